@@ -60,6 +60,10 @@ extern "C" {
 /* element types of x, y and the adapter weights */
 enum pl_dtype { PL_F32 = 0, PL_BF16 = 1, PL_F16 = 2 };
 
+/* a further element type, of paged key-value caches alone: 8-bit e4m3
+ * (finite values to 448, no infinities) */
+#define PL_F8E4M3 3
+
 /* epilogue rounding order of the expand (scale and add-back) */
 enum pl_epilogue {
   /* layers.py:127-128: d = T(acc); d = T(d * T(scale)); y = T(y + d) */
@@ -551,6 +555,81 @@ int pl_host_copy_async(void* dst, const void* src, int64_t nbytes, void* stream)
  * mask_dtype: 0 int64, 1 int32, 2 uint8/bool, 3 f32, 4 bf16, 5 f16. */
 int pl_check_right_padded(const void* mask, int32_t mask_dtype, int32_t B, int32_t S,
                           const int32_t* seq_lens, int32_t* flag, void* stream);
+
+/* ------------------------------------------------------------------------
+ * A decode step's work beside the Linears.  No counterpart in the reference,
+ * which leaves it to the wrapped model.
+ *
+ * A paged cache holds the keys (or values) of one layer in pages of
+ * page_size tokens (a power of two of at least 16): element (page, head,
+ * slot, d) at page * strides[0] + head * strides[1] + slot * strides[2] + d,
+ * so any order of page, head and slot.  page_table[row * table_ld + i] is
+ * the page of the row's tokens i * page_size and up; ids outside
+ * [0, num_pages) hold nothing.  The element type is the model's, or
+ * PL_F8E4M3 for 16-bit models, an element then standing for its value times
+ * k_scale[head] or v_scale[head] (else NULL).  Pointers and strides of the
+ * caches are whole 16-byte pieces; dim is a multiple of 16 up to 256. */
+
+/* Rotate the new tokens' q and k by position and append k and v to the rows'
+ * pages.  Token t of row b is live for t < min(seq_lens[b], row_len)
+ * (seq_lens NULL: row_len), has position past_lens[b] + t and goes to that
+ * place in the row's pages; a token whose position is outside [0, positions)
+ * or whose page the table does not hold is not live.  With c = cos[position]
+ * and s = sin[position], rows of rot / 2 fp32 values, and i below rot / 2,
+ *   x'[i] = x[i] c[i] - x[j] s[i],  x'[j] = x[j] c[i] + x[i] s[i],
+ * j = i + rot / 2, or, interleaved, the pairs (2i, 2i + 1) in place of
+ * (i, j); elements from rot on stay.  Computed in fp32 and rounded once; e4m3
+ * is the value over its scale, saturated.
+ * q [rows][row_len][heads][dim], k and v the same with kv_heads: strides of
+ * row, token and head, in elements.  q_out (and k_out, unless NULL) are
+ * contiguous and hold the rotated q (k), 0 for tokens that are not live; they
+ * do not overlap the inputs.  Two live tokens of one call never share a
+ * place in the pages. */
+int pl_rope_append(int32_t dtype, int32_t cache_dtype, const void* q, const int64_t* q_strides,
+                   const void* k, const int64_t* k_strides, const void* v,
+                   const int64_t* v_strides, void* q_out, void* k_out, void* key_cache,
+                   const int64_t* key_strides, void* value_cache, const int64_t* value_strides,
+                   int32_t num_pages, int32_t page_size, const int32_t* page_table,
+                   int64_t table_ld, int32_t max_pages, const int32_t* past_lens,
+                   const int32_t* seq_lens, int32_t rows, int32_t row_len, int32_t heads,
+                   int32_t kv_heads, int32_t dim, const float* cos, const float* sin,
+                   int32_t positions, int32_t rot, int32_t interleaved, const float* k_scale,
+                   const float* v_scale, void* stream);
+
+/* out[b][h] = sum over j of softmax_j(scale * q[b][h] . key_j) value_j, j over
+ * the last `window` (0: all) of the first min(lens[b], max_pages * page_size)
+ * tokens of row b's pages, key head h / (heads / kv_heads); tokens on pages
+ * the table does not hold are left out, and a row without a token gives 0.
+ * q [rows][heads][dim] with strides of row and head, out contiguous. */
+int pl_paged_attention(int32_t dtype, int32_t cache_dtype, const void* q,
+                       const int64_t* q_strides, const void* key_cache,
+                       const int64_t* key_strides, const void* value_cache,
+                       const int64_t* value_strides, int32_t num_pages, int32_t page_size,
+                       const int32_t* page_table, int64_t table_ld, int32_t max_pages,
+                       const int32_t* lens, int32_t rows, int32_t heads, int32_t kv_heads,
+                       int32_t dim, float scale, int32_t window, const float* k_scale,
+                       const float* v_scale, void* out, void* stream);
+
+/* Logits of one row for the choice of its next token, in fp32 and this order:
+ *   x = logits[b][v]
+ *   v among tokens[b][0 .. lens[b]):       x = x > 0 ? x / r : x * r,
+ *                                          r = repetition[b]
+ *   n > 0 times in [prompt_lens[b] ..):    x = x - (frequency[b] * n + presence[b])
+ *   entries j with bias_ids[b][j] == v:    x = x + (the sum of bias_values[b][j],
+ *                                          in the list's order)
+ *   bit v % 32 of allowed[b][v / 32] is 0: x = -infinity
+ * tokens (4 or 8 bytes each, at most 1048575 per row), bias lists (at most
+ * 2047 entries) and allowed may each be NULL, as may the three penalties
+ * and prompt_lens (then 0); ids outside [0, vocab) match nothing.  Row strides
+ * ld* are in elements, 0 for lists that all rows share.  out_dtype is PL_F32 or
+ * the logits' own type; out may be the logits (same type and stride). */
+int pl_adjust_logits(int32_t dtype, int32_t out_dtype, const void* logits, int64_t ld, void* out,
+                     int64_t ld_out, int32_t rows, int32_t vocab, const void* tokens,
+                     int32_t token_bytes, int64_t ld_tokens, int32_t history,
+                     const int32_t* lens, const int32_t* prompt_lens, const float* repetition,
+                     const float* presence, const float* frequency, const int32_t* bias_ids,
+                     const float* bias_values, int64_t ld_bias, int32_t n_bias,
+                     const int32_t* allowed, int64_t ld_allowed, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,6 +1,10 @@
 """polylora_amd — multi-LoRA inference with gfx950 HIP SGMV kernels.
 
 Same public names as the reference package ``polylora`` (src/polylora/__init__.py:1-18).
+What a decode step does beside the Linears is in ``polylora_amd.paged`` (append
+to a paged key-value cache, attention of one new token over it) and
+``polylora_amd.logits`` (penalties, biases and grammar masks), which the
+reference leaves to the wrapped model and its caller.
 """
 
 from .cache import GpuAdapterCache

@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import importlib.machinery
-from ctypes import c_int32, c_int64, c_void_p
+from ctypes import c_float, c_int32, c_int64, c_void_p
 from pathlib import Path
 
 import torch  # noqa: F401  (loads the HIP runtime the library must share)
@@ -18,6 +18,7 @@ LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libpolylora_hip.so"
 CALLS_PATH = LIB_PATH.parent / "_calls.so"
 
 PL_F32, PL_BF16, PL_F16 = 0, 1, 2
+PL_F8E4M3 = 3  # paged caches only
 PL_OK, PL_ERR_ARG, PL_ERR_ALIGN, PL_ERR_LAUNCH, PL_ERR_LIMIT = 0, 1, 2, 3, 4
 PL_EPI_FALLBACK, PL_EPI_TRITON = 0, 1
 PL_MAX_SLOTS = 4096
@@ -124,6 +125,22 @@ _SIGNATURES: dict[str, tuple] = {
     "pl_host_alloc": (c_int64,),
     "pl_host_free": (c_void_p,),
     "pl_slot_upload": (c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p),
+    "pl_rope_append": (
+        c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+        c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_int64, c_int32, c_void_p,
+        c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_int32, c_int32, c_int32,
+        c_void_p, c_void_p, c_void_p,
+    ),
+    "pl_paged_attention": (
+        c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32,
+        c_void_p, c_int64, c_int32, c_void_p, c_int32, c_int32, c_int32, c_int32, c_float, c_int32, c_void_p,
+        c_void_p, c_void_p, c_void_p,
+    ),
+    "pl_adjust_logits": (
+        c_int32, c_int32, c_void_p, c_int64, c_void_p, c_int64, c_int32, c_int32, c_void_p, c_int32, c_int64,
+        c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32,
+        c_void_p, c_int64, c_void_p,
+    ),
     "pl_check_right_padded": (c_void_p, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p),
 }
 _RESTYPES = {"pl_last_error": ctypes.c_char_p, "pl_plan_group_capacity": c_int64, "pl_shrink_workspace_bytes": c_int64,

@@ -28,7 +28,8 @@ CALLS_PATH = LIB_DIR / "_calls.so"
 INCLUDE_DIR = PACKAGE_DIR.parent / "include"
 
 ARCH = "gfx950"
-SOURCES = ("capi.hip", "plan.hip", "sgmv_tiled.hip", "sgmv_fused.hip", "sgmv_wide.hip", "sgmv_long.hip", "sgmv_rows.hip", "sgmv_refop.hip")
+SOURCES = ("capi.hip", "plan.hip", "sgmv_tiled.hip", "sgmv_fused.hip", "sgmv_wide.hip", "sgmv_long.hip", "sgmv_rows.hip", "sgmv_refop.hip",
+           "paged_append.hip", "paged_attention.hip", "logits.hip")
 HIPCC_FLAGS = (
     f"--offload-arch={ARCH}",
     "-O3",

@@ -221,6 +221,12 @@ inline pl_overlap pl_row_overlap(const void* x, int64_t ldx, int64_t K, const vo
                                                                     : pl_overlap::across;
 }
 
+// Whether two ranges of bytes meet.
+static inline bool pl_ranges_meet(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+  const uintptr_t p = reinterpret_cast<uintptr_t>(a), q = reinterpret_cast<uintptr_t>(b);
+  return a_bytes > 0 && b_bytes > 0 && p < q + (uint64_t)b_bytes && q < p + (uint64_t)a_bytes;
+}
+
 // The LoRA of rows straight from the row -> slot map and lengths, at any K, N,
 // stride and element alignment (sgmv_wide.hip), for rank capacities up to
 // kWideRankMax.  Returns PL_WIDE_DECLINED, having launched nothing, for what

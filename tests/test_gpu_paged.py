@@ -1,0 +1,426 @@
+"""The paged cache's operators against their 64-bit plain forms: sizes, types, layouts, masks, streams, refusals."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from oracle import decode as plain
+from polylora_amd.paged import paged_attention, rope_append, rope_table
+
+pytestmark = pytest.mark.gpu
+
+FP8 = torch.float8_e4m3fn
+# half a unit in the last place of each type, relative
+UNIT = {torch.float32: 2.0**-24, torch.bfloat16: 2.0**-8, torch.float16: 2.0**-11, FP8: 2.0**-4}
+# and the smallest step of its subnormals
+STEP = {torch.float32: 2.0**-149, torch.bfloat16: 2.0**-133, torch.float16: 2.0**-24, FP8: 2.0**-9}
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def pool(gen, rows, lens, kv_heads, dim, page, dtype, fp8=False, columns=0):
+    """CPU (key, value, table, k_scale, v_scale): random pages in random places, NaN in slots without a token."""
+    counts = [-(-n // page) for n in lens]
+    total = sum(counts) + 3
+    ids = torch.randperm(total, generator=gen).tolist()
+    width = max(1, columns, *counts)
+    table = torch.full((rows, width), -1, dtype=torch.int32)
+    held = torch.zeros(total, page, dtype=torch.bool)
+    at = 0
+    for b, n in enumerate(counts):
+        for i in range(n):
+            table[b, i] = ids[at]
+            held[ids[at], : min(page, lens[b] - i * page)] = True
+            at += 1
+    caches, scales = [], []
+    for _ in range(2):
+        x = torch.randn(total, kv_heads, page, dim, generator=gen)
+        scale = torch.rand(kv_heads, generator=gen) * 0.05 + 0.01
+        x = (x / scale[:, None, None]).clamp(-448, 448) if fp8 else x
+        x = x.masked_fill(~held[:, None, :, None], float("nan")).to(FP8 if fp8 else dtype)
+        caches.append(x)
+        scales.append(scale if fp8 else None)
+    return caches[0], caches[1], table, scales[0], scales[1]
+
+
+def put(x, gpu, order="head"):
+    """A cache on the GPU with its pages laid out by head or by slot."""
+    if x is None:
+        return None
+    if order == "head":
+        return x.to(gpu)
+    bits = x.view(torch.uint8) if x.dtype == FP8 else x
+    return bits.transpose(1, 2).contiguous().to(gpu).view(x.dtype).transpose(1, 2)
+
+
+def back(x):
+    return x.cpu().contiguous()
+
+
+# ----------------------------------------------------------------------------- append
+
+
+def check_append(got, want, unit_of, sizes):
+    """One rounding to the type, and fp32 products and sums before it (three roundings each)."""
+    got, want = back(got).double(), want
+    assert torch.equal(got.isnan(), want.isnan())
+    got, want, sizes = got.nan_to_num(0.0), want.nan_to_num(0.0), sizes.nan_to_num(0.0)
+    tol = UNIT[unit_of] * want.abs() + STEP[unit_of] / 2 + 2.0**-21 * sizes
+    assert bool(((got - want).abs() <= tol).all()), float(((got - want).abs() - tol).max())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,m,heads,kv_heads,dim,page,rot,interleaved,fp8,order", [
+    (1, 1, 4, 1, 16, 16, 16, False, False, "head"),
+    (3, 1, 32, 8, 128, 16, 128, False, False, "head"),
+    (5, 7, 6, 2, 80, 32, 80, False, False, "slot"),
+    (4, 37, 4, 4, 96, 16, 48, True, False, "head"),
+    (2, 5, 3, 1, 256, 64, 10, False, False, "slot"),
+    (2, 9, 5, 5, 48, 16, 30, True, False, "head"),
+    (3, 4, 2, 2, 64, 16, 0, False, False, "head"),
+    (3, 11, 8, 2, 128, 16, 128, False, True, "head"),
+    (2, 18, 4, 2, 80, 32, 40, False, True, "slot"),
+    (2, 3, 4, 2, 32, 16, 32, True, True, "head"),
+])
+def test_append_matches_the_plain_form(gpu, dtype, rows, m, heads, kv_heads, dim, page, rot, interleaved, fp8, order):
+    if fp8 and dtype == torch.float32:
+        pytest.skip("an 8-bit cache serves 16-bit models")
+    gen = torch.Generator().manual_seed(rows * 100 + m + dim)
+    past = torch.randint(0, 3 * page, (rows,), generator=gen)
+    seq = torch.randint(0, m + 3, (rows,), generator=gen)  # rows of no new token, and lengths above m
+    seq[0] = m
+    key, value, table, ks, vs = pool(gen, rows, [int(p) + m for p in past], kv_heads, dim, page, dtype, fp8)
+    if rows > 2:
+        table[-1, int(past[-1]) // page] = -1  # a page that the table does not hold
+    qkv = torch.randn(rows, m, heads + 2 * kv_heads, dim, generator=gen).to(dtype)
+    q, k, v = qkv.split((heads, kv_heads, kv_heads), 2)
+    cos, sin = rope_table(int(past.max()) + m, rot, 10000.0)
+    if fp8:
+        v[0, 0] *= 1000  # saturates
+    want = plain.rope_append(q, k, v, key, value, table, past, cos, sin, seq, interleaved, ks, vs)
+    # |x c| + |z s|, which the rounding errors are proportional to: the first of a pair with one sign, its second with the other
+    sizes = [plain.rope_append(q.abs(), k.abs(), v.abs(), key.double().abs(), value.double().abs(), table, past,
+                               cos.abs(), sign * sin.abs(), seq, interleaved, ks, vs) for sign in (-1, 1)]
+    qkv = qkv.to(gpu)
+    gq, gk, gv = qkv.split((heads, kv_heads, kv_heads), 2)
+    gkey, gvalue = put(key, gpu, order), put(value, gpu, order)
+    k_out = torch.full((rows, m, kv_heads, dim), 7.0, dtype=dtype, device=gpu)
+    up = {"k_scale": None if ks is None else ks.to(gpu), "v_scale": None if vs is None else vs.to(gpu)}
+    q_out = rope_append(gq, gk, gv, gkey, gvalue, table.to(gpu), past.int().to(gpu), cos.to(gpu), sin.to(gpu),
+                        seq_lens=seq.int().to(gpu), interleaved=interleaved, k_out=k_out, **up)
+    both = [torch.maximum(a, b) for a, b in zip(*sizes)]
+    check_append(q_out, want[0], dtype, both[0])
+    check_append(k_out, want[1], dtype, both[1])
+    cache_type = FP8 if fp8 else dtype
+    check_append(gkey, want[2], cache_type, both[2])
+    check_append(gvalue, want[3], cache_type, both[3])
+
+
+def test_append_keeps_every_other_byte_and_rounds_once(gpu):
+    """Values are copied bit for bit; bytes of other slots, pages and table columns stay."""
+    gen = torch.Generator().manual_seed(5)
+    dtype, page = torch.bfloat16, 16
+    past = [0, 15, 16, 31]
+    key, value, table, _, _ = pool(gen, 4, [p + 2 for p in past], 2, 64, page, dtype)
+    q = torch.randn(4, 2, 4, 64, generator=gen).to(dtype)
+    k, v = (torch.randn(4, 2, 2, 64, generator=gen).to(dtype) for _ in range(2))
+    cos, sin = torch.ones(64, 32), torch.zeros(64, 32)  # no turn: keys are copied too
+    gkey, gvalue = key.to(gpu), value.to(gpu)
+    q_out = rope_append(q.to(gpu), k.to(gpu), v.to(gpu), gkey, gvalue, table.to(gpu),
+                        torch.tensor(past, dtype=torch.int32, device=gpu), cos.to(gpu), sin.to(gpu))
+    for b, p in enumerate(past):
+        for t in range(2):
+            at = plain.place(table, b, p + t, key.shape[0], page)
+            key[at[0], :, at[1]], value[at[0], :, at[1]] = k[b, t], v[b, t]
+    assert torch.equal(back(gkey).view(torch.int16), key.view(torch.int16))
+    assert torch.equal(back(gvalue).view(torch.int16), value.view(torch.int16))
+    assert torch.equal(q_out.cpu(), q)
+
+
+def test_append_takes_empty_batches(gpu):
+    key = torch.zeros(2, 1, 16, 16, device=gpu)
+    cos, sin = rope_table(4, 16, device=gpu)
+    for rows, m in ((0, 3), (2, 0)):
+        x = torch.zeros(rows, m, 1, 16, device=gpu)
+        table = torch.zeros(rows, 1, dtype=torch.int32, device=gpu)
+        past = torch.zeros(rows, dtype=torch.int32, device=gpu)
+        assert rope_append(x, x, x, key, key.clone(), table, past, cos, sin).shape == (rows, m, 1, 16)
+
+
+def test_append_skips_positions_outside_the_table_and_the_angles(gpu):
+    key = torch.zeros(2, 1, 16, 16, device=gpu)
+    value = torch.zeros(2, 1, 16, 16, device=gpu)
+    x = torch.ones(5, 1, 1, 16, device=gpu)
+    table = torch.tensor([[0], [0], [2], [-5], [1]], dtype=torch.int32, device=gpu)
+    past = torch.tensor([16, -1, 3, 3, 9], dtype=torch.int32, device=gpu)  # past the columns, below 0, no such page (2x), past cos
+    cos, sin = rope_table(9, 16, device=gpu)
+    q = rope_append(x, x, x, key, value, table, past, cos, sin)
+    assert not q.any() and not key.any() and not value.any()
+
+
+# ----------------------------------------------------------------------------- attention
+
+
+def attention_tolerance(want, spread, reach, dtype, dim, tokens):
+    """One rounding of the output; scores off by (dim + 8) fp32 roundings of |q| . |k| and exponents and factors by a
+    few more, which move each weight by that share; weights of 16-bit values kept to 2 ** -15; sums of at most one
+    addition for every 32 tokens and 64 more."""
+    weights = 2.0**-24 * (4 * (dim + 8) * reach + 16) + 2.0**-24 * (tokens / 32 + 64)
+    if dtype != torch.float32:
+        weights = weights + 2.0**-15
+    return UNIT[dtype] * want.abs() + STEP[dtype] + weights * spread
+
+
+def check_attention(gpu, dtype, lens, heads, kv_heads, dim, page, fp8=False, order="head", window=None, scale=None,
+                    seed=0, q_gain=1.5, holes=False, columns=0):
+    gen = torch.Generator().manual_seed(seed + dim + heads)
+    rows = len(lens)
+    held = [min(n, (columns or 10**9) * page) for n in lens]
+    key, value, table, ks, vs = pool(gen, rows, held, kv_heads, dim, page, dtype, fp8, columns=columns)
+    if holes:
+        table[::2, 0] = -1
+        table[1::2, 0] = key.shape[0]
+    q = (torch.randn(rows, heads + 1, dim, generator=gen) * q_gain).to(dtype)
+    n = torch.tensor(lens, dtype=torch.int32)
+    want, spread, reach = plain.paged_attention(q[:, 1:], key, value, table, n, scale, window, ks, vs)
+    up = {"k_scale": None if ks is None else ks.to(gpu), "v_scale": None if vs is None else vs.to(gpu)}
+    args = (q.to(gpu)[:, 1:], put(key, gpu, order), put(value, gpu, order), table.to(gpu), n.to(gpu))
+    got = paged_attention(*args, scale=scale, window=window, **up)
+    tol = attention_tolerance(want, spread, reach, dtype, dim, max(1, *lens))
+    err = (got.cpu().double() - want).abs()
+    assert not got.isnan().any()
+    assert bool((err <= tol).all()), (float((err / tol).max()), float(err.max()))
+    again = torch.full_like(got, 7.0)
+    assert paged_attention(*args, scale=scale, window=window, out=again, **up) is again
+    assert torch.equal(again, got)  # the same bits each time
+    return got
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads,kv_heads,dim,page", [
+    (1, 1, 16, 16), (4, 1, 32, 16), (32, 8, 128, 16), (12, 12, 80, 32), (28, 4, 96, 64), (9, 3, 256, 16),
+    (16, 1, 64, 128), (17, 1, 64, 16), (40, 2, 48, 16), (6, 2, 192, 32), (3, 1, 112, 16), (5, 5, 144, 16),
+])
+def test_attention_matches_the_plain_form(gpu, dtype, heads, kv_heads, dim, page):
+    check_attention(gpu, dtype, [1, 0, 2, 15, 16, 17, 33, 100, 257], heads, kv_heads, dim, page)
+
+
+@pytest.mark.parametrize("dtype", DTYPES[:2])
+@pytest.mark.parametrize("heads,kv_heads,dim,page,order", [
+    (4, 1, 16, 16, "head"), (32, 8, 128, 16, "slot"), (12, 4, 96, 32, "head"), (8, 8, 80, 16, "head"),
+    (20, 1, 64, 64, "slot"), (4, 2, 256, 16, "head"),
+])
+def test_attention_over_an_8_bit_cache(gpu, dtype, heads, kv_heads, dim, page, order):
+    check_attention(gpu, dtype, [3, 0, 31, 64, 65, 300], heads, kv_heads, dim, page, fp8=True, order=order)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("window", [1, 2, 16, 31, 63, 64, 1000])
+def test_attention_windows(gpu, dtype, window):
+    check_attention(gpu, dtype, [0, 1, 16, 40, 63, 64, 65, 200], 8, 2, 64, 16, window=window, order="slot")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lens,heads,kv_heads", [([5000], 8, 2), ([3000, 1, 2999], 4, 4), ([2049] * 4 + [0] * 9, 16, 1)])
+def test_attention_over_long_rows(gpu, dtype, lens, heads, kv_heads):
+    check_attention(gpu, dtype, lens, heads, kv_heads, 128, 16)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attention_of_many_rows(gpu, dtype):
+    gen = torch.Generator().manual_seed(3)
+    check_attention(gpu, dtype, torch.randint(0, 70, (700,), generator=gen).tolist(), 4, 2, 64, 16)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attention_leaves_out_pages_the_table_does_not_hold(gpu, dtype):
+    check_attention(gpu, dtype, [10, 16, 17, 40, 300], 8, 2, 64, 16, holes=True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attention_clamps_lengths_to_the_table(gpu, dtype):
+    check_attention(gpu, dtype, [10_000, 64, 65, 0], 8, 2, 64, 16, columns=4)
+
+
+def test_attention_of_negative_lengths_is_empty(gpu):
+    key = torch.ones(2, 1, 16, 64, dtype=torch.bfloat16, device=gpu)
+    table = torch.zeros(2, 1, dtype=torch.int32, device=gpu)
+    q = torch.ones(2, 1, 64, dtype=torch.bfloat16, device=gpu)
+    assert not paged_attention(q, key, key, table, torch.tensor([-1, -100], dtype=torch.int32, device=gpu)).any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("scale,gain", [(1.0, 20.0), (0.0, 1.0), (-0.3, 1.0), (0.125, 40.0)])
+def test_attention_scales_and_peaks(gpu, dtype, scale, gain):
+    """One token that takes all of the weight, all tokens alike, and a negative scale."""
+    check_attention(gpu, dtype, [1, 30, 64, 129, 1000], 4, 2, 64, 16, scale=scale, q_gain=gain)
+
+
+def test_attention_takes_no_rows_and_no_pages(gpu):
+    key = torch.zeros(0, 2, 16, 64, dtype=torch.bfloat16, device=gpu)
+    q = torch.zeros(0, 4, 64, dtype=torch.bfloat16, device=gpu)
+    none = torch.zeros(0, dtype=torch.int32, device=gpu)
+    assert paged_attention(q, key, key, none.view(0, 0), none).shape == (0, 4, 64)
+    q = torch.ones(3, 4, 64, dtype=torch.bfloat16, device=gpu)
+    table = torch.full((3, 2), -1, dtype=torch.int32, device=gpu)
+    assert not paged_attention(q, key, key, table, torch.full((3,), 20, dtype=torch.int32, device=gpu)).any()
+    assert not paged_attention(q, key, key, table[:, :0], torch.full((3,), 20, dtype=torch.int32, device=gpu)).any()
+
+
+# ----------------------------------------------------------------------------- streams and graphs
+
+
+def _step(gpu, gen, rows=6, dtype=torch.bfloat16, longest=900):
+    past = torch.randint(0, longest, (rows,), generator=gen)
+    key, value, table, _, _ = pool(gen, rows, [int(p) + 1 for p in past], 2, 64, 16, dtype)
+    q, k, v = (torch.randn(rows, 1, h, 64, generator=gen).to(dtype).to(gpu) for h in (8, 2, 2))
+    cos, sin = rope_table(longest + 1, 64, device=gpu)
+    key, value, table, past = key.to(gpu), value.to(gpu), table.to(gpu), past.int().to(gpu)
+
+    def run():
+        turned = rope_append(q, k, v, key, value, table, past, cos, sin)
+        return paged_attention(turned[:, 0], key, value, table, past + 1)
+
+    return run, q
+
+
+def test_append_then_attend_on_two_streams(gpu):
+    gen = torch.Generator().manual_seed(11)
+    steps = [_step(gpu, gen)[0] for _ in range(2)]
+    want = [s() for s in steps]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in steps]
+    for _ in range(3):
+        got = []
+        for s, step in zip(streams, steps):
+            with torch.cuda.stream(s):
+                got.append(step())
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("warm", [True, False])
+def test_append_then_attend_in_a_graph(gpu, warm):
+    """Replays with new inputs between them, and eager calls of other sizes on the same stream."""
+    gen = torch.Generator().manual_seed(12)
+    run, q = _step(gpu, gen)
+    other, _ = _step(gpu, gen, rows=3, longest=5000)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        if warm:
+            run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        out = run()
+    other_want = other()
+    for i in range(4):
+        q.copy_(torch.randn(q.shape, generator=gen).to(q.dtype))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        with torch.cuda.stream(stream):
+            assert torch.equal(other(), other_want)
+            assert torch.equal(run(), got)
+        torch.cuda.synchronize()
+
+
+# ----------------------------------------------------------------------------- refusals
+
+
+def _good(gpu, dtype=torch.bfloat16):
+    key = torch.zeros(3, 2, 16, 32, dtype=dtype, device=gpu)
+    i32 = dict(dtype=torch.int32, device=gpu)
+    a = {"q": torch.zeros(2, 4, 32, dtype=dtype, device=gpu), "key_cache": key, "value_cache": key.clone(),
+         "page_table": torch.zeros(2, 1, **i32), "lens": torch.ones(2, **i32)}
+    cos, sin = rope_table(4, 32, device=gpu)
+    x = torch.zeros(2, 1, 2, 32, dtype=dtype, device=gpu)
+    b = {"q": torch.zeros(2, 1, 4, 32, dtype=dtype, device=gpu), "k": x, "v": x.clone(), "key_cache": key,
+         "value_cache": key.clone(), "page_table": a["page_table"], "past_lens": torch.zeros(2, **i32), "cos": cos, "sin": sin}
+    return a, b
+
+
+def test_refusals_of_both(gpu):
+    attend, append = _good(gpu)
+    paged_attention(**attend)
+    rope_append(**append)
+    key = attend["key_cache"]
+    fp8 = torch.zeros(3, 2, 16, 32, dtype=FP8, device=gpu)
+    ones = torch.ones(2, device=gpu)
+    bad = [
+        ({"key_cache": key[:, :, :, :16]}, ValueError),  # another head size
+        ({"key_cache": key[:2]}, ValueError),  # caches of two sizes
+        ({"key_cache": key.float(), "value_cache": key.float()}, TypeError),
+        ({"value_cache": key.half()}, TypeError),
+        ({"key_cache": fp8, "value_cache": fp8}, ValueError),  # no scales
+        ({"key_cache": fp8, "value_cache": fp8, "k_scale": ones, "v_scale": ones[:1]}, ValueError),
+        ({"key_cache": fp8, "value_cache": fp8, "k_scale": ones, "v_scale": ones.double()}, TypeError),
+        ({"k_scale": ones, "v_scale": ones}, ValueError),  # scales without an 8-bit cache
+        ({"key_cache": key[:, :, :8], "value_cache": key[:, :, :8]}, ValueError),  # pages of 8 tokens
+        ({"key_cache": key.new_zeros(3, 2, 48, 32), "value_cache": key.new_zeros(3, 2, 48, 32)}, ValueError),
+        ({"key_cache": key.transpose(2, 3).contiguous().transpose(2, 3)}, ValueError),
+        ({"key_cache": key.cpu()}, (TypeError, ValueError)),
+        ({"page_table": attend["page_table"].long()}, TypeError),
+        ({"page_table": attend["page_table"][:1]}, ValueError),
+        ({"page_table": attend["page_table"][:, 0]}, ValueError),
+        ({"page_table": attend["page_table"].cpu()}, ValueError),
+        # strides that are no whole 16-byte pieces
+        ({"key_cache": key.new_zeros(3, 2, 16, 33)[..., :32]}, RuntimeError),
+    ]
+    for change, error in bad:
+        for fn, good in ((paged_attention, attend), (rope_append, append)):
+            with pytest.raises(error):
+                fn(**{**good, **change})
+
+
+def test_refusals_of_the_attention(gpu):
+    good, _ = _good(gpu)
+    q, key = good["q"], good["key_cache"]
+    odd = key.new_zeros(3, 2, 16, 24)
+    bad = [
+        ({"q": q.cpu()}, RuntimeError),
+        ({"q": q[:, :3]}, ValueError),  # three heads over two
+        ({"q": q[0]}, ValueError),
+        ({"q": q.double()}, TypeError),
+        ({"q": q.transpose(1, 2).contiguous().transpose(1, 2)}, ValueError),
+        ({"lens": good["lens"].long()}, TypeError),
+        ({"lens": good["lens"][:1]}, ValueError),
+        ({"window": 0}, ValueError),
+        ({"window": -4}, ValueError),
+        ({"out": torch.empty(2, 4, 32, device=gpu)}, TypeError),
+        ({"out": torch.empty(2, 4, 16, dtype=q.dtype, device=gpu)}, ValueError),
+        ({"out": q}, RuntimeError),  # over the queries
+        ({"q": q.new_zeros(2, 4, 24), "key_cache": odd, "value_cache": odd}, RuntimeError),  # heads of 24
+        ({"q": q.new_zeros(2, 4, 272), "key_cache": key.new_zeros(3, 2, 16, 272),
+          "value_cache": key.new_zeros(3, 2, 16, 272)}, RuntimeError),
+    ]
+    for change, error in bad:
+        with pytest.raises(error):
+            paged_attention(**{**good, **change})
+
+
+def test_refusals_of_the_append(gpu):
+    _, good = _good(gpu)
+    k, cos = good["k"], good["cos"]
+    bad = [
+        ({"q": good["q"].cpu()}, RuntimeError),
+        ({"q": good["q"][:, 0]}, ValueError),
+        ({"k": k[:1]}, ValueError),
+        ({"v": k[:, :, :1]}, ValueError),
+        ({"v": k.float()}, TypeError),
+        ({"k": k[:, :, :1], "v": k[:, :, :1]}, ValueError),  # fewer heads than the cache
+        ({"past_lens": good["past_lens"].long()}, TypeError),
+        ({"past_lens": good["past_lens"][:1]}, ValueError),
+        ({"seq_lens": good["past_lens"].long()}, TypeError),
+        ({"cos": cos.half()}, TypeError),
+        ({"sin": cos[:1]}, ValueError),
+        ({"cos": cos[:, :4].t(), "sin": cos[:, :4].t()}, ValueError),
+        ({"cos": torch.ones(4, 17, device=gpu), "sin": torch.ones(4, 17, device=gpu)}, ValueError),
+        ({"k_out": k[:, :, :1]}, ValueError),
+        ({"k_out": k}, RuntimeError),  # over the keys
+    ]
+    for change, error in bad:
+        with pytest.raises(error):
+            rope_append(**{**good, **change})
