@@ -600,7 +600,16 @@ int pl_rope_append(int32_t dtype, int32_t cache_dtype, const void* q, const int6
  * the last `window` (0: all) of the first min(lens[b], max_pages * page_size)
  * tokens of row b's pages, key head h / (heads / kv_heads); tokens on pages
  * the table does not hold are left out, and a row without a token gives 0.
- * q [rows][heads][dim] with strides of row and head, out contiguous. */
+ * q [rows][heads][dim] with strides of row and head, out contiguous and apart
+ * from q.  The rows are split over the workgroups by their tokens, found from
+ * lens on the device; parts of a row are joined inside the launch through the
+ * workspace (pl_paged_attention_workspace_bytes(dim) bytes, 128-byte aligned,
+ * not cleared) and counters (PL_ATTENTION_COUNTER_INTS int32s, zero before the
+ * first launch and zero again after each), which launches that overlap must not
+ * share.  The result does not depend on which workgroup ends last. */
+#define PL_ATTENTION_COUNTER_INTS 12288
+int64_t pl_paged_attention_workspace_bytes(int32_t dim);
+
 int pl_paged_attention(int32_t dtype, int32_t cache_dtype, const void* q,
                        const int64_t* q_strides, const void* key_cache,
                        const int64_t* key_strides, const void* value_cache,
@@ -608,7 +617,9 @@ int pl_paged_attention(int32_t dtype, int32_t cache_dtype, const void* q,
                        const int32_t* page_table, int64_t table_ld, int32_t max_pages,
                        const int32_t* lens, int32_t rows, int32_t heads, int32_t kv_heads,
                        int32_t dim, float scale, int32_t window, const float* k_scale,
-                       const float* v_scale, void* out, void* stream);
+                       const float* v_scale, void* out, void* workspace,
+                       int64_t workspace_bytes, int32_t* counters, int64_t counter_ints,
+                       void* stream);
 
 /* Logits of one row for the choice of its next token, in fp32 and this order:
  *   x = logits[b][v]

@@ -27,6 +27,7 @@ PL_MAX_STACKED_MODULES = 4
 PL_NOALLOC_SCRATCH_BYTES = 32 << 20
 PL_REF_PART_PLAN, PL_REF_PART_WEIGHTS, PL_REF_PART_SCRATCH = 0, 1, 2
 PL_REF_BUILD_PLAN, PL_REF_PACK_USED, PL_REF_PACK_ALL, PL_REF_KEEP_PACKED = 1, 2, 4, 8
+PL_ATTENTION_COUNTER_INTS = 12288
 SLOT_ENTRY_INT32S = 8  # sizeof(pl_slot_entry) / 4
 
 DTYPE_CODES = {torch.float32: PL_F32, torch.bfloat16: PL_BF16, torch.float16: PL_F16}
@@ -134,8 +135,9 @@ _SIGNATURES: dict[str, tuple] = {
     "pl_paged_attention": (
         c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32,
         c_void_p, c_int64, c_int32, c_void_p, c_int32, c_int32, c_int32, c_int32, c_float, c_int32, c_void_p,
-        c_void_p, c_void_p, c_void_p,
+        c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
     ),
+    "pl_paged_attention_workspace_bytes": (c_int32,),
     "pl_adjust_logits": (
         c_int32, c_int32, c_void_p, c_int64, c_void_p, c_int64, c_int32, c_int32, c_void_p, c_int32, c_int64,
         c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32,
@@ -146,7 +148,7 @@ _SIGNATURES: dict[str, tuple] = {
 _RESTYPES = {"pl_last_error": ctypes.c_char_p, "pl_plan_group_capacity": c_int64, "pl_shrink_workspace_bytes": c_int64,
              "pl_host_alloc": c_void_p, "pl_sgmv_ref_workspace_bytes": c_int64, "pl_decode_counter_ints": c_int64,
              "pl_sgmv_ref_part_bytes": c_int64, "pl_lora_long_workspace_bytes": c_int64,
-             "pl_stream_capture_id": c_int64}
+             "pl_stream_capture_id": c_int64, "pl_paged_attention_workspace_bytes": c_int64}
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 

@@ -1,9 +1,67 @@
 // Attention of one new token per row over a paged key-value cache.
+//
+// With s_j = scale * q . k_j over the tokens j of a row,
+//   out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),   m = max_j s_j,
+// in one pass over keys and values: a running maximum m, sum l and unscaled
+// output o, all fp32; a larger maximum rescales l and o by exp(m_old - m), and
+// two partial results (m, l, o) of disjoint tokens join by the same rule.
+//
+// Each key and value element is read once and takes 2 * heads / kv_heads
+// operations a head, a few per byte: memory bounds it.  What carries it is
+// that every wave has whole tiles of loads in flight and nothing is staged:
+// keys and values go from their pages straight into the registers that feed
+// the matrix instructions.
+//
+// A wave takes tiles of 32 tokens (16 in fp32) of one (row, key head) and the
+// up to 16 query heads that share it, one per column of a 16x16 matrix
+// product; lane l stands for column l % 16 and lane group l / 16.
+//   S^T = K Q^T   lane (i, g) supplies 16-byte pieces of token i's key and of
+//                 query i; it gets the scores of query i with tokens 4g .. 4g+3
+//                 of each 16.
+//   O^T = V^T P^T the contraction over tokens may take them in any order that
+//                 both operands share, so each lane keeps the tokens whose
+//                 scores it got: the weights never leave their lane, and the
+//                 lane reads those tokens' values, dim / 16 consecutive
+//                 elements of each, and pairs them up by byte permutes.  It
+//                 gets the outputs of query i, so the maximum, the sum and the
+//                 rescaling of a query all stay in the lanes of its column.
+// Weights go into the product as two 16-bit numbers, p = hi + lo, which keeps
+// them to 2^-16 (bf16) or better: one product more on matrix units that have
+// little else to do, and the output keeps the error of its own rounding.
+//
+// Work is split by tokens: the launch is a fixed number of workgroups, and
+// each takes an equal run of the batch's atoms (kAtom tokens of one row and
+// key head), found from the lengths on the device, so no length is needed on
+// the host and ragged batches come out even.  A run that covers a (row, key
+// head) whole writes its output; a run that ends inside one leaves (m, l, o) in
+// the workspace, and the workgroup that arrives last on the pair's counter
+// joins the parts in order (the same bits whichever arrives last).
 #include "pl_paged.h"
 
 namespace {
 
 constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * 64;
+constexpr int kCols = 16;  // query heads of a workgroup's products
+
+// Workgroups of a launch: three (or as many as registers allow) on each CU.
+constexpr int kWorkersMax = 768;
+constexpr int kCounterStride = 16;  // int32s: 64 bytes for each counter
+
+template <int DT, int CT, int DP>
+struct shape {
+  static constexpr int E = pl_traits<DT>::E;         // elements of a 16-byte piece
+  static constexpr int kSubs = DT == PL_F32 ? 1 : 2; // 16-token parts of a tile
+  static constexpr int kTile = 16 * kSubs;
+  static constexpr int kAtom = 32 * kWaves;
+  static constexpr int kSteps = DP / (4 * E);        // products of 4 pieces along a key
+  static constexpr int kCsize = CT == PL_F8E4M3 ? 1 : DT == PL_F32 ? 4 : 2;
+  static constexpr int kKeyLoads = DP * kCsize / 64; // 16-byte loads of a lane per 16 keys
+  static constexpr int V = DP / 16;                  // value elements of a lane per token
+  static constexpr int kVWords = V * kCsize / 4;
+  static constexpr int kTokens = 4 * kSubs;          // tokens of a lane per tile
+  static constexpr int kPerCu = DP <= 128 ? 3 : DT == PL_F32 ? 1 : 2;
+};
 
 struct attend_args {
   const void* q;
@@ -13,81 +71,446 @@ struct attend_args {
   const int32_t* lens;
   const float *k_scale, *v_scale;
   void* out;  // contiguous [rows][heads][dim]
+  float* parts;
+  int32_t* counters;
   float scale;
-  int32_t rows, heads, kv_heads, dim, window;
+  int32_t rows, heads, kv_heads, dim, window, group, col_tiles;
 };
 
-template <int CT>
-__device__ __forceinline__ float from_cache(typename pl_cache_elem<CT>::T x) {
-  if constexpr (CT == PL_F8E4M3)
-    return __builtin_amdgcn_cvt_f32_fp8((int)x, 0);
-  else
-    return (float)x;
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// The largest of the four lanes of a column, and their sum.
+__device__ __forceinline__ float column_max(float x) {
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float column_sum(float x) {
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// One workgroup per (row, query head).  Each wave walks every kWaves-th token
-// with a running maximum, sum and output of its own, its lanes holding dim / 64
-// elements each; the waves' are joined in LDS at the end.
-template <int DT, int CT>
-__global__ __launch_bounds__(kWaves * 64) void pl_paged_attention_kernel(attend_args a) {
-  typedef typename pl_traits<DT>::T T;
-  typedef typename pl_cache_elem<CT>::T C;
-  constexpr int kPer = kHeadDimMax / 64;
-  const int b = (int)(blockIdx.x / a.heads), h = (int)(blockIdx.x % a.heads);
-  const int hk = h / (a.heads / a.kv_heads);
-  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
-  const int64_t cap = (int64_t)a.table.max_pages << a.table.page_shift;
-  const int len = (int)min((int64_t)max(a.lens[b], 0), cap);
-  const int first = a.window > 0 ? max(0, len - a.window) : 0;
-  float q[kPer], o[kPer], m = -INFINITY, l = 0.f;
-  const float scale = a.scale * (CT == PL_F8E4M3 ? a.k_scale[hk] : 1.f);
+template <int N>
+__device__ __forceinline__ void load_words(const char* p, bool ok, uint32_t (&w)[N]) {
+  p = ok ? p : reinterpret_cast<const char*>(pl_zero64);
+  if constexpr (N % 4 == 0) {
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int d = lane + 64 * i;
-    q[i] = d < a.dim ? (float)((const T*)a.q)[b * a.q_row + h * a.q_head + d] * scale : 0.f;
-    o[i] = 0.f;
+    for (int i = 0; i < N / 4; ++i) {
+      const pl_u32x4 x = pl_ld16(p + 16 * i);
+      w[4 * i] = x.x, w[4 * i + 1] = x.y, w[4 * i + 2] = x.z, w[4 * i + 3] = x.w;
+    }
+  } else if constexpr (N == 2) {
+    typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+    const u2 x = *reinterpret_cast<const u2*>(p);
+    w[0] = x.x, w[1] = x.y;
+  } else {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
   }
-  for (int j = first + wave; j < len; j += kWaves) {
-    const int page = a.table.p[b * a.table.ld + (j >> a.table.page_shift)];
-    if (page < 0 || page >= a.table.num_pages) continue;
-    const int slot = j & ((1 << a.table.page_shift) - 1);
-    const C* k = (const C*)a.key.p + page * a.key.s_page + hk * a.key.s_head + slot * a.key.s_slot;
-    const C* v =
-        (const C*)a.value.p + page * a.value.s_page + hk * a.value.s_head + slot * a.value.s_slot;
-    float s = 0.f, x[kPer];
+}
+
+// Two e4m3 values of a word as a pair of the model's 16-bit type (exact).
+template <int DT, bool HIGH>
+__device__ __forceinline__ uint32_t widen(uint32_t w) {
+  if constexpr (DT == PL_BF16)
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, HIGH));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, HIGH));
+}
+
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  typedef typename pl_traits<DT>::T T;
+  typedef T T2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, T2{(T)a, (T)b});
+}
+template <int DT>
+__device__ __forceinline__ float unpack(uint32_t w, int half) {
+  typedef typename pl_traits<DT>::T T;
+  typedef T T2 __attribute__((ext_vector_type(2)));
+  return (float)__builtin_bit_cast(T2, w)[half];
+}
+
+// What a wave holds of one (row, key head): its queries, and m (in units of
+// log2 e), l (this lane's tokens alone) and o of its tiles so far.
+template <int DT, int CT, int DP>
+struct wave_state {
+  typedef shape<DT, CT, DP> S;
+  pl_u32x4 q[S::kSteps];
+  pl_f32x4 o[S::V];
+  float m, l;
+};
+
+// The keys of one tile, as loaded.
+template <int DT, int CT, int DP>
+struct key_tile {
+  typedef shape<DT, CT, DP> S;
+  pl_u32x4 w[S::kSubs][S::kKeyLoads];
+};
+
+// First element of the 16-byte key piece that lane group g loads n-th.
+template <int CT>
+__device__ __forceinline__ int key_piece(int n, int g, int e) {
+  return (n * 4 + g) * (CT == PL_F8E4M3 ? 16 : e);
+}
+
+template <int DT, int CT, int DP>
+__device__ __forceinline__ void attend_tile(wave_state<DT, CT, DP>& st,
+                                            const key_tile<DT, CT, DP>& keys,
+                                            const uint32_t (&v)[shape<DT, CT, DP>::kTokens]
+                                                               [shape<DT, CT, DP>::kVWords],
+                                            float scale2, bool whole, uint32_t alive) {
+  typedef shape<DT, CT, DP> S;
+  pl_f32x4 s[S::kSubs];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int d = lane + 64 * i;
-      s += d < a.dim ? q[i] * from_cache<CT>(k[d]) : 0.f;
-      x[i] = d < a.dim ? from_cache<CT>(v[d]) : 0.f;
+  for (int u = 0; u < S::kSubs; ++u) {
+    s[u] = pl_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int n = 0; n < S::kKeyLoads; ++n) {
+      const pl_u32x4 w = keys.w[u][n];
+      if constexpr (CT == PL_F8E4M3) {
+        const pl_u32x4 a = {widen<DT, false>(w.x), widen<DT, true>(w.x), widen<DT, false>(w.y),
+                            widen<DT, true>(w.y)};
+        const pl_u32x4 b = {widen<DT, false>(w.z), widen<DT, true>(w.z), widen<DT, false>(w.w),
+                            widen<DT, true>(w.w)};
+        s[u] = pl_mfma_chunk<DT>(a, st.q[2 * n], s[u]);
+        s[u] = pl_mfma_chunk<DT>(b, st.q[2 * n + 1], s[u]);
+      } else {
+        s[u] = pl_mfma_chunk_short<DT>(w, st.q[n], s[u]);
+      }
+    }
+  }
+  float p[S::kTokens], top = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < S::kTokens; ++j) {
+    p[j] = s[j / 4][j % 4] * scale2;
+    if (!whole) p[j] = (alive >> j & 1) ? p[j] : -INFINITY;
+    top = fmaxf(top, p[j]);
+  }
+  top = fmaxf(st.m, column_max(top));
+  // nothing alive yet: any finite reference gives weights of 0
+  const float ref = top == -INFINITY ? 0.f : top;
+  if (__any(top > st.m)) {
+    const float keep = exp2_fast(st.m - ref);
+    st.l *= keep;
+#pragma unroll
+    for (int i = 0; i < S::V; ++i) st.o[i] *= keep;
+    st.m = top;
+  }
+#pragma unroll
+  for (int j = 0; j < S::kTokens; ++j) {
+    p[j] = exp2_fast(p[j] - ref);
+    st.l += p[j];
+  }
+  if constexpr (DT == PL_F32) {
+#pragma unroll
+    for (int i = 0; i < S::V; ++i) {
+      pl_f32x4 part = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < S::kTokens; ++j)
+        part = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[j][i]), p[j], part, 0, 0, 0);
+      st.o[i] += part;
+    }
+  } else {
+    pl_u32x4 hi, lo;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      hi[j] = pack2<DT>(p[2 * j], p[2 * j + 1]);
+      lo[j] = pack2<DT>(p[2 * j] - unpack<DT>(hi[j], 0), p[2 * j + 1] - unpack<DT>(hi[j], 1));
     }
 #pragma unroll
-    for (int w = 32; w > 0; w >>= 1) s += __shfl_xor(s, w);
-    const float top = fmaxf(m, s);
-    const float keep = m == top ? 1.f : __expf(m - top), p = s == top ? 1.f : __expf(s - top);
-    l = l * keep + p;
+    for (int i = 0; i < S::V / 2; ++i) {
+      uint32_t w[8];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) o[i] = o[i] * keep + p * x[i];
-    m = top;
+      for (int j = 0; j < 8; ++j) {
+        if constexpr (CT == PL_F8E4M3)
+          w[j] = i % 2 ? widen<DT, true>(v[j][i / 2]) : widen<DT, false>(v[j][i / 2]);
+        else
+          w[j] = v[j][i];
+      }
+      pl_u32x4 a, b;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        a[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x05040100);
+        b[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x07060302);
+      }
+      st.o[2 * i] = pl_mfma_chunk<DT>(a, hi, st.o[2 * i]);
+      st.o[2 * i + 1] = pl_mfma_chunk<DT>(b, hi, st.o[2 * i + 1]);
+      st.o[2 * i] = pl_mfma_chunk<DT>(a, lo, st.o[2 * i]);
+      st.o[2 * i + 1] = pl_mfma_chunk<DT>(b, lo, st.o[2 * i + 1]);
+    }
   }
-  __shared__ float s_m[kWaves], s_l[kWaves], s_o[kWaves][kHeadDimMax];
-  if (lane == 0) s_m[wave] = m, s_l[wave] = l;
+}
+
+// A row's tokens that count: [first, len), its atoms starting at base.
+struct row_span {
+  int first, len, base, atoms;
+};
+template <int ATOM>
+__device__ __forceinline__ row_span span_of(const attend_args& a, int len) {
+  const int64_t cap = a.table.num_pages ? (int64_t)a.table.max_pages << a.table.page_shift : 0;
+  row_span r;
+  r.len = (int)min((int64_t)max(len, 0), cap);
+  r.first = a.window > 0 ? max(0, r.len - a.window) : 0;
+  r.base = r.first & ~31;
+  r.atoms = max(1, (r.len - r.base + ATOM - 1) / ATOM);  // an empty row's output is an atom too
+  return r;
+}
+
+// Floats of one part: o [kCols][DP], then m and l of each column.
+constexpr int part_floats(int dp) { return kCols * dp + 2 * kCols; }
+
+template <int DT, int CT, int DP>
+__global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kPerCu)) void pl_paged_attention_kernel(
+    attend_args a) {
+  typedef shape<DT, CT, DP> S;
+  typedef typename pl_traits<DT>::T T;
+  constexpr int kPad = 4;
+  __shared__ float s_o[kWaves][kCols][DP + kPad];
+  __shared__ float s_m[kWaves][kCols], s_l[kWaves][kCols];
+  __shared__ int64_t s_scan[kWaves];
+  __shared__ int s_row, s_last;
+  __shared__ int64_t s_before;
+  const int tid = (int)threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int li = lane & 15, lg = lane >> 4;
+  const int per_row = a.kv_heads * a.col_tiles;
+
+  // atoms of the batch, then this workgroup's run of them
+  int64_t mine = 0;
+  for (int b = tid; b < a.rows; b += kThreads) mine += span_of<S::kAtom>(a, a.lens[b]).atoms;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) s_o[wave][lane + 64 * i] = o[i];
+  for (int w = 32; w > 0; w >>= 1) mine += __shfl_xor(mine, w);
+  if (lane == 0) s_scan[wave] = mine;
   __syncthreads();
-  const int d = (int)threadIdx.x;
-  if (d >= a.dim) return;
-  float top = -INFINITY, sum = 0.f, acc = 0.f;
-  for (int w = 0; w < kWaves; ++w) top = fmaxf(top, s_m[w]);
-  for (int w = 0; w < kWaves; ++w) {
-    const float f = s_l[w] > 0.f ? (s_m[w] == top ? 1.f : __expf(s_m[w] - top)) : 0.f;
-    sum += f * s_l[w], acc += f * s_o[w][d];
+  int64_t total = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) total += s_scan[w];
+  total *= per_row;
+  const int64_t per = (total + gridDim.x - 1) / gridDim.x;
+  const int64_t from = blockIdx.x * per, to = min(total, from + per);
+  if (from >= to) return;
+  // the row of its first atom: the first whose atoms up to and with it pass `from`
+  if (tid < 64) {
+    int64_t before = 0;
+    for (int b0 = 0;; b0 += 64) {
+      const int b = b0 + lane;
+      int64_t n = b < a.rows ? (int64_t)span_of<S::kAtom>(a, a.lens[b]).atoms * per_row : 0;
+      int64_t upto = n;
+#pragma unroll
+      for (int w = 1; w < 64; w <<= 1) {
+        const int64_t x = __shfl_up(upto, w);
+        if (lane >= w) upto += x;
+      }
+      upto += before;
+      const uint64_t past = __ballot(upto > from);
+      if (past || b0 + 64 >= a.rows) {
+        const int hit = past ? __ffsll((long long)past) - 1 : 63;
+        if (lane == hit) s_row = b, s_before = upto - n;
+        break;
+      }
+      before = __shfl(upto, 63);
+    }
   }
-  const float y = sum > 0.f ? acc / sum * (CT == PL_F8E4M3 ? a.v_scale[hk] : 1.f) : sum;
-  ((T*)a.out)[((int64_t)b * a.heads + h) * a.dim + d] = (T)y;
+  __syncthreads();
+  int row = s_row;
+  int64_t row_start = s_before;  // atom index of the row's first
+  int64_t at = from;
+  while (at < to) {
+    const row_span r = span_of<S::kAtom>(a, a.lens[row]);
+    const int64_t in_row = at - row_start;
+    if (in_row >= (int64_t)r.atoms * per_row) {
+      row_start += (int64_t)r.atoms * per_row;
+      ++row;
+      continue;
+    }
+    const int combo = (int)(in_row / r.atoms);
+    const int64_t pair_start = row_start + (int64_t)combo * r.atoms;
+    const int first_atom = (int)(at - pair_start);
+    const int last_atom = (int)min((int64_t)r.atoms, to - pair_start);
+    const int hk = combo / a.col_tiles, ct = combo % a.col_tiles;
+    const int cols = min(kCols, a.group - ct * kCols);
+
+    wave_state<DT, CT, DP> st;
+    st.m = -INFINITY, st.l = 0.f;
+#pragma unroll
+    for (int i = 0; i < S::V; ++i) st.o[i] = pl_f32x4{0.f, 0.f, 0.f, 0.f};
+    const int head0 = hk * a.group + ct * kCols;
+    {
+      const T* q = (const T*)a.q + row * a.q_row + (head0 + (li < cols ? li : 0)) * a.q_head;
+#pragma unroll
+      for (int n = 0; n < S::kSteps; ++n) {
+        const int d = CT == PL_F8E4M3 ? key_piece<CT>(n / 2, lg, S::E) + (n % 2) * 8
+                                      : key_piece<CT>(n, lg, S::E);
+        const bool ok = li < cols && d < a.dim;
+#pragma unroll
+        for (int e = 0; e < S::E; ++e) {
+          // rows of q have the alignment of their elements alone
+          const T x = ok ? q[d + e] : (T)0.f;
+          if constexpr (DT == PL_F32)
+            st.q[n][e] = __float_as_uint(x);
+          else if (e % 2 == 0)
+            st.q[n][e / 2] = __builtin_bit_cast(uint16_t, x);
+          else
+            st.q[n][e / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, x) << 16;
+        }
+      }
+    }
+    const float scale2 =
+        a.scale * 1.44269504088896f * (CT == PL_F8E4M3 ? a.k_scale[hk] : 1.f);
+
+    // this wave's tiles: every kWaves-th of the run's
+    const int end = min(r.len, r.base + last_atom * S::kAtom);
+    const char* key0 = (const char*)a.key.p + (int64_t)hk * a.key.s_head * S::kCsize;
+    const char* value0 = (const char*)a.value.p + (int64_t)hk * a.value.s_head * S::kCsize;
+    const int32_t* pages = a.table.p + row * a.table.ld;
+    const int mask = (1 << a.table.page_shift) - 1;
+    const int64_t key_slot = a.key.s_slot * S::kCsize, value_slot = a.value.s_slot * S::kCsize;
+    const int64_t key_page = a.key.s_page * S::kCsize, value_page = a.value.s_page * S::kCsize;
+    for (int t = r.base + first_atom * S::kAtom + wave * S::kTile; t < end; t += kWaves * S::kTile) {
+      key_tile<DT, CT, DP> keys;
+      uint32_t v[S::kTokens][S::kVWords];
+      bool whole = t >= r.first && t + S::kTile <= r.len;
+      uint32_t alive = 0;
+      const char *kp[S::kSubs], *vp[S::kSubs];
+#pragma unroll
+      for (int u = 0; u < S::kSubs; ++u) {
+        const int tu = t + 16 * u;
+        // 16 tokens from a multiple of 16 share a page; one without tokens here is not looked up
+        int page = tu < r.len ? pages[tu >> a.table.page_shift] : -1;
+        const bool held = page >= 0 && page < a.table.num_pages;
+        whole = whole && held;
+        page = held ? page : 0;
+        if (held) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int token = tu + 4 * lg + j;
+            alive |= (uint32_t)(token >= r.first && token < r.len) << (4 * u + j);
+          }
+        }
+        kp[u] = key0 + page * key_page + (tu & mask) * key_slot + li * key_slot;
+        vp[u] = value0 + page * value_page + (tu & mask) * value_slot + 4 * lg * value_slot +
+                li * S::V * S::kCsize;
+      }
+#pragma unroll
+      for (int u = 0; u < S::kSubs; ++u)
+#pragma unroll
+        for (int n = 0; n < S::kKeyLoads; ++n) {
+          const int d = key_piece<CT>(n, lg, S::E);
+          keys.w[u][n] = pl_ld16_or0(kp[u] + d * S::kCsize, d < a.dim);
+        }
+#pragma unroll
+      for (int j = 0; j < S::kTokens; ++j)
+        load_words(vp[j / 4] + (j % 4) * value_slot, li * S::V < a.dim, v[j]);
+      if (!whole) {
+        // slots without a token may hold anything, NaN too: no weight of 0 takes that out
+#pragma unroll
+        for (int j = 0; j < S::kTokens; ++j)
+#pragma unroll
+          for (int i = 0; i < S::kVWords; ++i) v[j][i] = (alive >> j & 1) ? v[j][i] : 0u;
+      }
+      attend_tile<DT, CT, DP>(st, keys, v, scale2, whole, alive);
+    }
+
+    // join the waves
+    st.l = column_sum(st.l);
+    if (lg == 0) s_m[wave][li] = st.m, s_l[wave][li] = st.l;
+    if (li < cols) {
+#pragma unroll
+      for (int i = 0; i < S::V; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s_o[wave][li][(4 * lg + e) * S::V + i] = st.o[i][e];
+    }
+    __syncthreads();
+    const bool complete = first_atom == 0 && last_atom == r.atoms;
+    const float v_scale = CT == PL_F8E4M3 ? a.v_scale[hk] : 1.f;
+    T* out = (T*)a.out + ((int64_t)row * a.heads + head0) * a.dim;
+    float* part = a.parts + (2 * (int64_t)blockIdx.x + (at == from ? 0 : 1)) * part_floats(DP);
+    for (int i = tid; i < cols * DP; i += kThreads) {
+      const int c = i / DP, d = i % DP;
+      float m = -INFINITY, l = 0.f, o = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) m = fmaxf(m, s_m[w][c]);
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const float f = m == -INFINITY ? 0.f : exp2_fast(s_m[w][c] - m);
+        l += f * s_l[w][c], o += f * s_o[w][c][d];
+      }
+      if (complete) {
+        if (d < a.dim) out[c * a.dim + d] = (T)(m == -INFINITY ? 0.f : o / l * v_scale);
+      } else {
+        __hip_atomic_store(part + i, o, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (d == 0) {
+          __hip_atomic_store(part + kCols * DP + 2 * c, m, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          __hip_atomic_store(part + kCols * DP + 2 * c + 1, l, __ATOMIC_RELAXED,
+                             __HIP_MEMORY_SCOPE_AGENT);
+        }
+      }
+    }
+    if (!complete) {
+      // Parts are stored through to where every XCD sees them and acknowledged
+      // before the arrival is counted; the last to arrive reads them after an
+      // acquire, so no line it reads is older than its stores.
+      const int64_t w0 = pair_start / per, w1 = (pair_start + r.atoms - 1) / per;
+      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+      __syncthreads();
+      if (tid == 0) {
+        int32_t* counter = a.counters + w0 * kCounterStride;
+        const int old = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        s_last = old == (int)(w1 - w0);
+        if (s_last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+      __syncthreads();
+      if (s_last) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+        const int n = (int)(w1 - w0) + 1;
+        // the first part is its workgroup's second when that workgroup began earlier
+        const int64_t slot0 = 2 * w0 + (w0 * per == pair_start ? 0 : 1);
+        for (int i = tid; i < cols * DP; i += kThreads) {
+          const int c = i / DP, d = i % DP;
+          float m = -INFINITY, l = 0.f, o = 0.f;
+          for (int w = 0; w < n; ++w) {
+            const float* p = a.parts + (w ? 2 * (w0 + w) : slot0) * part_floats(DP);
+            m = fmaxf(m, p[kCols * DP + 2 * c]);
+          }
+          for (int w = 0; w < n; ++w) {
+            const float* p = a.parts + (w ? 2 * (w0 + w) : slot0) * part_floats(DP);
+            const float f = m == -INFINITY ? 0.f : exp2_fast(p[kCols * DP + 2 * c] - m);
+            l += f * p[kCols * DP + 2 * c + 1], o += f * p[i];
+          }
+          if (d < a.dim) out[c * a.dim + d] = (T)(m == -INFINITY ? 0.f : o / l * v_scale);
+        }
+      }
+    }
+    __syncthreads();  // the shared arrays are free again
+    at = pair_start + last_atom;
+  }
+}
+
+template <int DT, int CT>
+int launch(const attend_args& a, int64_t atoms_most, hipStream_t s) {
+  const int per_cu = a.dim <= 128 ? 3 : DT == PL_F32 ? 1 : 2;
+  const int64_t blocks = atoms_most < 256 * per_cu ? atoms_most : 256 * per_cu;
+  const dim3 grid((unsigned)blocks);
+  if (a.dim <= 64)
+    pl_paged_attention_kernel<DT, CT, 64><<<grid, kThreads, 0, s>>>(a);
+  else if (a.dim <= 128)
+    pl_paged_attention_kernel<DT, CT, 128><<<grid, kThreads, 0, s>>>(a);
+  else
+    pl_paged_attention_kernel<DT, CT, 256><<<grid, kThreads, 0, s>>>(a);
+  return pl_launch_status("pl_paged_attention");
 }
 
 }  // namespace
+
+static_assert(PL_ATTENTION_COUNTER_INTS == kWorkersMax * kCounterStride, "one counter per workgroup");
+
+extern "C" int64_t pl_paged_attention_workspace_bytes(int32_t dim) {
+  const int dp = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
+  return dim < 1 || dim > kHeadDimMax ? 0 : 2ll * kWorkersMax * part_floats(dp) * (int64_t)sizeof(float);
+}
 
 extern "C" int pl_paged_attention(int32_t dtype, int32_t cache_dtype, const void* q,
                                   const int64_t* q_strides, const void* key_cache,
@@ -97,7 +520,8 @@ extern "C" int pl_paged_attention(int32_t dtype, int32_t cache_dtype, const void
                                   int32_t max_pages, const int32_t* lens, int32_t rows,
                                   int32_t heads, int32_t kv_heads, int32_t dim, float scale,
                                   int32_t window, const float* k_scale, const float* v_scale,
-                                  void* out, void* stream) {
+                                  void* out, void* workspace, int64_t workspace_bytes,
+                                  int32_t* counters, int64_t counter_ints, void* stream) {
   const int rc = pl_check_paged("pl_paged_attention", dtype, cache_dtype, key_cache, key_strides,
                                 value_cache, value_strides, num_pages, page_size, page_table,
                                 table_ld, max_pages, rows, heads, kv_heads, dim, k_scale, v_scale);
@@ -118,9 +542,12 @@ extern "C" int pl_paged_attention(int32_t dtype, int32_t cache_dtype, const void
     pl_set_error("pl_paged_attention: out overlaps q");
     return PL_ERR_ARG;
   }
-  if (!pl_grid_fits((int64_t)rows * heads, kWaves * 64)) {
-    pl_set_error("pl_paged_attention: too many rows (%d)", rows);
-    return PL_ERR_LIMIT;
+  if (!workspace || workspace_bytes < pl_paged_attention_workspace_bytes(dim) || !counters ||
+      counter_ints < PL_ATTENTION_COUNTER_INTS) {
+    pl_set_error("pl_paged_attention: workspace of %lld bytes and %lld counters, %lld and %d needed",
+                 (long long)workspace_bytes, (long long)counter_ints,
+                 (long long)pl_paged_attention_workspace_bytes(dim), PL_ATTENTION_COUNTER_INTS);
+    return PL_ERR_ARG;
   }
   attend_args a;
   a.q = q, a.q_row = q_strides[0], a.q_head = q_strides[1];
@@ -129,19 +556,19 @@ extern "C" int pl_paged_attention(int32_t dtype, int32_t cache_dtype, const void
   a.table = {page_table, table_ld, max_pages, num_pages, pl_log2_exact(page_size)};
   a.lens = lens, a.k_scale = k_scale, a.v_scale = v_scale, a.out = out, a.scale = scale;
   a.rows = rows, a.heads = heads, a.kv_heads = kv_heads, a.dim = dim, a.window = window;
+  a.group = heads / kv_heads, a.col_tiles = (a.group + kCols - 1) / kCols;
+  a.parts = static_cast<float*>(workspace), a.counters = counters;
+  // atoms at most: every row as long as its pages or its window allow
+  int64_t longest = (int64_t)max_pages * page_size;
+  if (window > 0 && longest > (int64_t)window + 31) longest = (int64_t)window + 31;
+  const int64_t atom = 32 * kWaves, per_pair = longest > atom ? (longest + atom - 1) / atom : 1;
+  const int64_t pairs = (int64_t)rows * kv_heads * a.col_tiles;
+  const int64_t atoms_most = pairs >= kWorkersMax ? pairs : pairs * per_pair;
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)(rows * heads));
-  if (cache_dtype == PL_F8E4M3) {
-    if (dtype == PL_BF16)
-      pl_paged_attention_kernel<PL_BF16, PL_F8E4M3><<<grid, kWaves * 64, 0, s>>>(a);
-    else
-      pl_paged_attention_kernel<PL_F16, PL_F8E4M3><<<grid, kWaves * 64, 0, s>>>(a);
-  } else if (dtype == PL_F32) {
-    pl_paged_attention_kernel<PL_F32, PL_F32><<<grid, kWaves * 64, 0, s>>>(a);
-  } else if (dtype == PL_BF16) {
-    pl_paged_attention_kernel<PL_BF16, PL_BF16><<<grid, kWaves * 64, 0, s>>>(a);
-  } else {
-    pl_paged_attention_kernel<PL_F16, PL_F16><<<grid, kWaves * 64, 0, s>>>(a);
-  }
-  return pl_launch_status("pl_paged_attention");
+  if (cache_dtype == PL_F8E4M3)
+    return dtype == PL_BF16 ? launch<PL_BF16, PL_F8E4M3>(a, atoms_most, s)
+                            : launch<PL_F16, PL_F8E4M3>(a, atoms_most, s);
+  if (dtype == PL_F32) return launch<PL_F32, PL_F32>(a, atoms_most, s);
+  return dtype == PL_BF16 ? launch<PL_BF16, PL_BF16>(a, atoms_most, s)
+                          : launch<PL_F16, PL_F16>(a, atoms_most, s);
 }

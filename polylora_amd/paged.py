@@ -16,7 +16,7 @@ from __future__ import annotations
 
 import torch
 
-from . import _native
+from . import _native, sgmv
 
 __all__ = ["paged_attention", "rope_append", "rope_table"]
 
@@ -142,6 +142,20 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_cache: to
     return q_out
 
 
+# One set of counters for each (device, stream), kept as the decode launch's are.
+_COUNTERS: dict[tuple[int, int], sgmv._HandoffCounters] = {}
+
+
+def _scratch(device: int, stream: int, dim: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """The stream's workspace for parts of rows and its zeroed arrival counters."""
+    held = _COUNTERS.get((device, stream))
+    if held is None:
+        held = _COUNTERS[device, stream] = sgmv._HandoffCounters(torch.device("cuda", device))
+    nbytes = _native.load().pl_paged_attention_workspace_bytes(dim)
+    return (sgmv._workspace(held.device, stream, "attention").get(nbytes),
+            held.get(_native.PL_ATTENTION_COUNTER_INTS))
+
+
 def paged_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, page_table: torch.Tensor,
                     lens: torch.Tensor, *, scale: float | None = None, window: int | None = None,
                     k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
@@ -173,12 +187,15 @@ def paged_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch
         out = torch.empty((rows, heads, dim), dtype=dtype, device=q.device)
     else:
         _check_tensor("out", out, dtype, device, (rows, heads, dim))
+    stream = torch._C._cuda_getCurrentRawStream(device)
+    ws, counters = _scratch(device, stream, dim)
     rc = _native.calls().pl_paged_attention(
         code, cache_code, q.data_ptr(), q.stride()[:2], key_cache.data_ptr(), key_cache.stride()[:3],
         value_cache.data_ptr(), value_cache.stride()[:3], key_cache.shape[0], key_cache.shape[2],
         page_table.data_ptr(), page_table.stride(0), page_table.shape[1], lens.data_ptr(), rows, heads, kv_heads, dim,
         dim ** -0.5 if scale is None else scale, window or 0, None if k_scale is None else k_scale.data_ptr(),
-        None if v_scale is None else v_scale.data_ptr(), out.data_ptr(), torch._C._cuda_getCurrentRawStream(device))
+        None if v_scale is None else v_scale.data_ptr(), out.data_ptr(), ws.data_ptr(), ws.numel(),
+        counters.data_ptr(), counters.numel(), stream)
     if rc:
         _native.check(rc, "pl_paged_attention")
     return out
