@@ -77,6 +77,7 @@ struct attend_args {
   int32_t rows, heads, kv_heads, dim, window, group, col_tiles;
 };
 
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // The largest of the four lanes of a column, and their sum.
@@ -93,9 +94,10 @@ __device__ __forceinline__ float column_sum(float x) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// 4 * N bytes at `off` from a base that the wave shares.
 template <int N>
-__device__ __forceinline__ void load_words(const char* p, bool ok, uint32_t (&w)[N]) {
-  p = ok ? p : reinterpret_cast<const char*>(pl_zero64);
+__device__ __forceinline__ void load_words(const char* base, uint32_t off, uint32_t (&w)[N]) {
+  const char* p = base + off;
   if constexpr (N % 4 == 0) {
 #pragma unroll
     for (int i = 0; i < N / 4; ++i) {
@@ -133,6 +135,12 @@ __device__ __forceinline__ float unpack(uint32_t w, int half) {
   return (float)__builtin_bit_cast(T2, w)[half];
 }
 
+// First element of the 16-byte key piece that lane group g loads n-th.
+template <int CT>
+__device__ __forceinline__ int key_piece(int n, int g, int e) {
+  return (n * 4 + g) * (CT == PL_F8E4M3 ? 16 : e);
+}
+
 // What a wave holds of one (row, key head): its queries, and m (in units of
 // log2 e), l (this lane's tokens alone) and o of its tiles so far.
 template <int DT, int CT, int DP>
@@ -143,25 +151,52 @@ struct wave_state {
   float m, l;
 };
 
-// The keys of one tile, as loaded.
-template <int DT, int CT, int DP>
-struct key_tile {
-  typedef shape<DT, CT, DP> S;
-  pl_u32x4 w[S::kSubs][S::kKeyLoads];
-};
-
-// First element of the 16-byte key piece that lane group g loads n-th.
-template <int CT>
-__device__ __forceinline__ int key_piece(int n, int g, int e) {
-  return (n * 4 + g) * (CT == PL_F8E4M3 ? 16 : e);
+// A row's page ids, read through the scalar cache: every lane wants the same.
+typedef const __attribute__((address_space(4))) int32_t* scalar_i32;
+__device__ __forceinline__ scalar_i32 as_scalar(const int32_t* p) {
+  return (scalar_i32)(reinterpret_cast<uintptr_t>(p));
 }
 
-template <int DT, int CT, int DP>
-__device__ __forceinline__ void attend_tile(wave_state<DT, CT, DP>& st,
-                                            const key_tile<DT, CT, DP>& keys,
-                                            const uint32_t (&v)[shape<DT, CT, DP>::kTokens]
-                                                               [shape<DT, CT, DP>::kVWords],
-                                            float scale2, bool whole, uint32_t alive) {
+// Where a tile's keys and values lie, for each 16 tokens of it (16 tokens from
+// a multiple of 16 share a page), and what of it counts.
+template <int SUBS>
+struct tile_place {
+  const char *key[SUBS], *value[SUBS];
+  bool held[SUBS];
+};
+
+// What the walk over one (row, key head) needs; all of it is the wave's.
+struct walk {
+  const char *key, *value;  // the key head's
+  scalar_i32 pages;
+  int64_t key_page, value_page;  // bytes
+  uint32_t key_slot, value_slot;
+  int first, len, shift, num_pages;
+};
+
+template <int SUBS>
+__device__ __forceinline__ tile_place<SUBS> place_tile(const walk& w, int t) {
+  tile_place<SUBS> r;
+#pragma unroll
+  for (int u = 0; u < SUBS; ++u) {
+    const int tu = t + 16 * u;
+    // no look-up for 16 tokens past the row's end: its table row may end there
+    const int id = tu < w.len ? w.pages[tu >> w.shift] : -1;
+    r.held[u] = id >= 0 && id < w.num_pages;
+    const int64_t page = r.held[u] ? id : 0;  // page 0 is there, and none of it counts
+    const uint32_t slot = (uint32_t)tu & ((1u << w.shift) - 1);
+    r.key[u] = w.key + page * w.key_page + (uint64_t)slot * w.key_slot;
+    r.value[u] = w.value + page * w.value_page + (uint64_t)slot * w.value_slot;
+  }
+  return r;
+}
+
+// Scores of a tile's tokens with the wave's queries, in units of log2 e.
+template <int DT, int CT, int DP, bool FULL>
+__device__ __forceinline__ void score_tile(
+    const wave_state<DT, CT, DP>& st,
+    const pl_u32x4 (&keys)[shape<DT, CT, DP>::kSubs][shape<DT, CT, DP>::kKeyLoads], int lg,
+    int dim, float scale2, float (&p)[shape<DT, CT, DP>::kTokens]) {
   typedef shape<DT, CT, DP> S;
   pl_f32x4 s[S::kSubs];
 #pragma unroll
@@ -169,7 +204,9 @@ __device__ __forceinline__ void attend_tile(wave_state<DT, CT, DP>& st,
     s[u] = pl_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int n = 0; n < S::kKeyLoads; ++n) {
-      const pl_u32x4 w = keys.w[u][n];
+      pl_u32x4 w = keys[u][n];
+      // pieces past the head's end were loaded from its start: they count as 0
+      if (!FULL && key_piece<CT>(n, lg, S::E) >= dim) w = pl_u32x4{0, 0, 0, 0};
       if constexpr (CT == PL_F8E4M3) {
         const pl_u32x4 a = {widen<DT, false>(w.x), widen<DT, true>(w.x), widen<DT, false>(w.y),
                             widen<DT, true>(w.y)};
@@ -178,17 +215,24 @@ __device__ __forceinline__ void attend_tile(wave_state<DT, CT, DP>& st,
         s[u] = pl_mfma_chunk<DT>(a, st.q[2 * n], s[u]);
         s[u] = pl_mfma_chunk<DT>(b, st.q[2 * n + 1], s[u]);
       } else {
-        s[u] = pl_mfma_chunk_short<DT>(w, st.q[n], s[u]);
+        s[u] = pl_mfma_chunk<DT>(w, st.q[n], s[u]);
       }
     }
   }
-  float p[S::kTokens], top = -INFINITY;
 #pragma unroll
-  for (int j = 0; j < S::kTokens; ++j) {
-    p[j] = s[j / 4][j % 4] * scale2;
-    if (!whole) p[j] = (alive >> j & 1) ? p[j] : -INFINITY;
-    top = fmaxf(top, p[j]);
-  }
+  for (int j = 0; j < S::kTokens; ++j) p[j] = s[j / 4][j % 4] * scale2;
+}
+
+// Takes scores p and values v of a tile into the running maximum, sum and output.
+template <int DT, int CT, int DP>
+__device__ __forceinline__ void weigh_tile(wave_state<DT, CT, DP>& st,
+                                           float (&p)[shape<DT, CT, DP>::kTokens],
+                                           const uint32_t (&v)[shape<DT, CT, DP>::kTokens]
+                                                              [shape<DT, CT, DP>::kVWords]) {
+  typedef shape<DT, CT, DP> S;
+  float top = p[0];
+#pragma unroll
+  for (int j = 1; j < S::kTokens; ++j) top = fmaxf(top, p[j]);
   top = fmaxf(st.m, column_max(top));
   // nothing alive yet: any finite reference gives weights of 0
   const float ref = top == -INFINITY ? 0.f : top;
@@ -212,6 +256,7 @@ __device__ __forceinline__ void attend_tile(wave_state<DT, CT, DP>& st,
       for (int j = 0; j < S::kTokens; ++j)
         part = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[j][i]), p[j], part, 0, 0, 0);
       st.o[i] += part;
+      if (i % 2) __builtin_amdgcn_sched_barrier(0);
     }
   } else {
     pl_u32x4 hi, lo;
@@ -240,6 +285,8 @@ __device__ __forceinline__ void attend_tile(wave_state<DT, CT, DP>& st,
       st.o[2 * i + 1] = pl_mfma_chunk<DT>(b, hi, st.o[2 * i + 1]);
       st.o[2 * i] = pl_mfma_chunk<DT>(a, lo, st.o[2 * i]);
       st.o[2 * i + 1] = pl_mfma_chunk<DT>(b, lo, st.o[2 * i + 1]);
+      // in this order: pairing up all values first would take as many registers again
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 }
@@ -262,7 +309,67 @@ __device__ __forceinline__ row_span span_of(const attend_args& a, int len) {
 // Floats of one part: o [kCols][DP], then m and l of each column.
 constexpr int part_floats(int dp) { return kCols * dp + 2 * kCols; }
 
-template <int DT, int CT, int DP>
+// Joins n parts (the first in slot `slot0`, part w in slot `slot` + 2 w) and
+// hands each 4 finished elements of a column to `store`.  A thread takes 4
+// elements over every lanes-th part, kBatch parts' loads at a time; the lanes
+// join through `scratch` (6 floats a thread).
+template <int DP, typename Store>
+__device__ __forceinline__ void join_parts(const float* parts, int slot0, int slot, int n, int cols,
+                                           float* scratch, Store store) {
+  constexpr int kBatch = 8;
+  const int tid = (int)threadIdx.x, items = cols * (DP / 4);
+  const int lanes = max(1, kThreads / items);
+  for (int i0 = 0; i0 < items; i0 += kThreads) {
+    const int item = i0 + (items <= kThreads ? tid % items : tid), first = items <= kThreads ? tid / items : 0;
+    const bool busy = item < items && first < lanes;
+    const int c = item / (DP / 4), d = item % (DP / 4) * 4;
+    float m = -INFINITY, l = 0.f;
+    pl_f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int w0 = first; busy && w0 < n; w0 += kBatch * lanes) {
+      pl_f32x4 x[kBatch];
+      float pm[kBatch], pl[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const int w = min(w0 + j * lanes, n - 1);  // the last again, with no weight
+        const float* p = parts + (int64_t)(w ? slot + 2 * w : slot0) * part_floats(DP);
+        x[j] = *reinterpret_cast<const pl_f32x4*>(p + c * DP + d);
+        pm[j] = p[kCols * DP + 2 * c], pl[j] = p[kCols * DP + 2 * c + 1];
+      }
+      float top = m;
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        pm[j] = w0 + j * lanes < n ? pm[j] : -INFINITY;
+        top = fmaxf(top, pm[j]);
+      }
+      const float ref = top == -INFINITY ? 0.f : top, keep = exp2_fast(m - ref);
+      l *= keep, o *= keep, m = top;
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const float f = exp2_fast(pm[j] - ref);
+        l += f * pl[j], o += f * x[j];
+      }
+    }
+    if (lanes > 1) {
+      __syncthreads();
+      if (busy) {
+        float* s = scratch + 6 * tid;
+        s[0] = m, s[1] = l, s[2] = o.x, s[3] = o.y, s[4] = o.z, s[5] = o.w;
+      }
+      __syncthreads();
+      if (busy && first == 0)
+        for (int k = 1; k < lanes; ++k) {
+          const float* s = scratch + 6 * (k * items + item);
+          const float top = fmaxf(m, s[0]), ref = top == -INFINITY ? 0.f : top;
+          const float keep = exp2_fast(m - ref), f = exp2_fast(s[0] - ref);
+          l = l * keep + f * s[1], m = top;
+          o = o * keep + pl_f32x4{s[2], s[3], s[4], s[5]} * f;
+        }
+    }
+    if (busy && first == 0) store(c, d, m == -INFINITY ? pl_f32x4{0.f, 0.f, 0.f, 0.f} : o / l);
+  }
+}
+
+template <int DT, int CT, int DP, bool FULL>
 __global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kPerCu)) void pl_paged_attention_kernel(
     attend_args a) {
   typedef shape<DT, CT, DP> S;
@@ -270,38 +377,37 @@ __global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kPerCu)) void pl_page
   constexpr int kPad = 4;
   __shared__ float s_o[kWaves][kCols][DP + kPad];
   __shared__ float s_m[kWaves][kCols], s_l[kWaves][kCols];
-  __shared__ int64_t s_scan[kWaves];
-  __shared__ int s_row, s_last;
-  __shared__ int64_t s_before;
+  __shared__ int s_scan[kWaves];
+  __shared__ int s_row, s_before, s_last;
   const int tid = (int)threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int li = lane & 15, lg = lane >> 4;
   const int per_row = a.kv_heads * a.col_tiles;
 
   // atoms of the batch, then this workgroup's run of them
-  int64_t mine = 0;
+  int mine = 0;
   for (int b = tid; b < a.rows; b += kThreads) mine += span_of<S::kAtom>(a, a.lens[b]).atoms;
 #pragma unroll
   for (int w = 32; w > 0; w >>= 1) mine += __shfl_xor(mine, w);
   if (lane == 0) s_scan[wave] = mine;
   __syncthreads();
-  int64_t total = 0;
+  int total = 0;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) total += s_scan[w];
-  total *= per_row;
-  const int64_t per = (total + gridDim.x - 1) / gridDim.x;
-  const int64_t from = blockIdx.x * per, to = min(total, from + per);
-  if (from >= to) return;
+  total = uniform(total) * per_row;
+  const int per = (int)((total + gridDim.x - 1) / gridDim.x);
+  const int from = (int)min((int64_t)blockIdx.x * per, (int64_t)total), to = min(total - per, from) + per;
+  if (from >= total) return;
   // the row of its first atom: the first whose atoms up to and with it pass `from`
   if (tid < 64) {
-    int64_t before = 0;
+    int before = 0;
     for (int b0 = 0;; b0 += 64) {
       const int b = b0 + lane;
-      int64_t n = b < a.rows ? (int64_t)span_of<S::kAtom>(a, a.lens[b]).atoms * per_row : 0;
-      int64_t upto = n;
+      const int n = b < a.rows ? span_of<S::kAtom>(a, a.lens[b]).atoms * per_row : 0;
+      int upto = n;
 #pragma unroll
       for (int w = 1; w < 64; w <<= 1) {
-        const int64_t x = __shfl_up(upto, w);
+        const int x = __shfl_up(upto, w);
         if (lane >= w) upto += x;
       }
       upto += before;
@@ -315,21 +421,21 @@ __global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kPerCu)) void pl_page
     }
   }
   __syncthreads();
-  int row = s_row;
-  int64_t row_start = s_before;  // atom index of the row's first
-  int64_t at = from;
+  int row = uniform(s_row);
+  int row_start = uniform(s_before);  // atom index of the row's first
+  int at = from;
   while (at < to) {
-    const row_span r = span_of<S::kAtom>(a, a.lens[row]);
-    const int64_t in_row = at - row_start;
-    if (in_row >= (int64_t)r.atoms * per_row) {
-      row_start += (int64_t)r.atoms * per_row;
+    const row_span r = span_of<S::kAtom>(a, as_scalar(a.lens)[row]);
+    const int in_row = at - row_start;
+    if (in_row >= r.atoms * per_row) {
+      row_start += r.atoms * per_row;
       ++row;
       continue;
     }
-    const int combo = (int)(in_row / r.atoms);
-    const int64_t pair_start = row_start + (int64_t)combo * r.atoms;
-    const int first_atom = (int)(at - pair_start);
-    const int last_atom = (int)min((int64_t)r.atoms, to - pair_start);
+    const int combo = in_row / r.atoms;
+    const int pair_start = row_start + combo * r.atoms;
+    const int first_atom = at - pair_start;
+    const int last_atom = min(r.atoms, to - pair_start);
     const int hk = combo / a.col_tiles, ct = combo % a.col_tiles;
     const int cols = min(kCols, a.group - ct * kCols);
 
@@ -344,18 +450,11 @@ __global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kPerCu)) void pl_page
       for (int n = 0; n < S::kSteps; ++n) {
         const int d = CT == PL_F8E4M3 ? key_piece<CT>(n / 2, lg, S::E) + (n % 2) * 8
                                       : key_piece<CT>(n, lg, S::E);
-        const bool ok = li < cols && d < a.dim;
-#pragma unroll
-        for (int e = 0; e < S::E; ++e) {
-          // rows of q have the alignment of their elements alone
-          const T x = ok ? q[d + e] : (T)0.f;
-          if constexpr (DT == PL_F32)
-            st.q[n][e] = __float_as_uint(x);
-          else if (e % 2 == 0)
-            st.q[n][e / 2] = __builtin_bit_cast(uint16_t, x);
-          else
-            st.q[n][e / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, x) << 16;
-        }
+        const bool ok = li < cols && (FULL || d < a.dim);
+        // rows of q have the alignment of their elements alone
+        pl_u32x4 x;
+        __builtin_memcpy(&x, q + (FULL || d < a.dim ? d : 0), 16);
+        st.q[n] = ok ? x : pl_u32x4{0, 0, 0, 0};
       }
     }
     const float scale2 =
@@ -363,55 +462,67 @@ __global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kPerCu)) void pl_page
 
     // this wave's tiles: every kWaves-th of the run's
     const int end = min(r.len, r.base + last_atom * S::kAtom);
-    const char* key0 = (const char*)a.key.p + (int64_t)hk * a.key.s_head * S::kCsize;
-    const char* value0 = (const char*)a.value.p + (int64_t)hk * a.value.s_head * S::kCsize;
-    const int32_t* pages = a.table.p + row * a.table.ld;
-    const int mask = (1 << a.table.page_shift) - 1;
-    const int64_t key_slot = a.key.s_slot * S::kCsize, value_slot = a.value.s_slot * S::kCsize;
-    const int64_t key_page = a.key.s_page * S::kCsize, value_page = a.value.s_page * S::kCsize;
-    for (int t = r.base + first_atom * S::kAtom + wave * S::kTile; t < end; t += kWaves * S::kTile) {
-      key_tile<DT, CT, DP> keys;
-      uint32_t v[S::kTokens][S::kVWords];
-      bool whole = t >= r.first && t + S::kTile <= r.len;
-      uint32_t alive = 0;
-      const char *kp[S::kSubs], *vp[S::kSubs];
+    walk w;
+    w.key = (const char*)a.key.p + (int64_t)hk * a.key.s_head * S::kCsize;
+    w.value = (const char*)a.value.p + (int64_t)hk * a.value.s_head * S::kCsize;
+    w.pages = as_scalar(a.table.p + row * a.table.ld);
+    w.key_page = a.key.s_page * S::kCsize, w.value_page = a.value.s_page * S::kCsize;
+    w.key_slot = (uint32_t)a.key.s_slot * S::kCsize;
+    w.value_slot = (uint32_t)a.value.s_slot * S::kCsize;
+    w.first = r.first, w.len = r.len, w.shift = a.table.page_shift;
+    w.num_pages = a.table.num_pages;
+    uint32_t key_off[S::kKeyLoads];
 #pragma unroll
-      for (int u = 0; u < S::kSubs; ++u) {
-        const int tu = t + 16 * u;
-        // 16 tokens from a multiple of 16 share a page; one without tokens here is not looked up
-        int page = tu < r.len ? pages[tu >> a.table.page_shift] : -1;
-        const bool held = page >= 0 && page < a.table.num_pages;
-        whole = whole && held;
-        page = held ? page : 0;
-        if (held) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int token = tu + 4 * lg + j;
-            alive |= (uint32_t)(token >= r.first && token < r.len) << (4 * u + j);
-          }
-        }
-        kp[u] = key0 + page * key_page + (tu & mask) * key_slot + li * key_slot;
-        vp[u] = value0 + page * value_page + (tu & mask) * value_slot + 4 * lg * value_slot +
-                li * S::V * S::kCsize;
-      }
+    for (int n = 0; n < S::kKeyLoads; ++n) {
+      const int d = key_piece<CT>(n, lg, S::E);
+      key_off[n] = li * w.key_slot + (FULL || d < a.dim ? d : 0) * S::kCsize;
+    }
+    // lanes past the head's end read its start: what they make is not stored
+    const uint32_t value_off =
+        4 * lg * w.value_slot + (FULL || li * S::V < a.dim ? li * S::V : 0) * S::kCsize;
+
+    // Keys of the next tile are asked for as soon as this tile's have gone into
+    // the scores, values as soon as the wave is at the tile: one or the other
+    // is in flight all the time, in no more registers than one tile takes.
+    pl_u32x4 keys[S::kSubs][S::kKeyLoads];
+    auto load_keys = [&](const tile_place<S::kSubs>& at) {
 #pragma unroll
       for (int u = 0; u < S::kSubs; ++u)
 #pragma unroll
-        for (int n = 0; n < S::kKeyLoads; ++n) {
-          const int d = key_piece<CT>(n, lg, S::E);
-          keys.w[u][n] = pl_ld16_or0(kp[u] + d * S::kCsize, d < a.dim);
-        }
+        for (int n = 0; n < S::kKeyLoads; ++n) keys[u][n] = pl_ld16(at.key[u] + key_off[n]);
+    };
+    int tile = r.base + first_atom * S::kAtom + wave * S::kTile;
+    tile_place<S::kSubs> place;
+    if (tile < end) {
+      place = place_tile<S::kSubs>(w, tile);
+      load_keys(place);
+    }
+    for (; tile < end; tile += kWaves * S::kTile) {
+      uint32_t v[S::kTokens][S::kVWords];
 #pragma unroll
       for (int j = 0; j < S::kTokens; ++j)
-        load_words(vp[j / 4] + (j % 4) * value_slot, li * S::V < a.dim, v[j]);
+        load_words(place.value[j / 4], value_off + (j % 4) * w.value_slot, v[j]);
+      const tile_place<S::kSubs> here = place;
+      const int next = tile + kWaves * S::kTile;
+      if (next < end) place = place_tile<S::kSubs>(w, next);
+      float p[S::kTokens];
+      score_tile<DT, CT, DP, FULL>(st, keys, lg, a.dim, scale2, p);
+      if (next < end) load_keys(place);
+      bool whole = tile >= r.first && tile + S::kTile <= r.len;
+#pragma unroll
+      for (int u = 0; u < S::kSubs; ++u) whole = whole && here.held[u];
       if (!whole) {
         // slots without a token may hold anything, NaN too: no weight of 0 takes that out
 #pragma unroll
-        for (int j = 0; j < S::kTokens; ++j)
+        for (int j = 0; j < S::kTokens; ++j) {
+          const int token = tile + 16 * (j / 4) + 4 * lg + j % 4;
+          const bool alive = here.held[j / 4] && token >= r.first && token < r.len;
+          p[j] = alive ? p[j] : -INFINITY;
 #pragma unroll
-          for (int i = 0; i < S::kVWords; ++i) v[j][i] = (alive >> j & 1) ? v[j][i] : 0u;
+          for (int i = 0; i < S::kVWords; ++i) v[j][i] = alive ? v[j][i] : 0u;
+        }
       }
-      attend_tile<DT, CT, DP>(st, keys, v, scale2, whole, alive);
+      weigh_tile<DT, CT, DP>(st, p, v);
     }
 
     // join the waves
@@ -453,40 +564,39 @@ __global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kPerCu)) void pl_page
       // Parts are stored through to where every XCD sees them and acknowledged
       // before the arrival is counted; the last to arrive reads them after an
       // acquire, so no line it reads is older than its stores.
-      const int64_t w0 = pair_start / per, w1 = (pair_start + r.atoms - 1) / per;
+      const int w0 = pair_start / per, w1 = (pair_start + r.atoms - 1) / per;
       __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
       __syncthreads();
       if (tid == 0) {
         int32_t* counter = a.counters + w0 * kCounterStride;
         const int old = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        s_last = old == (int)(w1 - w0);
+        s_last = old == w1 - w0;
         if (s_last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       }
       __syncthreads();
       if (s_last) {
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-        const int n = (int)(w1 - w0) + 1;
         // the first part is its workgroup's second when that workgroup began earlier
-        const int64_t slot0 = 2 * w0 + (w0 * per == pair_start ? 0 : 1);
-        for (int i = tid; i < cols * DP; i += kThreads) {
-          const int c = i / DP, d = i % DP;
-          float m = -INFINITY, l = 0.f, o = 0.f;
-          for (int w = 0; w < n; ++w) {
-            const float* p = a.parts + (w ? 2 * (w0 + w) : slot0) * part_floats(DP);
-            m = fmaxf(m, p[kCols * DP + 2 * c]);
-          }
-          for (int w = 0; w < n; ++w) {
-            const float* p = a.parts + (w ? 2 * (w0 + w) : slot0) * part_floats(DP);
-            const float f = m == -INFINITY ? 0.f : exp2_fast(p[kCols * DP + 2 * c] - m);
-            l += f * p[kCols * DP + 2 * c + 1], o += f * p[i];
-          }
-          if (d < a.dim) out[c * a.dim + d] = (T)(m == -INFINITY ? 0.f : o / l * v_scale);
-        }
+        const int slot0 = 2 * w0 + (w0 * per == pair_start ? 0 : 1);
+        join_parts<DP>(a.parts, slot0, 2 * w0, w1 - w0 + 1, cols, &s_o[0][0][0],
+                       [&](int c, int d, pl_f32x4 o) {
+#pragma unroll
+                         for (int e = 0; e < 4; ++e)
+                           if (FULL || d + e < a.dim) out[c * a.dim + d + e] = (T)(o[e] * v_scale);
+                       });
       }
     }
     __syncthreads();  // the shared arrays are free again
     at = pair_start + last_atom;
   }
+}
+
+template <int DT, int CT, int DP>
+void launch_dim(const attend_args& a, dim3 grid, hipStream_t s) {
+  if (a.dim == DP)
+    pl_paged_attention_kernel<DT, CT, DP, true><<<grid, kThreads, 0, s>>>(a);
+  else
+    pl_paged_attention_kernel<DT, CT, DP, false><<<grid, kThreads, 0, s>>>(a);
 }
 
 template <int DT, int CT>
@@ -495,11 +605,11 @@ int launch(const attend_args& a, int64_t atoms_most, hipStream_t s) {
   const int64_t blocks = atoms_most < 256 * per_cu ? atoms_most : 256 * per_cu;
   const dim3 grid((unsigned)blocks);
   if (a.dim <= 64)
-    pl_paged_attention_kernel<DT, CT, 64><<<grid, kThreads, 0, s>>>(a);
+    launch_dim<DT, CT, 64>(a, grid, s);
   else if (a.dim <= 128)
-    pl_paged_attention_kernel<DT, CT, 128><<<grid, kThreads, 0, s>>>(a);
+    launch_dim<DT, CT, 128>(a, grid, s);
   else
-    pl_paged_attention_kernel<DT, CT, 256><<<grid, kThreads, 0, s>>>(a);
+    launch_dim<DT, CT, 256>(a, grid, s);
   return pl_launch_status("pl_paged_attention");
 }
 
@@ -532,6 +642,14 @@ extern "C" int pl_paged_attention(int32_t dtype, int32_t cache_dtype, const void
     return PL_ERR_ARG;
   }
   if (rows == 0) return PL_OK;
+  // lanes address the 16 slots of a tile with 32-bit byte offsets
+  const int64_t slot_most = INT32_MAX / 16 / pl_cache_elem_size(cache_dtype);
+  if (key_strides[2] < 0 || key_strides[2] > slot_most || value_strides[2] < 0 ||
+      value_strides[2] > slot_most) {
+    pl_set_error("pl_paged_attention: slot strides of %lld and %lld elements",
+                 (long long)key_strides[2], (long long)value_strides[2]);
+    return PL_ERR_LIMIT;
+  }
   if (!q || !q_strides || !lens || !out) {
     pl_set_error("pl_paged_attention: null pointer");
     return PL_ERR_ARG;
@@ -563,7 +681,12 @@ extern "C" int pl_paged_attention(int32_t dtype, int32_t cache_dtype, const void
   if (window > 0 && longest > (int64_t)window + 31) longest = (int64_t)window + 31;
   const int64_t atom = 32 * kWaves, per_pair = longest > atom ? (longest + atom - 1) / atom : 1;
   const int64_t pairs = (int64_t)rows * kv_heads * a.col_tiles;
-  const int64_t atoms_most = pairs >= kWorkersMax ? pairs : pairs * per_pair;
+  if (pairs > INT32_MAX / per_pair) {
+    pl_set_error("pl_paged_attention: %lld rows and key heads of up to %lld tokens are too many",
+                 (long long)pairs, (long long)longest);
+    return PL_ERR_LIMIT;
+  }
+  const int64_t atoms_most = pairs * per_pair;
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (cache_dtype == PL_F8E4M3)
     return dtype == PL_BF16 ? launch<PL_BF16, PL_F8E4M3>(a, atoms_most, s)

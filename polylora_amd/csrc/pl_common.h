@@ -111,9 +111,6 @@ __device__ __forceinline__ int64_t pl_tile_off(int i, int c, int R, int C) {
 // Sixteen zero bytes in device memory: the source of every masked-off lane.
 static __device__ __attribute__((aligned(16))) uint32_t pl_zero16[4];
 
-// Sixty-four of them, for lanes that load more at a time.
-static __device__ __attribute__((aligned(64))) uint32_t pl_zero64[16];
-
 // Branch-free guarded load: lanes with !ok read pl_zero16 instead of p.  The
 // guard only selects an address, so no exec-masked branch and no select on
 // the loaded value: the compiler can keep a wave's loads in flight together.
