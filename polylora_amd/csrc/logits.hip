@@ -1,16 +1,24 @@
 // Penalties of repeated tokens, biases and grammar masks on logits.
 #include "pl_common.h"
 
+// One pass over the logits, 8 at a time: memory bounds it (each is read once
+// and written once).  A workgroup takes a slice of one row's vocabulary.  What
+// is particular to single tokens lies in a table of one LDS word per entry of
+// the slice, which the pass reads beside the logits: the workgroup first
+// counts the row's history into it (the tokens that fall into the slice;
+// integer atomics, the same result in any order) and puts the places of
+// biases there.  The history is read again for each slice, from L2, so slices
+// grow with the batch (slice_of).
 namespace {
 
-constexpr int kThreads = 256;
-// Vocabulary entries of one workgroup: a word of LDS for each.
-constexpr int kSlice = 4096;
 // A word of the slice's table: how often the token was generated, the place
-// plus one of its first entry in the bias list, whether it was seen at all.
+// plus one of its sum among the slice's biases, whether it was seen at all.
 constexpr uint32_t kCountMask = (1u << 20) - 1, kBiasShift = 20, kBiasMask = 0x7ff;
 constexpr uint32_t kSeen = 1u << 31;
 constexpr int kHistoryMax = (int)kCountMask, kBiasMax = (int)kBiasMask;
+constexpr int kVec = 8;     // logits of a thread's load
+constexpr int kPasses = 2;  // loads of a thread: its share of the slice
+constexpr int kWide = 1 << 22;  // logits from which slices are twice as large
 
 struct logits_args {
   const void* logits;
@@ -25,57 +33,155 @@ struct logits_args {
   int32_t rows, vocab, history, n_bias, wide_tokens, slices;
 };
 
-// One workgroup per (row, slice of the vocabulary): it counts the row's
-// history and looks up its biases in LDS, then walks its logits once.
-template <int DT, int OT>
-__global__ __launch_bounds__(kThreads) void pl_adjust_logits_kernel(logits_args a) {
+struct penalties {
+  float r, f, p;
+};
+
+// One logit: its word of the table, the slice's bias sums, its mask bit.
+__device__ __forceinline__ float adjust(float x, uint32_t w, const penalties& pen,
+                                        const float* sums, bool allowed) {
+  if (w & kSeen) {
+    x = x > 0.f ? x / pen.r : x * pen.r;
+    const uint32_t c = w & kCountMask;
+    if (c) x -= pen.f * (float)c + pen.p;
+  }
+  const int j = (int)((w >> kBiasShift) & kBiasMask);
+  if (j) x += sums[j - 1];
+  return allowed ? x : -INFINITY;
+}
+
+template <int DT, int OT, int THREADS>
+__global__ __launch_bounds__(THREADS) void pl_adjust_logits_kernel(logits_args a) {
   typedef typename pl_traits<DT>::T T;
   typedef typename pl_traits<OT>::T O;
-  __shared__ uint32_t table[kSlice];
+  constexpr int kSlice = THREADS * kVec * kPasses;
+  __shared__ __attribute__((aligned(16))) uint32_t table[kSlice];
+  extern __shared__ uint32_t dynamic[];  // the slice's biases: ids, values, sums
+  __shared__ int s_biases;
   const int b = (int)(blockIdx.x / a.slices), tid = (int)threadIdx.x;
   const int lo = (int)(blockIdx.x % a.slices) * kSlice, hi = min(lo + kSlice, a.vocab);
-  for (int i = tid; i < kSlice; i += kThreads) table[i] = 0;
-  __syncthreads();
+  const T* in = (const T*)a.logits + b * a.ld;
+  O* out = (O*)a.out + b * a.ld_out;
+  // rows have the alignment of their elements alone
+  T x[kPasses][kVec];
+#pragma unroll
+  for (int k = 0; k < kPasses; ++k) {
+    const int v = lo + (k * THREADS + tid) * kVec;
+    if (v + kVec <= hi) __builtin_memcpy(x[k], in + v, sizeof(x[k]));
+  }
   const int n = a.tokens ? min(max(a.lens[b], 0), a.history) : 0;
-  const int prompt = a.prompt_lens ? a.prompt_lens[b] : 0;
-  for (int i = tid; i < n; i += kThreads) {
-    const int64_t id = a.wide_tokens ? ((const int64_t*)a.tokens)[b * a.ld_tokens + i]
-                                     : ((const int32_t*)a.tokens)[b * a.ld_tokens + i];
-    if (id < lo || id >= hi) continue;
-    atomicOr(&table[id - lo], kSeen);
-    if (i >= prompt) atomicAdd(&table[id - lo], 1u);
-  }
-  const int32_t* ids = a.bias_ids + b * a.ld_bias;
-  const float* values = a.bias_values + b * a.ld_bias;
-  for (int j = tid; j < a.n_bias; j += kThreads) {
-    const int id = ids[j];
-    if (id < lo || id >= hi) continue;
-    bool first = true;
-    for (int i = 0; i < j; ++i) first = first && ids[i] != id;
-    if (first) atomicOr(&table[id - lo], (uint32_t)(j + 1) << kBiasShift);
-  }
-  __syncthreads();
-  const float r = a.repetition ? a.repetition[b] : 1.f;
-  const float f = a.frequency ? a.frequency[b] : 0.f, p = a.presence ? a.presence[b] : 0.f;
-  for (int v = lo + tid; v < hi; v += kThreads) {
-    float x = (float)((const T*)a.logits)[b * a.ld + v];
-    const uint32_t w = table[v - lo];
-    if (w & kSeen) {
-      x = x > 0.f ? x / r : x * r;
-      const uint32_t c = w & kCountMask;
-      if (c) x -= f * (float)c + p;
+  const bool special = n > 0 || a.n_bias > 0;
+  if (special) {
+    for (int i = tid; i < kSlice / 4; i += THREADS)
+      reinterpret_cast<pl_u32x4*>(table)[i] = pl_u32x4{0, 0, 0, 0};
+    __syncthreads();
+    const int prompt = a.prompt_lens ? a.prompt_lens[b] : 0;
+    constexpr int kBatch = 4;
+    for (int i0 = tid; i0 < n; i0 += kBatch * THREADS) {
+      int64_t id[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const int i = min(i0 + j * THREADS, n - 1);
+        id[j] = a.wide_tokens ? ((const int64_t*)a.tokens)[b * a.ld_tokens + i]
+                              : ((const int32_t*)a.tokens)[b * a.ld_tokens + i];
+      }
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const int i = i0 + j * THREADS;
+        if (i >= n || id[j] < lo || id[j] >= hi) continue;
+        if (i >= prompt) atomicAdd(&table[id[j] - lo], 1u);
+        atomicOr(&table[id[j] - lo], kSeen);
+      }
     }
-    const int j = (int)((w >> kBiasShift) & kBiasMask);
-    if (j) {
-      float bias = 0.f;
-      for (int i = j - 1; i < a.n_bias; ++i)
-        if (ids[i] == v) bias += values[i];
-      x += bias;
-    }
-    if (a.allowed && !((uint32_t)a.allowed[b * a.ld_allowed + (v >> 5)] >> (v & 31) & 1))
-      x = -INFINITY;
-    ((O*)a.out)[b * a.ld_out + v] = (O)x;
   }
+  int* ids = reinterpret_cast<int*>(dynamic);
+  float* values = reinterpret_cast<float*>(dynamic + a.n_bias);
+  float* sums = reinterpret_cast<float*>(dynamic + 2 * a.n_bias);
+  if (a.n_bias > 0) {
+    // one wave puts the slice's biases together in the list's order
+    if (tid < 64) {
+      const int32_t* list = a.bias_ids + b * a.ld_bias;
+      const float* list_values = a.bias_values + b * a.ld_bias;
+      int count = 0;
+      for (int j0 = 0; j0 < a.n_bias; j0 += 64) {
+        const int j = j0 + tid;
+        const int id = j < a.n_bias ? list[j] : -1;
+        const float value = j < a.n_bias ? list_values[j] : 0.f;
+        const bool mine = id >= lo && id < hi;
+        const uint64_t all = __ballot(mine);
+        if (mine) {
+          const int at = count + __popcll(all & ((1ull << tid) - 1));
+          ids[at] = id, values[at] = value;
+        }
+        count += __popcll(all);
+      }
+      if (tid == 0) s_biases = count;
+    }
+    __syncthreads();
+    // an id's first entry sums all of them
+    const int count = s_biases;
+    for (int j = tid; j < count; j += THREADS) {
+      const int id = ids[j];
+      bool first = true;
+      float sum = 0.f;
+      for (int i = 0; i < count; ++i) {
+        const bool same = ids[i] == id;
+        first = first && !(same && i < j);
+        sum += same ? values[i] : 0.f;
+      }
+      sums[j] = sum;
+      if (first) atomicOr(&table[id - lo], (uint32_t)(j + 1) << kBiasShift);
+    }
+  }
+  if (special) __syncthreads();
+  penalties pen;
+  pen.r = a.repetition ? a.repetition[b] : 1.f;
+  pen.f = a.frequency ? a.frequency[b] : 0.f;
+  pen.p = a.presence ? a.presence[b] : 0.f;
+  const uint8_t* allowed = reinterpret_cast<const uint8_t*>(a.allowed + b * a.ld_allowed);
+#pragma unroll
+  for (int k = 0; k < kPasses; ++k) {
+    const int v = lo + (k * THREADS + tid) * kVec;
+    if (v >= hi) break;
+    const uint32_t mask = a.allowed ? allowed[v >> 3] : 0xff;
+    uint32_t w[kVec] = {};
+    if (special) __builtin_memcpy(w, __builtin_assume_aligned(&table[v - lo], 16), sizeof(w));
+    O y[kVec];
+    if (v + kVec <= hi) {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) y[e] = (O)adjust((float)x[k][e], w[e], pen, sums, mask >> e & 1);
+      __builtin_memcpy(out + v, y, sizeof(y));
+    } else {
+      for (int e = 0; v + e < hi; ++e)
+        out[v + e] = (O)adjust((float)in[v + e], special ? table[v - lo + e] : 0u, pen, sums,
+                               mask >> e & 1);
+    }
+  }
+}
+
+// Threads of a workgroup, each with kVec * kPasses logits.  Larger slices read
+// the history less often, smaller ones put a small batch on more CUs.
+int threads_of(int64_t logits) {
+  return logits >= (int64_t)kWide ? 512 : 256;
+}
+
+template <int DT, int OT>
+int launch(logits_args a, hipStream_t s) {
+  const int threads = threads_of((int64_t)a.rows * a.vocab);
+  const int slice = threads * kVec * kPasses;
+  a.slices = (a.vocab + slice - 1) / slice;
+  const int64_t blocks = (int64_t)a.rows * a.slices;
+  if (!pl_grid_fits(blocks, threads)) {
+    pl_set_error("pl_adjust_logits: too many rows (%d)", a.rows);
+    return PL_ERR_LIMIT;
+  }
+  const dim3 grid((unsigned)blocks);
+  const size_t lds = (size_t)a.n_bias * 12;
+  if (threads == 512)
+    pl_adjust_logits_kernel<DT, OT, 512><<<grid, 512, lds, s>>>(a);
+  else
+    pl_adjust_logits_kernel<DT, OT, 256><<<grid, 256, lds, s>>>(a);
+  return pl_launch_status("pl_adjust_logits");
 }
 
 }  // namespace
@@ -122,23 +228,10 @@ extern "C" int pl_adjust_logits(int32_t dtype, int32_t out_dtype, const void* lo
   a.bias_ids = bias_ids, a.bias_values = bias_values, a.allowed = allowed;
   a.ld = ld, a.ld_out = ld_out, a.ld_tokens = ld_tokens, a.ld_bias = ld_bias;
   a.ld_allowed = ld_allowed, a.rows = rows, a.vocab = vocab, a.history = history;
-  a.n_bias = n_bias, a.wide_tokens = token_bytes == 8, a.slices = (vocab + kSlice - 1) / kSlice;
-  const int64_t blocks = (int64_t)rows * a.slices;
-  if (!pl_grid_fits(blocks, kThreads)) {
-    pl_set_error("pl_adjust_logits: too many rows (%d)", rows);
-    return PL_ERR_LIMIT;
-  }
+  a.n_bias = n_bias, a.wide_tokens = token_bytes == 8;
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)blocks);
-  if (dtype == PL_F32)
-    pl_adjust_logits_kernel<PL_F32, PL_F32><<<grid, kThreads, 0, s>>>(a);
-  else if (dtype == PL_BF16 && out_dtype == PL_F32)
-    pl_adjust_logits_kernel<PL_BF16, PL_F32><<<grid, kThreads, 0, s>>>(a);
-  else if (dtype == PL_BF16)
-    pl_adjust_logits_kernel<PL_BF16, PL_BF16><<<grid, kThreads, 0, s>>>(a);
-  else if (out_dtype == PL_F32)
-    pl_adjust_logits_kernel<PL_F16, PL_F32><<<grid, kThreads, 0, s>>>(a);
-  else
-    pl_adjust_logits_kernel<PL_F16, PL_F16><<<grid, kThreads, 0, s>>>(a);
-  return pl_launch_status("pl_adjust_logits");
+  if (dtype == PL_F32) return launch<PL_F32, PL_F32>(a, s);
+  if (dtype == PL_BF16)
+    return out_dtype == PL_F32 ? launch<PL_BF16, PL_F32>(a, s) : launch<PL_BF16, PL_BF16>(a, s);
+  return out_dtype == PL_F32 ? launch<PL_F16, PL_F32>(a, s) : launch<PL_F16, PL_F16>(a, s);
 }

@@ -62,6 +62,8 @@ int pl_check_paged(const char* what, int32_t dtype, int32_t cache_dtype, const v
 namespace {
 
 constexpr int kThreads = 256;
+// Workgroups that fill the GPU (eight on each of 256 CUs).
+constexpr int kFullGrid = 2048;
 
 struct append_args {
   const void *q, *k, *v;
@@ -73,65 +75,183 @@ struct append_args {
   const float *cos, *sin;  // [positions][rot / 2]
   const float *k_scale, *v_scale;
   int32_t rows, row_len, heads, kv_heads, dim, positions, half, interleaved;
+  int32_t turns, units, group;  // places of a head that turn, all of them, tokens of a workgroup
 };
 
-// x as stored: rounded to the cache's type, e4m3 after division by the scale
-// and saturated (NaN stays NaN).
-template <int CT>
-__device__ __forceinline__ typename pl_cache_elem<CT>::T to_cache(float x, float scale) {
-  if constexpr (CT == PL_F8E4M3) {
-    const float y = x / scale;
-    const float c = y != y ? y : fminf(fmaxf(y, -kE4M3Max), kE4M3Max);
-    return (uint8_t)(__builtin_amdgcn_cvt_pk_fp8_f32(c, c, 0, false) & 0xff);
+// One value as an e4m3 byte: over the scale, saturated (NaN stays NaN).
+__device__ __forceinline__ float to_e4m3_range(float x, float scale) {
+  const float y = x / scale;
+  return y != y ? y : fminf(fmaxf(y, -kE4M3Max), kE4M3Max);
+}
+
+// VEC elements of a row as fp32, and their stores.
+template <int DT, int VEC>
+__device__ __forceinline__ void load_vec(const void* p, int64_t at, float (&x)[VEC]) {
+  typedef typename pl_traits<DT>::T T;
+  typedef T TV __attribute__((ext_vector_type(VEC)));
+  const T* q = (const T*)p + at;
+  if constexpr (VEC == 1) {
+    x[0] = (float)*q;
   } else {
-    return (typename pl_cache_elem<CT>::T)x;
+    const TV v = *reinterpret_cast<const TV*>(q);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) x[e] = (float)v[e];
+  }
+}
+template <int DT, int VEC>
+__device__ __forceinline__ void store_vec(void* p, int64_t at, const float (&x)[VEC]) {
+  typedef typename pl_traits<DT>::T T;
+  typedef T TV __attribute__((ext_vector_type(VEC)));
+  T* q = (T*)p + at;
+  if constexpr (VEC == 1) {
+    *q = (T)x[0];
+  } else {
+    TV v;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = (T)x[e];
+    *reinterpret_cast<TV*>(q) = v;
+  }
+}
+template <int DT, int CT, int VEC>
+__device__ __forceinline__ void store_cache(void* p, int64_t at, const float (&x)[VEC], float scale) {
+  if constexpr (CT == PL_F8E4M3) {
+    uint8_t* q = (uint8_t*)p + at;
+    uint32_t w[(VEC + 3) / 4] = {};
+#pragma unroll
+    for (int e = 0; e < VEC; e += 2) {
+      const float lo = to_e4m3_range(x[e], scale);
+      const float hi = e + 1 < VEC ? to_e4m3_range(x[e + 1], scale) : lo;
+      w[e / 4] = e % 4 ? __builtin_amdgcn_cvt_pk_fp8_f32(lo, hi, (int)w[e / 4], true)
+                       : __builtin_amdgcn_cvt_pk_fp8_f32(lo, hi, (int)w[e / 4], false);
+    }
+    __builtin_memcpy(__builtin_assume_aligned(q, VEC), w, VEC);
+  } else {
+    store_vec<DT, VEC>(p, at, x);
   }
 }
 
-// One workgroup per token: its threads walk the elements of q, k and v.
-template <int DT, int CT>
+// A workgroup takes `group` tokens.  A thread keeps one place of the head,
+// VEC elements and, split in halves, the VEC that turn against them, and
+// walks the token's query and key heads with it, so that it reads its part of
+// cos and sin once; the threads then copy the values.  The tokens' lengths,
+// pages and angles take two dependent reads, the second beside the heads'.
+//
+// Bound by memory: every element of q, k and v is read and written once.
+template <int DT, int CT, int VEC>
 __global__ __launch_bounds__(kThreads) void pl_rope_append_kernel(append_args a) {
-  typedef typename pl_traits<DT>::T T;
-  typedef typename pl_cache_elem<CT>::T C;
-  const int b = (int)(blockIdx.x / a.row_len), t = (int)(blockIdx.x % a.row_len);
+  const int tid = (int)threadIdx.x;
+  // threads of a token, and this thread's
+  const int part = kThreads / a.group;
+  const int sub = tid / part, rank = tid - sub * part;
+  const int64_t token = (int64_t)blockIdx.x * a.group + sub;
+  if (token >= (int64_t)a.rows * a.row_len) return;
+  const int b = (int)(token / a.row_len), t = (int)(token - (int64_t)b * a.row_len);
   const int n = a.seq_lens ? min(a.seq_lens[b], a.row_len) : a.row_len;
-  const int64_t pos = (int64_t)a.past[b] + t;
-  const int64_t column = pos >> a.table.page_shift;
+  const int64_t pos = (int64_t)a.past[b] + t, column = pos >> a.table.page_shift;
   int page = -1;
   if (t < n && pos >= 0 && pos < a.positions && column < a.table.max_pages)
     page = a.table.p[b * a.table.ld + column];
   const bool live = page >= 0 && page < a.table.num_pages;
   const int64_t slot = pos & ((1 << a.table.page_shift) - 1);
-  const int all = (a.heads + 2 * a.kv_heads) * a.dim;
-  for (int i = (int)threadIdx.x; i < all; i += kThreads) {
-    const int h = i / a.dim, d = i % a.dim;
-    const bool is_q = h < a.heads, is_k = !is_q && h < a.heads + a.kv_heads;
-    const int hh = is_q ? h : is_k ? h - a.heads : h - a.heads - a.kv_heads;
-    const T* x = is_q   ? (const T*)a.q + b * a.qs[0] + t * a.qs[1] + hh * a.qs[2]
-                 : is_k ? (const T*)a.k + b * a.ks[0] + t * a.ks[1] + hh * a.ks[2]
-                        : (const T*)a.v + b * a.vs[0] + t * a.vs[1] + hh * a.vs[2];
-    float y = 0.f;
-    if (live) {
-      y = (float)x[d];
-      if ((is_q || is_k) && d < 2 * a.half) {
-        const int p = a.interleaved ? d >> 1 : d % a.half;
-        const bool second = a.interleaved ? (d & 1) : d >= a.half;
-        const int other = a.interleaved ? d ^ 1 : second ? d - a.half : d + a.half;
-        const float c = a.cos[pos * a.half + p], s = a.sin[pos * a.half + p], z = (float)x[other];
-        y = second ? y * c + z * s : y * c - z * s;
+
+  // query and key heads: place u of the head for heads lane, lane + lanes, ...
+  const int lanes = part / a.units, lane = rank / a.units, u = rank - lane * a.units;
+  if (lane < lanes) {
+    // the first `turns` places turn, each against the place half a rotation on
+    // or, interleaved, in pairs inside (a place of one element against the
+    // next); the rest are copied
+    const bool turn = u < a.turns, split = turn && (VEC == 1 || !a.interleaved);
+    const int d = !turn                           ? 2 * a.half + (u - a.turns) * VEC
+                  : VEC == 1 && a.interleaved ? 2 * u
+                                                  : u * VEC;
+    const int d2 = !split ? d : a.interleaved ? d + 1 : d + a.half;
+    float c[VEC], s[VEC];  // interleaved: VEC / 2 of them
+    if (turn && live) {
+      const int64_t i = pos * a.half + (a.interleaved ? d >> 1 : d);
+      if (VEC > 1 && a.interleaved) {
+        __builtin_memcpy(c, a.cos + i, VEC / 2 * sizeof(float));
+        __builtin_memcpy(s, a.sin + i, VEC / 2 * sizeof(float));
+      } else {
+        __builtin_memcpy(c, a.cos + i, VEC * sizeof(float));
+        __builtin_memcpy(s, a.sin + i, VEC * sizeof(float));
       }
     }
-    const int64_t token = (int64_t)b * a.row_len + t;
-    if (is_q) {
-      ((T*)a.q_out)[(token * a.heads + hh) * a.dim + d] = (T)y;
-    } else {
-      const pl_cache_view& cache = is_k ? a.key : a.value;
-      if (live)
-        ((C*)cache.p)[page * cache.s_page + hh * cache.s_head + slot * cache.s_slot + d] =
-            to_cache<CT>(y, CT == PL_F8E4M3 ? (is_k ? a.k_scale : a.v_scale)[hh] : 1.f);
-      if (is_k && a.k_out) ((T*)a.k_out)[(token * a.kv_heads + hh) * a.dim + d] = (T)y;
+    for (int h = lane; h < a.heads + a.kv_heads; h += lanes) {
+      const bool is_q = h < a.heads;
+      const int hh = is_q ? h : h - a.heads;
+      float x[VEC], y[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) x[e] = y[e] = 0.f;
+      if (live) {
+        const void* src = is_q ? a.q : a.k;
+        const int64_t at = is_q ? b * a.qs[0] + t * a.qs[1] + hh * a.qs[2]
+                                : b * a.ks[0] + t * a.ks[1] + hh * a.ks[2];
+        load_vec<DT, VEC>(src, at + d, x);
+        if (split) load_vec<DT, VEC>(src, at + d2, y);
+        if (split) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            const float x0 = x[e], y0 = y[e];
+            x[e] = x0 * c[e] - y0 * s[e];
+            y[e] = y0 * c[e] + x0 * s[e];
+          }
+        } else if (turn) {
+#pragma unroll
+          for (int e = 0; e + 1 < VEC; e += 2) {
+            const float x0 = x[e], y0 = x[e + 1];
+            x[e] = x0 * c[e / 2] - y0 * s[e / 2];
+            x[e + 1] = y0 * c[e / 2] + x0 * s[e / 2];
+          }
+        }
+      }
+      void* dense = is_q ? a.q_out : a.k_out;
+      if (dense) {
+        const int64_t at = (token * (is_q ? a.heads : a.kv_heads) + hh) * a.dim;
+        store_vec<DT, VEC>(dense, at + d, x);
+        if (split) store_vec<DT, VEC>(dense, at + d2, y);
+      }
+      if (!is_q && live) {
+        const int64_t at = page * a.key.s_page + hh * a.key.s_head + slot * a.key.s_slot;
+        const float scale = CT == PL_F8E4M3 ? a.k_scale[hh] : 1.f;
+        store_cache<DT, CT, VEC>(a.key.p, at + d, x, scale);
+        if (split) store_cache<DT, CT, VEC>(a.key.p, at + d2, y, scale);
+      }
     }
   }
+  if (!live) return;
+  const int places = a.dim / VEC;
+  for (int i = rank; i < a.kv_heads * places; i += part) {
+    const int hh = i / places, d = (i - hh * places) * VEC;
+    float x[VEC];
+    load_vec<DT, VEC>(a.v, b * a.vs[0] + t * a.vs[1] + hh * a.vs[2] + d, x);
+    store_cache<DT, CT, VEC>(a.value.p,
+                             page * a.value.s_page + hh * a.value.s_head + slot * a.value.s_slot + d,
+                             x, CT == PL_F8E4M3 ? a.v_scale[hh] : 1.f);
+  }
+}
+
+template <int DT, int CT>
+int launch(append_args a, int vec, hipStream_t s) {
+  // places of a head that a thread may keep
+  a.turns = (a.interleaved && vec > 1 ? 2 * a.half : a.half) / vec;
+  a.units = a.turns + (a.dim - 2 * a.half) / vec;
+  const int64_t tokens = (int64_t)a.rows * a.row_len;
+  // one token per workgroup while that leaves some idle, then enough of them
+  // that every thread walks several heads with the angles it has read
+  a.group = 1;
+  while (a.group < 4 && tokens / (2 * a.group) >= kFullGrid && kThreads / (2 * a.group) >= a.units)
+    a.group *= 2;
+  const dim3 grid((unsigned)((tokens + a.group - 1) / a.group));
+  if (vec == 8) {
+    if constexpr (DT != PL_F32) pl_rope_append_kernel<DT, CT, 8><<<grid, kThreads, 0, s>>>(a);
+  } else if (vec == 4) {
+    pl_rope_append_kernel<DT, CT, 4><<<grid, kThreads, 0, s>>>(a);
+  } else if (vec == 2) {
+    pl_rope_append_kernel<DT, CT, 2><<<grid, kThreads, 0, s>>>(a);
+  } else {
+    pl_rope_append_kernel<DT, CT, 1><<<grid, kThreads, 0, s>>>(a);
+  }
+  return pl_launch_status("pl_rope_append");
 }
 
 }  // namespace
@@ -192,19 +312,23 @@ extern "C" int pl_rope_append(int32_t dtype, int32_t cache_dtype, const void* q,
   a.k_scale = k_scale, a.v_scale = v_scale;
   a.rows = rows, a.row_len = row_len, a.heads = heads, a.kv_heads = kv_heads, a.dim = dim;
   a.positions = positions, a.half = rot / 2, a.interleaved = interleaved;
+  // Elements a thread moves at once: 16 bytes' worth where the halves of a
+  // rotation, and every pointer and stride, are whole pieces of that many.
+  auto whole = [&](int vec) {
+    const uintptr_t bytes = (uintptr_t)vec * es;
+    bool ok = (a.interleaved ? rot : rot / 2) % vec == 0 && dim % vec == 0;
+    const void* pointers[5] = {q, k, v, q_out, k_out};
+    for (const void* p : pointers) ok = ok && reinterpret_cast<uintptr_t>(p) % bytes == 0;
+    for (int i = 0; i < 3; ++i)
+      ok = ok && a.qs[i] % vec == 0 && a.ks[i] % vec == 0 && a.vs[i] % vec == 0;
+    return ok;
+  };
+  int vec = (int)(16 / es);
+  while (vec > 1 && !whole(vec)) vec /= 2;
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)tokens);
-  if (cache_dtype == PL_F8E4M3) {
-    if (dtype == PL_BF16)
-      pl_rope_append_kernel<PL_BF16, PL_F8E4M3><<<grid, kThreads, 0, s>>>(a);
-    else
-      pl_rope_append_kernel<PL_F16, PL_F8E4M3><<<grid, kThreads, 0, s>>>(a);
-  } else if (dtype == PL_F32) {
-    pl_rope_append_kernel<PL_F32, PL_F32><<<grid, kThreads, 0, s>>>(a);
-  } else if (dtype == PL_BF16) {
-    pl_rope_append_kernel<PL_BF16, PL_BF16><<<grid, kThreads, 0, s>>>(a);
-  } else {
-    pl_rope_append_kernel<PL_F16, PL_F16><<<grid, kThreads, 0, s>>>(a);
-  }
-  return pl_launch_status("pl_rope_append");
+  if (cache_dtype == PL_F8E4M3)
+    return dtype == PL_BF16 ? launch<PL_BF16, PL_F8E4M3>(a, vec, s)
+                            : launch<PL_F16, PL_F8E4M3>(a, vec, s);
+  if (dtype == PL_F32) return launch<PL_F32, PL_F32>(a, vec, s);
+  return dtype == PL_BF16 ? launch<PL_BF16, PL_BF16>(a, vec, s) : launch<PL_F16, PL_F16>(a, vec, s);
 }
