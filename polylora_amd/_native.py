@@ -16,6 +16,7 @@ import torch  # noqa: F401  (loads the HIP runtime the library must share)
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libpolylora_hip.so"
 CALLS_PATH = LIB_PATH.parent / "_calls.so"
+TENSOR_CALLS_PATH = LIB_PATH.parent / "_tensor_calls.so"
 
 PL_F32, PL_BF16, PL_F16 = 0, 1, 2
 PL_F8E4M3 = 3  # paged caches only
@@ -154,6 +155,7 @@ EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 
 _lib = None
 _calls = None
+_tensor_calls = None
 _checked_runtime = False
 
 
@@ -180,19 +182,33 @@ def load() -> ctypes.CDLL:
     return lib
 
 
+def _extension(path: Path):
+    """A CPython extension module built beside the library, which is loaded first (one instance for every binding)."""
+    load()
+    if not path.exists():
+        raise NativeLibraryMissing(f"{path} not found; build it with `python -m polylora_amd.build`")
+    loader = importlib.machinery.ExtensionFileLoader(path.stem, str(path))
+    module = loader.create_module(importlib.machinery.ModuleSpec(path.stem, loader, origin=str(path)))
+    loader.exec_module(module)
+    return module
+
+
 def calls():
     """The library's per-call functions as CPython entry points (csrc/pycalls.cpp): the C functions' arguments in
     their order as ints (None for a null pointer, a tuple for a host array of per-module values); each returns the
     status for ``check``."""
     global _calls
     if _calls is None:
-        load()  # the one instance of the library both bindings use
-        if not CALLS_PATH.exists():
-            raise NativeLibraryMissing(f"{CALLS_PATH} not found; build it with `python -m polylora_amd.build`")
-        loader = importlib.machinery.ExtensionFileLoader("_calls", str(CALLS_PATH))
-        _calls = loader.create_module(importlib.machinery.ModuleSpec("_calls", loader, origin=str(CALLS_PATH)))
-        loader.exec_module(_calls)
+        _calls = _extension(CALLS_PATH)
     return _calls
+
+
+def tensor_calls():
+    """The entry points that take torch tensors and check them themselves (csrc/tensorcalls.cpp)."""
+    global _tensor_calls
+    if _tensor_calls is None:
+        _tensor_calls = _extension(TENSOR_CALLS_PATH)
+    return _tensor_calls
 
 
 def check(status: int, what: str) -> None:

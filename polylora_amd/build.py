@@ -1,11 +1,13 @@
 """Build the gfx950 HIP library ``polylora_amd/_lib/libpolylora_hip.so``.
 
 Run ``python -m polylora_amd.build``.  Also builds ``_lib/_calls.so``, the
-CPython entry points of the per-call functions (``csrc/pycalls.cpp``), linked
+CPython entry points of the per-call functions (``csrc/pycalls.cpp``), and
+``_lib/_tensor_calls.so``, those that take torch tensors
+(``csrc/tensorcalls.cpp``, host code against the running torch), both linked
 against the library.  Every source under ``csrc/`` is
 compiled with ``hipcc --offload-arch=gfx950`` into an object under
 ``polylora_amd/_build/`` and the objects are linked into one shared library
-with a plain C ABI (``include/polylora_hip.h``); nothing links against
+with a plain C ABI (``include/polylora_hip.h``); it does not link against
 libtorch, so the library binds to whichever HIP runtime the process already
 loaded (torch's, when torch is imported first).
 """
@@ -25,6 +27,7 @@ BUILD_DIR = PACKAGE_DIR / "_build"
 LIB_DIR = PACKAGE_DIR / "_lib"
 LIB_PATH = LIB_DIR / "libpolylora_hip.so"
 CALLS_PATH = LIB_DIR / "_calls.so"
+TENSOR_CALLS_PATH = LIB_DIR / "_tensor_calls.so"
 INCLUDE_DIR = PACKAGE_DIR.parent / "include"
 
 ARCH = "gfx950"
@@ -102,15 +105,26 @@ def build(verbose: bool = False) -> Path:
 
 
 def _build_calls(hipcc: str) -> None:
-    """csrc/pycalls.cpp, host code only, for the running interpreter."""
+    """csrc/pycalls.cpp and csrc/tensorcalls.cpp, host code only, for the running interpreter and its torch."""
+    import torch
+
     cxx = [found] if (found := shutil.which("g++")) else [hipcc, "-x", "c++"]
-    tmp = CALLS_PATH.with_suffix(".so.tmp")
-    cmd = [*cxx, "-O2", "-fPIC", "-std=c++17", "-Wall", "-shared", f"-I{sysconfig.get_paths()['include']}",
-           str(CSRC_DIR / "pycalls.cpp"), "-o", str(tmp), f"-L{LIB_DIR}", "-lpolylora_hip", "-Wl,-rpath,$ORIGIN"]
-    proc = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
-    if proc.returncode != 0:
-        raise RuntimeError(f"build failed: {' '.join(cmd)}\n{proc.stdout}")
-    os.replace(tmp, CALLS_PATH)
+    torch_dir = Path(torch.__file__).resolve().parent
+    torch_flags = [f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{torch_dir / 'include'}",
+                   f"-I{torch_dir / 'include' / 'torch' / 'csrc' / 'api' / 'include'}"]
+    torch_libs = [f"-L{torch_dir / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    running = []
+    for source, target, flags, libs in (("pycalls.cpp", CALLS_PATH, [], []),
+                                        ("tensorcalls.cpp", TENSOR_CALLS_PATH, torch_flags, torch_libs)):
+        tmp = target.with_suffix(".so.tmp")
+        cmd = [*cxx, "-O2", "-fPIC", "-std=c++17", "-Wall", "-shared", f"-I{sysconfig.get_paths()['include']}", *flags,
+               str(CSRC_DIR / source), "-o", str(tmp), f"-L{LIB_DIR}", "-lpolylora_hip", *libs, "-Wl,-rpath,$ORIGIN"]
+        running.append((cmd, tmp, target, _run(cmd)))
+    for cmd, tmp, target, proc in running:
+        out, _ = proc.communicate()
+        if proc.returncode != 0:
+            raise RuntimeError(f"build failed: {' '.join(cmd)}\n{out}")
+        os.replace(tmp, target)
 
 
 if __name__ == "__main__":

@@ -35,7 +35,7 @@ bool to_pointer(PyObject* o, void** out) {
 
 template <typename A>
 struct Arg {  // int32_t and int64_t
-  static_assert(std::is_integral<A>::value, "integers, floats and pointers only");
+  static_assert(std::is_integral<A>::value, "integers and pointers only");
   A v;
   bool set(PyObject* o) {
     int64_t w;
@@ -48,17 +48,6 @@ struct Arg {  // int32_t and int64_t
     return true;
   }
   A get() { return v; }
-};
-
-template <>
-struct Arg<float> {
-  float v;
-  bool set(PyObject* o) {
-    const double w = PyFloat_AsDouble(o);
-    v = (float)w;
-    return w != -1.0 || !PyErr_Occurred();
-  }
-  float get() { return v; }
 };
 
 template <typename P>
@@ -134,9 +123,6 @@ PyMethodDef methods[] = {PL_CALL(pl_lora_apply),
                          PL_CALL(pl_sgmv_expand_stacked),
                          PL_CALL(pl_sgmv_lora_a_ref_parts),
                          PL_CALL(pl_sgmv_lora_b_ref_parts),
-                         PL_CALL(pl_rope_append),
-                         PL_CALL(pl_paged_attention),
-                         PL_CALL(pl_adjust_logits),
                          {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods,
