@@ -29,13 +29,13 @@
 // them to 2^-16 (bf16) or better: one product more on matrix units that have
 // little else to do, and the output keeps the error of its own rounding.
 //
-// Work is split by tokens: the launch is a fixed number of workgroups, and
-// each takes an equal run of the batch's atoms (kAtom tokens of one row and
-// key head), found from the lengths on the device, so no length is needed on
-// the host and ragged batches come out even.  A run that covers a (row, key
-// head) whole writes its output; a run that ends inside one leaves (m, l, o) in
-// the workspace, and the workgroup that arrives last on the pair's counter
-// joins the parts in order (the same bits whichever arrives last).
+// Work is split by tokens: the launch is a fixed number of workgroups, and the
+// batch's atoms (kAtom tokens of one row and key head) are dealt out in equal
+// runs, found from the lengths on the device, so no length is needed on the
+// host and ragged batches come out even (deal below says how runs are taken).
+// Where runs end inside a (row, key head), each leaves (m, l, o) in the
+// workspace, and the workgroup that arrives last on the pair's counter joins
+// the parts in order (the same bits whichever arrives last).
 #include "pl_paged.h"
 
 namespace {
@@ -60,8 +60,11 @@ struct shape {
   static constexpr int V = DP / 16;                  // value elements of a lane per token
   static constexpr int kVWords = V * kCsize / 4;
   static constexpr int kTokens = 4 * kSubs;          // tokens of a lane per tile
-  static constexpr int kPerCu = DP <= 128 ? 3 : DT == PL_F32 ? 1 : 2;
+  static constexpr int kPerCu = DP <= 128 ? 3 : 2;  // workgroups of a CU
+  // Queries in LDS where keys, values and outputs fill the registers.
+  static constexpr bool kQueryLds = DP == 256 || DT == PL_F32;
 };
+typedef pl_u32x4 __attribute__((may_alias)) shared_u32x4;
 
 struct attend_args {
   const void* q;
@@ -80,6 +83,26 @@ struct attend_args {
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// Sum (and, of values that are not negative, maximum) of a lane's and all lower
+// lanes' values: shifts by 1, 2, 4 and 8 inside rows of 16, then each row's
+// last lane into the rows above.  Lanes that a step does not write add 0.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int from_lower(int x) {
+  return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int scan_sum(int x) {
+  x += from_lower<0x111, 0xf>(x), x += from_lower<0x112, 0xf>(x);
+  x += from_lower<0x114, 0xf>(x), x += from_lower<0x118, 0xf>(x);
+  x += from_lower<0x142, 0xa>(x);
+  return x + from_lower<0x143, 0xc>(x);
+}
+__device__ __forceinline__ int scan_max(int x) {
+  x = max(x, from_lower<0x111, 0xf>(x)), x = max(x, from_lower<0x112, 0xf>(x));
+  x = max(x, from_lower<0x114, 0xf>(x)), x = max(x, from_lower<0x118, 0xf>(x));
+  x = max(x, from_lower<0x142, 0xa>(x));
+  return max(x, from_lower<0x143, 0xc>(x));
+}
+
 // The largest of the four lanes of a column, and their sum.
 __device__ __forceinline__ float column_max(float x) {
   auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -94,22 +117,29 @@ __device__ __forceinline__ float column_sum(float x) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// 4 * N bytes at `off` from a base that the wave shares.
+// Memory that a wave's lanes read through a buffer descriptor, all of it in
+// scalar registers: `bytes` from `p`; reads past them give 0 and touch nothing.
+typedef __amdgpu_buffer_rsrc_t pl_buffer;
+__device__ __forceinline__ pl_buffer make_buffer(uintptr_t p, uint32_t bytes) {
+  const uint32_t lo = (uint32_t)uniform((int)(uint32_t)p), hi = (uint32_t)uniform((int)(p >> 32));
+  return __builtin_amdgcn_make_buffer_rsrc(
+      reinterpret_cast<void*>((uintptr_t)lo | (uintptr_t)hi << 32), 0, uniform((int)bytes), 0x00027000);
+}
 template <int N>
-__device__ __forceinline__ void load_words(const char* base, uint32_t off, uint32_t (&w)[N]) {
-  const char* p = base + off;
+__device__ __forceinline__ void load_words(pl_buffer r, uint32_t lane_off, uint32_t wave_off,
+                                           uint32_t (&w)[N]) {
   if constexpr (N % 4 == 0) {
 #pragma unroll
     for (int i = 0; i < N / 4; ++i) {
-      const pl_u32x4 x = pl_ld16(p + 16 * i);
+      const pl_u32x4 x = __builtin_bit_cast(
+          pl_u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, lane_off + 16 * i, wave_off, 0));
       w[4 * i] = x.x, w[4 * i + 1] = x.y, w[4 * i + 2] = x.z, w[4 * i + 3] = x.w;
     }
   } else if constexpr (N == 2) {
-    typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-    const u2 x = *reinterpret_cast<const u2*>(p);
-    w[0] = x.x, w[1] = x.y;
+    const auto x = __builtin_amdgcn_raw_buffer_load_b64(r, lane_off, wave_off, 0);
+    w[0] = x[0], w[1] = x[1];
   } else {
-    w[0] = *reinterpret_cast<const uint32_t*>(p);
+    w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, lane_off, wave_off, 0);
   }
 }
 
@@ -146,44 +176,55 @@ __device__ __forceinline__ int key_piece(int n, int g, int e) {
 template <int DT, int CT, int DP>
 struct wave_state {
   typedef shape<DT, CT, DP> S;
-  pl_u32x4 q[S::kSteps];
+  pl_u32x4 q[S::kQueryLds ? 1 : S::kSteps];
+  shared_u32x4* q_lds;  // this lane's pieces, 64 apart
+  __device__ __forceinline__ pl_u32x4 query(int n) const {
+    if constexpr (S::kQueryLds)
+      return q_lds[n * 64];
+    else
+      return q[n];
+  }
   pl_f32x4 o[S::V];
   float m, l;
 };
 
 // A row's page ids, read through the scalar cache: every lane wants the same.
 typedef const __attribute__((address_space(4))) int32_t* scalar_i32;
+typedef const __attribute__((address_space(4))) float* scalar_f32;
 __device__ __forceinline__ scalar_i32 as_scalar(const int32_t* p) {
   return (scalar_i32)(reinterpret_cast<uintptr_t>(p));
 }
-
-// Where a tile's keys and values lie, for each 16 tokens of it (16 tokens from
-// a multiple of 16 share a page), and what of it counts.
-template <int SUBS>
-struct tile_place {
-  const char *key[SUBS], *value[SUBS];
-  bool held[SUBS];
-};
+__device__ __forceinline__ scalar_f32 as_scalar(const float* p) {
+  return (scalar_f32)(reinterpret_cast<uintptr_t>(p));
+}
 
 // What the walk over one (row, key head) needs; all of it is the wave's.
 struct walk {
-  const char *key, *value;  // the key head's
+  uintptr_t key, value;  // the key head's
   scalar_i32 pages;
   int64_t key_page, value_page;  // bytes
   uint32_t key_slot, value_slot;
-  int first, len, shift, num_pages;
+  int end, shift, num_pages;
 };
 
+// Where a tile's keys and values lie, for each 16 tokens of it (16 tokens from
+// a multiple of 16 share a page).  Tokens past the walk's end and on pages that
+// the table does not hold have no bytes: reading them gives 0.
+template <int SUBS>
+struct tile_place {
+  uintptr_t key[SUBS], value[SUBS];
+  bool held[SUBS];
+};
 template <int SUBS>
 __device__ __forceinline__ tile_place<SUBS> place_tile(const walk& w, int t) {
   tile_place<SUBS> r;
 #pragma unroll
   for (int u = 0; u < SUBS; ++u) {
     const int tu = t + 16 * u;
-    // no look-up for 16 tokens past the row's end: its table row may end there
-    const int id = tu < w.len ? w.pages[tu >> w.shift] : -1;
+    // no look-up past the end: the table's row may end there
+    const int id = tu < w.end ? w.pages[tu >> w.shift] : -1;
     r.held[u] = id >= 0 && id < w.num_pages;
-    const int64_t page = r.held[u] ? id : 0;  // page 0 is there, and none of it counts
+    const int64_t page = r.held[u] ? id : 0;
     const uint32_t slot = (uint32_t)tu & ((1u << w.shift) - 1);
     r.key[u] = w.key + page * w.key_page + (uint64_t)slot * w.key_slot;
     r.value[u] = w.value + page * w.value_page + (uint64_t)slot * w.value_slot;
@@ -212,10 +253,10 @@ __device__ __forceinline__ void score_tile(
                             widen<DT, true>(w.y)};
         const pl_u32x4 b = {widen<DT, false>(w.z), widen<DT, true>(w.z), widen<DT, false>(w.w),
                             widen<DT, true>(w.w)};
-        s[u] = pl_mfma_chunk<DT>(a, st.q[2 * n], s[u]);
-        s[u] = pl_mfma_chunk<DT>(b, st.q[2 * n + 1], s[u]);
+        s[u] = pl_mfma_chunk<DT>(a, st.query(2 * n), s[u]);
+        s[u] = pl_mfma_chunk<DT>(b, st.query(2 * n + 1), s[u]);
       } else {
-        s[u] = pl_mfma_chunk<DT>(w, st.q[n], s[u]);
+        s[u] = pl_mfma_chunk<DT>(w, st.query(n), s[u]);
       }
     }
   }
@@ -369,64 +410,92 @@ __device__ __forceinline__ void join_parts(const float* parts, int slot0, int sl
   }
 }
 
+// How the batch's atoms are dealt out, from their number, the (row, key head)
+// pairs and the longest pair.  Times are in tiles of a wave (one after the
+// other, about as long as it waits for one): starting and ending a pair costs
+// a team of waves about kStart of them and joining parts about kJoin.
+struct deal {
+  int team;    // waves on a pair: kWaves, or 1 (no waves to join, no barrier)
+  bool whole;  // pairs go whole to the run that their first atom falls in
+};
+constexpr float kStart = 4.f, kJoin = 5.f;
+__device__ __forceinline__ deal choose_deal(int total, int pairs, int longest) {
+  const float w = (float)gridDim.x, n = (float)total, p = (float)pairs, top = (float)longest;
+  const float alone = kWaves * top * w + n + w + p / kWaves;
+  const float team = top * w + n + kStart * (w + p);
+  const float split = w + n + kStart * (w + p) + kJoin * w;
+  if (alone < team && alone < split) return {1, true};
+  return {kWaves, team < split};
+}
+
 template <int DT, int CT, int DP, bool FULL>
 __global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kPerCu)) void pl_paged_attention_kernel(
     attend_args a) {
   typedef shape<DT, CT, DP> S;
   typedef typename pl_traits<DT>::T T;
   constexpr int kPad = 4;
-  __shared__ float s_o[kWaves][kCols][DP + kPad];
+  __shared__ __attribute__((aligned(16))) float s_o[kWaves][kCols][DP + kPad];
   __shared__ float s_m[kWaves][kCols], s_l[kWaves][kCols];
-  __shared__ int s_scan[kWaves];
-  __shared__ int s_row, s_before, s_last;
+  __shared__ int s_last;
   const int tid = (int)threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int li = lane & 15, lg = lane >> 4;
   const int per_row = a.kv_heads * a.col_tiles;
 
-  // atoms of the batch, then this workgroup's run of them
-  int mine = 0;
-  for (int b = tid; b < a.rows; b += kThreads) mine += span_of<S::kAtom>(a, a.lens[b]).atoms;
+  // Each wave works out the deal for itself: 64 rows to a look, no barrier.
+  constexpr int kLooks = 4;  // that stay in registers
+  int atoms[kLooks], total = 0, longest = 0;
 #pragma unroll
-  for (int w = 32; w > 0; w >>= 1) mine += __shfl_xor(mine, w);
-  if (lane == 0) s_scan[wave] = mine;
-  __syncthreads();
-  int total = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) total += s_scan[w];
-  total = uniform(total) * per_row;
-  const int per = (int)((total + gridDim.x - 1) / gridDim.x);
-  const int from = (int)min((int64_t)blockIdx.x * per, (int64_t)total), to = min(total - per, from) + per;
+  for (int k = 0; k < kLooks; ++k) {
+    const int b = k * 64 + lane;
+    const int len = b < a.rows ? a.lens[b] : 0;
+    atoms[k] = b < a.rows ? span_of<S::kAtom>(a, len).atoms : 0;
+    total += atoms[k], longest = max(longest, atoms[k]);
+  }
+  for (int b = kLooks * 64 + lane; b < a.rows; b += 64) {
+    const int n = span_of<S::kAtom>(a, a.lens[b]).atoms;
+    total += n, longest = max(longest, n);
+  }
+  total = __builtin_amdgcn_readlane(scan_sum(total), 63) * per_row;
+  longest = __builtin_amdgcn_readlane(scan_max(longest), 63);
+  const deal how = choose_deal(total, a.rows * per_row, longest);
+  const int workers = (int)gridDim.x * kWaves / how.team;
+  const int worker = how.team == 1 ? (int)blockIdx.x * kWaves + wave : (int)blockIdx.x;
+  const int per = (total + workers - 1) / workers;
+  const int from = (int)min((int64_t)worker * per, (int64_t)total), to = min(total - per, from) + per;
   if (from >= total) return;
   // the row of its first atom: the first whose atoms up to and with it pass `from`
-  if (tid < 64) {
-    int before = 0;
-    for (int b0 = 0;; b0 += 64) {
-      const int b = b0 + lane;
-      const int n = b < a.rows ? span_of<S::kAtom>(a, a.lens[b]).atoms * per_row : 0;
-      int upto = n;
+  int row = 0, row_start = 0;
+  for (int b0 = 0;; b0 += 64) {
+    const int b = b0 + lane;
+    int n = atoms[0];
 #pragma unroll
-      for (int w = 1; w < 64; w <<= 1) {
-        const int x = __shfl_up(upto, w);
-        if (lane >= w) upto += x;
-      }
-      upto += before;
-      const uint64_t past = __ballot(upto > from);
-      if (past || b0 + 64 >= a.rows) {
-        const int hit = past ? __ffsll((long long)past) - 1 : 63;
-        if (lane == hit) s_row = b, s_before = upto - n;
-        break;
-      }
-      before = __shfl(upto, 63);
+    for (int k = 1; k < kLooks; ++k) n = b0 == k * 64 ? atoms[k] : n;
+    if (b0 >= kLooks * 64) n = b < a.rows ? span_of<S::kAtom>(a, a.lens[b]).atoms : 0;
+    n *= per_row;
+    const int upto = scan_sum(n) + row_start;
+    const uint64_t past = __ballot(upto > from);
+    if (past || b0 + 64 >= a.rows) {
+      const int hit = past ? __ffsll((long long)past) - 1 : 63;
+      row = b0 + hit;
+      row_start = __builtin_amdgcn_readlane(upto - n, hit);
+      break;
     }
+    row_start = __builtin_amdgcn_readlane(upto, 63);
   }
-  __syncthreads();
-  int row = uniform(s_row);
-  int row_start = uniform(s_before);  // atom index of the row's first
+  row = uniform(row);
+
   int at = from;
+  bool skip = how.whole;  // to the first pair that starts in the run
   while (at < to) {
     const row_span r = span_of<S::kAtom>(a, as_scalar(a.lens)[row]);
-    const int in_row = at - row_start;
+    int in_row = at - row_start;
+    if (skip) {
+      in_row = (in_row + r.atoms - 1) / r.atoms * r.atoms;
+      at = row_start + in_row;
+      skip = false;
+      if (at >= to) return;
+    }
     if (in_row >= r.atoms * per_row) {
       row_start += r.atoms * per_row;
       ++row;
@@ -435,42 +504,34 @@ __global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kPerCu)) void pl_page
     const int combo = in_row / r.atoms;
     const int pair_start = row_start + combo * r.atoms;
     const int first_atom = at - pair_start;
-    const int last_atom = min(r.atoms, to - pair_start);
+    const int last_atom = how.whole ? r.atoms : min(r.atoms, to - pair_start);
     const int hk = combo / a.col_tiles, ct = combo % a.col_tiles;
     const int cols = min(kCols, a.group - ct * kCols);
+    const int head0 = hk * a.group + ct * kCols;
 
     wave_state<DT, CT, DP> st;
     st.m = -INFINITY, st.l = 0.f;
+    st.q_lds = reinterpret_cast<shared_u32x4*>(&s_o[wave][0][0]) + lane;
 #pragma unroll
     for (int i = 0; i < S::V; ++i) st.o[i] = pl_f32x4{0.f, 0.f, 0.f, 0.f};
-    const int head0 = hk * a.group + ct * kCols;
-    {
-      const T* q = (const T*)a.q + row * a.q_row + (head0 + (li < cols ? li : 0)) * a.q_head;
-#pragma unroll
-      for (int n = 0; n < S::kSteps; ++n) {
-        const int d = CT == PL_F8E4M3 ? key_piece<CT>(n / 2, lg, S::E) + (n % 2) * 8
-                                      : key_piece<CT>(n, lg, S::E);
-        const bool ok = li < cols && (FULL || d < a.dim);
-        // rows of q have the alignment of their elements alone
-        pl_u32x4 x;
-        __builtin_memcpy(&x, q + (FULL || d < a.dim ? d : 0), 16);
-        st.q[n] = ok ? x : pl_u32x4{0, 0, 0, 0};
-      }
-    }
     const float scale2 =
-        a.scale * 1.44269504088896f * (CT == PL_F8E4M3 ? a.k_scale[hk] : 1.f);
+        a.scale * 1.44269504088896f * (CT == PL_F8E4M3 ? as_scalar(a.k_scale)[hk] : 1.f);
 
-    // this wave's tiles: every kWaves-th of the run's
+    // the tiles of this wave: every team-th of the run's
     const int end = min(r.len, r.base + last_atom * S::kAtom);
+    const int step = how.team * S::kTile;
     walk w;
-    w.key = (const char*)a.key.p + (int64_t)hk * a.key.s_head * S::kCsize;
-    w.value = (const char*)a.value.p + (int64_t)hk * a.value.s_head * S::kCsize;
+    w.key = reinterpret_cast<uintptr_t>(a.key.p) + (int64_t)hk * a.key.s_head * S::kCsize;
+    w.value = reinterpret_cast<uintptr_t>(a.value.p) + (int64_t)hk * a.value.s_head * S::kCsize;
     w.pages = as_scalar(a.table.p + row * a.table.ld);
     w.key_page = a.key.s_page * S::kCsize, w.value_page = a.value.s_page * S::kCsize;
     w.key_slot = (uint32_t)a.key.s_slot * S::kCsize;
     w.value_slot = (uint32_t)a.value.s_slot * S::kCsize;
-    w.first = r.first, w.len = r.len, w.shift = a.table.page_shift;
+    w.end = end, w.shift = a.table.page_shift;
     w.num_pages = a.table.num_pages;
+    // bytes from the first of 16 slots to the end of the last
+    const uint32_t key_span = 15 * w.key_slot + (uint32_t)a.dim * S::kCsize;
+    const uint32_t value_span = 15 * w.value_slot + (uint32_t)a.dim * S::kCsize;
     uint32_t key_off[S::kKeyLoads];
 #pragma unroll
     for (int n = 0; n < S::kKeyLoads; ++n) {
@@ -484,30 +545,52 @@ __global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kPerCu)) void pl_page
     // Keys of the next tile are asked for as soon as this tile's have gone into
     // the scores, values as soon as the wave is at the tile: one or the other
     // is in flight all the time, in no more registers than one tile takes.
+    // Past the last tile the loads stay, of no bytes: a load that is made in
+    // one turn of the loop and not in another would have to be waited for in
+    // every turn.
     pl_u32x4 keys[S::kSubs][S::kKeyLoads];
     auto load_keys = [&](const tile_place<S::kSubs>& at) {
 #pragma unroll
-      for (int u = 0; u < S::kSubs; ++u)
+      for (int u = 0; u < S::kSubs; ++u) {
+        const pl_buffer r = make_buffer(at.key[u], at.held[u] ? key_span : 0);
 #pragma unroll
-        for (int n = 0; n < S::kKeyLoads; ++n) keys[u][n] = pl_ld16(at.key[u] + key_off[n]);
+        for (int n = 0; n < S::kKeyLoads; ++n)
+          keys[u][n] = __builtin_bit_cast(
+              pl_u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, key_off[n], 0, 0));
+      }
     };
-    int tile = r.base + first_atom * S::kAtom + wave * S::kTile;
-    tile_place<S::kSubs> place;
+    int tile = r.base + first_atom * S::kAtom + (how.team == 1 ? 0 : wave * S::kTile);
     if (tile < end) {
-      place = place_tile<S::kSubs>(w, tile);
+      tile_place<S::kSubs> place = place_tile<S::kSubs>(w, tile);
+      const T* q = (const T*)a.q + row * a.q_row + (head0 + (li < cols ? li : 0)) * a.q_head;
+#pragma unroll
+      for (int n = 0; n < S::kSteps; ++n) {
+        const int d = CT == PL_F8E4M3 ? key_piece<CT>(n / 2, lg, S::E) + (n % 2) * 8
+                                      : key_piece<CT>(n, lg, S::E);
+        // rows of q have the alignment of their elements alone
+        pl_u32x4 x;
+        __builtin_memcpy(&x, q + (FULL || d < a.dim ? d : 0), 16);
+        x = li < cols && (FULL || d < a.dim) ? x : pl_u32x4{0, 0, 0, 0};
+        if constexpr (S::kQueryLds)
+          st.q_lds[n * 64] = x;
+        else
+          st.q[n] = x;
+      }
       load_keys(place);
-    }
-    for (; tile < end; tile += kWaves * S::kTile) {
+      do {
       uint32_t v[S::kTokens][S::kVWords];
 #pragma unroll
-      for (int j = 0; j < S::kTokens; ++j)
-        load_words(place.value[j / 4], value_off + (j % 4) * w.value_slot, v[j]);
+      for (int u = 0; u < S::kSubs; ++u) {
+        const pl_buffer b = make_buffer(place.value[u], place.held[u] ? value_span : 0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) load_words(b, value_off, j * w.value_slot, v[4 * u + j]);
+      }
       const tile_place<S::kSubs> here = place;
-      const int next = tile + kWaves * S::kTile;
-      if (next < end) place = place_tile<S::kSubs>(w, next);
+      const int next = tile + step;
+      place = place_tile<S::kSubs>(w, next);
       float p[S::kTokens];
       score_tile<DT, CT, DP, FULL>(st, keys, lg, a.dim, scale2, p);
-      if (next < end) load_keys(place);
+      load_keys(place);
       bool whole = tile >= r.first && tile + S::kTile <= r.len;
 #pragma unroll
       for (int u = 0; u < S::kSubs; ++u) whole = whole && here.held[u];
@@ -523,21 +606,41 @@ __global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kPerCu)) void pl_page
         }
       }
       weigh_tile<DT, CT, DP>(st, p, v);
+      tile = next;
+      } while (tile < end);
     }
 
-    // join the waves
     st.l = column_sum(st.l);
+    const float v_scale = CT == PL_F8E4M3 ? as_scalar(a.v_scale)[hk] : 1.f;
+    T* out = (T*)a.out + ((int64_t)row * a.heads + head0) * a.dim;
+    if (how.team == 1) {
+      if (li < cols) {
+        const float f = st.m == -INFINITY ? 0.f : v_scale / st.l;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int d = (4 * lg + e) * S::V;
+          T y[S::V];
+#pragma unroll
+          for (int i = 0; i < S::V; ++i) y[i] = (T)(st.o[i][e] * f);
+          // out has the alignment of its elements alone
+          if (FULL || d < a.dim) __builtin_memcpy(out + li * a.dim + d, y, sizeof(y));
+        }
+      }
+      at = pair_start + last_atom;
+      continue;
+    }
+    // join the waves
     if (lg == 0) s_m[wave][li] = st.m, s_l[wave][li] = st.l;
     if (li < cols) {
 #pragma unroll
-      for (int i = 0; i < S::V; ++i)
+      for (int e = 0; e < 4; ++e)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s_o[wave][li][(4 * lg + e) * S::V + i] = st.o[i][e];
+        for (int i = 0; i < S::V; i += 4)
+          *reinterpret_cast<pl_f32x4*>(&s_o[wave][li][(4 * lg + e) * S::V + i]) =
+              pl_f32x4{st.o[i][e], st.o[i + 1][e], st.o[i + 2][e], st.o[i + 3][e]};
     }
     __syncthreads();
     const bool complete = first_atom == 0 && last_atom == r.atoms;
-    const float v_scale = CT == PL_F8E4M3 ? a.v_scale[hk] : 1.f;
-    T* out = (T*)a.out + ((int64_t)row * a.heads + head0) * a.dim;
     float* part = a.parts + (2 * (int64_t)blockIdx.x + (at == from ? 0 : 1)) * part_floats(DP);
     for (int i = tid; i < cols * DP; i += kThreads) {
       const int c = i / DP, d = i % DP;
@@ -601,7 +704,7 @@ void launch_dim(const attend_args& a, dim3 grid, hipStream_t s) {
 
 template <int DT, int CT>
 int launch(const attend_args& a, int64_t atoms_most, hipStream_t s) {
-  const int per_cu = a.dim <= 128 ? 3 : DT == PL_F32 ? 1 : 2;
+  const int per_cu = a.dim <= 128 ? 3 : 2;
   const int64_t blocks = atoms_most < 256 * per_cu ? atoms_most : 256 * per_cu;
   const dim3 grid((unsigned)blocks);
   if (a.dim <= 64)
