@@ -59,6 +59,12 @@ struct shape {
   static constexpr int kKeyLoads = DP * kCsize / 64; // 16-byte loads of a lane per 16 keys
   static constexpr int V = DP / 16;                  // value elements of a lane per token
   static constexpr int kVWords = V * kCsize / 4;
+  // They come in pieces of at most 16 bytes, 16 lanes' pieces side by side.
+  static constexpr int kPiece = V * kCsize <= 16 ? V : 16 / kCsize;
+  static constexpr int kPieces = V / kPiece;
+  static __device__ __forceinline__ int value_at(int lane, int piece) {
+    return (piece * 16 + lane) * kPiece;
+  }
   static constexpr int kTokens = 4 * kSubs;          // tokens of a lane per tile
   static constexpr int kPerCu = DP <= 128 ? 3 : 2;  // workgroups of a CU
   // Queries in LDS where keys, values and outputs fill the registers.
@@ -125,21 +131,21 @@ __device__ __forceinline__ pl_buffer make_buffer(uintptr_t p, uint32_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(
       reinterpret_cast<void*>((uintptr_t)lo | (uintptr_t)hi << 32), 0, uniform((int)bytes), 0x00027000);
 }
-template <int N>
+// N words (1, 2 or 4) at lane_off + wave_off; STREAM marks lines as read once.
+template <int N, bool STREAM>
 __device__ __forceinline__ void load_words(pl_buffer r, uint32_t lane_off, uint32_t wave_off,
-                                           uint32_t (&w)[N]) {
-  if constexpr (N % 4 == 0) {
+                                           uint32_t* w) {
+  constexpr int kPolicy = STREAM ? 2 : 0;
+  if constexpr (N == 4) {
+    const auto x = __builtin_amdgcn_raw_buffer_load_b128(r, lane_off, wave_off, kPolicy);
 #pragma unroll
-    for (int i = 0; i < N / 4; ++i) {
-      const pl_u32x4 x = __builtin_bit_cast(
-          pl_u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, lane_off + 16 * i, wave_off, 0));
-      w[4 * i] = x.x, w[4 * i + 1] = x.y, w[4 * i + 2] = x.z, w[4 * i + 3] = x.w;
-    }
+    for (int i = 0; i < 4; ++i) w[i] = x[i];
   } else if constexpr (N == 2) {
-    const auto x = __builtin_amdgcn_raw_buffer_load_b64(r, lane_off, wave_off, 0);
+    const auto x = __builtin_amdgcn_raw_buffer_load_b64(r, lane_off, wave_off, kPolicy);
     w[0] = x[0], w[1] = x[1];
   } else {
-    w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, lane_off, wave_off, 0);
+    static_assert(N == 1, "loads of 4, 8 or 16 bytes");
+    w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, lane_off, wave_off, kPolicy);
   }
 }
 
@@ -539,8 +545,16 @@ __global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kPerCu)) void pl_page
       key_off[n] = li * w.key_slot + (FULL || d < a.dim ? d : 0) * S::kCsize;
     }
     // lanes past the head's end read its start: what they make is not stored
-    const uint32_t value_off =
-        4 * lg * w.value_slot + (FULL || li * S::V < a.dim ? li * S::V : 0) * S::kCsize;
+    uint32_t value_off[S::kPieces];
+#pragma unroll
+    for (int n = 0; n < S::kPieces; ++n) {
+      const int d = S::value_at(li, n);
+      value_off[n] = 4 * lg * w.value_slot + (FULL || d < a.dim ? d : 0) * S::kCsize;
+    }
+    // Lines are read once, and marking them so takes 256 rows of up to 1024
+    // tokens from 123 to 116 us.  Heads that are no whole lines share them
+    // between loads, which then fetch them twice (fp32, 80 elements: 40 -> 56 us).
+    constexpr bool kStream = FULL;
 
     // Keys of the next tile are asked for as soon as this tile's have gone into
     // the scores, values as soon as the wave is at the tile: one or the other
@@ -554,9 +568,11 @@ __global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kPerCu)) void pl_page
       for (int u = 0; u < S::kSubs; ++u) {
         const pl_buffer r = make_buffer(at.key[u], at.held[u] ? key_span : 0);
 #pragma unroll
-        for (int n = 0; n < S::kKeyLoads; ++n)
-          keys[u][n] = __builtin_bit_cast(
-              pl_u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, key_off[n], 0, 0));
+        for (int n = 0; n < S::kKeyLoads; ++n) {
+          uint32_t x[4];
+          load_words<4, kStream>(r, key_off[n], 0, x);
+          keys[u][n] = pl_u32x4{x[0], x[1], x[2], x[3]};
+        }
       }
     };
     int tile = r.base + first_atom * S::kAtom + (how.team == 1 ? 0 : wave * S::kTile);
@@ -583,7 +599,11 @@ __global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kPerCu)) void pl_page
       for (int u = 0; u < S::kSubs; ++u) {
         const pl_buffer b = make_buffer(place.value[u], place.held[u] ? value_span : 0);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) load_words(b, value_off, j * w.value_slot, v[4 * u + j]);
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int n = 0; n < S::kPieces; ++n)
+            load_words<S::kVWords / S::kPieces, kStream>(b, value_off[n], j * w.value_slot,
+                                                         v[4 * u + j] + n * (S::kVWords / S::kPieces));
       }
       const tile_place<S::kSubs> here = place;
       const int next = tile + step;
@@ -617,14 +637,16 @@ __global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kPerCu)) void pl_page
       if (li < cols) {
         const float f = st.m == -INFINITY ? 0.f : v_scale / st.l;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int d = (4 * lg + e) * S::V;
-          T y[S::V];
+        for (int e = 0; e < 4; ++e)
 #pragma unroll
-          for (int i = 0; i < S::V; ++i) y[i] = (T)(st.o[i][e] * f);
-          // out has the alignment of its elements alone
-          if (FULL || d < a.dim) __builtin_memcpy(out + li * a.dim + d, y, sizeof(y));
-        }
+          for (int n = 0; n < S::kPieces; ++n) {
+            const int d = S::value_at(4 * lg + e, n);
+            T y[S::kPiece];
+#pragma unroll
+            for (int i = 0; i < S::kPiece; ++i) y[i] = (T)(st.o[n * S::kPiece + i][e] * f);
+            // out has the alignment of its elements alone
+            if (FULL || d < a.dim) __builtin_memcpy(out + li * a.dim + d, y, sizeof(y));
+          }
       }
       at = pair_start + last_atom;
       continue;
@@ -636,7 +658,8 @@ __global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kPerCu)) void pl_page
       for (int e = 0; e < 4; ++e)
 #pragma unroll
         for (int i = 0; i < S::V; i += 4)
-          *reinterpret_cast<pl_f32x4*>(&s_o[wave][li][(4 * lg + e) * S::V + i]) =
+          *reinterpret_cast<pl_f32x4*>(
+              &s_o[wave][li][S::value_at(4 * lg + e, i / S::kPiece) + i % S::kPiece]) =
               pl_f32x4{st.o[i][e], st.o[i + 1][e], st.o[i + 2][e], st.o[i + 3][e]};
     }
     __syncthreads();
