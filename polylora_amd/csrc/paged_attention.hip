@@ -71,6 +71,7 @@ struct shape {
   static constexpr bool kQueryLds = DP == 256 || DT == PL_F32;
 };
 typedef pl_u32x4 __attribute__((may_alias)) shared_u32x4;
+typedef float pl_f32x2 __attribute__((ext_vector_type(2)));
 
 struct attend_args {
   const void* q;
@@ -353,6 +354,18 @@ __device__ __forceinline__ row_span span_of(const attend_args& a, int len) {
   return r;
 }
 
+// Four outputs, rounded (out has the alignment of its elements alone).
+template <typename T>
+__device__ __forceinline__ void store4(T* p, pl_f32x4 x) {
+  const T y[4] = {(T)x.x, (T)x.y, (T)x.z, (T)x.w};
+  __builtin_memcpy(p, y, sizeof(y));
+}
+// Two floats, 8-byte aligned, stored through to where every XCD sees them.
+__device__ __forceinline__ void store_agent(float* p, float x, float y) {
+  const uint64_t w = (uint64_t)__float_as_uint(y) << 32 | __float_as_uint(x);
+  __hip_atomic_store(reinterpret_cast<uint64_t*>(p), w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
 // Floats of one part: o [kCols][DP], then m and l of each column.
 constexpr int part_floats(int dp) { return kCols * dp + 2 * kCols; }
 
@@ -380,7 +393,8 @@ __device__ __forceinline__ void join_parts(const float* parts, int slot0, int sl
         const int w = min(w0 + j * lanes, n - 1);  // the last again, with no weight
         const float* p = parts + (int64_t)(w ? slot + 2 * w : slot0) * part_floats(DP);
         x[j] = *reinterpret_cast<const pl_f32x4*>(p + c * DP + d);
-        pm[j] = p[kCols * DP + 2 * c], pl[j] = p[kCols * DP + 2 * c + 1];
+        const pl_f32x2 ml = *reinterpret_cast<const pl_f32x2*>(p + kCols * DP + 2 * c);
+        pm[j] = ml.x, pl[j] = ml.y;
       }
       float top = m;
 #pragma unroll
@@ -418,15 +432,18 @@ __device__ __forceinline__ void join_parts(const float* parts, int slot0, int sl
 
 // How the batch's atoms are dealt out, from their number, the (row, key head)
 // pairs and the longest pair.  Times are in tiles of a wave (one after the
-// other, about as long as it waits for one): starting and ending a pair costs
-// a team of waves about kStart of them and joining parts about kJoin.
+// other, about as long as it waits for one), of which a team of waves takes
+// TILES for an atom: starting and ending a pair costs a team about kStart of
+// them and joining parts about kJoin.
 struct deal {
   int team;    // waves on a pair: kWaves, or 1 (no waves to join, no barrier)
   bool whole;  // pairs go whole to the run that their first atom falls in
 };
 constexpr float kStart = 4.f, kJoin = 5.f;
+template <int TILES>
 __device__ __forceinline__ deal choose_deal(int total, int pairs, int longest) {
-  const float w = (float)gridDim.x, n = (float)total, p = (float)pairs, top = (float)longest;
+  const float w = (float)gridDim.x, p = (float)pairs;
+  const float n = (float)total * TILES, top = (float)longest * TILES;
   const float alone = kWaves * top * w + n + w + p / kWaves;
   const float team = top * w + n + kStart * (w + p);
   const float split = w + n + kStart * (w + p) + kJoin * w;
@@ -450,12 +467,12 @@ __global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kPerCu)) void pl_page
 
   // Each wave works out the deal for itself: 64 rows to a look, no barrier.
   constexpr int kLooks = 4;  // that stay in registers
-  int atoms[kLooks], total = 0, longest = 0;
+  int atoms[kLooks], lens[kLooks], total = 0, longest = 0;
 #pragma unroll
   for (int k = 0; k < kLooks; ++k) {
     const int b = k * 64 + lane;
-    const int len = b < a.rows ? a.lens[b] : 0;
-    atoms[k] = b < a.rows ? span_of<S::kAtom>(a, len).atoms : 0;
+    lens[k] = b < a.rows ? a.lens[b] : 0;
+    atoms[k] = b < a.rows ? span_of<S::kAtom>(a, lens[k]).atoms : 0;
     total += atoms[k], longest = max(longest, atoms[k]);
   }
   for (int b = kLooks * 64 + lane; b < a.rows; b += 64) {
@@ -464,20 +481,26 @@ __global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kPerCu)) void pl_page
   }
   total = __builtin_amdgcn_readlane(scan_sum(total), 63) * per_row;
   longest = __builtin_amdgcn_readlane(scan_max(longest), 63);
-  const deal how = choose_deal(total, a.rows * per_row, longest);
+  const deal how = choose_deal<S::kAtom / (kWaves * S::kTile)>(total, a.rows * per_row, longest);
   const int workers = (int)gridDim.x * kWaves / how.team;
   const int worker = how.team == 1 ? (int)blockIdx.x * kWaves + wave : (int)blockIdx.x;
   const int per = (total + workers - 1) / workers;
   const int from = (int)min((int64_t)worker * per, (int64_t)total), to = min(total - per, from) + per;
   if (from >= total) return;
   // the row of its first atom: the first whose atoms up to and with it pass `from`
-  int row = 0, row_start = 0;
+  int row = 0, row_start = 0, row_len = 0;
   for (int b0 = 0;; b0 += 64) {
     const int b = b0 + lane;
-    int n = atoms[0];
+    int n = atoms[0], len = lens[0];
 #pragma unroll
-    for (int k = 1; k < kLooks; ++k) n = b0 == k * 64 ? atoms[k] : n;
-    if (b0 >= kLooks * 64) n = b < a.rows ? span_of<S::kAtom>(a, a.lens[b]).atoms : 0;
+    for (int k = 1; k < kLooks; ++k) {
+      n = b0 == k * 64 ? atoms[k] : n;
+      len = b0 == k * 64 ? lens[k] : len;
+    }
+    if (b0 >= kLooks * 64) {
+      len = b < a.rows ? a.lens[b] : 0;
+      n = b < a.rows ? span_of<S::kAtom>(a, len).atoms : 0;
+    }
     n *= per_row;
     const int upto = scan_sum(n) + row_start;
     const uint64_t past = __ballot(upto > from);
@@ -485,6 +508,7 @@ __global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kPerCu)) void pl_page
       const int hit = past ? __ffsll((long long)past) - 1 : 63;
       row = b0 + hit;
       row_start = __builtin_amdgcn_readlane(upto - n, hit);
+      row_len = __builtin_amdgcn_readlane(len, hit);
       break;
     }
     row_start = __builtin_amdgcn_readlane(upto, 63);
@@ -494,7 +518,7 @@ __global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kPerCu)) void pl_page
   int at = from;
   bool skip = how.whole;  // to the first pair that starts in the run
   while (at < to) {
-    const row_span r = span_of<S::kAtom>(a, as_scalar(a.lens)[row]);
+    const row_span r = span_of<S::kAtom>(a, row_len);
     int in_row = at - row_start;
     if (skip) {
       in_row = (in_row + r.atoms - 1) / r.atoms * r.atoms;
@@ -504,7 +528,7 @@ __global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kPerCu)) void pl_page
     }
     if (in_row >= r.atoms * per_row) {
       row_start += r.atoms * per_row;
-      ++row;
+      row_len = as_scalar(a.lens)[++row];
       continue;
     }
     const int combo = in_row / r.atoms;
@@ -665,25 +689,25 @@ __global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kPerCu)) void pl_page
     __syncthreads();
     const bool complete = first_atom == 0 && last_atom == r.atoms;
     float* part = a.parts + (2 * (int64_t)blockIdx.x + (at == from ? 0 : 1)) * part_floats(DP);
-    for (int i = tid; i < cols * DP; i += kThreads) {
-      const int c = i / DP, d = i % DP;
-      float m = -INFINITY, l = 0.f, o = 0.f;
+    for (int i = tid; i < cols * (DP / 4); i += kThreads) {
+      const int c = i / (DP / 4), d = i % (DP / 4) * 4;
+      float m = -INFINITY, l = 0.f;
+      pl_f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) m = fmaxf(m, s_m[w][c]);
+      const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) {
-        const float f = m == -INFINITY ? 0.f : exp2_fast(s_m[w][c] - m);
-        l += f * s_l[w][c], o += f * s_o[w][c][d];
+        const float f = exp2_fast(s_m[w][c] - ref);
+        l += f * s_l[w][c];
+        o += f * *reinterpret_cast<const pl_f32x4*>(&s_o[w][c][d]);
       }
       if (complete) {
-        if (d < a.dim) out[c * a.dim + d] = (T)(m == -INFINITY ? 0.f : o / l * v_scale);
+        if (FULL || d < a.dim) store4(out + c * a.dim + d, o * (m == -INFINITY ? 0.f : v_scale / l));
       } else {
-        __hip_atomic_store(part + i, o, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (d == 0) {
-          __hip_atomic_store(part + kCols * DP + 2 * c, m, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-          __hip_atomic_store(part + kCols * DP + 2 * c + 1, l, __ATOMIC_RELAXED,
-                             __HIP_MEMORY_SCOPE_AGENT);
-        }
+        store_agent(part + c * DP + d, o.x, o.y);
+        store_agent(part + c * DP + d + 2, o.z, o.w);
+        if (d == 0) store_agent(part + kCols * DP + 2 * c, m, l);
       }
     }
     if (!complete) {
@@ -706,9 +730,7 @@ __global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kPerCu)) void pl_page
         const int slot0 = 2 * w0 + (w0 * per == pair_start ? 0 : 1);
         join_parts<DP>(a.parts, slot0, 2 * w0, w1 - w0 + 1, cols, &s_o[0][0][0],
                        [&](int c, int d, pl_f32x4 o) {
-#pragma unroll
-                         for (int e = 0; e < 4; ++e)
-                           if (FULL || d + e < a.dim) out[c * a.dim + d + e] = (T)(o[e] * v_scale);
+                         if (FULL || d < a.dim) store4(out + c * a.dim + d, o * v_scale);
                        });
       }
     }
