@@ -1,14 +1,15 @@
 // Penalties of repeated tokens, biases and grammar masks on logits.
 #include "pl_common.h"
 
-// One pass over the logits, 8 at a time: memory bounds it (each is read once
-// and written once).  A workgroup takes a slice of one row's vocabulary.  What
+// One pass over the logits, 4 at a time (16 bytes of fp32 output, so that a
+// wave's stores fill whole lines): memory bounds it (each is read once and
+// written once).  A workgroup takes a slice of one row's vocabulary.  What
 // is particular to single tokens lies in a table of one LDS word per entry of
 // the slice, which the pass reads beside the logits: the workgroup first
 // counts the row's history into it (the tokens that fall into the slice;
 // integer atomics, the same result in any order) and puts the places of
 // biases there.  The history is read again for each slice, from L2, so slices
-// grow with the batch (slice_of).
+// are larger for a long one.
 namespace {
 
 // A word of the slice's table: how often the token was generated, the place
@@ -16,9 +17,8 @@ namespace {
 constexpr uint32_t kCountMask = (1u << 20) - 1, kBiasShift = 20, kBiasMask = 0x7ff;
 constexpr uint32_t kSeen = 1u << 31;
 constexpr int kHistoryMax = (int)kCountMask, kBiasMax = (int)kBiasMask;
-constexpr int kVec = 8;     // logits of a thread's load
-constexpr int kPasses = 2;  // loads of a thread: its share of the slice
-constexpr int kWide = 1 << 22;  // logits from which slices are twice as large
+constexpr int kVec = 4;     // logits of a thread's load
+constexpr int kPasses = 4;  // loads of a thread: its share of the slice
 
 struct logits_args {
   const void* logits;
@@ -56,7 +56,7 @@ __global__ __launch_bounds__(THREADS) void pl_adjust_logits_kernel(logits_args a
   typedef typename pl_traits<OT>::T O;
   constexpr int kSlice = THREADS * kVec * kPasses;
   __shared__ __attribute__((aligned(16))) uint32_t table[kSlice];
-  extern __shared__ uint32_t dynamic[];  // the slice's biases: ids, values, sums
+  extern __shared__ __attribute__((aligned(16))) uint32_t dynamic[];  // the slice's biases: ids, values, sums
   __shared__ int s_biases;
   const int b = (int)(blockIdx.x / a.slices), tid = (int)threadIdx.x;
   const int lo = (int)(blockIdx.x % a.slices) * kSlice, hi = min(lo + kSlice, a.vocab);
@@ -64,27 +64,73 @@ __global__ __launch_bounds__(THREADS) void pl_adjust_logits_kernel(logits_args a
   O* out = (O*)a.out + b * a.ld_out;
   // rows have the alignment of their elements alone
   T x[kPasses][kVec];
+  uint32_t mask[kPasses];
+  const uint8_t* allowed = reinterpret_cast<const uint8_t*>(a.allowed + b * a.ld_allowed);
 #pragma unroll
   for (int k = 0; k < kPasses; ++k) {
     const int v = lo + (k * THREADS + tid) * kVec;
     if (v + kVec <= hi) __builtin_memcpy(x[k], in + v, sizeof(x[k]));
+    mask[k] = a.allowed && v < hi ? allowed[v >> 3] : 0xff;
   }
+  // kBatch tokens of the history, THREADS apart, from i on (the last one again
+  // past its end).
+  constexpr int kBatch = 4;
+  int64_t id[kBatch];
+  auto look = [&](int i, int end) {
+    if (a.wide_tokens) {
+      const int64_t* p = (const int64_t*)a.tokens + b * a.ld_tokens;
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) id[j] = p[min(i + j * THREADS, end - 1)];
+    } else {
+      const int32_t* p = (const int32_t*)a.tokens + b * a.ld_tokens;
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) id[j] = p[min(i + j * THREADS, end - 1)];
+    }
+  };
+  // The first of them are asked for beside their number: the list is there
+  // whole, and what lies beyond `lens` is not counted.
+  if (a.tokens && a.history > 0) look(tid, a.history);
   const int n = a.tokens ? min(max(a.lens[b], 0), a.history) : 0;
-  const bool special = n > 0 || a.n_bias > 0;
+  const int prompt = a.prompt_lens ? a.prompt_lens[b] : 0;
+  const bool special = a.tokens || a.n_bias > 0;
+  const int room = (a.n_bias + 3) & ~3;
+  int* ids = reinterpret_cast<int*>(dynamic);
+  float* values = reinterpret_cast<float*>(dynamic + room);
+  float* sums = reinterpret_cast<float*>(dynamic + 2 * room);
   if (special) {
     for (int i = tid; i < kSlice / 4; i += THREADS)
       reinterpret_cast<pl_u32x4*>(table)[i] = pl_u32x4{0, 0, 0, 0};
-    __syncthreads();
-    const int prompt = a.prompt_lens ? a.prompt_lens[b] : 0;
-    constexpr int kBatch = 4;
-    for (int i0 = tid; i0 < n; i0 += kBatch * THREADS) {
-      int64_t id[kBatch];
+    if (a.n_bias > 0 && tid < 64) {
+      // one wave puts the slice's biases together in the list's order
+      constexpr int kLook = 4;  // 64 entries each, asked for at once
+      const int32_t* list = a.bias_ids + b * a.ld_bias;
+      const float* list_values = a.bias_values + b * a.ld_bias;
+      int count = 0;
+      for (int j0 = 0; j0 < a.n_bias; j0 += 64 * kLook) {
+        int entry[kLook];
+        float value[kLook];
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        const int i = min(i0 + j * THREADS, n - 1);
-        id[j] = a.wide_tokens ? ((const int64_t*)a.tokens)[b * a.ld_tokens + i]
-                              : ((const int32_t*)a.tokens)[b * a.ld_tokens + i];
+        for (int k = 0; k < kLook; ++k) {
+          const int j = j0 + 64 * k + tid;
+          entry[k] = j < a.n_bias ? list[j] : -1;
+          value[k] = j < a.n_bias ? list_values[j] : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < kLook; ++k) {
+          const bool mine = entry[k] >= lo && entry[k] < hi;
+          const uint64_t all = __ballot(mine);
+          if (mine) {
+            const int at = count + __popcll(all & ((1ull << tid) - 1));
+            ids[at] = entry[k], values[at] = value[k];
+          }
+          count += __popcll(all);
+        }
       }
+      if (tid == 0) s_biases = count;
+    }
+    __syncthreads();
+    for (int i0 = tid; i0 < n; i0 += kBatch * THREADS) {
+      if (i0 != tid) look(i0, n);
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
         const int i = i0 + j * THREADS;
@@ -93,81 +139,66 @@ __global__ __launch_bounds__(THREADS) void pl_adjust_logits_kernel(logits_args a
         atomicOr(&table[id[j] - lo], kSeen);
       }
     }
-  }
-  int* ids = reinterpret_cast<int*>(dynamic);
-  float* values = reinterpret_cast<float*>(dynamic + a.n_bias);
-  float* sums = reinterpret_cast<float*>(dynamic + 2 * a.n_bias);
-  if (a.n_bias > 0) {
-    // one wave puts the slice's biases together in the list's order
-    if (tid < 64) {
-      const int32_t* list = a.bias_ids + b * a.ld_bias;
-      const float* list_values = a.bias_values + b * a.ld_bias;
-      int count = 0;
-      for (int j0 = 0; j0 < a.n_bias; j0 += 64) {
-        const int j = j0 + tid;
-        const int id = j < a.n_bias ? list[j] : -1;
-        const float value = j < a.n_bias ? list_values[j] : 0.f;
-        const bool mine = id >= lo && id < hi;
-        const uint64_t all = __ballot(mine);
-        if (mine) {
-          const int at = count + __popcll(all & ((1ull << tid) - 1));
-          ids[at] = id, values[at] = value;
+    if (a.n_bias > 0) {
+      // an id's first entry sums all of them, in order; four to a look
+      const int count = s_biases;
+      for (int j = tid; j < count; j += THREADS) {
+        const int id0 = ids[j];
+        bool first = true;
+        float sum = 0.f;
+        for (int i = 0; i < count; i += 4) {
+          int look[4];
+          float add[4];
+          __builtin_memcpy(look, __builtin_assume_aligned(ids + i, 16), 16);
+          __builtin_memcpy(add, __builtin_assume_aligned(values + i, 16), 16);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const bool same = i + e < count && look[e] == id0;
+            first = first && !(same && i + e < j);
+            sum += same ? add[e] : 0.f;
+          }
         }
-        count += __popcll(all);
+        sums[j] = sum;
+        if (first) atomicOr(&table[id0 - lo], (uint32_t)(j + 1) << kBiasShift);
       }
-      if (tid == 0) s_biases = count;
     }
     __syncthreads();
-    // an id's first entry sums all of them
-    const int count = s_biases;
-    for (int j = tid; j < count; j += THREADS) {
-      const int id = ids[j];
-      bool first = true;
-      float sum = 0.f;
-      for (int i = 0; i < count; ++i) {
-        const bool same = ids[i] == id;
-        first = first && !(same && i < j);
-        sum += same ? values[i] : 0.f;
-      }
-      sums[j] = sum;
-      if (first) atomicOr(&table[id - lo], (uint32_t)(j + 1) << kBiasShift);
-    }
   }
-  if (special) __syncthreads();
   penalties pen;
   pen.r = a.repetition ? a.repetition[b] : 1.f;
   pen.f = a.frequency ? a.frequency[b] : 0.f;
   pen.p = a.presence ? a.presence[b] : 0.f;
-  const uint8_t* allowed = reinterpret_cast<const uint8_t*>(a.allowed + b * a.ld_allowed);
 #pragma unroll
   for (int k = 0; k < kPasses; ++k) {
     const int v = lo + (k * THREADS + tid) * kVec;
     if (v >= hi) break;
-    const uint32_t mask = a.allowed ? allowed[v >> 3] : 0xff;
+    const uint32_t may = mask[k] >> (v & 4);
     uint32_t w[kVec] = {};
     if (special) __builtin_memcpy(w, __builtin_assume_aligned(&table[v - lo], 16), sizeof(w));
-    O y[kVec];
     if (v + kVec <= hi) {
+      typedef O OV __attribute__((ext_vector_type(kVec), aligned(sizeof(O))));
+      OV y;
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) y[e] = (O)adjust((float)x[k][e], w[e], pen, sums, mask >> e & 1);
-      __builtin_memcpy(out + v, y, sizeof(y));
+      for (int e = 0; e < kVec; ++e) y[e] = (O)adjust((float)x[k][e], w[e], pen, sums, may >> e & 1);
+      // past the caches: the output is read by another launch, whole (256 rows: 41 -> 31 us)
+      __builtin_nontemporal_store(y, reinterpret_cast<OV*>(out + v));
     } else {
       for (int e = 0; v + e < hi; ++e)
         out[v + e] = (O)adjust((float)in[v + e], special ? table[v - lo + e] : 0u, pen, sums,
-                               mask >> e & 1);
+                               may >> e & 1);
     }
   }
 }
 
-// Threads of a workgroup, each with kVec * kPasses logits.  Larger slices read
-// the history less often, smaller ones put a small batch on more CUs.
-int threads_of(int64_t logits) {
-  return logits >= (int64_t)kWide ? 512 : 256;
-}
+// Threads of a workgroup, each with kVec * kPasses logits.  Small slices put a
+// small batch on more CUs and cost nothing while the history is short; a long
+// one is read less often by large slices (32 rows, 8000 tokens: 12.0 -> 9.9
+// us; 256 rows, 2000 tokens: 41 us either way).
+constexpr int kLongHistory = 4096;
 
 template <int DT, int OT>
 int launch(logits_args a, hipStream_t s) {
-  const int threads = threads_of((int64_t)a.rows * a.vocab);
+  const int threads = a.history > kLongHistory ? 1024 : 256;
   const int slice = threads * kVec * kPasses;
   a.slices = (a.vocab + slice - 1) / slice;
   const int64_t blocks = (int64_t)a.rows * a.slices;
@@ -176,9 +207,9 @@ int launch(logits_args a, hipStream_t s) {
     return PL_ERR_LIMIT;
   }
   const dim3 grid((unsigned)blocks);
-  const size_t lds = (size_t)a.n_bias * 12;
-  if (threads == 512)
-    pl_adjust_logits_kernel<DT, OT, 512><<<grid, 512, lds, s>>>(a);
+  const size_t lds = (size_t)((a.n_bias + 3) & ~3) * 12;
+  if (threads == 1024)
+    pl_adjust_logits_kernel<DT, OT, 1024><<<grid, 1024, lds, s>>>(a);
   else
     pl_adjust_logits_kernel<DT, OT, 256><<<grid, 256, lds, s>>>(a);
   return pl_launch_status("pl_adjust_logits");

@@ -109,7 +109,7 @@ __device__ __forceinline__ void store_vec(void* p, int64_t at, const float (&x)[
     TV v;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) v[e] = (T)x[e];
-    *reinterpret_cast<TV*>(q) = v;
+    __builtin_nontemporal_store(v, reinterpret_cast<TV*>(q));
   }
 }
 template <int DT, int CT, int VEC>

@@ -77,6 +77,14 @@ def test_matches_the_plain_form(gpu, dtype, rows, vocab, history, bias, grammar,
     assert torch.equal(check(gpu, a), wide)
 
 
+def test_the_longest_lists(gpu):
+    """A history beyond one look of a workgroup and a bias list at its limit, most of it in one slice."""
+    gen = torch.Generator().manual_seed(6)
+    a = build(gen, 2, 20000, torch.bfloat16, 9000, 2047, True)
+    a["bias_ids"][1] = a["bias_ids"][1] % 600
+    check(gpu, a)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_in_place_rows_of_any_stride(gpu, dtype):
     gen = torch.Generator().manual_seed(1)
