@@ -64,6 +64,12 @@ namespace {
 constexpr int kThreads = 256;
 // Workgroups that fill the GPU (eight on each of 256 CUs).
 constexpr int kFullGrid = 2048;
+// Workgroups up to which a token's heads are shared out.
+constexpr int kFewTokens = 512;
+// Outputs above this pass by the caches, where the next launch, on other XCDs,
+// would hardly find them (32 x 1024 prompt tokens 135 -> 127 us, 8 x 64 5.6 ->
+// 4.9; 256 single tokens are not worth it, 4.8 -> 5.0).
+constexpr int64_t kCacheBytes = 4 << 20;
 
 struct append_args {
   const void *q, *k, *v;
@@ -78,9 +84,11 @@ struct append_args {
   int32_t turns, units, group;  // places of a head that turn, all of them, tokens of a workgroup
 };
 
-// One value as an e4m3 byte: over the scale, saturated (NaN stays NaN).
-__device__ __forceinline__ float to_e4m3_range(float x, float scale) {
-  const float y = x / scale;
+// A value over the scale (times its reciprocal, taken once for a head: within
+// one fp32 rounding of the quotient, 2^-20 of an e4m3 step), saturated (NaN
+// stays NaN).
+__device__ __forceinline__ float to_e4m3_range(float x, float per_scale) {
+  const float y = x * per_scale;
   return y != y ? y : fminf(fmaxf(y, -kE4M3Max), kE4M3Max);
 }
 
@@ -98,7 +106,8 @@ __device__ __forceinline__ void load_vec(const void* p, int64_t at, float (&x)[V
     for (int e = 0; e < VEC; ++e) x[e] = (float)v[e];
   }
 }
-template <int DT, int VEC>
+// STREAM: past the caches, for outputs larger than they are.
+template <int DT, int VEC, bool STREAM>
 __device__ __forceinline__ void store_vec(void* p, int64_t at, const float (&x)[VEC]) {
   typedef typename pl_traits<DT>::T T;
   typedef T TV __attribute__((ext_vector_type(VEC)));
@@ -109,35 +118,39 @@ __device__ __forceinline__ void store_vec(void* p, int64_t at, const float (&x)[
     TV v;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) v[e] = (T)x[e];
-    __builtin_nontemporal_store(v, reinterpret_cast<TV*>(q));
+    if constexpr (STREAM)
+      __builtin_nontemporal_store(v, reinterpret_cast<TV*>(q));
+    else
+      *reinterpret_cast<TV*>(q) = v;
   }
 }
-template <int DT, int CT, int VEC>
-__device__ __forceinline__ void store_cache(void* p, int64_t at, const float (&x)[VEC], float scale) {
+template <int DT, int CT, int VEC, bool STREAM>
+__device__ __forceinline__ void store_cache(void* p, int64_t at, const float (&x)[VEC], float per_scale) {
   if constexpr (CT == PL_F8E4M3) {
     uint8_t* q = (uint8_t*)p + at;
     uint32_t w[(VEC + 3) / 4] = {};
 #pragma unroll
     for (int e = 0; e < VEC; e += 2) {
-      const float lo = to_e4m3_range(x[e], scale);
-      const float hi = e + 1 < VEC ? to_e4m3_range(x[e + 1], scale) : lo;
+      const float lo = to_e4m3_range(x[e], per_scale);
+      const float hi = e + 1 < VEC ? to_e4m3_range(x[e + 1], per_scale) : lo;
       w[e / 4] = e % 4 ? __builtin_amdgcn_cvt_pk_fp8_f32(lo, hi, (int)w[e / 4], true)
                        : __builtin_amdgcn_cvt_pk_fp8_f32(lo, hi, (int)w[e / 4], false);
     }
     __builtin_memcpy(__builtin_assume_aligned(q, VEC), w, VEC);
   } else {
-    store_vec<DT, VEC>(p, at, x);
+    store_vec<DT, VEC, STREAM>(p, at, x);
   }
 }
 
-// A workgroup takes `group` tokens.  A thread keeps one place of the head,
+// A workgroup takes `group` tokens (or one of gridDim.y shares of them).  A
+// thread keeps one place of the head,
 // VEC elements and, split in halves, the VEC that turn against them, and
 // walks the token's query and key heads with it, so that it reads its part of
 // cos and sin once; the threads then copy the values.  The tokens' lengths,
 // pages and angles take two dependent reads, the second beside the heads'.
 //
 // Bound by memory: every element of q, k and v is read and written once.
-template <int DT, int CT, int VEC>
+template <int DT, int CT, int VEC, bool STREAM>
 __global__ __launch_bounds__(kThreads) void pl_rope_append_kernel(append_args a) {
   const int tid = (int)threadIdx.x;
   // threads of a token, and this thread's
@@ -176,7 +189,8 @@ __global__ __launch_bounds__(kThreads) void pl_rope_append_kernel(append_args a)
         __builtin_memcpy(s, a.sin + i, VEC * sizeof(float));
       }
     }
-    for (int h = lane; h < a.heads + a.kv_heads; h += lanes) {
+    const int step = lanes * (int)gridDim.y;
+    for (int h = (int)blockIdx.y * lanes + lane; h < a.heads + a.kv_heads; h += step) {
       const bool is_q = h < a.heads;
       const int hh = is_q ? h : h - a.heads;
       float x[VEC], y[VEC];
@@ -207,26 +221,39 @@ __global__ __launch_bounds__(kThreads) void pl_rope_append_kernel(append_args a)
       void* dense = is_q ? a.q_out : a.k_out;
       if (dense) {
         const int64_t at = (token * (is_q ? a.heads : a.kv_heads) + hh) * a.dim;
-        store_vec<DT, VEC>(dense, at + d, x);
-        if (split) store_vec<DT, VEC>(dense, at + d2, y);
+        store_vec<DT, VEC, STREAM>(dense, at + d, x);
+        if (split) store_vec<DT, VEC, STREAM>(dense, at + d2, y);
       }
       if (!is_q && live) {
         const int64_t at = page * a.key.s_page + hh * a.key.s_head + slot * a.key.s_slot;
-        const float scale = CT == PL_F8E4M3 ? a.k_scale[hh] : 1.f;
-        store_cache<DT, CT, VEC>(a.key.p, at + d, x, scale);
-        if (split) store_cache<DT, CT, VEC>(a.key.p, at + d2, y, scale);
+        const float per_scale = CT == PL_F8E4M3 ? 1.f / a.k_scale[hh] : 1.f;
+        store_cache<DT, CT, VEC, STREAM>(a.key.p, at + d, x, per_scale);
+        if (split) store_cache<DT, CT, VEC, STREAM>(a.key.p, at + d2, y, per_scale);
       }
     }
   }
   if (!live) return;
   const int places = a.dim / VEC;
-  for (int i = rank; i < a.kv_heads * places; i += part) {
+  for (int i = (int)blockIdx.y * part + rank; i < a.kv_heads * places; i += part * (int)gridDim.y) {
     const int hh = i / places, d = (i - hh * places) * VEC;
     float x[VEC];
     load_vec<DT, VEC>(a.v, b * a.vs[0] + t * a.vs[1] + hh * a.vs[2] + d, x);
-    store_cache<DT, CT, VEC>(a.value.p,
+    store_cache<DT, CT, VEC, STREAM>(a.value.p,
                              page * a.value.s_page + hh * a.value.s_head + slot * a.value.s_slot + d,
-                             x, CT == PL_F8E4M3 ? a.v_scale[hh] : 1.f);
+                             x, CT == PL_F8E4M3 ? 1.f / a.v_scale[hh] : 1.f);
+  }
+}
+
+template <int DT, int CT, bool STREAM>
+void launch_vec(const append_args& a, int vec, dim3 grid, hipStream_t s) {
+  if (vec == 8) {
+    if constexpr (DT != PL_F32) pl_rope_append_kernel<DT, CT, 8, STREAM><<<grid, kThreads, 0, s>>>(a);
+  } else if (vec == 4) {
+    pl_rope_append_kernel<DT, CT, 4, STREAM><<<grid, kThreads, 0, s>>>(a);
+  } else if (vec == 2) {
+    pl_rope_append_kernel<DT, CT, 2, STREAM><<<grid, kThreads, 0, s>>>(a);
+  } else {
+    pl_rope_append_kernel<DT, CT, 1, STREAM><<<grid, kThreads, 0, s>>>(a);
   }
 }
 
@@ -241,16 +268,16 @@ int launch(append_args a, int vec, hipStream_t s) {
   a.group = 1;
   while (a.group < 4 && tokens / (2 * a.group) >= kFullGrid && kThreads / (2 * a.group) >= a.units)
     a.group *= 2;
-  const dim3 grid((unsigned)((tokens + a.group - 1) / a.group));
-  if (vec == 8) {
-    if constexpr (DT != PL_F32) pl_rope_append_kernel<DT, CT, 8><<<grid, kThreads, 0, s>>>(a);
-  } else if (vec == 4) {
-    pl_rope_append_kernel<DT, CT, 4><<<grid, kThreads, 0, s>>>(a);
-  } else if (vec == 2) {
-    pl_rope_append_kernel<DT, CT, 2><<<grid, kThreads, 0, s>>>(a);
-  } else {
-    pl_rope_append_kernel<DT, CT, 1><<<grid, kThreads, 0, s>>>(a);
-  }
+  // few tokens: as many workgroups to each as have a head for every thread
+  // (2 tokens of 64 + 8 heads of 256: 8.5 -> 4.1 us)
+  int shares = 1;
+  while (tokens * shares < kFewTokens && (a.heads + a.kv_heads) * a.units > kThreads * shares) shares *= 2;
+  const dim3 grid((unsigned)((tokens + a.group - 1) / a.group), (unsigned)shares);
+  const int64_t bytes = tokens * (a.heads + 2 * a.kv_heads) * a.dim * pl_elem_size(DT);
+  if (bytes > kCacheBytes)
+    launch_vec<DT, CT, true>(a, vec, grid, s);
+  else
+    launch_vec<DT, CT, false>(a, vec, grid, s);
   return pl_launch_status("pl_rope_append");
 }
 
