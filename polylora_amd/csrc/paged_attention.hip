@@ -451,7 +451,7 @@ __device__ __forceinline__ deal choose_deal(int total, int pairs, int longest) {
   return {kWaves, team < split};
 }
 
-template <int DT, int CT, int DP, bool FULL>
+template <int DT, int CT, int DP, bool FULL, bool STREAM>
 __global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kPerCu)) void pl_paged_attention_kernel(
     attend_args a) {
   typedef shape<DT, CT, DP> S;
@@ -469,10 +469,11 @@ __global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kPerCu)) void pl_page
   constexpr int kLooks = 4;  // that stay in registers
   int atoms[kLooks], lens[kLooks], total = 0, longest = 0;
 #pragma unroll
+  for (int k = 0; k < kLooks; ++k) lens[k] = a.lens[min(k * 64 + lane, a.rows - 1)];
+#pragma unroll
   for (int k = 0; k < kLooks; ++k) {
-    const int b = k * 64 + lane;
-    lens[k] = b < a.rows ? a.lens[b] : 0;
-    atoms[k] = b < a.rows ? span_of<S::kAtom>(a, lens[k]).atoms : 0;
+    const int n = span_of<S::kAtom>(a, lens[k]).atoms;
+    atoms[k] = k * 64 + lane < a.rows ? n : 0;
     total += atoms[k], longest = max(longest, atoms[k]);
   }
   for (int b = kLooks * 64 + lane; b < a.rows; b += 64) {
@@ -575,11 +576,6 @@ __global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kPerCu)) void pl_page
       const int d = S::value_at(li, n);
       value_off[n] = 4 * lg * w.value_slot + (FULL || d < a.dim ? d : 0) * S::kCsize;
     }
-    // Lines are read once, and marking them so takes 256 rows of up to 1024
-    // tokens from 123 to 116 us.  Heads that are no whole lines share them
-    // between loads, which then fetch them twice (fp32, 80 elements: 40 -> 56 us).
-    constexpr bool kStream = FULL;
-
     // Keys of the next tile are asked for as soon as this tile's have gone into
     // the scores, values as soon as the wave is at the tile: one or the other
     // is in flight all the time, in no more registers than one tile takes.
@@ -594,7 +590,7 @@ __global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kPerCu)) void pl_page
 #pragma unroll
         for (int n = 0; n < S::kKeyLoads; ++n) {
           uint32_t x[4];
-          load_words<4, kStream>(r, key_off[n], 0, x);
+          load_words<4, STREAM>(r, key_off[n], 0, x);
           keys[u][n] = pl_u32x4{x[0], x[1], x[2], x[3]};
         }
       }
@@ -626,7 +622,7 @@ __global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kPerCu)) void pl_page
         for (int j = 0; j < 4; ++j)
 #pragma unroll
           for (int n = 0; n < S::kPieces; ++n)
-            load_words<S::kVWords / S::kPieces, kStream>(b, value_off[n], j * w.value_slot,
+            load_words<S::kVWords / S::kPieces, STREAM>(b, value_off[n], j * w.value_slot,
                                                          v[4 * u + j] + n * (S::kVWords / S::kPieces));
       }
       const tile_place<S::kSubs> here = place;
@@ -739,25 +735,36 @@ __global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kPerCu)) void pl_page
   }
 }
 
+// Lines read once are marked so where a pool of pages is too large to stay in
+// the GPU's last cache (256 rows of up to 1024 tokens 129 -> 120 us; 256 rows of
+// up to 128, 134 MB, 20.9 -> 23.1).  Not where a line is read again: by the next
+// 16 query heads of a key head (204 rows, 20 for each 120 -> 144 us), or,
+// in heads that are no whole lines, by another load (fp32, 80 elements: 40 -> 56).
+constexpr int64_t kLastCache = 256 << 20;
+
 template <int DT, int CT, int DP>
-void launch_dim(const attend_args& a, dim3 grid, hipStream_t s) {
-  if (a.dim == DP)
-    pl_paged_attention_kernel<DT, CT, DP, true><<<grid, kThreads, 0, s>>>(a);
+void launch_dim(const attend_args& a, int64_t pool_bytes, dim3 grid, hipStream_t s) {
+  if (a.dim != DP)
+    pl_paged_attention_kernel<DT, CT, DP, false, false><<<grid, kThreads, 0, s>>>(a);
+  else if (pool_bytes > kLastCache && a.col_tiles == 1)
+    pl_paged_attention_kernel<DT, CT, DP, true, true><<<grid, kThreads, 0, s>>>(a);
   else
-    pl_paged_attention_kernel<DT, CT, DP, false><<<grid, kThreads, 0, s>>>(a);
+    pl_paged_attention_kernel<DT, CT, DP, true, false><<<grid, kThreads, 0, s>>>(a);
 }
 
 template <int DT, int CT>
 int launch(const attend_args& a, int64_t atoms_most, hipStream_t s) {
+  const int64_t pool_bytes = 2ll * a.table.num_pages * ((int64_t)a.kv_heads * a.dim << a.table.page_shift) *
+                             pl_cache_elem_size(CT);
   const int per_cu = a.dim <= 128 ? 3 : 2;
   const int64_t blocks = atoms_most < 256 * per_cu ? atoms_most : 256 * per_cu;
   const dim3 grid((unsigned)blocks);
   if (a.dim <= 64)
-    launch_dim<DT, CT, 64>(a, grid, s);
+    launch_dim<DT, CT, 64>(a, pool_bytes, grid, s);
   else if (a.dim <= 128)
-    launch_dim<DT, CT, 128>(a, grid, s);
+    launch_dim<DT, CT, 128>(a, pool_bytes, grid, s);
   else
-    launch_dim<DT, CT, 256>(a, grid, s);
+    launch_dim<DT, CT, 256>(a, pool_bytes, grid, s);
   return pl_launch_status("pl_paged_attention");
 }
 
