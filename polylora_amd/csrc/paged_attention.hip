@@ -243,18 +243,17 @@ __device__ __forceinline__ tile_place<SUBS> place_tile(const walk& w, int t) {
 template <int DT, int CT, int DP, bool FULL>
 __device__ __forceinline__ void score_tile(
     const wave_state<DT, CT, DP>& st,
-    const pl_u32x4 (&keys)[shape<DT, CT, DP>::kSubs][shape<DT, CT, DP>::kKeyLoads], int lg,
+    const pl_u32x4 (&keys)[shape<DT, CT, DP>::kSubs][shape<DT, CT, DP>::kKeyLoads],
     int dim, float scale2, float (&p)[shape<DT, CT, DP>::kTokens]) {
   typedef shape<DT, CT, DP> S;
   pl_f32x4 s[S::kSubs];
 #pragma unroll
   for (int u = 0; u < S::kSubs; ++u) {
     s[u] = pl_f32x4{0.f, 0.f, 0.f, 0.f};
+    pl_f32x4 odd = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int n = 0; n < S::kKeyLoads; ++n) {
-      pl_u32x4 w = keys[u][n];
-      // pieces past the head's end were loaded from its start: they count as 0
-      if (!FULL && key_piece<CT>(n, lg, S::E) >= dim) w = pl_u32x4{0, 0, 0, 0};
+      const pl_u32x4 w = keys[u][n];
       if constexpr (CT == PL_F8E4M3) {
         const pl_u32x4 a = {widen<DT, false>(w.x), widen<DT, true>(w.x), widen<DT, false>(w.y),
                             widen<DT, true>(w.y)};
@@ -262,10 +261,19 @@ __device__ __forceinline__ void score_tile(
                             widen<DT, true>(w.w)};
         s[u] = pl_mfma_chunk<DT>(a, st.query(2 * n), s[u]);
         s[u] = pl_mfma_chunk<DT>(b, st.query(2 * n + 1), s[u]);
+      } else if constexpr (DT == PL_F32) {
+        // two sums side by side, of the pieces that the head has
+        if (FULL || n * 4 * S::E < dim) {
+          if (n % 2)
+            odd = pl_mfma_chunk<DT>(w, st.query(n), odd);
+          else
+            s[u] = pl_mfma_chunk<DT>(w, st.query(n), s[u]);
+        }
       } else {
         s[u] = pl_mfma_chunk<DT>(w, st.query(n), s[u]);
       }
     }
+    if constexpr (DT == PL_F32) s[u] += odd;
   }
 #pragma unroll
   for (int j = 0; j < S::kTokens; ++j) p[j] = s[j / 4][j % 4] * scale2;
@@ -563,18 +571,19 @@ __global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kPerCu)) void pl_page
     // bytes from the first of 16 slots to the end of the last
     const uint32_t key_span = 15 * w.key_slot + (uint32_t)a.dim * S::kCsize;
     const uint32_t value_span = 15 * w.value_slot + (uint32_t)a.dim * S::kCsize;
+    // lanes past the head's end ask for what no descriptor holds, and get 0
+    constexpr uint32_t kNowhere = 0x80000000u;
     uint32_t key_off[S::kKeyLoads];
 #pragma unroll
     for (int n = 0; n < S::kKeyLoads; ++n) {
       const int d = key_piece<CT>(n, lg, S::E);
-      key_off[n] = li * w.key_slot + (FULL || d < a.dim ? d : 0) * S::kCsize;
+      key_off[n] = FULL || d < a.dim ? li * w.key_slot + d * S::kCsize : kNowhere;
     }
-    // lanes past the head's end read its start: what they make is not stored
     uint32_t value_off[S::kPieces];
 #pragma unroll
     for (int n = 0; n < S::kPieces; ++n) {
       const int d = S::value_at(li, n);
-      value_off[n] = 4 * lg * w.value_slot + (FULL || d < a.dim ? d : 0) * S::kCsize;
+      value_off[n] = FULL || d < a.dim ? 4 * lg * w.value_slot + d * S::kCsize : kNowhere;
     }
     // Keys of the next tile are asked for as soon as this tile's have gone into
     // the scores, values as soon as the wave is at the tile: one or the other
@@ -629,7 +638,7 @@ __global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kPerCu)) void pl_page
       const int next = tile + step;
       place = place_tile<S::kSubs>(w, next);
       float p[S::kTokens];
-      score_tile<DT, CT, DP, FULL>(st, keys, lg, a.dim, scale2, p);
+      score_tile<DT, CT, DP, FULL>(st, keys, a.dim, scale2, p);
       load_keys(place);
       bool whole = tile >= r.first && tile + S::kTile <= r.len;
 #pragma unroll
