@@ -607,7 +607,7 @@ int pl_rope_append(int32_t dtype, int32_t cache_dtype, const void* q, const int6
  * not cleared) and counters (PL_ATTENTION_COUNTER_INTS int32s, zero before the
  * first launch and zero again after each), which launches that overlap must not
  * share.  The result does not depend on which workgroup ends last. */
-#define PL_ATTENTION_COUNTER_INTS 12288
+#define PL_ATTENTION_COUNTER_INTS 8192
 int64_t pl_paged_attention_workspace_bytes(int32_t dim);
 
 int pl_paged_attention(int32_t dtype, int32_t cache_dtype, const void* q,

@@ -28,7 +28,7 @@ PL_MAX_STACKED_MODULES = 4
 PL_NOALLOC_SCRATCH_BYTES = 32 << 20
 PL_REF_PART_PLAN, PL_REF_PART_WEIGHTS, PL_REF_PART_SCRATCH = 0, 1, 2
 PL_REF_BUILD_PLAN, PL_REF_PACK_USED, PL_REF_PACK_ALL, PL_REF_KEEP_PACKED = 1, 2, 4, 8
-PL_ATTENTION_COUNTER_INTS = 12288
+PL_ATTENTION_COUNTER_INTS = 8192
 SLOT_ENTRY_INT32S = 8  # sizeof(pl_slot_entry) / 4
 
 DTYPE_CODES = {torch.float32: PL_F32, torch.bfloat16: PL_BF16, torch.float16: PL_F16}

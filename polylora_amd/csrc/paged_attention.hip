@@ -44,8 +44,17 @@ constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * 64;
 constexpr int kCols = 16;  // query heads of a workgroup's products
 
-// Workgroups of a launch: three (or as many as registers allow) on each CU.
-constexpr int kWorkersMax = 768;
+// Workgroups of a launch: two on each CU, of which a batch of many tokens takes
+// one.  A CU's waves are served oldest first, so its workgroups end one after
+// the other, and the memory is as busy with the fewer of them: with three,
+// two and one on a CU, a row of 131072 tokens takes 103, 96 and 91 us, 256 rows
+// of up to 1024 121, 118 and 115; 64 rows of up to 512, starting and ending
+// more than reading, 22, 22 and 25; fp32, 37 x 12 windows of 500, 42, 34 and 39;
+// 51 rows of up to 18000 over an 8-bit cache of 80 elements, 75 with two and 83
+// with one.
+constexpr int kCus = 256;
+constexpr int kWorkersMax = 2 * kCus;
+constexpr int kManyAtoms = 8 * kCus;
 constexpr int kCounterStride = 16;  // int32s: 64 bytes for each counter
 
 template <int DT, int CT, int DP>
@@ -59,6 +68,9 @@ struct shape {
   static constexpr int kKeyLoads = DP * kCsize / 64; // 16-byte loads of a lane per 16 keys
   static constexpr int V = DP / 16;                  // value elements of a lane per token
   static constexpr int kVWords = V * kCsize / 4;
+  // Waves of a SIMD that the compiler is to leave registers for: schedules
+  // for fewer were slower (fp32, 64 x 12 x 2048 tokens: 161 -> 169 us).
+  static constexpr int kWavesPerSimd = DP <= 128 ? 3 : 2;
   // They come in pieces of at most 16 bytes, 16 lanes' pieces side by side.
   static constexpr int kPiece = V * kCsize <= 16 ? V : 16 / kCsize;
   static constexpr int kPieces = V / kPiece;
@@ -66,7 +78,6 @@ struct shape {
     return (piece * 16 + lane) * kPiece;
   }
   static constexpr int kTokens = 4 * kSubs;          // tokens of a lane per tile
-  static constexpr int kPerCu = DP <= 128 ? 3 : 2;  // workgroups of a CU
   // Queries in LDS where keys, values and outputs fill the registers.
   static constexpr bool kQueryLds = DP == 256 || DT == PL_F32;
 };
@@ -449,8 +460,8 @@ struct deal {
 };
 constexpr float kStart = 4.f, kJoin = 5.f;
 template <int TILES>
-__device__ __forceinline__ deal choose_deal(int total, int pairs, int longest) {
-  const float w = (float)gridDim.x, p = (float)pairs;
+__device__ __forceinline__ deal choose_deal(int teams, int total, int pairs, int longest) {
+  const float w = (float)teams, p = (float)pairs;
   const float n = (float)total * TILES, top = (float)longest * TILES;
   const float alone = kWaves * top * w + n + w + p / kWaves;
   const float team = top * w + n + kStart * (w + p);
@@ -460,7 +471,7 @@ __device__ __forceinline__ deal choose_deal(int total, int pairs, int longest) {
 }
 
 template <int DT, int CT, int DP, bool FULL, bool STREAM>
-__global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kPerCu)) void pl_paged_attention_kernel(
+__global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kWavesPerSimd)) void pl_paged_attention_kernel(
     attend_args a) {
   typedef shape<DT, CT, DP> S;
   typedef typename pl_traits<DT>::T T;
@@ -490,8 +501,13 @@ __global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kPerCu)) void pl_page
   }
   total = __builtin_amdgcn_readlane(scan_sum(total), 63) * per_row;
   longest = __builtin_amdgcn_readlane(scan_max(longest), 63);
-  const deal how = choose_deal<S::kAtom / (kWaves * S::kTile)>(total, a.rows * per_row, longest);
-  const int workers = (int)gridDim.x * kWaves / how.team;
+  // one wave of a SIMD keeps the memory busy if its tiles are large and its products few
+  const bool many =
+      DT != PL_F32 && DP <= 128 && a.dim * S::kCsize >= 128 && total >= kManyAtoms;
+  const int teams = many ? min((int)gridDim.x, kCus) : (int)gridDim.x;
+  const deal how =
+      choose_deal<S::kAtom / (kWaves * S::kTile)>(teams, total, a.rows * per_row, longest);
+  const int workers = how.team == 1 ? (int)gridDim.x * kWaves : teams;
   const int worker = how.team == 1 ? (int)blockIdx.x * kWaves + wave : (int)blockIdx.x;
   const int per = (total + workers - 1) / workers;
   const int from = (int)min((int64_t)worker * per, (int64_t)total), to = min(total - per, from) + per;
@@ -765,8 +781,7 @@ template <int DT, int CT>
 int launch(const attend_args& a, int64_t atoms_most, hipStream_t s) {
   const int64_t pool_bytes = 2ll * a.table.num_pages * ((int64_t)a.kv_heads * a.dim << a.table.page_shift) *
                              pl_cache_elem_size(CT);
-  const int per_cu = a.dim <= 128 ? 3 : 2;
-  const int64_t blocks = atoms_most < 256 * per_cu ? atoms_most : 256 * per_cu;
+  const int64_t blocks = atoms_most < kWorkersMax ? atoms_most : kWorkersMax;
   const dim3 grid((unsigned)blocks);
   if (a.dim <= 64)
     launch_dim<DT, CT, 64>(a, pool_bytes, grid, s);
