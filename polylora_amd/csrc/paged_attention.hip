@@ -450,22 +450,27 @@ __device__ __forceinline__ void join_parts(const float* parts, int slot0, int sl
 }
 
 // How the batch's atoms are dealt out, from their number, the (row, key head)
-// pairs and the longest pair.  Times are in tiles of a wave (one after the
-// other, about as long as it waits for one), of which a team of waves takes
-// TILES for an atom: starting and ending a pair costs a team about kStart of
-// them and joining parts about kJoin.
+// pairs and the longest pair.  Times are in tiles of a wave, of which a team of
+// waves takes TILES for an atom: a team's first pair costs it about kFirst of
+// them to begin, each pair kPair, joining parts kJoin, and waves alone read a
+// batch that fills the memory kAlone times as slowly.  Measured against each other (us alone /
+// team, whole / team, split): 1 row of up to 300 tokens 11.0 / 8.2 / 8.6, 64 of
+// 512 19.2 / 22.5 / 26.8, 256 of 512 62 / 85 / 85, 256 of 2048 229 / 216 / 209, 1
+// of 4000 88 / 39 / 11; what this takes is within a tenth of the best of them.
 struct deal {
   int team;    // waves on a pair: kWaves, or 1 (no waves to join, no barrier)
   bool whole;  // pairs go whole to the run that their first atom falls in
 };
-constexpr float kStart = 4.f, kJoin = 5.f;
+constexpr float kFirst = 2.f, kPair = 8.6f, kJoin = 5.f, kAlone = 2.1f;
 template <int TILES>
 __device__ __forceinline__ deal choose_deal(int teams, int total, int pairs, int longest) {
   const float w = (float)teams, p = (float)pairs;
   const float n = (float)total * TILES, top = (float)longest * TILES;
-  const float alone = kWaves * top * w + n + w + p / kWaves;
-  const float team = top * w + n + kStart * (w + p);
-  const float split = w + n + kStart * (w + p) + kJoin * w;
+  // each times w; waves enough for a pair each wait for the longest, else for a run and it
+  const bool each = pairs <= (int)gridDim.x * kWaves;
+  const float alone = fmaxf(kWaves * top * w + (each ? 0.f : n), kAlone * n) + w + p / kWaves;
+  const float ends = kFirst * w + kPair * p;
+  const float team = top * w + n + ends, split = w + n + ends + kJoin * w;
   if (alone < team && alone < split) return {1, true};
   return {kWaves, team < split};
 }
@@ -508,13 +513,16 @@ __global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kWavesPerSimd)) void 
   const deal how =
       choose_deal<S::kAtom / (kWaves * S::kTile)>(teams, total, a.rows * per_row, longest);
   const int workers = how.team == 1 ? (int)gridDim.x * kWaves : teams;
-  const int worker = how.team == 1 ? (int)blockIdx.x * kWaves + wave : (int)blockIdx.x;
+  const int worker = how.team == 1 ? wave * (int)gridDim.x + (int)blockIdx.x : (int)blockIdx.x;
+  // waves enough for a pair each: no runs, whose atoms come by ones, twos and threes
+  const bool each = how.team == 1 && a.rows * per_row <= workers;
   const int per = (total + workers - 1) / workers;
-  const int from = (int)min((int64_t)worker * per, (int64_t)total), to = min(total - per, from) + per;
-  if (from >= total) return;
+  const int from = (int)min((int64_t)worker * per, (int64_t)total);
+  int to = min(total - per, from) + per;
+  if (each ? worker >= a.rows * per_row : from >= total) return;
   // the row of its first atom: the first whose atoms up to and with it pass `from`
-  int row = 0, row_start = 0, row_len = 0;
-  for (int b0 = 0;; b0 += 64) {
+  int row = 0, row_start = 0, row_len = 0, at = from;
+  for (int b0 = 0; !each; b0 += 64) {
     const int b = b0 + lane;
     int n = atoms[0], len = lens[0];
 #pragma unroll
@@ -539,9 +547,15 @@ __global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kWavesPerSimd)) void 
     row_start = __builtin_amdgcn_readlane(upto, 63);
   }
   row = uniform(row);
-
-  int at = from;
-  bool skip = how.whole;  // to the first pair that starts in the run
+  if (each) {
+    // its pair, as if the rows before it had no atoms
+    row = worker / per_row;
+    row_len = as_scalar(a.lens)[row];
+    row_start = 0;
+    at = worker % per_row * span_of<S::kAtom>(a, row_len).atoms;
+    to = at + 1;
+  }
+  bool skip = how.whole && !each;  // to the first pair that starts in the run
   while (at < to) {
     const row_span r = span_of<S::kAtom>(a, row_len);
     int in_row = at - row_start;
