@@ -90,6 +90,10 @@ __global__ __launch_bounds__(THREADS) void pl_adjust_logits_kernel(logits_args a
   // The first of them are asked for beside their number: the list is there
   // whole, and what lies beyond `lens` is not counted.
   if (a.tokens && a.history > 0) look(tid, a.history);
+  penalties pen;
+  pen.r = a.repetition ? a.repetition[b] : 1.f;
+  pen.f = a.frequency ? a.frequency[b] : 0.f;
+  pen.p = a.presence ? a.presence[b] : 0.f;
   const int n = a.tokens ? min(max(a.lens[b], 0), a.history) : 0;
   const int prompt = a.prompt_lens ? a.prompt_lens[b] : 0;
   const bool special = a.tokens || a.n_bias > 0;
@@ -164,10 +168,6 @@ __global__ __launch_bounds__(THREADS) void pl_adjust_logits_kernel(logits_args a
     }
     __syncthreads();
   }
-  penalties pen;
-  pen.r = a.repetition ? a.repetition[b] : 1.f;
-  pen.f = a.frequency ? a.frequency[b] : 0.f;
-  pen.p = a.presence ? a.presence[b] : 0.f;
 #pragma unroll
   for (int k = 0; k < kPasses; ++k) {
     const int v = lo + (k * THREADS + tid) * kVec;

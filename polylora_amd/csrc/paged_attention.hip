@@ -21,10 +21,10 @@
 //   O^T = V^T P^T the contraction over tokens may take them in any order that
 //                 both operands share, so each lane keeps the tokens whose
 //                 scores it got: the weights never leave their lane, and the
-//                 lane reads those tokens' values, dim / 16 consecutive
-//                 elements of each, and pairs them up by byte permutes.  It
-//                 gets the outputs of query i, so the maximum, the sum and the
-//                 rescaling of a query all stay in the lanes of its column.
+//                 lane reads those tokens' values, a sixteenth of each, and
+//                 pairs them up by byte permutes.  It gets the outputs of
+//                 query i, so the maximum, the sum and the rescaling of a query
+//                 all stay in the lanes of its column.
 // Weights go into the product as two 16-bit numbers, p = hi + lo, which keeps
 // them to 2^-16 (bf16) or better: one product more on matrix units that have
 // little else to do, and the output keeps the error of its own rounding.
@@ -653,39 +653,39 @@ __global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kWavesPerSimd)) void 
       }
       load_keys(place);
       do {
-      uint32_t v[S::kTokens][S::kVWords];
+        uint32_t v[S::kTokens][S::kVWords];
 #pragma unroll
-      for (int u = 0; u < S::kSubs; ++u) {
-        const pl_buffer b = make_buffer(place.value[u], place.held[u] ? value_span : 0);
+        for (int u = 0; u < S::kSubs; ++u) {
+          const pl_buffer b = make_buffer(place.value[u], place.held[u] ? value_span : 0);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+          for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int n = 0; n < S::kPieces; ++n)
-            load_words<S::kVWords / S::kPieces, STREAM>(b, value_off[n], j * w.value_slot,
-                                                         v[4 * u + j] + n * (S::kVWords / S::kPieces));
-      }
-      const tile_place<S::kSubs> here = place;
-      const int next = tile + step;
-      place = place_tile<S::kSubs>(w, next);
-      float p[S::kTokens];
-      score_tile<DT, CT, DP, FULL>(st, keys, a.dim, scale2, p);
-      load_keys(place);
-      bool whole = tile >= r.first && tile + S::kTile <= r.len;
-#pragma unroll
-      for (int u = 0; u < S::kSubs; ++u) whole = whole && here.held[u];
-      if (!whole) {
-        // slots without a token may hold anything, NaN too: no weight of 0 takes that out
-#pragma unroll
-        for (int j = 0; j < S::kTokens; ++j) {
-          const int token = tile + 16 * (j / 4) + 4 * lg + j % 4;
-          const bool alive = here.held[j / 4] && token >= r.first && token < r.len;
-          p[j] = alive ? p[j] : -INFINITY;
-#pragma unroll
-          for (int i = 0; i < S::kVWords; ++i) v[j][i] = alive ? v[j][i] : 0u;
+            for (int n = 0; n < S::kPieces; ++n)
+              load_words<S::kVWords / S::kPieces, STREAM>(b, value_off[n], j * w.value_slot,
+                                                           v[4 * u + j] + n * (S::kVWords / S::kPieces));
         }
-      }
-      weigh_tile<DT, CT, DP>(st, p, v);
-      tile = next;
+        const tile_place<S::kSubs> here = place;
+        const int next = tile + step;
+        place = place_tile<S::kSubs>(w, next);
+        float p[S::kTokens];
+        score_tile<DT, CT, DP, FULL>(st, keys, a.dim, scale2, p);
+        load_keys(place);
+        bool whole = tile >= r.first && tile + S::kTile <= r.len;
+#pragma unroll
+        for (int u = 0; u < S::kSubs; ++u) whole = whole && here.held[u];
+        if (!whole) {
+          // slots without a token may hold anything, NaN too: no weight of 0 takes that out
+#pragma unroll
+          for (int j = 0; j < S::kTokens; ++j) {
+            const int token = tile + 16 * (j / 4) + 4 * lg + j % 4;
+            const bool alive = here.held[j / 4] && token >= r.first && token < r.len;
+            p[j] = alive ? p[j] : -INFINITY;
+#pragma unroll
+            for (int i = 0; i < S::kVWords; ++i) v[j][i] = alive ? v[j][i] : 0u;
+          }
+        }
+        weigh_tile<DT, CT, DP>(st, p, v);
+        tile = next;
       } while (tile < end);
     }
 
