@@ -200,6 +200,7 @@ def check_attention(gpu, dtype, lens, heads, kv_heads, dim, page, fp8=False, ord
 @pytest.mark.parametrize("heads,kv_heads,dim,page", [
     (1, 1, 16, 16), (4, 1, 32, 16), (32, 8, 128, 16), (12, 12, 80, 32), (28, 4, 96, 64), (9, 3, 256, 16),
     (16, 1, 64, 128), (17, 1, 64, 16), (40, 2, 48, 16), (6, 2, 192, 32), (3, 1, 112, 16), (5, 5, 144, 16),
+    (48, 1, 64, 16), (71, 1, 64, 16), (66, 2, 128, 16), (130, 1, 256, 16), (64, 2, 80, 32),
 ])
 def test_attention_matches_the_plain_form(gpu, dtype, heads, kv_heads, dim, page):
     check_attention(gpu, dtype, [1, 0, 2, 15, 16, 17, 33, 100, 257], heads, kv_heads, dim, page)
@@ -221,7 +222,8 @@ def test_attention_windows(gpu, dtype, window):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("lens,heads,kv_heads", [([5000], 8, 2), ([3000, 1, 2999], 4, 4), ([2049] * 4 + [0] * 9, 16, 1)])
+@pytest.mark.parametrize("lens,heads,kv_heads", [([5000], 8, 2), ([3000, 1, 2999], 4, 4), ([2049] * 4 + [0] * 9, 16, 1),
+                                                 ([4000, 700], 40, 2), ([3000], 71, 1)])
 def test_attention_over_long_rows(gpu, dtype, lens, heads, kv_heads):
     check_attention(gpu, dtype, lens, heads, kv_heads, 128, 16)
 
