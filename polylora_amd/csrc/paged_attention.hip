@@ -25,9 +25,13 @@
 //                 pairs them up by byte permutes.  It gets the outputs of
 //                 query i, so the maximum, the sum and the rescaling of a query
 //                 all stay in the lanes of its column.
-// Weights go into the product as two 16-bit numbers, p = hi + lo, which keeps
-// them to 2^-16 (bf16) or better: one product more on matrix units that have
-// little else to do, and the output keeps the error of its own rounding.
+// Weights go into the product as two 16-bit numbers, p = hi + lo: one product
+// more on matrix units that have little else to do, and the output keeps the
+// error of its own rounding.  bf16 keeps them to 2^-16 of themselves.  fp16 ends
+// at 2^-24, so its weights are taken 2^15 times as large, to 32768 for the
+// highest score (l and o alike, so the factor goes out in o / l), and kept to
+// 2^-22 of themselves or 2^-40 of the largest.  Without it tokens 17.3 and more
+// below the highest score counted in l and not in o.
 //
 // Work is split by tokens: the launch is a fixed number of workgroups, and the
 // batch's atoms (kAtom tokens of one row and key head) are dealt out in equal
@@ -80,6 +84,8 @@ struct shape {
   static constexpr int kTokens = 4 * kSubs;          // tokens of a lane per tile
   // Queries in LDS where keys, values and outputs fill the registers.
   static constexpr bool kQueryLds = DP == 256 || DT == PL_F32;
+  // log2 of what weights are multiplied by, that their 16-bit parts keep small ones.
+  static constexpr float kLift = DT == PL_F16 ? 15.f : 0.f;
 };
 typedef pl_u32x4 __attribute__((may_alias)) shared_u32x4;
 typedef uint32_t pl_u32x2 __attribute__((ext_vector_type(2)));
@@ -313,7 +319,7 @@ __device__ __forceinline__ void weigh_tile(wave_state<DT, CT, DP>& st,
   }
 #pragma unroll
   for (int j = 0; j < S::kTokens; ++j) {
-    p[j] = exp2_fast(p[j] - ref);
+    p[j] = exp2_fast(S::kLift ? p[j] - ref + S::kLift : p[j] - ref);
     st.l += p[j];
   }
   if constexpr (DT == PL_F32) {

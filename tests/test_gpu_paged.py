@@ -269,6 +269,38 @@ def test_attention_takes_no_rows_and_no_pages(gpu):
     assert not paged_attention(q, key, key, table[:, :0], torch.full((3,), 20, dtype=torch.int32, device=gpu)).any()
 
 
+# ----------------------------------------------------------------------------- values that are easily lost
+
+
+# rows that a wave has to itself, rows that a workgroup takes whole, a row that is split over workgroups
+DEALS = {"alone": [300] * 300, "whole": [600] * 128, "split": [8192]}
+
+
+@pytest.mark.parametrize("deal", DEALS)
+@pytest.mark.parametrize("dtype,fp8", [(d, False) for d in DTYPES] + [(d, True) for d in DTYPES[:2]])
+def test_attention_keeps_tokens_far_below_the_highest_score(gpu, deal, dtype, fp8):
+    """A first token of value 0 that stands 2 to 22 above all others: the output is the others' alone."""
+    lens, kv_heads, dim, page = DEALS[deal], 2, 64, 64
+    above = torch.tensor([2.0, 12.0, 14.0, 16.0, 18.0, 20.0, 22.0])
+    gen = torch.Generator().manual_seed(21)
+    key, value, table, ks, vs = pool(gen, len(lens), lens, kv_heads, dim, page, dtype, fp8)
+    key = torch.where(key.float().isnan(), float("nan"), 0.0)
+    value = value.float().abs()
+    first = table[:, 0].long()
+    key[first, :, 0, 0], value[first, :, 0] = 1.0, 0.0
+    key, value, ks = key.to(FP8 if fp8 else dtype), value.to(FP8 if fp8 else dtype), torch.ones(kv_heads) if fp8 else None
+    q = torch.zeros(len(lens), kv_heads * len(above), dim, dtype=dtype)
+    q[:, :, 0] = above.repeat(kv_heads)
+    n = torch.tensor(lens, dtype=torch.int32)
+    want, spread, reach = plain.paged_attention(q, key, value, table, n, 1.0, None, ks, vs)
+    up = {"k_scale": ks.to(gpu), "v_scale": vs.to(gpu)} if fp8 else {}
+    got = paged_attention(q.to(gpu), key.to(gpu), value.to(gpu), table.to(gpu), n.to(gpu), scale=1.0, **up)
+    # the first token's value of 0 adds nothing to `spread`: what is allowed is relative to the output
+    tol = attention_tolerance(want, spread, reach, dtype, dim, max(lens))
+    err = (got.cpu().double() - want).abs()
+    assert bool((err <= tol).all()), float((err / tol).max())
+
+
 # ----------------------------------------------------------------------------- streams and graphs
 
 
