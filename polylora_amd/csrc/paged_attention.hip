@@ -465,7 +465,8 @@ __device__ __forceinline__ void join_parts(const attend_args& a, int slot0, int 
           o = o * keep + pl_f32x4{s[2], s[3], s[4], s[5]} * f;
         }
     }
-    if (busy && first == 0) store(c, d, m == -INFINITY ? pl_f32x4{0.f, 0.f, 0.f, 0.f} : o / l);
+    // no token gives 0; NaN, which no maximum shows, is in l and stays
+    if (busy && first == 0) store(c, d, l == 0.f ? pl_f32x4{0.f, 0.f, 0.f, 0.f} : o / l);
   }
 }
 

@@ -301,6 +301,47 @@ def test_attention_keeps_tokens_far_below_the_highest_score(gpu, deal, dtype, fp
     assert bool((err <= tol).all()), float((err / tol).max())
 
 
+def _finite_batch(gpu, dtype, deal, fp8=False):
+    """Arguments on the GPU, two query heads to each of two key heads, and the page and slot of a token in the middle
+    of the last row."""
+    lens, page = DEALS[deal], 16
+    gen = torch.Generator().manual_seed(22)
+    key, value, table, ks, vs = pool(gen, len(lens), lens, 2, 64, page, dtype, fp8)
+    q = torch.randn(len(lens), 4, 64, generator=gen).to(dtype)
+    at = plain.place(table, len(lens) - 1, lens[-1] // 2, key.shape[0], page)
+    args = [x.to(gpu) for x in (q, key, value, table, torch.tensor(lens, dtype=torch.int32))]
+    return args, {"k_scale": ks.to(gpu), "v_scale": vs.to(gpu)} if fp8 else {}, at
+
+
+@pytest.mark.parametrize("deal", DEALS)
+@pytest.mark.parametrize("dtype,fp8", [(d, False) for d in DTYPES] + [(torch.bfloat16, True)])
+def test_attention_hands_on_nan_that_counts(gpu, deal, dtype, fp8):
+    """NaN in a query, in a key and in a value: NaN comes out where it goes in, and nowhere else."""
+    (q, key, value, table, lens), scales, (page, slot) = _finite_batch(gpu, dtype, deal, fp8)
+    clean = paged_attention(q, key, value, table, lens, **scales)
+    assert not clean.isnan().any()
+
+    def check(where, *args):
+        got = paged_attention(*args, table, lens, **scales)
+        assert torch.equal(got.isnan(), where)
+        assert torch.equal(got[~where], clean[~where])
+
+    where = torch.zeros(clean.shape, dtype=torch.bool, device=gpu)
+    bad = q.clone()
+    bad[-1, 1, 5] = float("nan")
+    where[-1, 1] = True
+    check(where, bad, key, value)
+    bits = torch.tensor(float("nan")).to(key.dtype).view(torch.uint8 if fp8 else key.dtype).to(gpu)
+    bad = key.clone()
+    (bad.view(torch.uint8) if fp8 else bad)[page, 1, slot, 7] = bits
+    where.zero_()[-1, 2:] = True
+    check(where, q, bad, value)
+    bad = value.clone()
+    (bad.view(torch.uint8) if fp8 else bad)[page, 1, slot, 7] = bits
+    where.zero_()[-1, 2:, 7] = True
+    check(where, q, key, bad)
+
+
 # ----------------------------------------------------------------------------- streams and graphs
 
 
