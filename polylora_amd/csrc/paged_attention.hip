@@ -27,10 +27,10 @@
 //                 all stay in the lanes of its column.
 // Weights go into the product as two 16-bit numbers, p = hi + lo: one product
 // more on matrix units that have little else to do, and the output keeps the
-// error of its own rounding.  bf16 keeps them to 2^-16 of themselves.  fp16 ends
+// error of its own rounding.  bf16 keeps them to 2^-15 of themselves.  fp16 ends
 // at 2^-24, so its weights are taken 2^15 times as large, to 32768 for the
 // highest score (l and o alike, so the factor goes out in o / l), and kept to
-// 2^-22 of themselves or 2^-40 of the largest.  Without it tokens 17.3 and more
+// 2^-21 of themselves or 2^-39 of the largest.  Without it tokens 17.3 and more
 // below the highest score counted in l and not in o.
 //
 // Work is split by tokens: the launch is a fixed number of workgroups, and the
@@ -190,6 +190,21 @@ __device__ __forceinline__ float unpack(uint32_t w, int half) {
   return (float)__builtin_bit_cast(T2, w)[half];
 }
 
+// The same, rounded towards 0.
+template <int DT>
+__device__ __forceinline__ uint32_t pack2_down(float a, float b) {
+  if constexpr (DT == PL_BF16)
+    return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302);
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+}
+// lo, but at least the smallest fp16 number where hi is not 0 (neither is negative).
+__device__ __forceinline__ uint32_t least_beside(uint32_t hi, uint32_t lo) {
+  typedef uint16_t pair __attribute__((ext_vector_type(2)));
+  const pair least = __builtin_elementwise_min(__builtin_bit_cast(pair, hi), pair{1, 1});
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(pair, lo), least));
+}
+
 // First element of the 16-byte key piece that lane group g loads n-th.
 template <int CT>
 __device__ __forceinline__ int key_piece(int n, int g, int e) {
@@ -336,8 +351,14 @@ __device__ __forceinline__ void weigh_tile(wave_state<DT, CT, DP>& st,
     pl_u32x4 hi, lo;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      hi[j] = pack2<DT>(p[2 * j], p[2 * j + 1]);
-      lo[j] = pack2<DT>(p[2 * j] - unpack<DT>(hi[j], 0), p[2 * j + 1] - unpack<DT>(hi[j], 1));
+      // neither part is negative, and lo not 0 where hi is not: an infinite value
+      // times both is infinite, not NaN
+      float x[2] = {p[2 * j], p[2 * j + 1]};
+      if constexpr (DT == PL_BF16)
+        for (float& e : x) e = __uint_as_float(__float_as_uint(e) | 1u);  // below fp32's rounding
+      hi[j] = pack2_down<DT>(x[0], x[1]);
+      lo[j] = pack2<DT>(x[0] - unpack<DT>(hi[j], 0), x[1] - unpack<DT>(hi[j], 1));
+      if constexpr (DT == PL_F16) lo[j] = least_beside(hi[j], lo[j]);
     }
 #pragma unroll
     for (int i = 0; i < S::V / 2; ++i) {

@@ -342,6 +342,21 @@ def test_attention_hands_on_nan_that_counts(gpu, deal, dtype, fp8):
     check(where, q, key, bad)
 
 
+@pytest.mark.parametrize("deal", DEALS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attention_hands_on_infinite_values(gpu, deal, dtype):
+    """An infinite value has a weight above 0, so its sum is infinite; the largest score's, whose weight is 1, among them."""
+    (q, key, value, table, lens), _, (page, slot) = _finite_batch(gpu, dtype, deal)
+    key[page, 1, slot] = q[-1, 2] * 2  # the highest score of one query head, an ordinary one of the other
+    clean = paged_attention(q, key, value, table, lens)
+    value[page, 1, slot, 7], value[page, 1, slot, 60] = float("inf"), float("-inf")
+    got = paged_attention(q, key, value, table, lens)
+    assert bool((got[-1, 2:, 7] == float("inf")).all()) and bool((got[-1, 2:, 60] == float("-inf")).all())
+    same = torch.ones(clean.shape, dtype=torch.bool, device=gpu)
+    same[-1, 2:, 7] = same[-1, 2:, 60] = False
+    assert torch.equal(got[same], clean[same])
+
+
 # ----------------------------------------------------------------------------- streams and graphs
 
 
