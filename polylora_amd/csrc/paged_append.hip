@@ -84,11 +84,22 @@ struct append_args {
   int32_t turns, units, group;  // places of a head that turn, all of them, tokens of a workgroup
 };
 
-// A value over the scale (times its reciprocal, taken once for a head: within
-// one fp32 rounding of the quotient, 2^-20 of an e4m3 step), saturated (NaN
-// stays NaN).
-__device__ __forceinline__ float to_e4m3_range(float x, float per_scale) {
-  const float y = x * per_scale;
+// The scale of an e4m3 cache's head and its reciprocal.
+struct e4m3_scale {
+  float s, per;
+};
+template <int CT>
+__device__ __forceinline__ e4m3_scale head_scale(const float* scales, int head) {
+  const float s = CT == PL_F8E4M3 ? scales[head] : 1.f;
+  return {s, 1.f / s};
+}
+// A value over the scale, saturated (NaN stays NaN).  The product with the
+// scale's reciprocal, taken once for a head, is off by its roundings, which show
+// half way between two e4m3 numbers; what it leaves of x corrects it, where it
+// is not saturated anyway (dividing each value: 24 x 77 tokens 7.3 -> 8.1 us).
+__device__ __forceinline__ float to_e4m3_range(float x, e4m3_scale scale) {
+  const float z = x * scale.per;
+  const float y = fabsf(z) < 2 * kE4M3Max ? fmaf(fmaf(-z, scale.s, x), scale.per, z) : z;
   return y != y ? y : fminf(fmaxf(y, -kE4M3Max), kE4M3Max);
 }
 
@@ -125,14 +136,14 @@ __device__ __forceinline__ void store_vec(void* p, int64_t at, const float (&x)[
   }
 }
 template <int DT, int CT, int VEC, bool STREAM>
-__device__ __forceinline__ void store_cache(void* p, int64_t at, const float (&x)[VEC], float per_scale) {
+__device__ __forceinline__ void store_cache(void* p, int64_t at, const float (&x)[VEC], e4m3_scale scale) {
   if constexpr (CT == PL_F8E4M3) {
     uint8_t* q = (uint8_t*)p + at;
     uint32_t w[(VEC + 3) / 4] = {};
 #pragma unroll
     for (int e = 0; e < VEC; e += 2) {
-      const float lo = to_e4m3_range(x[e], per_scale);
-      const float hi = e + 1 < VEC ? to_e4m3_range(x[e + 1], per_scale) : lo;
+      const float lo = to_e4m3_range(x[e], scale);
+      const float hi = e + 1 < VEC ? to_e4m3_range(x[e + 1], scale) : lo;
       w[e / 4] = e % 4 ? __builtin_amdgcn_cvt_pk_fp8_f32(lo, hi, (int)w[e / 4], true)
                        : __builtin_amdgcn_cvt_pk_fp8_f32(lo, hi, (int)w[e / 4], false);
     }
@@ -226,9 +237,9 @@ __global__ __launch_bounds__(kThreads) void pl_rope_append_kernel(append_args a)
       }
       if (!is_q && live) {
         const int64_t at = page * a.key.s_page + hh * a.key.s_head + slot * a.key.s_slot;
-        const float per_scale = CT == PL_F8E4M3 ? 1.f / a.k_scale[hh] : 1.f;
-        store_cache<DT, CT, VEC, STREAM>(a.key.p, at + d, x, per_scale);
-        if (split) store_cache<DT, CT, VEC, STREAM>(a.key.p, at + d2, y, per_scale);
+        const e4m3_scale scale = head_scale<CT>(a.k_scale, hh);
+        store_cache<DT, CT, VEC, STREAM>(a.key.p, at + d, x, scale);
+        if (split) store_cache<DT, CT, VEC, STREAM>(a.key.p, at + d2, y, scale);
       }
     }
   }
@@ -239,8 +250,8 @@ __global__ __launch_bounds__(kThreads) void pl_rope_append_kernel(append_args a)
     float x[VEC];
     load_vec<DT, VEC>(a.v, b * a.vs[0] + t * a.vs[1] + hh * a.vs[2] + d, x);
     store_cache<DT, CT, VEC, STREAM>(a.value.p,
-                             page * a.value.s_page + hh * a.value.s_head + slot * a.value.s_slot + d,
-                             x, CT == PL_F8E4M3 ? 1.f / a.v_scale[hh] : 1.f);
+                                     page * a.value.s_page + hh * a.value.s_head + slot * a.value.s_slot + d,
+                                     x, head_scale<CT>(a.v_scale, hh));
   }
 }
 

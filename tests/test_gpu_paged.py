@@ -357,6 +357,24 @@ def test_attention_hands_on_infinite_values(gpu, deal, dtype):
     assert torch.equal(got[same], clean[same])
 
 
+@pytest.mark.parametrize("dtype", DTYPES[:2])
+def test_append_stores_quotients_in_8_bits(gpu, dtype):
+    """Values half way between two e4m3 numbers, over scales whose reciprocals are rounded: the even one, as x / scale is."""
+    heads = torch.arange(3, 8 if dtype == torch.bfloat16 else 64, 2)
+    scale = heads / 256.0
+    x = (torch.arange(16, 32) / 16.0)[None] * scale[:, None]
+    k = x.to(dtype)[None, None]
+    assert torch.equal(k.float()[0, 0], x)
+    want = (k.float()[0, 0] / scale[:, None]).to(FP8).float()
+    key = torch.zeros(1, len(heads), 16, 16, device=gpu).to(FP8)
+    value, k, up = key.clone(), k.to(gpu), scale.to(gpu)
+    cos, sin = rope_table(4, 0, device=gpu)
+    zero = torch.zeros(1, dtype=torch.int32, device=gpu)
+    rope_append(k, k, k, key, value, zero[None], zero, cos, sin, k_scale=up, v_scale=up)
+    assert torch.equal(key[0, :, 0].float().cpu(), want)
+    assert torch.equal(value[0, :, 0].float().cpu(), want)
+
+
 # ----------------------------------------------------------------------------- streams and graphs
 
 
