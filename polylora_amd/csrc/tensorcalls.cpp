@@ -11,6 +11,7 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -56,9 +57,19 @@ std::string type_text(at::ScalarType t) {
   }
 }
 
+// No argument may be part of a graph that wants derivatives: none of the calls has any.
+void check_no_grad(const at::Tensor& t, const char* name) {
+  if (t.requires_grad() && c10::GradMode::is_enabled())
+    runtime_error(std::string(name) + " requires a gradient, and the call has no backward: call it under torch.no_grad()");
+  if (t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
+    runtime_error(std::string(name) + " carries a tangent, and the call has no forward derivative");
+}
+
 const at::Tensor& tensor(PyObject* o, const char* name) {
   if (!THPVariable_Check(o)) type_error(std::string(name) + " must be a torch.Tensor");
-  return THPVariable_Unpack(o);
+  const at::Tensor& t = THPVariable_Unpack(o);
+  check_no_grad(t, name);
+  return t;
 }
 const at::Tensor* maybe(PyObject* o, const char* name) {
   return o == Py_None ? nullptr : &tensor(o, name);
@@ -93,18 +104,13 @@ int32_t dtype_code(at::ScalarType t) {
   }
 }
 
-// The tensor that sets the call's GPU: on one, and not part of a graph that wants gradients.
+// The tensor that sets the call's GPU is on one.
 void check_lead(const at::Tensor& t, const char* what) {
   if (!t.is_cuda())
     runtime_error(std::string(what) +
                   ": polylora_amd computes only on a ROCm GPU through its HIP library; got a CPU "
                   "tensor (there is no CPU fallback)");
 }
-void check_no_grad(const at::Tensor& t, const char* what) {
-  if (t.requires_grad() && c10::GradMode::is_enabled())
-    runtime_error(std::string(what) + " has no backward: call it under torch.no_grad()");
-}
-
 void check_type(const at::Tensor& t, const char* name, at::ScalarType type, int device) {
   if (t.scalar_type() != type)
     type_error(std::string(name) + " must be " + type_text(type) + ", not " + type_text(t.scalar_type()));
@@ -211,10 +217,7 @@ PyObject* rope_append(PyObject* const* a) {
   check_type(k, "k", type, device);
   check_type(v, "v", type, device);
   check_shape(v, "v", k.sizes());
-  for (const at::Tensor* t : {&q, &k, &v}) {
-    check_last(*t, "q, k and v");
-    check_no_grad(*t, "rope_append");
-  }
+  for (const at::Tensor* t : {&q, &k, &v}) check_last(*t, "q, k and v");
   const Cache c = check_cache(tensor(a[3], "key_cache"), tensor(a[4], "value_cache"), tensor(a[5], "page_table"),
                               rows, dim, type, device, maybe(a[11], "k_scale"), maybe(a[12], "v_scale"));
   if (c.kv_heads != kv_heads || kv_heads == 0 || heads % kv_heads)
@@ -266,7 +269,6 @@ PyObject* paged_attention(PyObject* const* a) {
   const at::ScalarType type = q.scalar_type();
   const int32_t code = dtype_code(type);
   check_last(q, "q");
-  check_no_grad(q, "paged_attention");
   const Cache c = check_cache(tensor(a[1], "key_cache"), tensor(a[2], "value_cache"), tensor(a[3], "page_table"),
                               rows, dim, type, device, maybe(a[7], "k_scale"), maybe(a[8], "v_scale"));
   if (c.kv_heads == 0 || heads % c.kv_heads)
@@ -327,7 +329,6 @@ PyObject* adjust_logits(PyObject* const* a) {
   const at::ScalarType type = logits.scalar_type();
   const int32_t code = dtype_code(type);
   check_last(logits, "logits");
-  check_no_grad(logits, "adjust_logits");
   const at::Tensor* given = maybe(a[10], "out");
   if (given) {
     if (given->scalar_type() != at::kFloat && given->scalar_type() != type)

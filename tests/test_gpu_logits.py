@@ -199,3 +199,21 @@ def test_refusals(gpu):
     wide = torch.zeros(2, 65, device=gpu)
     with pytest.raises(RuntimeError):  # over the logits, one element on
         adjust_logits(wide[:, :64], out=wide[:, 1:])
+
+
+def test_tensors_that_want_derivatives_are_refused(gpu):
+    """Any floating-point argument, not only the logits; under no_grad they are taken."""
+    good = {name: t.to(gpu) for name, t in build(torch.Generator().manual_seed(8), 2, 40, torch.float32, 5, 3).items()}
+    good["out"] = torch.empty_like(good["logits"])
+    for name, t in good.items():
+        if t.dtype != torch.float32:
+            continue
+        held = t.detach().clone().requires_grad_()
+        with pytest.raises(RuntimeError, match="no backward"):
+            adjust_logits(**{**good, name: held})
+        with torch.no_grad():
+            adjust_logits(**{**good, name: held})
+        with torch.autograd.forward_ad.dual_level():
+            dual = torch.autograd.forward_ad.make_dual(t.detach().clone(), torch.ones_like(t))
+            with pytest.raises(RuntimeError, match="no forward derivative"):
+                adjust_logits(**{**good, name: dual})

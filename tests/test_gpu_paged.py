@@ -532,3 +532,28 @@ def test_refusals_of_the_append(gpu):
     for change, error in bad:
         with pytest.raises(error):
             rope_append(**{**good, **change})
+
+
+def test_tensors_that_want_derivatives_are_refused(gpu):
+    """Any floating-point argument, not only the queries; under no_grad they are taken."""
+    dtype = torch.bfloat16
+    attend, append = _good(gpu, dtype)
+    fp8 = torch.zeros(3, 2, 16, 32, device=gpu).to(FP8)
+    ones = torch.ones(2, device=gpu)
+    scaled = {"key_cache": fp8, "value_cache": fp8.clone(), "k_scale": ones, "v_scale": ones.clone()}
+    attend["out"] = torch.empty_like(attend["q"])
+    append["k_out"] = torch.empty_like(append["k"])
+    for fn, good in ((paged_attention, attend), (rope_append, append), (paged_attention, {**attend, **scaled}),
+                     (rope_append, {**append, **scaled})):
+        for name, t in good.items():
+            if t.dtype not in (torch.float32, dtype):
+                continue
+            held = t.detach().clone().requires_grad_()
+            with pytest.raises(RuntimeError, match="no backward"):
+                fn(**{**good, name: held})
+            with torch.no_grad():
+                fn(**{**good, name: held})
+            with torch.autograd.forward_ad.dual_level():
+                dual = torch.autograd.forward_ad.make_dual(t.detach().clone(), torch.ones_like(t))
+                with pytest.raises(RuntimeError, match="no forward derivative"):
+                    fn(**{**good, name: dual})
