@@ -633,7 +633,8 @@ int pl_paged_attention(int32_t dtype, int32_t cache_dtype, const void* q,
  * 2047 entries) and allowed may each be NULL, as may the three penalties
  * and prompt_lens (then 0); ids outside [0, vocab) match nothing.  Row strides
  * ld* are in elements, 0 for lists that all rows share.  out_dtype is PL_F32 or
- * the logits' own type; out may be the logits (same type and stride). */
+ * the logits' own type; out may be the logits (same type and stride), and its
+ * rows do not overlap. */
 int pl_adjust_logits(int32_t dtype, int32_t out_dtype, const void* logits, int64_t ld, void* out,
                      int64_t ld_out, int32_t rows, int32_t vocab, const void* tokens,
                      int32_t token_bytes, int64_t ld_tokens, int32_t history,

@@ -246,6 +246,11 @@ extern "C" int pl_adjust_logits(int32_t dtype, int32_t out_dtype, const void* lo
     pl_set_error("pl_adjust_logits: null pointer, or tokens of %d bytes", token_bytes);
     return PL_ERR_ARG;
   }
+  if (rows > 1 && ld_out < vocab) {
+    pl_set_error("pl_adjust_logits: rows of out %lld elements apart overlap (vocab %d)",
+                 (long long)ld_out, vocab);
+    return PL_ERR_ARG;
+  }
   const int64_t in_bytes = ((rows - 1) * ld + vocab) * pl_elem_size(dtype);
   const int64_t out_bytes = ((rows - 1) * ld_out + vocab) * pl_elem_size(out_dtype);
   if (pl_ranges_meet(logits, in_bytes, out, out_bytes) &&

@@ -170,3 +170,14 @@ def test_plain_rotation_is_a_complex_product():
     assert torch.equal(y[:, 6:], x[:, 6:])
     half = plain.rotate(x[:, [0, 2, 4, 1, 3, 5, 6, 7]], angle.cos(), angle.sin(), False)
     torch.testing.assert_close(half[:, [0, 3, 1, 4, 2, 5, 6, 7]], y)
+
+
+def test_logits_rows_of_the_output_never_overlap():
+    lib = _native.load()
+    p = 4096
+    args = dict(dtype=1, out_dtype=0, logits=p, ld=64, out=1 << 20, ld_out=63, rows=2, vocab=64, tokens=None, token_bytes=0,
+                ld_tokens=0, history=0, lens=None, prompt=None, rep=None, pres=None, freq=None, ids=None, values=None,
+                ld_bias=0, n_bias=0, allowed=None, ld_allowed=0, stream=None)
+    assert _refused(lib.pl_adjust_logits, args) == _native.PL_ERR_ARG
+    assert _refused(lib.pl_adjust_logits, args, ld_out=0) == _native.PL_ERR_ARG  # one row expanded to all
+    assert _refused(lib.pl_adjust_logits, args, ld=0, out=p, out_dtype=1, ld_out=0) == _native.PL_ERR_ARG  # in place
