@@ -584,7 +584,8 @@ int pl_check_right_padded(const void* mask, int32_t mask_dtype, int32_t B, int32
  * row, token and head, in elements.  q_out (and k_out, unless NULL) are
  * contiguous and hold the rotated q (k), 0 for tokens that are not live; they
  * do not overlap the inputs.  Two live tokens of one call never share a
- * place in the pages. */
+ * place in the pages, nor do two elements of the caches: in the order of their
+ * strides, each dimension steps past what the smaller ones reach. */
 int pl_rope_append(int32_t dtype, int32_t cache_dtype, const void* q, const int64_t* q_strides,
                    const void* k, const int64_t* k_strides, const void* v,
                    const int64_t* v_strides, void* q_out, void* k_out, void* key_cache,

@@ -1,4 +1,6 @@
 // Rotation by position and append to a paged key-value cache.
+#include <algorithm>
+
 #include "pl_paged.h"
 
 int pl_check_paged(const char* what, int32_t dtype, int32_t cache_dtype, const void* key_cache,
@@ -292,6 +294,23 @@ int launch(append_args a, int vec, hipStream_t s) {
   return pl_launch_status("pl_rope_append");
 }
 
+// Whether no two elements of a cache share a place: from the smallest stride up,
+// each dimension steps past all that those before it reach.
+bool elements_apart(const int64_t* strides, int32_t pages, int32_t kv_heads, int32_t page_size,
+                    int32_t dim) {
+  struct {
+    int64_t stride, size;
+  } d[3] = {{strides[0], pages}, {strides[1], kv_heads}, {strides[2], page_size}};
+  std::sort(d, d + 3, [](const auto& x, const auto& y) { return x.stride < y.stride; });
+  int64_t reach = dim;
+  for (const auto& x : d) {
+    if (x.size == 1) continue;
+    if (x.stride < reach) return false;
+    reach += (x.size - 1) * x.stride;
+  }
+  return true;
+}
+
 }  // namespace
 
 extern "C" int pl_rope_append(int32_t dtype, int32_t cache_dtype, const void* q,
@@ -338,6 +357,12 @@ extern "C" int pl_rope_append(int32_t dtype, int32_t cache_dtype, const void* q,
   if (!pl_grid_fits(tokens, kThreads)) {
     pl_set_error("pl_rope_append: too many tokens (%lld)", (long long)tokens);
     return PL_ERR_LIMIT;
+  }
+  if (num_pages > 0 && (key_cache == value_cache ||
+                        !elements_apart(key_strides, num_pages, kv_heads, page_size, dim) ||
+                        !elements_apart(value_strides, num_pages, kv_heads, page_size, dim))) {
+    pl_set_error("pl_rope_append: elements of the caches share their places");
+    return PL_ERR_ARG;
   }
   append_args a;
   a.q = q, a.k = k, a.v = v;

@@ -181,3 +181,20 @@ def test_logits_rows_of_the_output_never_overlap():
     assert _refused(lib.pl_adjust_logits, args) == _native.PL_ERR_ARG
     assert _refused(lib.pl_adjust_logits, args, ld_out=0) == _native.PL_ERR_ARG  # one row expanded to all
     assert _refused(lib.pl_adjust_logits, args, ld=0, out=p, out_dtype=1, ld_out=0) == _native.PL_ERR_ARG  # in place
+
+
+def test_append_never_writes_a_place_twice():
+    lib = _native.load()
+    s, p = _i64(64, 32, 16), 4096
+    dense, other = _i64(512, 256, 16), _i64(512, 16, 32)  # pages by head and by slot
+    args = dict(dtype=1, cache=1, q=p, qs=s, k=2 * p, ks=s, v=3 * p, vs=s, out=1 << 20, k_out=None, key=4 * p, keys=dense,
+                value=64 * p, values=other, pages=4, page=16, table=p, ld=2, cols=2, past=p, seq=None, rows=1, m=2, heads=2,
+                kv=2, dim=16, cos=p, sin=p, positions=8, rot=16, inter=0, ksc=None, vsc=None, stream=None)
+    one = lib.pl_rope_append
+    for bad in (_i64(0, 256, 16), _i64(512, 0, 16), _i64(512, 256, 0), _i64(504, 256, 16), _i64(512, 16, 16), _i64(512, 256, 8)):
+        assert _refused(one, args, keys=bad) == _native.PL_ERR_ARG
+        assert b"share their places" in lib.pl_last_error()
+        assert _refused(one, args, values=bad) == _native.PL_ERR_ARG
+        assert b"share their places" in lib.pl_last_error()
+    assert _refused(one, args, value=4 * p) == _native.PL_ERR_ARG
+    assert b"share their places" in lib.pl_last_error()

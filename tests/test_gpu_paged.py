@@ -557,3 +557,22 @@ def test_tensors_that_want_derivatives_are_refused(gpu):
                 dual = torch.autograd.forward_ad.make_dual(t.detach().clone(), torch.ones_like(t))
                 with pytest.raises(RuntimeError, match="no forward derivative"):
                     fn(**{**good, name: dual})
+
+
+def test_append_into_caches_of_any_layout_that_is_apart(gpu):
+    """Slices of wider buffers, keys beside values, one page or one key head of any stride."""
+    gen = torch.Generator().manual_seed(31)
+    cos, sin = rope_table(20, 32, device=gpu)
+    past = torch.tensor([3], dtype=torch.int32, device=gpu)
+    one = torch.zeros(1, 1, dtype=torch.int32, device=gpu)
+    for kv, pages in ((2, 3), (1, 3), (2, 1), (1, 1)):
+        x = torch.randn(1, 2, kv, 32, generator=gen).to(gpu)
+        wide = torch.zeros(pages, 2, kv, 16, 48, device=gpu)
+        by_slot = torch.zeros(pages, 16, kv, 2, 32, device=gpu).permute(3, 0, 2, 1, 4)
+        want = None
+        for key, value in ((wide[:, 0, :, :, :32], wide[:, 1, :, :, 16:]), (by_slot[0], by_slot[1]),
+                           (torch.zeros(pages, kv, 16, 32, device=gpu), torch.zeros(kv, 16, pages, 32, device=gpu).permute(2, 0, 1, 3))):
+            rope_append(x, x, x, key, value, one, past, cos, sin)
+            got = torch.stack((key, value))
+            want = got if want is None else want
+            assert torch.equal(got, want) and bool((got[:, 0, :, 3:5] != 0).any())
