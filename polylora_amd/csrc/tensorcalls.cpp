@@ -12,11 +12,13 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <c10/core/AutogradState.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
 #include <exception>
+#include <optional>
 #include <string>
 
 #include "../../include/polylora_hip.h"
@@ -111,6 +113,17 @@ void check_lead(const at::Tensor& t, const char* what) {
                   ": polylora_amd computes only on a ROCm GPU through its HIP library; got a CPU "
                   "tensor (there is no CPU fallback)");
 }
+// Launches go to the current GPU: the tensor's, for as long as this lives.
+class OnDevice {
+ public:
+  explicit OnDevice(const at::Tensor& t) {
+    if (c10::impl::getDeviceGuardImpl(c10::DeviceType::CUDA)->getDevice() != t.device()) guard_.emplace(t.device());
+  }
+
+ private:
+  std::optional<c10::DeviceGuard> guard_;
+};
+
 void check_type(const at::Tensor& t, const char* name, at::ScalarType type, int device) {
   if (t.scalar_type() != type)
     type_error(std::string(name) + " must be " + type_text(type) + ", not " + type_text(t.scalar_type()));
@@ -208,6 +221,7 @@ PyObject* rope_append(PyObject* const* a) {
   const at::Tensor* k_out = maybe(a[13], "k_out");
   check_lead(q, "rope_append");
   const int device = q.get_device();
+  const OnDevice current(q);
   if (q.dim() != 4 || k.dim() != 4 || q.size(0) != k.size(0) || q.size(1) != k.size(1) || q.size(3) != k.size(3))
     value_error("q and k must be [rows, M, heads, dim] and [rows, M, kv_heads, dim], not " +
                 shape_text(q.sizes()) + " and " + shape_text(k.sizes()));
@@ -264,6 +278,7 @@ PyObject* paged_attention(PyObject* const* a) {
   const at::Tensor& q = tensor(a[0], "q");
   check_lead(q, "paged_attention");
   const int device = q.get_device();
+  const OnDevice current(q);
   if (q.dim() != 3) value_error("q must be [rows, heads, dim], not " + shape_text(q.sizes()));
   const int64_t rows = q.size(0), heads = q.size(1), dim = q.size(2);
   const at::ScalarType type = q.scalar_type();
@@ -324,6 +339,7 @@ PyObject* adjust_logits(PyObject* const* a) {
   const at::Tensor& logits = tensor(a[0], "logits");
   check_lead(logits, "adjust_logits");
   const int device = logits.get_device();
+  const OnDevice current(logits);
   if (logits.dim() != 2) value_error("logits must be [rows, vocab], not " + shape_text(logits.sizes()));
   const int64_t rows = logits.size(0), vocab = logits.size(1);
   const at::ScalarType type = logits.scalar_type();

@@ -576,3 +576,16 @@ def test_append_into_caches_of_any_layout_that_is_apart(gpu):
             got = torch.stack((key, value))
             want = got if want is None else want
             assert torch.equal(got, want) and bool((got[:, 0, :, 3:5] != 0).any())
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs a second GPU")
+def test_tensors_of_a_gpu_that_is_not_the_current_one(gpu):
+    other = torch.device("cuda", 1)
+    with torch.cuda.device(other):
+        attend, append = _good(other)
+        attend["lens"].fill_(9)
+        attend["value_cache"].fill_(2.0)
+        want, turned = paged_attention(**attend), rope_append(**append)
+    with torch.cuda.device(gpu):
+        assert torch.equal(paged_attention(**attend), want) and torch.equal(rope_append(**append), turned)
+        assert torch.cuda.current_device() == gpu.index
