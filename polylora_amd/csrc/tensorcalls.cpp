@@ -406,6 +406,13 @@ PyObject* adjust_logits(PyObject* const* a) {
   return THPVariable_Wrap(std::move(out));
 }
 
+// (stream) -> pl_stream_capture_id of it
+PyObject* stream_capture_id(PyObject* const* a) {
+  void* stream = PyLong_AsVoidPtr(a[0]);
+  if (!stream && PyErr_Occurred()) throw Raised{};
+  return PyLong_FromLongLong(pl_stream_capture_id(stream));
+}
+
 template <PyObject* (*Fn)(PyObject* const*), Py_ssize_t N>
 PyObject* guarded(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (n != N) {
@@ -431,7 +438,8 @@ constexpr PyMethodDef method(const char* name) {
 }
 
 PyMethodDef methods[] = {method<rope_append, 15>("rope_append"), method<paged_attention, 15>("paged_attention"),
-                         method<adjust_logits, 12>("adjust_logits"), {nullptr, nullptr, 0, nullptr}};
+                         method<adjust_logits, 12>("adjust_logits"),
+                         method<stream_capture_id, 1>("stream_capture_id"), {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensor_calls", nullptr, -1, methods,
                       nullptr,               nullptr,         nullptr, nullptr};

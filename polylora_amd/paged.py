@@ -14,6 +14,8 @@ No counterpart in the reference, which leaves attention to the wrapped model.  T
 
 from __future__ import annotations
 
+import threading
+
 import torch
 
 from . import _native, sgmv
@@ -28,7 +30,6 @@ def rope_table(positions: int, rot: int, base: float = 10000.0, device=None) -> 
     i = torch.arange(rot // 2, dtype=torch.float64, device=device)
     angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * base ** (-2.0 * i / max(1, rot))
     return angle.cos().float(), angle.sin().float()
-
 
 
 def _stream(t: torch.Tensor) -> int:
@@ -58,34 +59,51 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_cache: to
 
 
 class _Scratch:
-    """What the attention's launches on one (device, stream) use: the workspace for parts of rows, and arrival
-    counters that are zero between launches (kept as the decode launch's hand-off counters are)."""
+    """What the attention's launches use that run one after the other: the workspace for parts of rows, and arrival
+    counters that are zero between launches."""
 
-    def __init__(self, device: int, stream: int) -> None:
-        where = torch.device("cuda", device)
-        self.workspace = sgmv._workspace(where, stream, "attention")
-        self.counters = sgmv._HandoffCounters(where)
-        self.bytes: dict[int, int] = {}  # by head size
+    def __init__(self, device: int) -> None:
+        self.workspace = sgmv._Workspace(torch.device("cuda", device))
+        self.counters: torch.Tensor | None = None
+        self.args: dict[int, tuple[int, int, int, int]] = {}  # by head size; replaced workspaces stay allocated
 
     def get(self, dim: int) -> tuple[int, int, int, int]:
-        need = self.bytes.get(dim)
-        if need is None:
-            need = self.bytes[dim] = int(_native.load().pl_paged_attention_workspace_bytes(dim))
-        buf = self.workspace.get(need)
-        counters = self.counters.get(_native.PL_ATTENTION_COUNTER_INTS)
-        return buf.data_ptr(), buf.numel(), counters.data_ptr(), counters.numel()
+        return self.args.get(dim) or self._make(dim)
+
+    def _make(self, dim: int) -> tuple[int, int, int, int]:
+        with _LOCK:
+            buf = self.workspace.get(int(_native.load().pl_paged_attention_workspace_bytes(dim)))
+            if self.counters is None:
+                # by a fill kernel on the current stream, the launch's, which a HIP graph records like any other
+                self.counters = torch.empty(_native.PL_ATTENTION_COUNTER_INTS, dtype=torch.int32, device=buf.device).zero_()
+            args = buf.data_ptr(), buf.numel(), self.counters.data_ptr(), self.counters.numel()
+            self.args[dim] = args
+            return args
 
 
+_LOCK = threading.Lock()
+# One for each (device, stream), for the life of the process.
 _SCRATCH: dict[tuple[int, int], _Scratch] = {}
+# What the last HIP graph captured on a (device, stream) got: (capture id, its own).  Graphs captured on one stream may
+# be replayed beside each other and beside the stream's own work, so they share nothing with either.  The memory is
+# the graph's, from the pool that it is captured into, and lasts as long as that.
+_CAPTURED: dict[tuple[int, int], tuple[int, _Scratch]] = {}
 
 
 def _scratch(t: torch.Tensor, stream: int) -> tuple[int, int, int, int]:
     device = t.get_device()
     if device < 0 or t.dim() == 0:
         return 0, 0, 0, 0  # the call refuses the tensor
-    held = _SCRATCH.get((device, stream))
+    key = device, stream
+    capture = _native.tensor_calls().stream_capture_id(stream)
+    if capture:
+        held = _CAPTURED.get(key)
+        if held is None or held[0] != capture or capture < 0:  # below 0: a capture of unknown id
+            held = _CAPTURED[key] = capture, _Scratch(device)
+        return held[1].get(t.shape[-1])
+    held = _SCRATCH.get(key)
     if held is None:
-        held = _SCRATCH[device, stream] = _Scratch(device, stream)
+        held = _SCRATCH.setdefault(key, _Scratch(device))
     return held.get(t.shape[-1])
 
 

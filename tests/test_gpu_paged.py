@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+from concurrent.futures import ThreadPoolExecutor
+
 import pytest
 import torch
 
@@ -433,6 +435,82 @@ def test_append_then_attend_in_a_graph(gpu, warm):
             assert torch.equal(other(), other_want)
             assert torch.equal(run(), got)
         torch.cuda.synchronize()
+
+
+def _capture(fn, stream=None):
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        out = fn()
+    return graph, out
+
+
+@pytest.mark.parametrize("warm", [True, False])
+def test_graphs_of_one_capture_stream_replayed_beside_each_other(gpu, warm):
+    """Two graphs captured on the same stream, with rows that are split, on two other streams at once, and eager calls
+    on the capture stream beside them."""
+    gen = torch.Generator().manual_seed(13)
+    steps = [_step(gpu, gen, rows=2, longest=9000)[0] for _ in range(3)]
+    want = [s() for s in steps]
+    capture = torch.cuda.Stream()
+    capture.wait_stream(torch.cuda.current_stream())
+    if warm:
+        with torch.cuda.stream(capture):
+            steps[2]()
+    torch.cuda.synchronize()
+    graphs = [_capture(s, capture) for s in steps[:2]]
+    streams = [torch.cuda.Stream() for _ in graphs]
+    got = [[], [], []]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for stream, (graph, out), kept in zip(streams, graphs, got):
+            with torch.cuda.stream(stream):
+                graph.replay()
+                kept.append(out.clone())
+        with torch.cuda.stream(capture):
+            got[2].append(steps[2]())
+    torch.cuda.synchronize()
+    for kept, one in zip(got, want):
+        assert all(torch.equal(x, one) for x in kept)
+
+
+def test_a_graph_keeps_its_scratch_when_others_are_captured(gpu):
+    """Head sizes that need larger workspaces, graphs captured and dropped, and eager allocations between replays."""
+    gen = torch.Generator().manual_seed(14)
+    run, _ = _step(gpu, gen, rows=2, longest=9000)
+    want = run()
+    torch.cuda.synchronize()
+    graph, out = _capture(run)
+    for i in range(4):
+        other, _ = _step(gpu, gen, rows=2, longest=3000 + i)
+        torch.cuda.synchronize()
+        dropped, _ = _capture(other)
+        dropped.replay()
+        torch.cuda.synchronize()
+        del dropped
+        noise = [torch.full((1 << 20,), -1, dtype=torch.int32, device=gpu) for _ in range(8)]
+        torch.cuda.synchronize()
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and all(bool((x == -1).all()) for x in noise)
+
+
+def test_threads_that_share_a_stream(gpu):
+    gen = torch.Generator().manual_seed(15)
+    steps = [_step(gpu, gen, rows=2, longest=5000)[0] for _ in range(2)]
+    want = [s() for s in steps]
+    stream = torch.cuda.Stream()  # no scratch yet
+    torch.cuda.synchronize()
+
+    def work(step):
+        with torch.cuda.stream(stream):
+            return [step() for _ in range(30)]
+
+    with ThreadPoolExecutor(2) as pool:
+        got = list(pool.map(work, steps))
+    torch.cuda.synchronize()
+    for kept, one in zip(got, want):
+        assert all(torch.equal(x, one) for x in kept)
 
 
 # ----------------------------------------------------------------------------- refusals
