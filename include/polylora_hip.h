@@ -564,8 +564,8 @@ int pl_check_right_padded(const void* mask, int32_t mask_dtype, int32_t B, int32
  * page_size tokens (a power of two of at least 16): element (page, head,
  * slot, d) at page * strides[0] + head * strides[1] + slot * strides[2] + d,
  * so any order of page, head and slot.  page_table[row * table_ld + i] is
- * the page of the row's tokens i * page_size and up; ids outside
- * [0, num_pages) hold nothing.  The element type is the model's, or
+ * the page of the row's tokens i * page_size and up (table_ld 0: one list that
+ * all rows share); ids outside [0, num_pages) hold nothing.  The element type is the model's, or
  * PL_F8E4M3 for 16-bit models, an element then standing for its value times
  * k_scale[head] or v_scale[head] (else NULL).  Pointers and strides of the
  * caches are whole 16-byte pieces; dim is a multiple of 16 up to 256. */

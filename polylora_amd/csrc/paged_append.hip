@@ -36,7 +36,7 @@ int pl_check_paged(const char* what, int32_t dtype, int32_t cache_dtype, const v
                  page_size);
     return PL_ERR_LIMIT;
   }
-  if (num_pages < 0 || max_pages < 0 || table_ld < max_pages ||
+  if (num_pages < 0 || max_pages < 0 || (table_ld < max_pages && table_ld != 0) ||
       (int64_t)max_pages * page_size > INT32_MAX) {
     pl_set_error("%s: bad page table (pages %d, columns %d, row stride %lld)", what, num_pages,
                  max_pages, (long long)table_ld);

@@ -198,3 +198,17 @@ def test_append_never_writes_a_place_twice():
         assert b"share their places" in lib.pl_last_error()
     assert _refused(one, args, value=4 * p) == _native.PL_ERR_ARG
     assert b"share their places" in lib.pl_last_error()
+
+
+def test_a_shared_page_table_is_no_reason_to_refuse():
+    """table_ld 0 passes the table's check and meets the next one; a row that runs into the next is refused as before."""
+    lib = _native.load()
+    s, p = _i64(64, 32, 16), 4096
+    args = dict(dtype=1, cache=1, q=p, qs=_i64(64, 16), key=p, keys=s, value=p, values=s, pages=4, page=16, table=p, ld=0,
+                cols=2, lens=None, rows=2, heads=2, kv=2, dim=16, scale=1.0, window=0, ksc=None, vsc=None, out=1 << 20,
+                ws=p, wsb=1 << 30, counters=p, ints=_native.PL_ATTENTION_COUNTER_INTS, stream=None)
+    _refused(lib.pl_paged_attention, args)
+    assert b"null pointer" in lib.pl_last_error()
+    for ld in (1, -2):
+        _refused(lib.pl_paged_attention, args, ld=ld)
+        assert b"page table" in lib.pl_last_error()

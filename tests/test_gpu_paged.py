@@ -667,3 +667,21 @@ def test_tensors_of_a_gpu_that_is_not_the_current_one(gpu):
     with torch.cuda.device(gpu):
         assert torch.equal(paged_attention(**attend), want) and torch.equal(rope_append(**append), turned)
         assert torch.cuda.current_device() == gpu.index
+
+
+def test_rows_that_share_one_page_table(gpu):
+    """A table expanded over the rows: several continuations of one prompt, of lengths of their own."""
+    gen = torch.Generator().manual_seed(32)
+    key, value, table, _, _ = pool(gen, 1, [400], 2, 64, 16, torch.bfloat16)
+    key, value, table = key.to(gpu), value.to(gpu), table.to(gpu)
+    q = torch.randn(5, 4, 64, generator=gen).to(torch.bfloat16).to(gpu)
+    lens = torch.tensor([400, 1, 0, 17, 399], dtype=torch.int32, device=gpu)
+    want = paged_attention(q, key, value, table.repeat(5, 1), lens)
+    assert torch.equal(paged_attention(q, key, value, table.expand(5, -1), lens), want)
+    x = torch.randn(5, 1, 2, 64, generator=gen).to(torch.bfloat16).to(gpu)
+    past = torch.tensor([0, 31, 16, 350, 128], dtype=torch.int32, device=gpu)
+    cos, sin = rope_table(400, 64, device=gpu)
+    caches = [[c.clone() for c in (key, value)] for _ in range(2)]
+    for (k, v), t in zip(caches, (table.repeat(5, 1), table.expand(5, -1))):
+        rope_append(x, x, x, k, v, t, past, cos, sin)
+    assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(*caches))
