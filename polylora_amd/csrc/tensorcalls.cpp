@@ -330,7 +330,8 @@ List list(const at::Tensor& t, const char* name, at::ScalarType type, int device
     value_error(std::string(name) + " must be [" + std::to_string(rows) + ", n], or [n] for all rows, not " +
                 shape_text(t.sizes()));
   check_last(t, name);
-  return {t.const_data_ptr(), size32(t.size(-1), name), t.dim() == 2 ? t.stride(0) : 0};
+  // the stride of a single row says nothing
+  return {t.const_data_ptr(), size32(t.size(-1), name), t.dim() == 2 && rows > 1 ? t.stride(0) : 0};
 }
 
 // (logits, tokens, lens, prompt_lens, repetition, presence, frequency, bias_ids, bias_values, allowed, out,

@@ -217,3 +217,14 @@ def test_tensors_that_want_derivatives_are_refused(gpu):
             dual = torch.autograd.forward_ad.make_dual(t.detach().clone(), torch.ones_like(t))
             with pytest.raises(RuntimeError, match="no forward derivative"):
                 adjust_logits(**{**good, name: dual})
+
+
+def test_lists_of_one_row_of_any_stride(gpu):
+    """A single row's ids as a slice of a wider buffer beside dense values."""
+    a = {name: t.to(gpu) for name, t in build(torch.Generator().manual_seed(9), 1, 300, torch.bfloat16, 20, 6, True).items()}
+    want = adjust_logits(**a)
+    for name in ("bias_ids", "tokens", "allowed"):
+        wide = torch.zeros(1, a[name].shape[1] + 5, dtype=a[name].dtype, device=gpu)
+        wide[:, : a[name].shape[1]] = a[name]
+        assert torch.equal(adjust_logits(**{**a, name: wide[:, : a[name].shape[1]]}), want)
+    assert torch.equal(adjust_logits(**{**a, "bias_values": a["bias_values"][0]}), want)  # one list, a row or not
