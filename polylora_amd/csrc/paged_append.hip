@@ -52,7 +52,9 @@ int pl_check_paged(const char* what, int32_t dtype, int32_t cache_dtype, const v
     const int64_t e = 16 / pl_cache_elem_size(cache_dtype);
     bool ok = reinterpret_cast<uintptr_t>(key_cache) % 16 == 0 &&
               reinterpret_cast<uintptr_t>(value_cache) % 16 == 0;
-    for (int i = 0; i < 3; ++i) ok = ok && key_strides[i] % e == 0 && value_strides[i] % e == 0;
+    const int32_t sizes[3] = {num_pages, kv_heads, page_size};
+    for (int i = 0; i < 3; ++i)  // a dimension of one is never stepped along
+      ok = ok && (sizes[i] <= 1 || (key_strides[i] % e == 0 && value_strides[i] % e == 0));
     if (!ok) {
       pl_set_error("%s: cache pointers and strides must be whole 16-byte pieces", what);
       return PL_ERR_ALIGN;

@@ -138,7 +138,7 @@ void check_dense(const at::Tensor& t, const char* name) {
   if (!t.is_contiguous()) value_error(std::string(name) + " must be contiguous");
 }
 void check_last(const at::Tensor& t, const char* name) {
-  if (t.numel() && t.stride(-1) != 1)
+  if (t.numel() && t.size(-1) > 1 && t.stride(-1) != 1)
     value_error(std::string("the last dimension of ") + name + " must be contiguous");
 }
 // A contiguous int32 or fp32 vector of n elements; null where the tensor is.

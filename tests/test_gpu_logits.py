@@ -228,3 +228,14 @@ def test_lists_of_one_row_of_any_stride(gpu):
         wide[:, : a[name].shape[1]] = a[name]
         assert torch.equal(adjust_logits(**{**a, name: wide[:, : a[name].shape[1]]}), want)
     assert torch.equal(adjust_logits(**{**a, "bias_values": a["bias_values"][0]}), want)  # one list, a row or not
+
+
+def test_dimensions_of_one_may_have_any_stride(gpu):
+    """A vocabulary of one, a history of one token, a list of one bias."""
+    x = torch.tensor([[2.0, 3.0]], device=gpu).t()
+    one = torch.zeros(1, 2, dtype=torch.int32, device=gpu).t()
+    lens = torch.ones(2, dtype=torch.int32, device=gpu)
+    assert x.stride(1) == one.stride(1) == 2
+    got = adjust_logits(x, tokens=one, lens=lens, presence=torch.ones(2, device=gpu), bias_ids=one,
+                        bias_values=torch.full((1, 2), 0.5, device=gpu).t())
+    assert got.tolist() == [[1.5], [2.5]]

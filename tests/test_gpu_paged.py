@@ -685,3 +685,22 @@ def test_rows_that_share_one_page_table(gpu):
     for (k, v), t in zip(caches, (table.repeat(5, 1), table.expand(5, -1))):
         rope_append(x, x, x, k, v, t, past, cos, sin)
     assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(*caches))
+
+
+def test_dimensions_of_one_may_have_any_stride(gpu):
+    """One key head, one page or one column of a table, out of buffers whose other strides are odd."""
+    gen = torch.Generator().manual_seed(33)
+    key, value = (torch.randn(1, 1, 16, 32, generator=gen).to(gpu) for _ in range(2))
+    x = torch.randn(3, 1, 2, 32, generator=gen).to(gpu)
+    lens = torch.tensor([16, 3, 9], dtype=torch.int32, device=gpu)
+    table = torch.zeros(3, 1, dtype=torch.int32, device=gpu)
+    odd_key, odd_value = (torch.as_strided(c.clone(), (1, 1, 16, 32), (515, 513, 32, 1)) for c in (key, value))
+    odd_table = torch.zeros(1, 3, dtype=torch.int32, device=gpu).t()
+    assert odd_table.stride(1) == 3
+    want = paged_attention(x[:, 0], key, value, table, lens)
+    assert torch.equal(paged_attention(x[:, 0], odd_key, odd_value, odd_table, lens), want)
+    cos, sin = rope_table(16, 32, device=gpu)
+    past = torch.tensor([4, 5, 6], dtype=torch.int32, device=gpu)
+    rope_append(x, x[:, :, :1], x[:, :, 1:], key, value, table, past, cos, sin)
+    rope_append(x, x[:, :, :1], x[:, :, 1:], odd_key, odd_value, odd_table, past, cos, sin)
+    assert torch.equal(odd_key, key) and torch.equal(odd_value, value)
