@@ -156,7 +156,8 @@ void check_status(int rc, const char* what) {
     runtime_error(std::string(what) + " failed (status " + std::to_string(rc) + "): " + pl_last_error());
 }
 
-// The cache arguments of both calls over a paged cache.
+// The cache arguments of both calls over a paged cache.  A written cache that
+// shares its memory until then (a lazy clone) gets its own.
 struct Cache {
   int32_t code, num_pages, page_size, kv_heads, max_pages;
   void *key, *value;
@@ -168,7 +169,7 @@ struct Cache {
 
 Cache check_cache(const at::Tensor& key, const at::Tensor& value, const at::Tensor& table, int64_t rows,
                   int64_t dim, at::ScalarType type, int device, const at::Tensor* k_scale,
-                  const at::Tensor* v_scale) {
+                  const at::Tensor* v_scale, bool written) {
   if (key.dim() != 4 || key.sizes() != value.sizes())
     value_error("the caches must be [pages, kv_heads, page_size, head_dim], both alike, not " +
                 shape_text(key.sizes()) + " and " + shape_text(value.sizes()));
@@ -205,7 +206,8 @@ Cache check_cache(const at::Tensor& key, const at::Tensor& value, const at::Tens
   check_last(table, "page_table");
   c.num_pages = size32(key.size(0), "the cache"), c.page_size = size32(page_size, "a page");
   c.kv_heads = size32(kv_heads, "the cache"), c.max_pages = size32(table.size(1), "page_table");
-  c.key = const_cast<void*>(key.const_data_ptr()), c.value = const_cast<void*>(value.const_data_ptr());
+  c.key = written ? key.mutable_data_ptr() : const_cast<void*>(key.const_data_ptr());
+  c.value = written ? value.mutable_data_ptr() : const_cast<void*>(value.const_data_ptr());
   c.key_strides = key.strides().data(), c.value_strides = value.strides().data();
   c.table = static_cast<const int32_t*>(table.const_data_ptr());
   // a table of one row or column may have any stride there
@@ -233,7 +235,7 @@ PyObject* rope_append(PyObject* const* a) {
   check_shape(v, "v", k.sizes());
   for (const at::Tensor* t : {&q, &k, &v}) check_last(*t, "q, k and v");
   const Cache c = check_cache(tensor(a[3], "key_cache"), tensor(a[4], "value_cache"), tensor(a[5], "page_table"),
-                              rows, dim, type, device, maybe(a[11], "k_scale"), maybe(a[12], "v_scale"));
+                              rows, dim, type, device, maybe(a[11], "k_scale"), maybe(a[12], "v_scale"), true);
   if (c.kv_heads != kv_heads || kv_heads == 0 || heads % kv_heads)
     value_error(std::to_string(heads) + " heads and " + std::to_string(kv_heads) + " key heads over a cache of " +
                 std::to_string(c.kv_heads));
@@ -285,7 +287,7 @@ PyObject* paged_attention(PyObject* const* a) {
   const int32_t code = dtype_code(type);
   check_last(q, "q");
   const Cache c = check_cache(tensor(a[1], "key_cache"), tensor(a[2], "value_cache"), tensor(a[3], "page_table"),
-                              rows, dim, type, device, maybe(a[7], "k_scale"), maybe(a[8], "v_scale"));
+                              rows, dim, type, device, maybe(a[7], "k_scale"), maybe(a[8], "v_scale"), false);
   if (c.kv_heads == 0 || heads % c.kv_heads)
     value_error(std::to_string(heads) + " heads over a cache of " + std::to_string(c.kv_heads) + " key heads");
   const int32_t* lens = vector<int32_t>(&tensor(a[4], "lens"), "lens", at::kInt, device, rows);

@@ -704,3 +704,14 @@ def test_dimensions_of_one_may_have_any_stride(gpu):
     rope_append(x, x[:, :, :1], x[:, :, 1:], key, value, table, past, cos, sin)
     rope_append(x, x[:, :, :1], x[:, :, 1:], odd_key, odd_value, odd_table, past, cos, sin)
     assert torch.equal(odd_key, key) and torch.equal(odd_value, value)
+
+
+def test_append_into_a_lazy_clone_leaves_the_original(gpu):
+    _, good = _good(gpu)
+    key, value = good["key_cache"], good["value_cache"]
+    good["k"], good["v"] = torch.ones_like(good["k"]), torch.ones_like(good["v"])
+    good["page_table"] = torch.tensor([[0], [1]], dtype=torch.int32, device=gpu)
+    copies = torch._lazy_clone(key), torch._lazy_clone(value)
+    rope_append(**{**good, "key_cache": copies[0], "value_cache": copies[1]})
+    assert not key.any() and not value.any()
+    assert bool(copies[0].any()) and bool(copies[1].any())
