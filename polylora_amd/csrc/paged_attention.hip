@@ -918,7 +918,9 @@ extern "C" int pl_paged_attention(int32_t dtype, int32_t cache_dtype, const void
   if (window > 0 && longest > (int64_t)window + 31) longest = (int64_t)window + 31;
   const int64_t atom = 32 * kWaves, per_pair = longest > atom ? (longest + atom - 1) / atom : 1;
   const int64_t pairs = (int64_t)rows * kv_heads * a.col_tiles;
-  if (pairs > INT32_MAX / per_pair) {
+  // token and atom numbers are 32-bit, a tile past a row's end and a run past the last one included
+  if ((int64_t)max_pages * page_size > INT32_MAX - 2 * atom ||
+      pairs > (INT32_MAX - kWorkersMax * kWaves) / per_pair) {
     pl_set_error("pl_paged_attention: %lld rows and key heads of up to %lld tokens are too many",
                  (long long)pairs, (long long)longest);
     return PL_ERR_LIMIT;

@@ -212,3 +212,16 @@ def test_a_shared_page_table_is_no_reason_to_refuse():
     for ld in (1, -2):
         _refused(lib.pl_paged_attention, args, ld=ld)
         assert b"page table" in lib.pl_last_error()
+
+
+def test_attention_counts_stay_within_32_bits():
+    """Table columns whose last token's tile, and batches whose last run, would pass them."""
+    lib = _native.load()
+    s, p = _i64(64, 32, 16), 4096
+    args = dict(dtype=1, cache=1, q=p, qs=_i64(64, 16), key=p, keys=s, value=p, values=s, pages=4, page=16, table=p,
+                ld=1 << 27, cols=2, lens=p, rows=1, heads=2, kv=2, dim=16, scale=1.0, window=0, ksc=None, vsc=None, out=1 << 60,
+                ws=p, wsb=1 << 30, counters=p, ints=_native.PL_ATTENTION_COUNTER_INTS, stream=None)
+    one = lib.pl_paged_attention
+    assert _refused(one, args, cols=(1 << 27) - 1) == _native.PL_ERR_LIMIT
+    assert _refused(one, args, cols=(1 << 27) - 1, window=5) == _native.PL_ERR_LIMIT
+    assert _refused(one, args, rows=(1 << 30) - 1) == _native.PL_ERR_LIMIT
