@@ -19,6 +19,9 @@ constexpr uint32_t kSeen = 1u << 31;
 constexpr int kHistoryMax = (int)kCountMask, kBiasMax = (int)kBiasMask;
 constexpr int kVec = 4;     // logits of a thread's load
 constexpr int kPasses = 4;  // loads of a thread: its share of the slice
+constexpr int kThreadsMax = 1024;
+// Places up to the end of the last slice are 32-bit.
+constexpr int kVocabMax = INT32_MAX - kThreadsMax * kVec * kPasses;
 
 struct logits_args {
   const void* logits;
@@ -198,7 +201,7 @@ constexpr int kLongHistory = 4096;
 
 template <int DT, int OT>
 int launch(logits_args a, hipStream_t s) {
-  const int threads = a.history > kLongHistory ? 1024 : 256;
+  const int threads = a.history > kLongHistory ? kThreadsMax : 256;
   const int slice = threads * kVec * kPasses;
   a.slices = (a.vocab + slice - 1) / slice;
   const int64_t blocks = (int64_t)a.rows * a.slices;
@@ -208,8 +211,8 @@ int launch(logits_args a, hipStream_t s) {
   }
   const dim3 grid((unsigned)blocks);
   const size_t lds = (size_t)((a.n_bias + 3) & ~3) * 12;
-  if (threads == 1024)
-    pl_adjust_logits_kernel<DT, OT, 1024><<<grid, 1024, lds, s>>>(a);
+  if (threads == kThreadsMax)
+    pl_adjust_logits_kernel<DT, OT, kThreadsMax><<<grid, kThreadsMax, lds, s>>>(a);
   else
     pl_adjust_logits_kernel<DT, OT, 256><<<grid, 256, lds, s>>>(a);
   return pl_launch_status("pl_adjust_logits");
@@ -238,6 +241,10 @@ extern "C" int pl_adjust_logits(int32_t dtype, int32_t out_dtype, const void* lo
   if (history > kHistoryMax || n_bias > kBiasMax) {
     pl_set_error("pl_adjust_logits: at most %d tokens of history and %d biases (got %d and %d)",
                  kHistoryMax, kBiasMax, history, n_bias);
+    return PL_ERR_LIMIT;
+  }
+  if (vocab > kVocabMax) {
+    pl_set_error("pl_adjust_logits: at most %d logits a row (got %d)", kVocabMax, vocab);
     return PL_ERR_LIMIT;
   }
   if (rows == 0 || vocab == 0) return PL_OK;

@@ -225,3 +225,13 @@ def test_attention_counts_stay_within_32_bits():
     assert _refused(one, args, cols=(1 << 27) - 1) == _native.PL_ERR_LIMIT
     assert _refused(one, args, cols=(1 << 27) - 1, window=5) == _native.PL_ERR_LIMIT
     assert _refused(one, args, rows=(1 << 30) - 1) == _native.PL_ERR_LIMIT
+
+
+def test_logits_places_stay_within_32_bits():
+    lib = _native.load()
+    p = 4096
+    args = dict(dtype=1, out_dtype=0, logits=p, ld=1 << 31, out=1 << 60, ld_out=1 << 31, rows=1, vocab=(1 << 31) - 1, tokens=None,
+                token_bytes=0, ld_tokens=0, history=0, lens=None, prompt=None, rep=None, pres=None, freq=None, ids=None,
+                values=None, ld_bias=0, n_bias=0, allowed=None, ld_allowed=0, stream=None)
+    assert _refused(lib.pl_adjust_logits, args) == _native.PL_ERR_LIMIT
+    assert _refused(lib.pl_adjust_logits, args, vocab=(1 << 31) - (1 << 14)) == _native.PL_ERR_LIMIT
