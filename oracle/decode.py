@@ -68,8 +68,8 @@ def gather(key, value, table, lens, row: int, window=None, k_scale=None, v_scale
     pages, slots = (torch.tensor(x) for x in zip(*places))
     out = []
     for cache, scale in ((key, k_scale), (value, v_scale)):
-        x = cache.double() if cache.dtype == torch.float8_e4m3fn else cache
-        x = x[pages, :, slots].double()
+        bits = cache.view(torch.uint8) if cache.dtype == torch.float8_e4m3fn else cache  # 8-bit floats take no lists
+        x = bits[pages, :, slots].view(cache.dtype).double()
         out.append(x if scale is None else x * scale.double()[:, None])
     return out[0], out[1]
 

@@ -377,6 +377,121 @@ def test_append_stores_quotients_in_8_bits(gpu, dtype):
     assert torch.equal(value[0, :, 0].float().cpu(), want)
 
 
+# ----------------------------------------------------------------------------- what large batches alone reach
+
+
+def _ragged(gen, rows, low, high):
+    return torch.randint(low, high + 1, (rows,), generator=gen).tolist()
+
+
+@pytest.mark.parametrize("dtype,fp8", [(d, False) for d in DTYPES] + [(torch.float16, True)])
+@pytest.mark.parametrize("kv_heads,heads,dim", [(16, 16, 64), (16, 32, 128)])
+def test_attention_of_more_pairs_than_waves(gpu, dtype, fp8, kv_heads, heads, dim):
+    """4800 pairs: every wave takes a run of whole pairs, which begin and end inside rows, some of them empty."""
+    gen = torch.Generator().manual_seed(41)
+    check_attention(gpu, dtype, _ragged(gen, 300, 0, 200), heads, kv_heads, dim, 16, fp8=fp8)
+
+
+@pytest.mark.parametrize("dtype,fp8", [(torch.bfloat16, False), (torch.float16, False), (torch.bfloat16, True)])
+@pytest.mark.parametrize("rows,low,high", [(70, 400, 520), (6, 6000, 8192), (40, 1, 4000)])
+def test_attention_of_many_tokens(gpu, dtype, fp8, rows, low, high):
+    """2048 atoms and more: one workgroup on a CU, pairs alone and split."""
+    gen = torch.Generator().manual_seed(42)
+    check_attention(gpu, dtype, _ragged(gen, rows, low, high), 8, 8, 128, 64, fp8=fp8)
+
+
+@pytest.mark.parametrize("dtype,fp8", [(d, False) for d in DTYPES] + [(d, True) for d in DTYPES[:2]])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("lens", [[100] * 40 + [0, 1, 33], [3000, 17]])
+def test_attention_over_a_pool_larger_than_the_last_cache(gpu, dtype, fp8, dim, lens):
+    """Pages marked as read once, out of more than 256 MiB of them: the bits that a small pool gives."""
+    gen = torch.Generator().manual_seed(43)
+    kv_heads, page = 4, 64
+    key, value, table, ks, vs = pool(gen, len(lens), lens, kv_heads, dim, page, dtype, fp8)
+    n = key.shape[0]
+    large = (257 << 20) // (2 * kv_heads * page * dim * key.element_size()) + 1
+    ids = torch.randperm(large, generator=gen)[:n]
+    up = {"k_scale": ks.to(gpu), "v_scale": vs.to(gpu)} if fp8 else {}
+    q = torch.randn(len(lens), 8, dim, generator=gen).to(dtype).to(gpu)
+    lens = torch.tensor(lens, dtype=torch.int32, device=gpu)
+    want = paged_attention(q, key.to(gpu), value.to(gpu), table.to(gpu), lens, **up)
+    assert not want.isnan().any()
+    wide = []
+    for c in (key, value):
+        bits = c.view(torch.uint8) if fp8 else c
+        x = torch.full((large, *c.shape[1:]), 127 if fp8 else float("nan"), dtype=bits.dtype, device=gpu)
+        x[ids.to(gpu)] = bits.to(gpu)
+        wide.append(x.view(c.dtype))
+    moved = torch.where((table >= 0) & (table < n), ids[table.clamp(0, n - 1).long()], -1).int()
+    assert torch.equal(paged_attention(q, *wide, moved.to(gpu), lens, **up), want)
+
+
+def _append_by_rows(q, k, v, key, value, table, past, cos, sin, seq, interleaved, ks, vs):
+    """oracle.decode.rope_append, a row's tokens at once."""
+    m, page = q.shape[1], key.shape[2]
+    out = [torch.zeros(x.shape, dtype=torch.float64) for x in (q, k)]
+    caches = [key.double().clone(), value.double().clone()]
+    for b in range(q.shape[0]):
+        n = min(m, int(seq[b]))
+        pos = int(past[b]) + torch.arange(n)
+        c, s = (t[pos].double()[:, None] for t in (cos, sin))
+        h = c.shape[-1]
+        for x, y in zip((q, k), out):
+            x = x[b, :n].double()
+            i = torch.arange(h) * 2 if interleaved else torch.arange(h)
+            j = i + 1 if interleaved else i + h
+            y[b, :n] = x
+            y[b, :n, :, i], y[b, :n, :, j] = x[..., i] * c - x[..., j] * s, x[..., j] * c + x[..., i] * s
+        for cache, x, scale in zip(caches, (out[1][b, :n], v[b, :n].double()), (ks, vs)):
+            x = x if scale is None else (x / scale.double()[:, None]).clamp(-448, 448)
+            cache[table[b].long()[pos // page], :, pos % page] = x
+    return *out, *caches
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_the_plain_append_by_rows_is_the_plain_append(interleaved):
+    gen = torch.Generator().manual_seed(44)
+    key, value, table, ks, vs = pool(gen, 3, [40, 20, 33], 2, 32, 16, torch.bfloat16, True)
+    q, k, v = (torch.randn(3, 7, h, 32, generator=gen) for h in (4, 2, 2))
+    past, seq = torch.tensor([33, 5, 0]), torch.tensor([7, 0, 4])
+    cos, sin = rope_table(40, 20)
+    args = (q, k, v, key, value, table, past, cos, sin, seq, interleaved, ks, vs)
+    for a, b in zip(_append_by_rows(*args), plain.rope_append(*args)):
+        assert torch.equal(a.isnan(), b.isnan())
+        torch.testing.assert_close(a.nan_to_num(0.0), b.nan_to_num(0.0), rtol=1e-14, atol=1e-14)
+
+
+@pytest.mark.parametrize("dtype,fp8", [(d, False) for d in DTYPES] + [(d, True) for d in DTYPES[:2]])
+@pytest.mark.parametrize("rows,m,heads,kv_heads,dim,rot,interleaved", [
+    (1, 4099, 8, 2, 64, 64, False),  # two tokens to a workgroup, an odd number of them
+    (3, 2735, 4, 2, 64, 64, True),  # four
+    (3, 5461, 3, 1, 80, 40, False),
+    (2, 4100, 4, 1, 256, 256, False),  # as many as its places leave threads for
+    (5, 1700, 6, 2, 48, 30, True),  # single elements
+])
+def test_append_of_many_tokens(gpu, dtype, fp8, rows, m, heads, kv_heads, dim, rot, interleaved):
+    """Outputs past the caches and several tokens to a workgroup, the last one part full, rows part full."""
+    gen = torch.Generator().manual_seed(45)
+    past, page = torch.randint(0, 50, (rows,), generator=gen), 64
+    seq = torch.randint(m // 2, m + 1, (rows,), generator=gen)
+    seq[0] = m
+    key, value, table, ks, vs = pool(gen, rows, [int(p + n) for p, n in zip(past, seq)], kv_heads, dim, page, dtype, fp8)
+    q, k, v = torch.randn(rows, m, heads + 2 * kv_heads, dim, generator=gen).to(dtype).split((heads, kv_heads, kv_heads), 2)
+    cos, sin = rope_table(m + 50, rot)
+    args = (q, k, v, key, value, table, past, cos, sin, seq, interleaved, ks, vs)
+    want = _append_by_rows(*args)
+    sizes = [_append_by_rows(q.abs(), k.abs(), v.abs(), key.float().abs(), value.float().abs(), table, past, cos.abs(),
+                             sign * sin.abs(), seq, interleaved, ks, vs) for sign in (-1, 1)]
+    sizes = [torch.maximum(a, b) for a, b in zip(*sizes)]
+    gkey, gvalue, k_out = key.to(gpu), value.to(gpu), torch.full((rows, m, kv_heads, dim), 7.0, dtype=dtype, device=gpu)
+    up = {"k_scale": ks.to(gpu), "v_scale": vs.to(gpu)} if fp8 else {}
+    q_out = rope_append(q.to(gpu), k.to(gpu), v.to(gpu), gkey, gvalue, table.to(gpu), past.int().to(gpu), cos.to(gpu),
+                        sin.to(gpu), seq_lens=seq.int().to(gpu), interleaved=interleaved, k_out=k_out, **up)
+    for got, one, size, kind in zip((q_out, k_out, gkey, gvalue), want, sizes, (dtype, dtype, FP8 if fp8 else dtype,
+                                                                             FP8 if fp8 else dtype)):
+        check_append(got, one, kind, size)
+
+
 # ----------------------------------------------------------------------------- streams and graphs
 
 
