@@ -25,13 +25,15 @@
 //                 pairs them up by byte permutes.  It gets the outputs of
 //                 query i, so the maximum, the sum and the rescaling of a query
 //                 all stay in the lanes of its column.
-// Weights go into the product as two 16-bit numbers, p = hi + lo: one product
-// more on matrix units that have little else to do, and the output keeps the
-// error of its own rounding.  bf16 keeps them to 2^-15 of themselves.  fp16 ends
-// at 2^-24, so its weights are taken 2^15 times as large, to 32768 for the
-// highest score (l and o alike, so the factor goes out in o / l), and kept to
-// 2^-21 of themselves or 2^-39 of the largest.  Without it tokens 17.3 and more
-// below the highest score counted in l and not in o.
+// Weights go into the product as sums of 16-bit numbers, a product more for each
+// on matrix units that have little else to do: three bf16 are the fp32 weight
+// itself, two fp16 keep 2^-21 of it, and the output keeps the error of its own
+// rounding (two bf16, 2^-15 of a weight, put 8 times as many outputs on the other
+// side of theirs, 0.33 % of them, for 0.5 us of 110 over 256 rows to 1024 tokens
+// and 0.7 of 21 over 64 of 512).  fp16 ends at 2^-24, so its weights are taken
+// 2^15 times as large, to 32768 for the highest score (l and o alike, so the
+// factor goes out in o / l), and end at 2^-39 of the largest; without it tokens
+// 17.3 and more below the highest score counted in l and not in o.
 //
 // Work is split by tokens: the launch is a fixed number of workgroups, and the
 // batch's atoms (kAtom tokens of one row and key head) are dealt out in equal
@@ -84,6 +86,7 @@ struct shape {
   static constexpr int kTokens = 4 * kSubs;          // tokens of a lane per tile
   // Queries in LDS where keys, values and outputs fill the registers.
   static constexpr bool kQueryLds = DP == 256 || DT == PL_F32;
+  static constexpr int kParts = DT == PL_BF16 ? 3 : 2;  // 16-bit parts of a weight
   // log2 of what weights are multiplied by, that their 16-bit parts keep small ones.
   static constexpr float kLift = DT == PL_F16 ? 15.f : 0.f;
 };
@@ -198,11 +201,14 @@ __device__ __forceinline__ uint32_t pack2_down(float a, float b) {
   else
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
 }
-// lo, but at least the smallest fp16 number where hi is not 0 (neither is negative).
-__device__ __forceinline__ uint32_t least_beside(uint32_t hi, uint32_t lo) {
+// Numbers that are not negative, raised to the type's smallest normal one (fp16:
+// smallest of all) beside ones that are not 0 in `first`.
+template <int DT>
+__device__ __forceinline__ uint32_t at_least_smallest(uint32_t x, uint32_t first) {
   typedef uint16_t pair __attribute__((ext_vector_type(2)));
-  const pair least = __builtin_elementwise_min(__builtin_bit_cast(pair, hi), pair{1, 1});
-  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(pair, lo), least));
+  constexpr uint16_t kSmallest = DT == PL_BF16 ? 0x80 : 1;
+  const pair least = __builtin_elementwise_min(__builtin_bit_cast(pair, first), pair{kSmallest, kSmallest});
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(pair, x), least));
 }
 
 // First element of the 16-byte key piece that lane group g loads n-th.
@@ -348,17 +354,17 @@ __device__ __forceinline__ void weigh_tile(wave_state<DT, CT, DP>& st,
       if (i % 2) __builtin_amdgcn_sched_barrier(0);
     }
   } else {
-    pl_u32x4 hi, lo;
+    pl_u32x4 part[S::kParts];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      // neither part is negative, and lo not 0 where hi is not: an infinite value
-      // times both is infinite, not NaN
-      float x[2] = {p[2 * j], p[2 * j + 1]};
-      if constexpr (DT == PL_BF16)
-        for (float& e : x) e = __uint_as_float(__float_as_uint(e) | 1u);  // below fp32's rounding
-      hi[j] = pack2_down<DT>(x[0], x[1]);
-      lo[j] = pack2<DT>(x[0] - unpack<DT>(hi[j], 0), x[1] - unpack<DT>(hi[j], 1));
-      if constexpr (DT == PL_F16) lo[j] = least_beside(hi[j], lo[j]);
+      float a = p[2 * j], b = p[2 * j + 1];
+#pragma unroll
+      for (int k = 0; k < S::kParts; ++k) {
+        const uint32_t x = pack2_down<DT>(a, b);
+        a -= unpack<DT>(x, 0), b -= unpack<DT>(x, 1);
+        // no part negative, or 0 beside the others: an infinite value stays one
+        part[k][j] = k ? at_least_smallest<DT>(x, part[0][j]) : x;
+      }
     }
 #pragma unroll
     for (int i = 0; i < S::V / 2; ++i) {
@@ -376,10 +382,11 @@ __device__ __forceinline__ void weigh_tile(wave_state<DT, CT, DP>& st,
         a[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x05040100);
         b[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x07060302);
       }
-      st.o[2 * i] = pl_mfma_chunk<DT>(a, hi, st.o[2 * i]);
-      st.o[2 * i + 1] = pl_mfma_chunk<DT>(b, hi, st.o[2 * i + 1]);
-      st.o[2 * i] = pl_mfma_chunk<DT>(a, lo, st.o[2 * i]);
-      st.o[2 * i + 1] = pl_mfma_chunk<DT>(b, lo, st.o[2 * i + 1]);
+#pragma unroll
+      for (int k = 0; k < S::kParts; ++k) {
+        st.o[2 * i] = pl_mfma_chunk<DT>(a, part[k], st.o[2 * i]);
+        st.o[2 * i + 1] = pl_mfma_chunk<DT>(b, part[k], st.o[2 * i + 1]);
+      }
       // in this order: pairing up all values first would take as many registers again
       __builtin_amdgcn_sched_barrier(0);
     }
