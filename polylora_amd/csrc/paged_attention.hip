@@ -360,7 +360,8 @@ __device__ __forceinline__ void weigh_tile(wave_state<DT, CT, DP>& st,
       float a = p[2 * j], b = p[2 * j + 1];
 #pragma unroll
       for (int k = 0; k < S::kParts; ++k) {
-        const uint32_t x = pack2_down<DT>(a, b);
+        // bf16's last part is exact either way
+        const uint32_t x = k + 1 < S::kParts || DT == PL_BF16 ? pack2_down<DT>(a, b) : pack2<DT>(a, b);
         a -= unpack<DT>(x, 0), b -= unpack<DT>(x, 1);
         // no part negative, or 0 beside the others: an infinite value stays one
         part[k][j] = k ? at_least_smallest<DT>(x, part[0][j]) : x;
