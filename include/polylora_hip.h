@@ -600,7 +600,8 @@ int pl_rope_append(int32_t dtype, int32_t cache_dtype, const void* q, const int6
 /* out[b][h] = sum over j of softmax_j(scale * q[b][h] . key_j) value_j, j over
  * the last `window` (0: all) of the first min(lens[b], max_pages * page_size)
  * tokens of row b's pages, key head h / (heads / kv_heads); tokens on pages
- * the table does not hold are left out, and a row without a token gives 0.
+ * the table does not hold are left out, and a row without a token, or whose
+ * scores are all -infinity, gives 0.
  * q [rows][heads][dim] with strides of row and head, out contiguous and apart
  * from q.  The rows are split over the workgroups by their tokens, found from
  * lens on the device; parts of a row are joined inside the launch through the

@@ -65,7 +65,8 @@ __global__ __launch_bounds__(THREADS) void pl_adjust_logits_kernel(logits_args a
   const int lo = (int)(blockIdx.x % a.slices) * kSlice, hi = min(lo + kSlice, a.vocab);
   const T* in = (const T*)a.logits + b * a.ld;
   O* out = (O*)a.out + b * a.ld_out;
-  // rows have the alignment of their elements alone
+  // Rows have the alignment of their elements alone.  16-bit logits are widened
+  // at their load, whose branch then waits for it; fp32's are all in flight.
   T x[kPasses][kVec];
   uint32_t mask[kPasses];
   const uint8_t* allowed = reinterpret_cast<const uint8_t*>(a.allowed + b * a.ld_allowed);

@@ -158,13 +158,14 @@ __device__ __forceinline__ void store_cache(void* p, int64_t at, const float (&x
 }
 
 // A workgroup takes `group` tokens (or one of gridDim.y shares of them).  A
-// thread keeps one place of the head,
-// VEC elements and, split in halves, the VEC that turn against them, and
-// walks the token's query and key heads with it, so that it reads its part of
-// cos and sin once; the threads then copy the values.  The tokens' lengths,
-// pages and angles take two dependent reads, the second beside the heads'.
+// thread keeps one place of the head, VEC elements and, split in halves, the
+// VEC that turn against them, and walks the token's query and key heads with it,
+// so that it reads its part of cos and sin once; the threads then copy the values.
 //
-// Bound by memory: every element of q, k and v is read and written once.
+// Bound by memory: every element of q, k and v is read and written once.  Few
+// tokens are bound by reads that wait for each other: length, position, page
+// and angles, then of a head its first half and its second, an 8-bit cache's
+// scale, and after the heads the values (256 single tokens 4.4 us, 1.2 of it bytes).
 template <int DT, int CT, int VEC, bool STREAM>
 __global__ __launch_bounds__(kThreads) void pl_rope_append_kernel(append_args a) {
   const int tid = (int)threadIdx.x;

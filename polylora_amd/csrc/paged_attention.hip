@@ -84,7 +84,8 @@ struct shape {
     return (piece * 16 + lane) * kPiece;
   }
   static constexpr int kTokens = 4 * kSubs;          // tokens of a lane per tile
-  // Queries in LDS where keys, values and outputs fill the registers.
+  // Queries in LDS where keys, values and outputs fill the registers (heads of
+  // 144 to 240 elements spill a few all the same, 20 to 96 bytes a thread).
   static constexpr bool kQueryLds = DP == 256 || DT == PL_F32;
   static constexpr int kParts = DT == PL_BF16 ? 3 : 2;  // 16-bit parts of a weight
   // log2 of what weights are multiplied by, that their 16-bit parts keep small ones.
@@ -828,7 +829,8 @@ __global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kWavesPerSimd)) void 
 
 // Lines read once are marked so where a pool of pages is too large to stay in
 // the GPU's last cache (256 rows of up to 1024 tokens 129 -> 120 us; 256 rows of
-// up to 128, 134 MB, 20.9 -> 23.1).  Not where a line is read again: by the next
+// up to 128, 134 MB, 20.9 -> 23.1, which a batch as small in a larger pool loses:
+// how much of the pool it reads is known on the device alone).  Not where a line is read again: by the next
 // 16 query heads of a key head (204 rows, 20 for each 120 -> 144 us), or,
 // in heads that are no whole lines, by another load (fp32, 80 elements: 40 -> 56).
 constexpr int64_t kLastCache = 256 << 20;

@@ -38,8 +38,9 @@ def adjust_logits(logits: torch.Tensor, *, tokens: torch.Tensor | None = None, l
     tokens int32 or int64 ``[rows, n]`` (n to 1048575; right-padded, what is beyond lens is not read as tokens), lens
     and prompt_lens int32 ``[rows]``, the penalties fp32 ``[rows]``, bias_ids int32 and bias_values fp32 ``[rows, m]`` (or
     ``[m]`` for all rows; m to 2047), allowed int32 ``[rows, ceil(vocab / 32)]`` (or one row for all); each is optional,
-    ids outside the vocabulary match nothing.  Logits in float32, bfloat16 or float16, rows of any stride.  The result
-    goes into ``out`` (fp32, or the logits' dtype; the logits themselves too) or a new fp32 tensor.
+    ids outside the vocabulary match nothing; bias_ids and bias_values of several rows have one row stride.  Logits in
+    float32, bfloat16 or float16, rows of any stride.  The result goes into ``out`` (fp32, or the logits' dtype; the
+    logits themselves too; rows apart) or a new fp32 tensor.
     """
     return _native.tensor_calls().adjust_logits(logits, tokens, lens, prompt_lens, repetition, presence, frequency,
                                                 bias_ids, bias_values, allowed, out, _stream(logits))

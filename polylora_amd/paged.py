@@ -48,7 +48,8 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_cache: to
     fused projection too).  Token t of row b (``t < min(seq_lens[b], M)``; all M without seq_lens) has position
     ``past_lens[b] + t``; cos and sin are fp32 ``[positions, rot / 2]`` (``rope_table``) and rotate the first ``rot``
     elements of a head: its halves against each other, or the pairs (2i, 2i + 1) with ``interleaved``.  Both in fp32,
-    rounded once.  page_table, past_lens and seq_lens are int32.  An 8-bit cache takes ``x / scale``, saturated.
+    rounded once.  page_table ``[rows, columns]`` (rows may share one, expanded), past_lens and seq_lens ``[rows]`` are
+    int32.  An 8-bit cache takes ``x / scale``, saturated.  No two elements of the caches may share a place.
 
     The rotated q comes back as a new contiguous tensor, 0 for padding tokens; ``k_out``, a contiguous tensor like k,
     also receives the rotated k, for attention inside a prompt.  A token beyond the cos table or on a page the table
@@ -117,7 +118,11 @@ def paged_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch
     serving as many query heads in a row.  ``lens`` (int32) counts the row's tokens, the new one included (append it
     first); with ``window`` only the last that many of them count.  ``scale`` is ``dim ** -0.5`` unless given.  Sums and
     the softmax are fp32, the output is rounded once, into ``out`` (contiguous, like q) or a new tensor.  A row without
-    a token gives 0; slots of pages beyond a row's tokens are never part of a result, whatever they hold.
+    a token, or whose scores are all -inf, gives 0; slots of pages beyond a row's tokens are never part of a result,
+    whatever they hold.
+
+    Calls on one stream share a workspace and counters; a HIP graph has its own, so its replays may overlap other work,
+    but not each other.
     """
     stream = _stream(q)
     return _native.tensor_calls().paged_attention(q, key_cache, value_cache, page_table, lens, scale, window, k_scale,
