@@ -597,6 +597,26 @@ int pl_rope_append(int32_t dtype, int32_t cache_dtype, const void* q, const int6
                    int32_t positions, int32_t rot, int32_t interleaved, const float* k_scale,
                    const float* v_scale, void* stream);
 
+/* The same with the norms of queries and keys of each head before the rotation,
+ *   x / sqrt(mean(x^2) + eps) * w,
+ * in fp32 like the rest, w the head's dim weights of q_norm or k_norm (the model's
+ * type or PL_F32, norm_dtype for both; NULL for no norm of these), eps positive;
+ * and, unless depths is NULL, with position past_lens[b] + depths[b * depths_ld + t]
+ * in the angles (depths_ld 0: one list that all rows share).  The token's place
+ * in the pages stays past_lens[b] + t. */
+int pl_norm_rope_append(int32_t dtype, int32_t cache_dtype, const void* q,
+                        const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                        const void* v, const int64_t* v_strides, void* q_out, void* k_out,
+                        void* key_cache, const int64_t* key_strides, void* value_cache,
+                        const int64_t* value_strides, int32_t num_pages, int32_t page_size,
+                        const int32_t* page_table, int64_t table_ld, int32_t max_pages,
+                        const int32_t* past_lens, const int32_t* seq_lens, int32_t rows,
+                        int32_t row_len, int32_t heads, int32_t kv_heads, int32_t dim,
+                        const float* cos, const float* sin, int32_t positions, int32_t rot,
+                        int32_t interleaved, const float* k_scale, const float* v_scale,
+                        const void* q_norm, const void* k_norm, int32_t norm_dtype, float eps,
+                        const int32_t* depths, int64_t depths_ld, void* stream);
+
 /* out[b][h] = sum over j of softmax_j(scale * q[b][h] . key_j) value_j, j over
  * the last `window` (0: all) of the first min(lens[b], max_pages * page_size)
  * tokens of row b's pages, key head h / (heads / kv_heads); tokens on pages
@@ -622,6 +642,68 @@ int pl_paged_attention(int32_t dtype, int32_t cache_dtype, const void* q,
                        const float* v_scale, void* out, void* workspace,
                        int64_t workspace_bytes, int32_t* counters, int64_t counter_ints,
                        void* stream);
+
+/* Attention of the row_len drafted tokens of each row: token t of row b, live for
+ * t < min(seq_lens[b], row_len) (seq_lens NULL: row_len), lies at place
+ * past_lens[b] + t of the row's pages and attends, as above, to
+ *   places j below past_lens[b], with a window j > past_lens[b] + d - window, and
+ *   live drafted tokens: those up to t (with a window, past_lens[b] + t - window
+ *   < j too), or, where visible is not NULL, those whose bit is set: bit j % 32 of
+ *   visible[b * visible_row + t * visible_token + j / 32] for drafted token j.
+ * d is t, or depths[b * depths_row + t] where visible is not NULL; a window of a
+ * tree needs depths and is at least row_len.  A token that is not live gives 0, as
+ * does one that sees nothing; nothing is read at a place that no live token of the
+ * row sees.  q [rows][row_len][heads][dim] with strides of row, token and head, out
+ * contiguous and apart from q. */
+int pl_tree_attention(int32_t dtype, int32_t cache_dtype, const void* q, const int64_t* q_strides,
+                      const void* key_cache, const int64_t* key_strides, const void* value_cache,
+                      const int64_t* value_strides, int32_t num_pages, int32_t page_size,
+                      const int32_t* page_table, int64_t table_ld, int32_t max_pages,
+                      const int32_t* past_lens, const int32_t* seq_lens, const int32_t* visible,
+                      int64_t visible_row, int64_t visible_token, int32_t words,
+                      const int32_t* depths, int64_t depths_row, int32_t rows, int32_t row_len,
+                      int32_t heads, int32_t kv_heads, int32_t dim, float scale, int32_t window,
+                      const float* k_scale, const float* v_scale, void* out, void* stream);
+
+/* In every cache of `layers` layers (host arrays of pointers, all caches with
+ * these strides, none over another): what lies at place past_lens[b] +
+ * path[b * path_ld + i] of row b's pages moves to place past_lens[b] + i, for i
+ * below min(counts[b], columns) up to the first entry that is negative or not above
+ * the one before it; a move from or to a page that the table does not hold is left
+ * out.  dtype is the caches' element type. */
+int pl_keep_tokens(int32_t dtype, int32_t layers, void* const* key_caches,
+                   void* const* value_caches, const int64_t* strides, int32_t num_pages,
+                   int32_t page_size, int32_t kv_heads, int32_t dim, const int32_t* page_table,
+                   int64_t table_ld, int32_t max_pages, const int32_t* past_lens,
+                   const int32_t* path, int64_t path_ld, int32_t columns, const int32_t* counts,
+                   int32_t rows, void* stream);
+
+/* Which drafted tokens of each row stay, and the token behind them.  Token 0 of row b
+ * is the row's last one, tokens 1 to min(seq_lens[b], nodes) - 1 are drafts (seq_lens
+ * NULL: nodes), token n behind token parents[b * ld_parents + n] < n (ld_parents 0:
+ * one list for all rows; NULL: behind token n - 1).  With x the logits of what follows
+ * token n, t = temperature[b] (NULL: 1) and u = uniforms[b * ld_uniforms + n], in 64
+ * bits, from token 0 on:
+ *   e_v = exp((x_v - max x) / t), Z their sum, or, for t = 0, the first largest
+ *   logit has all the weight;
+ *   without draft_probs the first v with e_0 + ... + e_v > u Z follows: the row goes
+ *   on with the first draft behind n that holds v, or stops with v;
+ *   with draft_probs (a line; q the probabilities at draft_probs[b * ld_draft_row + n *
+ *   ld_draft_node] that draft n + 1, token d, came from) the row goes on where
+ *   u q_d Z < e_d.  Else it stops with the first v whose sum of max(e_i - q_i Z, 0),
+ *   i <= v, is above u' times the whole sum, u' the uniform of the row's last token;
+ *   where that is 0 everywhere, and behind the last draft, of e_i.
+ * Where x has NaN or +infinity or nothing above -infinity, or t is not at least 0 and
+ * finite, the row stops with token -1; so does a row of no token.
+ * path [rows][nodes] gets the numbers of the tokens that stay, from 0 on, -1 behind
+ * them; counts how many; next the token that follows. */
+int pl_verify_tokens(int32_t dtype, const void* logits, int64_t ld_row, int64_t ld_node,
+                     const void* tokens, int32_t token_bytes, int64_t ld_tokens,
+                     const float* uniforms, int64_t ld_uniforms, const int32_t* parents,
+                     int64_t ld_parents, const float* draft_probs, int64_t ld_draft_row,
+                     int64_t ld_draft_node, const float* temperature, const int32_t* seq_lens,
+                     int32_t rows, int32_t nodes, int32_t vocab, int32_t* path, int32_t* counts,
+                     int64_t* next, void* stream);
 
 /* Logits of one row for the choice of its next token, in fp32 and this order:
  *   x = logits[b][v]

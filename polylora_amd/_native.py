@@ -133,6 +133,26 @@ _SIGNATURES: dict[str, tuple] = {
         c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_int32, c_int32, c_int32,
         c_void_p, c_void_p, c_void_p,
     ),
+    "pl_norm_rope_append": (
+        c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+        c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_int64, c_int32, c_void_p,
+        c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_int32, c_int32, c_int32,
+        c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_float, c_void_p, c_int64, c_void_p,
+    ),
+    "pl_tree_attention": (
+        c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32,
+        c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int32, c_void_p, c_int64,
+        c_int32, c_int32, c_int32, c_int32, c_int32, c_float, c_int32, c_void_p, c_void_p, c_void_p, c_void_p,
+    ),
+    "pl_keep_tokens": (
+        c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_void_p, c_int64,
+        c_int32, c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_int32, c_void_p,
+    ),
+    "pl_verify_tokens": (
+        c_int32, c_void_p, c_int64, c_int64, c_void_p, c_int32, c_int64, c_void_p, c_int64, c_void_p, c_int64,
+        c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p,
+        c_void_p,
+    ),
     "pl_paged_attention": (
         c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32,
         c_void_p, c_int64, c_int32, c_void_p, c_int32, c_int32, c_int32, c_int32, c_float, c_int32, c_void_p,

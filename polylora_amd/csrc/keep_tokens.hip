@@ -1,0 +1,149 @@
+// Keys and values of the tokens of a row that stay, moved up behind one another in
+// the row's pages, in every layer's caches.
+#include "pl_paged.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kLayersMax = 64;  // of a launch: their pointers are its arguments
+constexpr int kBatch = 4;       // moves of a thread that are in flight
+
+struct keep_args {
+  void* caches[2 * kLayersMax];  // keys and values of each layer
+  int64_t s_page, s_head, s_slot;  // bytes
+  pl_page_table table;
+  const int32_t *past, *path, *counts;
+  int64_t path_ld;
+  int32_t columns, caches_n;
+  int32_t pieces, head_pieces;  // 16-byte pieces of a token and of a head
+  int32_t groups;               // workgroups of a row
+};
+
+// Memory bounds it: every element that moves is read and written once, and each
+// of a row's few moves is one slot of every cache.  A thread keeps one 16-byte
+// piece of one head of one cache and takes the row's moves in order, kBatch reads
+// ahead of their writes.  A path ascends, so a token never comes from a place
+// before its own, and no read follows the write of its place: that holds for
+// each thread by itself, and no other thread has its pieces.
+__global__ __launch_bounds__(kThreads) void pl_keep_tokens_kernel(keep_args a) {
+  __shared__ int64_t s_from[kThreads], s_to[kThreads];
+  __shared__ int s_count[kThreads / 64], s_end[kThreads / 64];
+  const int tid = (int)threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int b = (int)(blockIdx.x / a.groups), group = (int)blockIdx.x - b * a.groups;
+  const int n = min(a.counts[b], a.columns);
+  const int64_t past = a.past[b];
+  const int32_t* path = a.path + b * a.path_ld;
+  const int32_t* pages = a.table.p + b * a.table.ld;
+  const int mask = (1 << a.table.page_shift) - 1;
+  auto place = [&](int64_t at) -> int64_t {
+    const int64_t column = at >> a.table.page_shift;
+    if (at < 0 || column >= a.table.max_pages) return -1;
+    const int id = pages[column];
+    return id < 0 || id >= a.table.num_pages ? -1 : id * a.s_page + (at & mask) * a.s_slot;
+  };
+  bool going = true;
+  for (int t0 = 0; t0 < n && going; t0 += kThreads) {
+    // the moves among these tokens, in order; the path ends where it does not ascend
+    const int t = t0 + tid;
+    const int node = t < n ? path[t] : 0, before = t > 0 && t < n ? path[t - 1] : -1;
+    const uint64_t bad = __ballot(t < n && node <= before);
+    if (lane == 0) s_end[wave] = bad ? t0 + wave * 64 + __ffsll((long long)bad) - 1 : n;
+    __syncthreads();
+    int end = n;
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; ++w) end = min(end, s_end[w]);
+    going = end == n;
+    int64_t from = -1, to = -1;
+    if (t < end && node != t) from = place(past + node), to = place(past + t);
+    const bool moves = from >= 0 && to >= 0;
+    const uint64_t all = __ballot(moves);
+    if (lane == 0) s_count[wave] = __popcll(all);
+    __syncthreads();
+    int at = __popcll(all & ((1ull << lane) - 1)), total = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; ++w) {
+      at += w < wave ? s_count[w] : 0;
+      total += s_count[w];
+    }
+    if (moves) s_from[at] = from, s_to[at] = to;
+    __syncthreads();
+    for (int64_t i = (int64_t)group * kThreads + tid; total > 0 && i < (int64_t)a.caches_n * a.pieces;
+         i += (int64_t)a.groups * kThreads) {
+      const int cache = (int)(i / a.pieces), piece = (int)(i - (int64_t)cache * a.pieces);
+      const int head = piece / a.head_pieces;
+      uint8_t* p = static_cast<uint8_t*>(a.caches[cache]) + head * a.s_head + (piece - head * a.head_pieces) * 16;
+      for (int j0 = 0; j0 < total; j0 += kBatch) {
+        pl_u32x4 x[kBatch];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) x[j] = pl_ld16(p + s_from[min(j0 + j, total - 1)]);
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j)
+          if (j0 + j < total) *reinterpret_cast<pl_u32x4*>(p + s_to[j0 + j]) = x[j];
+      }
+    }
+    __syncthreads();
+  }
+}
+
+}  // namespace
+
+extern "C" int pl_keep_tokens(int32_t dtype, int32_t layers, void* const* key_caches, void* const* value_caches,
+                              const int64_t* strides, int32_t num_pages, int32_t page_size, int32_t kv_heads,
+                              int32_t dim, const int32_t* page_table, int64_t table_ld, int32_t max_pages,
+                              const int32_t* past_lens, const int32_t* path, int64_t path_ld, int32_t columns,
+                              const int32_t* counts, int32_t rows, void* stream) {
+  const char* what = "pl_keep_tokens";
+  if (dtype != PL_F32 && dtype != PL_BF16 && dtype != PL_F16 && dtype != PL_F8E4M3) {
+    pl_set_error("%s: unknown element type %d", what, dtype);
+    return PL_ERR_ARG;
+  }
+  if (layers < 0 || columns < 0 || rows < 0 || (rows > 1 && path_ld < columns && path_ld != 0)) {
+    pl_set_error("%s: bad sizes (layers %d, columns %d, rows %d, row stride %lld)", what, layers, columns, rows,
+                 (long long)path_ld);
+    return PL_ERR_ARG;
+  }
+  // the cache checks of the other calls, scales aside
+  const float unit = 0.f;
+  const float* scale = dtype == PL_F8E4M3 ? &unit : nullptr;
+  const int32_t model = dtype == PL_F8E4M3 ? PL_BF16 : dtype;
+  if (layers > 0 && (!key_caches || !value_caches)) {
+    pl_set_error("%s: null pointer", what);
+    return PL_ERR_ARG;
+  }
+  for (int i = 0; i < layers; ++i) {
+    const int rc = pl_check_paged(what, model, dtype, key_caches[i], strides, value_caches[i], strides, num_pages,
+                                  page_size, page_table, table_ld, max_pages, rows, kv_heads, kv_heads, dim, scale,
+                                  scale);
+    if (rc) return rc;
+  }
+  if (rows == 0 || layers == 0 || columns == 0 || num_pages == 0) return PL_OK;
+  if (!past_lens || !path || !counts) {
+    pl_set_error("%s: null pointer", what);
+    return PL_ERR_ARG;
+  }
+  if (!pl_elements_apart(strides, num_pages, kv_heads, page_size, dim)) {
+    pl_set_error("%s: elements of the caches share their places", what);
+    return PL_ERR_ARG;
+  }
+  const int64_t es = pl_cache_elem_size(dtype);
+  keep_args a;
+  a.s_page = strides[0] * es, a.s_head = strides[1] * es, a.s_slot = strides[2] * es;
+  a.table = {page_table, table_ld, max_pages, num_pages, pl_log2_exact(page_size)};
+  a.past = past_lens, a.path = path, a.counts = counts, a.path_ld = path_ld, a.columns = columns;
+  a.head_pieces = (int32_t)(dim * es / 16), a.pieces = a.head_pieces * kv_heads;
+  for (int l0 = 0; l0 < layers; l0 += kLayersMax) {
+    const int n = layers - l0 < kLayersMax ? layers - l0 : kLayersMax;
+    for (int i = 0; i < n; ++i) a.caches[2 * i] = key_caches[l0 + i], a.caches[2 * i + 1] = value_caches[l0 + i];
+    a.caches_n = 2 * n;
+    const int64_t items = (int64_t)a.caches_n * a.pieces;
+    a.groups = (int32_t)((items + kThreads - 1) / kThreads);
+    if (!pl_grid_fits((int64_t)rows * a.groups, kThreads)) {
+      pl_set_error("%s: too many rows (%d)", what, rows);
+      return PL_ERR_LIMIT;
+    }
+    pl_keep_tokens_kernel<<<dim3((unsigned)(rows * a.groups)), kThreads, 0, reinterpret_cast<hipStream_t>(stream)>>>(a);
+    const int rc = pl_launch_status(what);
+    if (rc) return rc;
+  }
+  return PL_OK;
+}

@@ -52,3 +52,8 @@ int pl_check_paged(const char* what, int32_t dtype, int32_t cache_dtype, const v
                    const int32_t* page_table, int64_t table_ld, int32_t max_pages, int32_t rows,
                    int32_t heads, int32_t kv_heads, int32_t dim, const float* k_scale,
                    const float* v_scale);
+
+// Whether no two elements of a cache share a place: from the smallest stride up,
+// each dimension steps past all that those before it reach.
+bool pl_elements_apart(const int64_t* strides, int32_t pages, int32_t kv_heads, int32_t page_size,
+                       int32_t dim);

@@ -1,5 +1,5 @@
 // CPython entry points that take torch tensors: the operators of a decode step
-// beside the Linears (polylora_amd.paged, polylora_amd.logits).
+// beside the Linears (polylora_amd.paged, polylora_amd.logits, polylora_amd.drafts).
 //
 // Their smallest calls take 4 us on the GPU, and checking ten tensor arguments
 // from Python alone takes twice that.  Here a call is one look at each tensor,
@@ -16,10 +16,12 @@
 #include <c10/core/GradMode.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cmath>
 #include <exception>
 #include <optional>
 #include <string>
+#include <vector>
 
 #include "../../include/polylora_hip.h"
 
@@ -141,6 +143,18 @@ void check_last(const at::Tensor& t, const char* name) {
   if (t.numel() && t.size(-1) > 1 && t.stride(-1) != 1)
     value_error(std::string("the last dimension of ") + name + " must be contiguous");
 }
+// The same for each of a sequence of tensors, kept alive by it.
+struct Sequence {
+  explicit Sequence(PyObject* o, const char* name) : held(PySequence_Fast(o, name)) {
+    if (!held) throw Raised{};
+  }
+  ~Sequence() { Py_DECREF(held); }
+  Sequence(const Sequence&) = delete;
+  Sequence& operator=(const Sequence&) = delete;
+  size_t size() const { return (size_t)PySequence_Fast_GET_SIZE(held); }
+  const at::Tensor& at(size_t i, const char* name) const { return tensor(PySequence_Fast_GET_ITEM(held, i), name); }
+  PyObject* held;
+};
 // A contiguous int32 or fp32 vector of n elements; null where the tensor is.
 template <typename E>
 const E* vector(const at::Tensor* t, const char* name, at::ScalarType type, int device, int64_t n) {
@@ -149,6 +163,22 @@ const E* vector(const at::Tensor* t, const char* name, at::ScalarType type, int 
   check_shape(*t, name, {n});
   check_dense(*t, name);
   return static_cast<const E*>(t->const_data_ptr());
+}
+
+// int32 numbers for each token, [rows, n], or [n] that all rows share (row stride 0).
+struct Rows {
+  const int32_t* p = nullptr;
+  int64_t ld = 0;
+};
+Rows row_numbers(const at::Tensor* t, const char* name, int device, int64_t rows, int64_t n) {
+  if (!t) return {};
+  check_type(*t, name, at::kInt, device);
+  if (t->dim() == 1)
+    check_shape(*t, name, {n});
+  else
+    check_shape(*t, name, {rows, n});
+  check_last(*t, name);
+  return {static_cast<const int32_t*>(t->const_data_ptr()), t->dim() == 2 && rows > 1 ? t->stride(0) : 0};
 }
 
 void check_status(int rc, const char* what) {
@@ -180,7 +210,7 @@ Cache check_cache(const at::Tensor& key, const at::Tensor& value, const at::Tens
   Cache c;
   c.k_scale = c.v_scale = nullptr;
   if (key.scalar_type() == type) {
-    c.code = dtype_code(type);
+    c.code = type == at::kFloat8_e4m3fn ? PL_F8E4M3 : dtype_code(type);  // 8 bits by themselves: bytes to move
     if (k_scale || v_scale) value_error("scales belong to an 8-bit cache");
   } else if (key.scalar_type() == at::kFloat8_e4m3fn && type != at::kFloat) {
     c.code = PL_F8E4M3;
@@ -216,7 +246,7 @@ Cache check_cache(const at::Tensor& key, const at::Tensor& value, const at::Tens
 }
 
 // (q, k, v, key_cache, value_cache, page_table, past_lens, cos, sin, seq_lens, interleaved, k_scale, v_scale,
-//  k_out, stream) -> the rotated q
+//  k_out, q_norm, k_norm, eps, depths, stream) -> the rotated q
 PyObject* rope_append(PyObject* const* a) {
   const at::Tensor &q = tensor(a[0], "q"), &k = tensor(a[1], "k"), &v = tensor(a[2], "v");
   const at::Tensor &cos = tensor(a[7], "cos"), &sin = tensor(a[8], "sin");
@@ -257,20 +287,39 @@ PyObject* rope_append(PyObject* const* a) {
   }
   const int interleaved = PyObject_IsTrue(a[10]);
   if (interleaved < 0) throw Raised{};
-  void* stream = PyLong_AsVoidPtr(a[14]);
+  const at::Tensor *q_norm = maybe(a[14], "q_norm"), *k_norm = maybe(a[15], "k_norm");
+  const at::Tensor* norm = q_norm ? q_norm : k_norm;
+  if (norm && norm->scalar_type() != at::kFloat && norm->scalar_type() != type)
+    type_error("norms must be torch.float32 or " + type_text(type) + ", not " + type_text(norm->scalar_type()));
+  const void* q_weights = vector<void>(q_norm, "q_norm", norm ? norm->scalar_type() : type, device, dim);
+  const void* k_weights = vector<void>(k_norm, "k_norm", norm ? norm->scalar_type() : type, device, dim);
+  const double eps = real(a[16]);
+  const at::Tensor* depths = maybe(a[17], "depths");
+  const Rows depth = row_numbers(depths, "depths", device, rows, m);
+  void* stream = PyLong_AsVoidPtr(a[18]);
   const int32_t r32 = size32(rows, "q"), m32 = size32(m, "q"), h32 = size32(heads, "q"), d32 = size32(dim, "q");
   const int32_t p32 = size32(cos.size(0), "cos");
   at::Tensor out = at::empty(q.sizes(), q.options());
   int rc;
   Py_BEGIN_ALLOW_THREADS;
-  rc = pl_rope_append(code, c.code, q.const_data_ptr(), q.strides().data(), k.const_data_ptr(), k.strides().data(),
-                      v.const_data_ptr(), v.strides().data(), out.data_ptr(), k_out ? k_out->data_ptr() : nullptr,
-                      c.key, c.key_strides, c.value, c.value_strides, c.num_pages, c.page_size, c.table, c.table_ld,
-                      c.max_pages, past, seq, r32, m32, h32, c.kv_heads, d32,
-                      static_cast<const float*>(cos.const_data_ptr()), static_cast<const float*>(sin.const_data_ptr()),
-                      p32, (int32_t)(2 * half), interleaved, c.k_scale, c.v_scale, stream);
+  if (norm || depths)
+    rc = pl_norm_rope_append(code, c.code, q.const_data_ptr(), q.strides().data(), k.const_data_ptr(), k.strides().data(),
+                             v.const_data_ptr(), v.strides().data(), out.data_ptr(), k_out ? k_out->data_ptr() : nullptr,
+                             c.key, c.key_strides, c.value, c.value_strides, c.num_pages, c.page_size, c.table, c.table_ld,
+                             c.max_pages, past, seq, r32, m32, h32, c.kv_heads, d32,
+                             static_cast<const float*>(cos.const_data_ptr()), static_cast<const float*>(sin.const_data_ptr()),
+                             p32, (int32_t)(2 * half), interleaved, c.k_scale, c.v_scale,
+                             q_weights, k_weights, norm ? dtype_code(norm->scalar_type()) : code, (float)eps, depth.p,
+                             depth.ld, stream);
+  else
+    rc = pl_rope_append(code, c.code, q.const_data_ptr(), q.strides().data(), k.const_data_ptr(), k.strides().data(),
+                        v.const_data_ptr(), v.strides().data(), out.data_ptr(), k_out ? k_out->data_ptr() : nullptr,
+                        c.key, c.key_strides, c.value, c.value_strides, c.num_pages, c.page_size, c.table, c.table_ld,
+                        c.max_pages, past, seq, r32, m32, h32, c.kv_heads, d32,
+                        static_cast<const float*>(cos.const_data_ptr()), static_cast<const float*>(sin.const_data_ptr()),
+                        p32, (int32_t)(2 * half), interleaved, c.k_scale, c.v_scale, stream);
   Py_END_ALLOW_THREADS;
-  check_status(rc, "pl_rope_append");
+  check_status(rc, norm || depths ? "pl_norm_rope_append" : "pl_rope_append");
   return THPVariable_Wrap(std::move(out));
 }
 
@@ -409,6 +458,188 @@ PyObject* adjust_logits(PyObject* const* a) {
   return THPVariable_Wrap(std::move(out));
 }
 
+// (q, key_cache, value_cache, page_table, past_lens, seq_lens, visible, depths, scale, window, k_scale, v_scale,
+//  out, stream) -> out; scale and window may be None
+PyObject* tree_attention(PyObject* const* a) {
+  const at::Tensor& q = tensor(a[0], "q");
+  check_lead(q, "tree_attention");
+  const int device = q.get_device();
+  const OnDevice current(q);
+  if (q.dim() != 4) value_error("q must be [rows, M, heads, dim], not " + shape_text(q.sizes()));
+  const int64_t rows = q.size(0), m = q.size(1), heads = q.size(2), dim = q.size(3);
+  const at::ScalarType type = q.scalar_type();
+  const int32_t code = dtype_code(type);
+  check_last(q, "q");
+  const Cache c = check_cache(tensor(a[1], "key_cache"), tensor(a[2], "value_cache"), tensor(a[3], "page_table"),
+                              rows, dim, type, device, maybe(a[10], "k_scale"), maybe(a[11], "v_scale"), false);
+  if (c.kv_heads == 0 || heads % c.kv_heads)
+    value_error(std::to_string(heads) + " heads over a cache of " + std::to_string(c.kv_heads) + " key heads");
+  const int32_t* past = vector<int32_t>(&tensor(a[4], "past_lens"), "past_lens", at::kInt, device, rows);
+  const int32_t* seq = vector<int32_t>(maybe(a[5], "seq_lens"), "seq_lens", at::kInt, device, rows);
+  const at::Tensor* visible = maybe(a[6], "visible");
+  const int32_t* masks = nullptr;
+  int64_t mask_row = 0, mask_token = 0, words = 0;
+  if (visible) {
+    check_type(*visible, "visible", at::kInt, device);
+    const int64_t nd = visible->dim();
+    if (nd < 2 || nd > 3 || visible->size(nd - 2) != m || (nd == 3 && visible->size(0) != rows) ||
+        visible->size(nd - 1) * 32 < m)
+      value_error("visible must be [" + std::to_string(rows) + ", " + std::to_string(m) + ", words], or one such [" +
+                  std::to_string(m) + ", words] for all rows, of a bit for each token, not " +
+                  shape_text(visible->sizes()));
+    check_last(*visible, "visible");
+    words = visible->size(nd - 1);
+    masks = static_cast<const int32_t*>(visible->const_data_ptr());
+    mask_row = nd == 3 && rows > 1 ? visible->stride(0) : 0;
+    mask_token = m > 1 ? visible->stride(nd - 2) : 0;
+  }
+  const at::Tensor* depths = maybe(a[7], "depths");
+  const Rows depth = row_numbers(depths, "depths", device, rows, m);
+  const double scale = a[8] == Py_None ? 1.0 / std::sqrt((double)dim) : real(a[8]);
+  int64_t window = 0;
+  if (a[9] != Py_None) {
+    window = integer(a[9]);
+    if (window < 1) value_error("window must be at least one token, not " + std::to_string(window));
+    if (visible && !depths) value_error("a window over a tree of drafts needs their depths");
+    if (visible && window < m)
+      value_error("a window of " + std::to_string(window) + " tokens over a tree of " + std::to_string(m) + " drafts");
+    if (window > INT32_MAX) window = 0;  // no row is that long
+  }
+  const at::Tensor* given = maybe(a[12], "out");
+  if (given) {
+    check_type(*given, "out", type, device);
+    check_shape(*given, "out", q.sizes());
+    check_dense(*given, "out");
+  }
+  void* stream = PyLong_AsVoidPtr(a[13]);
+  const int32_t r32 = size32(rows, "q"), m32 = size32(m, "q"), h32 = size32(heads, "q"), d32 = size32(dim, "q");
+  const int32_t w32 = size32(words, "visible");
+  at::Tensor out = given ? *given : at::empty(q.sizes(), q.options());
+  int rc;
+  Py_BEGIN_ALLOW_THREADS;
+  rc = pl_tree_attention(code, c.code, q.const_data_ptr(), q.strides().data(), c.key, c.key_strides, c.value,
+                         c.value_strides, c.num_pages, c.page_size, c.table, c.table_ld, c.max_pages, past, seq, masks,
+                         mask_row, mask_token, w32, depth.p, depth.ld, r32, m32, h32, c.kv_heads, d32, (float)scale,
+                         (int32_t)window, c.k_scale, c.v_scale, out.data_ptr(), stream);
+  Py_END_ALLOW_THREADS;
+  check_status(rc, "pl_tree_attention");
+  if (given) return Py_NewRef(a[12]);
+  return THPVariable_Wrap(std::move(out));
+}
+
+// (key_caches, value_caches, page_table, past_lens, path, counts, stream)
+PyObject* keep_tokens(PyObject* const* a) {
+  const Sequence keys(a[0], "key_caches must be a sequence of tensors");
+  const Sequence values(a[1], "value_caches must be a sequence of tensors");
+  if (keys.size() != values.size())
+    value_error(std::to_string(keys.size()) + " key caches and " + std::to_string(values.size()) + " value caches");
+  const at::Tensor &table = tensor(a[2], "page_table"), &path = tensor(a[4], "path");
+  check_lead(path, "keep_tokens");
+  const int device = path.get_device();
+  const OnDevice current(path);
+  check_type(path, "path", at::kInt, device);
+  if (path.dim() != 2) value_error("path must be [rows, n], not " + shape_text(path.sizes()));
+  check_last(path, "path");
+  const int64_t rows = path.size(0);
+  const int32_t* past = vector<int32_t>(&tensor(a[3], "past_lens"), "past_lens", at::kInt, device, rows);
+  const int32_t* counts = vector<int32_t>(&tensor(a[5], "counts"), "counts", at::kInt, device, rows);
+  const size_t layers = keys.size();
+  std::vector<void*> pointers(2 * layers);
+  Cache c = {};
+  const at::Tensor* lead = layers ? &keys.at(0, "key_caches") : nullptr;
+  for (size_t i = 0; i < 2 * layers; ++i) {
+    const at::Tensor& x = i < layers ? keys.at(i, "key_caches") : values.at(i - layers, "value_caches");
+    if (x.sizes() != lead->sizes() || x.scalar_type() != lead->scalar_type())
+      value_error("the caches must be alike, not " + shape_text(lead->sizes()) + " of " +
+                  type_text(lead->scalar_type()) + " and " + shape_text(x.sizes()) + " of " +
+                  type_text(x.scalar_type()));
+    if (i == 0) {
+      // an 8-bit cache's scales are not looked at: its bytes move
+      c = check_cache(x, x, table, rows, x.dim() == 4 ? x.size(3) : 0, x.scalar_type(), device, nullptr, nullptr, true);
+    } else {
+      check_type(x, "a cache", lead->scalar_type(), device);
+      check_last(x, "the caches");
+      for (int d = 0; d < 3; ++d)
+        if (x.size(d) > 1 && x.stride(d) != lead->stride(d)) value_error("the caches must have the same strides");
+    }
+    pointers[i] = x.mutable_data_ptr();
+  }
+  std::vector<void*> order(pointers);
+  std::sort(order.begin(), order.end());
+  if (lead && lead->numel() && std::adjacent_find(order.begin(), order.end()) != order.end())
+    value_error("a cache is there twice");
+  void* stream = PyLong_AsVoidPtr(a[6]);
+  const int32_t r32 = size32(rows, "path"), n32 = size32(path.size(1), "path"), l32 = size32((int64_t)layers, "layers");
+  if (layers) {
+    const int32_t d32 = size32(lead->size(3), "the cache");
+    int rc;
+    Py_BEGIN_ALLOW_THREADS;
+    rc = pl_keep_tokens(c.code, l32, pointers.data(), pointers.data() + layers, c.key_strides, c.num_pages,
+                        c.page_size, c.kv_heads, d32, c.table, c.table_ld, c.max_pages, past,
+                        static_cast<const int32_t*>(path.const_data_ptr()), rows > 1 ? path.stride(0) : path.size(1),
+                        n32, counts, r32, stream);
+    Py_END_ALLOW_THREADS;
+    check_status(rc, "pl_keep_tokens");
+  }
+  Py_RETURN_NONE;
+}
+
+// (logits, tokens, uniforms, parents, draft_probs, temperature, seq_lens, stream) -> (path, counts, next)
+PyObject* verify_tokens(PyObject* const* a) {
+  const at::Tensor &logits = tensor(a[0], "logits"), &tokens = tensor(a[1], "tokens");
+  const at::Tensor& uniforms = tensor(a[2], "uniforms");
+  check_lead(logits, "verify_tokens");
+  const int device = logits.get_device();
+  const OnDevice current(logits);
+  if (logits.dim() != 3) value_error("logits must be [rows, M, vocab], not " + shape_text(logits.sizes()));
+  const int64_t rows = logits.size(0), m = logits.size(1), vocab = logits.size(2);
+  const int32_t code = dtype_code(logits.scalar_type());
+  check_last(logits, "logits");
+  if (tokens.scalar_type() != at::kLong && tokens.scalar_type() != at::kInt)
+    type_error("tokens must be torch.int64 or torch.int32, not " + type_text(tokens.scalar_type()));
+  check_type(tokens, "tokens", tokens.scalar_type(), device);
+  check_shape(tokens, "tokens", {rows, m});
+  check_last(tokens, "tokens");
+  check_type(uniforms, "uniforms", at::kFloat, device);
+  check_shape(uniforms, "uniforms", {rows, m});
+  check_last(uniforms, "uniforms");
+  const at::Tensor *parents = maybe(a[3], "parents"), *draft_probs = maybe(a[4], "draft_probs");
+  if (parents && draft_probs) value_error("drafts with probabilities form a line: no parents beside draft_probs");
+  const Rows tree = row_numbers(parents, "parents", device, rows, m);
+  const float* probs = nullptr;
+  int64_t probs_row = 0, probs_node = 0;
+  if (draft_probs) {
+    check_type(*draft_probs, "draft_probs", at::kFloat, device);
+    check_shape(*draft_probs, "draft_probs", {rows, m > 0 ? m - 1 : 0, vocab});
+    check_last(*draft_probs, "draft_probs");
+    probs = static_cast<const float*>(draft_probs->const_data_ptr());
+    probs_row = draft_probs->stride(0), probs_node = draft_probs->stride(1);
+  }
+  const float* heat = vector<float>(maybe(a[5], "temperature"), "temperature", at::kFloat, device, rows);
+  const int32_t* seq = vector<int32_t>(maybe(a[6], "seq_lens"), "seq_lens", at::kInt, device, rows);
+  void* stream = PyLong_AsVoidPtr(a[7]);
+  const int32_t r32 = size32(rows, "logits"), m32 = size32(m, "logits"), v32 = size32(vocab, "logits");
+  const at::TensorOptions ints = logits.options().dtype(at::kInt);
+  at::Tensor path = at::empty({rows, m}, ints), counts = at::empty({rows}, ints);
+  at::Tensor next = at::empty({rows}, ints.dtype(at::kLong));
+  int rc;
+  Py_BEGIN_ALLOW_THREADS;
+  rc = pl_verify_tokens(code, logits.const_data_ptr(), logits.stride(0), logits.stride(1), tokens.const_data_ptr(),
+                        (int32_t)tokens.element_size(), tokens.stride(0),
+                        static_cast<const float*>(uniforms.const_data_ptr()), uniforms.stride(0), tree.p, tree.ld,
+                        draft_probs ? probs : nullptr, probs_row, probs_node, heat, seq, r32, m32, v32,
+                        static_cast<int32_t*>(path.data_ptr()), static_cast<int32_t*>(counts.data_ptr()),
+                        static_cast<int64_t*>(next.data_ptr()), stream);
+  Py_END_ALLOW_THREADS;
+  check_status(rc, "pl_verify_tokens");
+  PyObject* r = PyTuple_New(3);
+  if (!r) throw Raised{};
+  PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(std::move(path)));
+  PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(std::move(counts)));
+  PyTuple_SET_ITEM(r, 2, THPVariable_Wrap(std::move(next)));
+  return r;
+}
+
 // (stream) -> pl_stream_capture_id of it
 PyObject* stream_capture_id(PyObject* const* a) {
   void* stream = PyLong_AsVoidPtr(a[0]);
@@ -440,8 +671,9 @@ constexpr PyMethodDef method(const char* name) {
   return {name, (PyCFunction)(void (*)(void)) & guarded<Fn, N>, METH_FASTCALL, nullptr};
 }
 
-PyMethodDef methods[] = {method<rope_append, 15>("rope_append"), method<paged_attention, 15>("paged_attention"),
-                         method<adjust_logits, 12>("adjust_logits"),
+PyMethodDef methods[] = {method<rope_append, 19>("rope_append"), method<paged_attention, 15>("paged_attention"),
+                         method<adjust_logits, 12>("adjust_logits"), method<tree_attention, 14>("tree_attention"),
+                         method<keep_tokens, 7>("keep_tokens"), method<verify_tokens, 8>("verify_tokens"),
                          method<stream_capture_id, 1>("stream_capture_id"), {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensor_calls", nullptr, -1, methods,

@@ -1,9 +1,13 @@
-"""Paged key-value cache of a serving batch: append with the rotation by position, attention of one new token.
+"""Paged key-value cache of a serving batch: append with the rotation by position, attention of new and drafted tokens.
 
 Every row of a batch is a request with its own adapter and its own length; its keys and values lie in pages of one
 pool, in the order of its row of a page table.  ``rope_append`` rotates the new tokens' queries and keys and writes
 keys and values to their places, ``paged_attention`` reads them for the row's newest token.  Rows are right-padded as
 in the rest of the package: token t of row b counts for ``t < min(seq_lens[b], M)``.
+
+Where several tokens of a row are drafted and looked at in one pass, ``rope_append`` appends all of them (``depths``
+where they form a tree), ``tree_attention`` is their attention over the pages and over one another,
+``drafts.verify_tokens`` says which of them stay, and ``keep_tokens`` moves those up behind the row's tokens.
 
 A cache is ``[pages, kv_heads, page_size, head_dim]`` (any strides with a contiguous last dimension, so a permuted
 ``[pages, page_size, kv_heads, head_dim]`` too) in the model's dtype, or ``torch.float8_e4m3fn`` for 16-bit models with
@@ -20,7 +24,7 @@ import torch
 
 from . import _native, sgmv
 
-__all__ = ["paged_attention", "rope_append", "rope_table"]
+__all__ = ["keep_tokens", "paged_attention", "rope_append", "rope_table", "tree_attention"]
 
 
 def rope_table(positions: int, rot: int, base: float = 10000.0, device=None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -41,7 +45,9 @@ def _stream(t: torch.Tensor) -> int:
 def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
                 page_table: torch.Tensor, past_lens: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, *,
                 seq_lens: torch.Tensor | None = None, interleaved: bool = False, k_scale: torch.Tensor | None = None,
-                v_scale: torch.Tensor | None = None, k_out: torch.Tensor | None = None) -> torch.Tensor:
+                v_scale: torch.Tensor | None = None, k_out: torch.Tensor | None = None,
+                q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None, eps: float = 1e-6,
+                depths: torch.Tensor | None = None) -> torch.Tensor:
     """Rotate the new tokens' q and k by position, append k and v to the rows' pages; returns the rotated q.
 
     q ``[rows, M, heads, dim]``, k and v ``[rows, M, kv_heads, dim]`` with a contiguous last dimension (views of one
@@ -54,9 +60,16 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_cache: to
     The rotated q comes back as a new contiguous tensor, 0 for padding tokens; ``k_out``, a contiguous tensor like k,
     also receives the rotated k, for attention inside a prompt.  A token beyond the cos table or on a page the table
     does not hold (an id outside the pool) counts as padding.
+
+    With ``q_norm`` and ``k_norm`` (``[dim]``, fp32 or q's dtype, both of one; either may be None) each head of q and k is
+    first divided by ``sqrt(mean(x ** 2) + eps)`` and multiplied by the weights, in fp32 like the rest and not rounded in
+    between (its squares too: elements beyond 2 ** 59 may give 0).  ``depths`` (int32 ``[rows, M]``, or ``[M]`` for all
+    rows) is for tokens that form a tree: token t is rotated by position ``past_lens[b] + depths[b, t]``, its place in the
+    pages stays ``past_lens[b] + t``.
     """
     return _native.tensor_calls().rope_append(q, k, v, key_cache, value_cache, page_table, past_lens, cos, sin, seq_lens,
-                                              interleaved, k_scale, v_scale, k_out, _stream(q))
+                                              interleaved, k_scale, v_scale, k_out, q_norm, k_norm, eps, depths,
+                                              _stream(q))
 
 
 class _Scratch:
@@ -127,3 +140,35 @@ def paged_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch
     stream = _stream(q)
     return _native.tensor_calls().paged_attention(q, key_cache, value_cache, page_table, lens, scale, window, k_scale,
                                                   v_scale, out, *_scratch(q, stream), stream)
+
+
+def tree_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, page_table: torch.Tensor,
+                   past_lens: torch.Tensor, *, seq_lens: torch.Tensor | None = None,
+                   visible: torch.Tensor | None = None, depths: torch.Tensor | None = None,
+                   scale: float | None = None, window: int | None = None, k_scale: torch.Tensor | None = None,
+                   v_scale: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of several new tokens of each row, drafts or a piece of a prompt, over its pages and one another.
+
+    q ``[rows, M, heads, dim]`` (last dimension contiguous): token t of row b (``t < min(seq_lens[b], M)``) was appended
+    to place ``past_lens[b] + t`` (``rope_append``).  It sees the row's ``past_lens[b]`` tokens before these and, of
+    these, itself and those before it; or, with ``visible``, those whose bit is set in its mask: int32
+    ``[rows, M, words]`` (or ``[M, words]`` for all rows), bit ``j % 32`` of word ``j // 32`` for token j
+    (``drafts.tree_tables`` makes them from the tokens' parents).  With ``window`` a token sees the last that many, itself
+    included, by position; in a tree, of at most ``window`` tokens, that is by ``depths`` and holds for the tokens before
+    the tree.  scale, scales, precision, ``out`` and rows that see nothing are ``paged_attention``'s; padding tokens get 0.
+    """
+    return _native.tensor_calls().tree_attention(q, key_cache, value_cache, page_table, past_lens, seq_lens, visible,
+                                                 depths, scale, window, k_scale, v_scale, out, _stream(q))
+
+
+def keep_tokens(key_caches, value_caches, page_table: torch.Tensor, past_lens: torch.Tensor, path: torch.Tensor,
+                counts: torch.Tensor) -> None:
+    """Move the keys and values of the tokens that stay up behind the row's tokens, in every layer's caches.
+
+    ``key_caches`` and ``value_caches`` are sequences of caches, one for each layer, alike in shape, strides and dtype and
+    none over another.  Row b keeps the tokens at places ``past_lens[b] + path[b, i]``, ``i < counts[b]``: they move to
+    ``past_lens[b] + i``.  path is int32 ``[rows, n]`` and ascends (``drafts.verify_tokens`` gives it; a row's path ends at
+    an entry that does not); counts and past_lens are int32 ``[rows]``.  Moves from or to pages that the table does not
+    hold are left out.  Rows that move tokens do not share the pages they move them in.
+    """
+    _native.tensor_calls().keep_tokens(key_caches, value_caches, page_table, past_lens, path, counts, _stream(path))
