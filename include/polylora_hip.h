@@ -653,8 +653,12 @@ int pl_paged_attention(int32_t dtype, int32_t cache_dtype, const void* q,
  * d is t, or depths[b * depths_row + t] where visible is not NULL; a window of a
  * tree needs depths and is at least row_len.  A token that is not live gives 0, as
  * does one that sees nothing; nothing is read at a place that no live token of the
- * row sees.  q [rows][row_len][heads][dim] with strides of row, token and head, out
- * contiguous and apart from q. */
+ * row sees.  Depths below 0 count as 0.  q [rows][row_len][heads][dim] with strides of
+ * row, token and head, out contiguous and apart from q.  Workspace
+ * (pl_tree_attention_workspace_bytes(dim) bytes) and counters as above; the two may
+ * share them where they follow one another.  At most 2048 query heads to a key head. */
+int64_t pl_tree_attention_workspace_bytes(int32_t dim);
+
 int pl_tree_attention(int32_t dtype, int32_t cache_dtype, const void* q, const int64_t* q_strides,
                       const void* key_cache, const int64_t* key_strides, const void* value_cache,
                       const int64_t* value_strides, int32_t num_pages, int32_t page_size,
@@ -663,7 +667,9 @@ int pl_tree_attention(int32_t dtype, int32_t cache_dtype, const void* q, const i
                       int64_t visible_row, int64_t visible_token, int32_t words,
                       const int32_t* depths, int64_t depths_row, int32_t rows, int32_t row_len,
                       int32_t heads, int32_t kv_heads, int32_t dim, float scale, int32_t window,
-                      const float* k_scale, const float* v_scale, void* out, void* stream);
+                      const float* k_scale, const float* v_scale, void* out, void* workspace,
+                      int64_t workspace_bytes, int32_t* counters, int64_t counter_ints,
+                      void* stream);
 
 /* In every cache of `layers` layers (host arrays of pointers, all caches with
  * these strides, none over another): what lies at place past_lens[b] +

@@ -77,7 +77,7 @@ def tree_attention(q, key, value, table, past, seq_lens=None, visible=None, dept
             continue
         for t in range(n):
             places = seen_places(int(past[b]), n, t, m, None if visible is None else visible[b, t].tolist(),
-                                 None if depths is None else int(depths[b, t]), window)
+                                 None if depths is None else max(0, int(depths[b, t])), window)
             places = [place(table, b, p, num_pages, page_size) for p in places]
             places = [p for p in places if p is not None]
             if not places:

@@ -459,7 +459,7 @@ PyObject* adjust_logits(PyObject* const* a) {
 }
 
 // (q, key_cache, value_cache, page_table, past_lens, seq_lens, visible, depths, scale, window, k_scale, v_scale,
-//  out, stream) -> out; scale and window may be None
+//  out, workspace, workspace_bytes, counters, counter_ints, stream) -> out; scale and window may be None
 PyObject* tree_attention(PyObject* const* a) {
   const at::Tensor& q = tensor(a[0], "q");
   check_lead(q, "tree_attention");
@@ -511,7 +511,8 @@ PyObject* tree_attention(PyObject* const* a) {
     check_shape(*given, "out", q.sizes());
     check_dense(*given, "out");
   }
-  void* stream = PyLong_AsVoidPtr(a[13]);
+  void *workspace = PyLong_AsVoidPtr(a[13]), *counters = PyLong_AsVoidPtr(a[15]), *stream = PyLong_AsVoidPtr(a[17]);
+  const int64_t workspace_bytes = integer(a[14]), counter_ints = integer(a[16]);
   const int32_t r32 = size32(rows, "q"), m32 = size32(m, "q"), h32 = size32(heads, "q"), d32 = size32(dim, "q");
   const int32_t w32 = size32(words, "visible");
   at::Tensor out = given ? *given : at::empty(q.sizes(), q.options());
@@ -520,7 +521,8 @@ PyObject* tree_attention(PyObject* const* a) {
   rc = pl_tree_attention(code, c.code, q.const_data_ptr(), q.strides().data(), c.key, c.key_strides, c.value,
                          c.value_strides, c.num_pages, c.page_size, c.table, c.table_ld, c.max_pages, past, seq, masks,
                          mask_row, mask_token, w32, depth.p, depth.ld, r32, m32, h32, c.kv_heads, d32, (float)scale,
-                         (int32_t)window, c.k_scale, c.v_scale, out.data_ptr(), stream);
+                         (int32_t)window, c.k_scale, c.v_scale, out.data_ptr(), workspace, workspace_bytes,
+                         static_cast<int32_t*>(counters), counter_ints, stream);
   Py_END_ALLOW_THREADS;
   check_status(rc, "pl_tree_attention");
   if (given) return Py_NewRef(a[12]);
@@ -672,7 +674,7 @@ constexpr PyMethodDef method(const char* name) {
 }
 
 PyMethodDef methods[] = {method<rope_append, 19>("rope_append"), method<paged_attention, 15>("paged_attention"),
-                         method<adjust_logits, 12>("adjust_logits"), method<tree_attention, 14>("tree_attention"),
+                         method<adjust_logits, 12>("adjust_logits"), method<tree_attention, 18>("tree_attention"),
                          method<keep_tokens, 7>("keep_tokens"), method<verify_tokens, 8>("verify_tokens"),
                          method<stream_capture_id, 1>("stream_capture_id"), {nullptr, nullptr, 0, nullptr}};
 

@@ -79,19 +79,20 @@ class _Scratch:
     def __init__(self, device: int) -> None:
         self.workspace = sgmv._Workspace(torch.device("cuda", device))
         self.counters: torch.Tensor | None = None
-        self.args: dict[int, tuple[int, int, int, int]] = {}  # by head size; replaced workspaces stay allocated
+        # by call and head size; replaced workspaces stay allocated
+        self.args: dict[tuple[str, int], tuple[int, int, int, int]] = {}
 
-    def get(self, dim: int) -> tuple[int, int, int, int]:
-        return self.args.get(dim) or self._make(dim)
+    def get(self, call: str, dim: int) -> tuple[int, int, int, int]:
+        return self.args.get((call, dim)) or self._make(call, dim)
 
-    def _make(self, dim: int) -> tuple[int, int, int, int]:
+    def _make(self, call: str, dim: int) -> tuple[int, int, int, int]:
         with _LOCK:
-            buf = self.workspace.get(int(_native.load().pl_paged_attention_workspace_bytes(dim)))
+            buf = self.workspace.get(int(getattr(_native.load(), f"pl_{call}_workspace_bytes")(dim)))
             if self.counters is None:
                 # by a fill kernel on the current stream, the launch's, which a HIP graph records like any other
                 self.counters = torch.empty(_native.PL_ATTENTION_COUNTER_INTS, dtype=torch.int32, device=buf.device).zero_()
             args = buf.data_ptr(), buf.numel(), self.counters.data_ptr(), self.counters.numel()
-            self.args[dim] = args
+            self.args[call, dim] = args
             return args
 
 
@@ -104,7 +105,7 @@ _SCRATCH: dict[tuple[int, int], _Scratch] = {}
 _CAPTURED: dict[tuple[int, int], tuple[int, _Scratch]] = {}
 
 
-def _scratch(t: torch.Tensor, stream: int) -> tuple[int, int, int, int]:
+def _scratch(t: torch.Tensor, stream: int, call: str) -> tuple[int, int, int, int]:
     device = t.get_device()
     if device < 0 or t.dim() == 0:
         return 0, 0, 0, 0  # the call refuses the tensor
@@ -114,11 +115,11 @@ def _scratch(t: torch.Tensor, stream: int) -> tuple[int, int, int, int]:
         held = _CAPTURED.get(key)
         if held is None or held[0] != capture or capture < 0:  # below 0: a capture of unknown id
             held = _CAPTURED[key] = capture, _Scratch(device)
-        return held[1].get(t.shape[-1])
+        return held[1].get(call, t.shape[-1])
     held = _SCRATCH.get(key)
     if held is None:
         held = _SCRATCH.setdefault(key, _Scratch(device))
-    return held.get(t.shape[-1])
+    return held.get(call, t.shape[-1])
 
 
 def paged_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, page_table: torch.Tensor,
@@ -134,12 +135,12 @@ def paged_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch
     a token, or whose scores are all -inf, gives 0; slots of pages beyond a row's tokens are never part of a result,
     whatever they hold.
 
-    Calls on one stream share a workspace and counters; a HIP graph has its own, so its replays may overlap other work,
-    but not each other.
+    Calls on one stream share a workspace and counters (``tree_attention``'s too); a HIP graph has its own, so its replays
+    may overlap other work, but not each other.
     """
     stream = _stream(q)
     return _native.tensor_calls().paged_attention(q, key_cache, value_cache, page_table, lens, scale, window, k_scale,
-                                                  v_scale, out, *_scratch(q, stream), stream)
+                                                  v_scale, out, *_scratch(q, stream, "paged_attention"), stream)
 
 
 def tree_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, page_table: torch.Tensor,
@@ -157,8 +158,10 @@ def tree_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.
     included, by position; in a tree, of at most ``window`` tokens, that is by ``depths`` and holds for the tokens before
     the tree.  scale, scales, precision, ``out`` and rows that see nothing are ``paged_attention``'s; padding tokens get 0.
     """
+    stream = _stream(q)
     return _native.tensor_calls().tree_attention(q, key_cache, value_cache, page_table, past_lens, seq_lens, visible,
-                                                 depths, scale, window, k_scale, v_scale, out, _stream(q))
+                                                 depths, scale, window, k_scale, v_scale, out,
+                                                 *_scratch(q, stream, "tree_attention"), stream)
 
 
 def keep_tokens(key_caches, value_caches, page_table: torch.Tensor, past_lens: torch.Tensor, path: torch.Tensor,
