@@ -32,7 +32,7 @@ INCLUDE_DIR = PACKAGE_DIR.parent / "include"
 
 ARCH = "gfx950"
 SOURCES = ("capi.hip", "plan.hip", "sgmv_tiled.hip", "sgmv_fused.hip", "sgmv_wide.hip", "sgmv_long.hip", "sgmv_rows.hip", "sgmv_refop.hip",
-           "paged_append.hip", "paged_attention.hip", "logits.hip", "tree_attention.hip", "keep_tokens.hip", "verify.hip")
+           "paged_append.hip", "paged_attention.hip", "logits.hip", "tree_attention.hip", "tree_wide.hip", "keep_tokens.hip", "verify.hip")
 HIPCC_FLAGS = (
     f"--offload-arch={ARCH}",
     "-O3",
