@@ -702,14 +702,22 @@ int pl_keep_tokens(int32_t dtype, int32_t layers, void* const* key_caches,
  * Where x has NaN or +infinity or nothing above -infinity, or t is not at least 0 and
  * finite, the row stops with token -1; so does a row of no token.
  * path [rows][nodes] gets the numbers of the tokens that stay, from 0 on, -1 behind
- * them; counts how many; next the token that follows. */
+ * them; counts how many; next the token that follows.  At most 1024 tokens to a row
+ * and 2^24 logits to a token.  Workspace (pl_verify_workspace_bytes, 128-byte aligned,
+ * not cleared) and counters (pl_verify_counter_ints int32s, 8-byte aligned, zero before
+ * the first launch and zero again after each call) are not shared by calls that
+ * overlap. */
+int64_t pl_verify_workspace_bytes(int32_t rows, int32_t nodes, int32_t vocab);
+int64_t pl_verify_counter_ints(int32_t rows, int32_t nodes);
+
 int pl_verify_tokens(int32_t dtype, const void* logits, int64_t ld_row, int64_t ld_node,
                      const void* tokens, int32_t token_bytes, int64_t ld_tokens,
                      const float* uniforms, int64_t ld_uniforms, const int32_t* parents,
                      int64_t ld_parents, const float* draft_probs, int64_t ld_draft_row,
                      int64_t ld_draft_node, const float* temperature, const int32_t* seq_lens,
                      int32_t rows, int32_t nodes, int32_t vocab, int32_t* path, int32_t* counts,
-                     int64_t* next, void* stream);
+                     int64_t* next, void* workspace, int64_t workspace_bytes, int32_t* counters,
+                     int64_t counter_ints, void* stream);
 
 /* Logits of one row for the choice of its next token, in fp32 and this order:
  *   x = logits[b][v]

@@ -153,8 +153,10 @@ _SIGNATURES: dict[str, tuple] = {
     "pl_verify_tokens": (
         c_int32, c_void_p, c_int64, c_int64, c_void_p, c_int32, c_int64, c_void_p, c_int64, c_void_p, c_int64,
         c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p,
-        c_void_p,
+        c_void_p, c_int64, c_void_p, c_int64, c_void_p,
     ),
+    "pl_verify_workspace_bytes": (c_int32, c_int32, c_int32),
+    "pl_verify_counter_ints": (c_int32, c_int32),
     "pl_paged_attention": (
         c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32,
         c_void_p, c_int64, c_int32, c_void_p, c_int32, c_int32, c_int32, c_int32, c_float, c_int32, c_void_p,
@@ -172,7 +174,8 @@ _RESTYPES = {"pl_last_error": ctypes.c_char_p, "pl_plan_group_capacity": c_int64
              "pl_host_alloc": c_void_p, "pl_sgmv_ref_workspace_bytes": c_int64, "pl_decode_counter_ints": c_int64,
              "pl_sgmv_ref_part_bytes": c_int64, "pl_lora_long_workspace_bytes": c_int64,
              "pl_stream_capture_id": c_int64, "pl_paged_attention_workspace_bytes": c_int64,
-             "pl_tree_attention_workspace_bytes": c_int64}
+             "pl_tree_attention_workspace_bytes": c_int64, "pl_verify_workspace_bytes": c_int64,
+             "pl_verify_counter_ints": c_int64}
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 

@@ -586,7 +586,8 @@ PyObject* keep_tokens(PyObject* const* a) {
   Py_RETURN_NONE;
 }
 
-// (logits, tokens, uniforms, parents, draft_probs, temperature, seq_lens, stream) -> (path, counts, next)
+// (logits, tokens, uniforms, parents, draft_probs, temperature, seq_lens, workspace, workspace_bytes, counters,
+//  counter_ints, stream) -> (path, counts, next)
 PyObject* verify_tokens(PyObject* const* a) {
   const at::Tensor &logits = tensor(a[0], "logits"), &tokens = tensor(a[1], "tokens");
   const at::Tensor& uniforms = tensor(a[2], "uniforms");
@@ -619,7 +620,8 @@ PyObject* verify_tokens(PyObject* const* a) {
   }
   const float* heat = vector<float>(maybe(a[5], "temperature"), "temperature", at::kFloat, device, rows);
   const int32_t* seq = vector<int32_t>(maybe(a[6], "seq_lens"), "seq_lens", at::kInt, device, rows);
-  void* stream = PyLong_AsVoidPtr(a[7]);
+  void *workspace = PyLong_AsVoidPtr(a[7]), *counters = PyLong_AsVoidPtr(a[9]), *stream = PyLong_AsVoidPtr(a[11]);
+  const int64_t workspace_bytes = integer(a[8]), counter_ints = integer(a[10]);
   const int32_t r32 = size32(rows, "logits"), m32 = size32(m, "logits"), v32 = size32(vocab, "logits");
   const at::TensorOptions ints = logits.options().dtype(at::kInt);
   at::Tensor path = at::empty({rows, m}, ints), counts = at::empty({rows}, ints);
@@ -631,7 +633,8 @@ PyObject* verify_tokens(PyObject* const* a) {
                         static_cast<const float*>(uniforms.const_data_ptr()), uniforms.stride(0), tree.p, tree.ld,
                         draft_probs ? probs : nullptr, probs_row, probs_node, heat, seq, r32, m32, v32,
                         static_cast<int32_t*>(path.data_ptr()), static_cast<int32_t*>(counts.data_ptr()),
-                        static_cast<int64_t*>(next.data_ptr()), stream);
+                        static_cast<int64_t*>(next.data_ptr()), workspace, workspace_bytes,
+                        static_cast<int32_t*>(counters), counter_ints, stream);
   Py_END_ALLOW_THREADS;
   check_status(rc, "pl_verify_tokens");
   PyObject* r = PyTuple_New(3);
@@ -675,7 +678,7 @@ constexpr PyMethodDef method(const char* name) {
 
 PyMethodDef methods[] = {method<rope_append, 19>("rope_append"), method<paged_attention, 15>("paged_attention"),
                          method<adjust_logits, 12>("adjust_logits"), method<tree_attention, 18>("tree_attention"),
-                         method<keep_tokens, 7>("keep_tokens"), method<verify_tokens, 8>("verify_tokens"),
+                         method<keep_tokens, 7>("keep_tokens"), method<verify_tokens, 12>("verify_tokens"),
                          method<stream_capture_id, 1>("stream_capture_id"), {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensor_calls", nullptr, -1, methods,

@@ -12,7 +12,7 @@ from __future__ import annotations
 import torch
 
 from . import _native
-from .paged import _stream
+from .paged import _scratch, _stream
 
 __all__ = ["tree_tables", "verify_tokens"]
 
@@ -68,5 +68,7 @@ def verify_tokens(logits: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Te
     path (int32 ``[rows, M]``) has the numbers of the tokens that stay, from 0 on and -1 behind them, counts (int32
     ``[rows]``) how many they are, token 0 among them, as ``paged.keep_tokens`` takes them; next is int64 ``[rows]``.
     """
+    stream = _stream(logits)
+    sizes = logits.shape if logits.dim() == 3 and logits.numel() < 1 << 62 else (0, 0, 0)  # the call refuses others
     return _native.tensor_calls().verify_tokens(logits, tokens, uniforms, parents, draft_probs, temperature, seq_lens,
-                                                _stream(logits))
+                                                *_scratch(logits, stream, "verify", *sizes), stream)

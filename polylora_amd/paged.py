@@ -73,26 +73,35 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_cache: to
 
 
 class _Scratch:
-    """What the attention's launches use that run one after the other: the workspace for parts of rows, and arrival
-    counters that are zero between launches."""
+    """What launches use that run one after the other: a workspace for parts of the work, and arrival counters that are
+    zero between launches."""
 
     def __init__(self, device: int) -> None:
         self.workspace = sgmv._Workspace(torch.device("cuda", device))
         self.counters: torch.Tensor | None = None
-        # by call and head size; replaced workspaces stay allocated
-        self.args: dict[tuple[str, int], tuple[int, int, int, int]] = {}
+        self.retired: list[torch.Tensor] = []
+        # by call and its sizes; replaced buffers stay allocated
+        self.args: dict[tuple, tuple[int, int, int, int]] = {}
 
-    def get(self, call: str, dim: int) -> tuple[int, int, int, int]:
-        return self.args.get((call, dim)) or self._make(call, dim)
+    def get(self, call: str, *sizes: int) -> tuple[int, int, int, int]:
+        return self.args.get((call, *sizes)) or self._make(call, *sizes)
 
-    def _make(self, call: str, dim: int) -> tuple[int, int, int, int]:
+    def _make(self, call: str, *sizes: int) -> tuple[int, int, int, int]:
+        lib = _native.load()
         with _LOCK:
-            buf = self.workspace.get(int(getattr(_native.load(), f"pl_{call}_workspace_bytes")(dim)))
-            if self.counters is None:
+            buf = self.workspace.get(int(getattr(lib, f"pl_{call}_workspace_bytes")(*sizes)))
+            ints = int(lib.pl_verify_counter_ints(*sizes[:2])) if call == "verify" else 0
+            ints = max(ints, _native.PL_ATTENTION_COUNTER_INTS)
+            if self.counters is None or self.counters.numel() < ints:
+                if self.counters is not None:
+                    self.retired.append(self.counters)
+                    ints = max(ints, 2 * self.counters.numel())
                 # by a fill kernel on the current stream, the launch's, which a HIP graph records like any other
-                self.counters = torch.empty(_native.PL_ATTENTION_COUNTER_INTS, dtype=torch.int32, device=buf.device).zero_()
+                self.counters = torch.empty(ints, dtype=torch.int32, device=buf.device).zero_()
             args = buf.data_ptr(), buf.numel(), self.counters.data_ptr(), self.counters.numel()
-            self.args[call, dim] = args
+            if len(self.args) >= 4096:  # a batch of every size
+                self.args.clear()
+            self.args[(call, *sizes)] = args
             return args
 
 
@@ -105,9 +114,9 @@ _SCRATCH: dict[tuple[int, int], _Scratch] = {}
 _CAPTURED: dict[tuple[int, int], tuple[int, _Scratch]] = {}
 
 
-def _scratch(t: torch.Tensor, stream: int, call: str) -> tuple[int, int, int, int]:
+def _scratch(t: torch.Tensor, stream: int, call: str, *sizes: int) -> tuple[int, int, int, int]:
     device = t.get_device()
-    if device < 0 or t.dim() == 0:
+    if device < 0:
         return 0, 0, 0, 0  # the call refuses the tensor
     key = device, stream
     capture = _native.tensor_calls().stream_capture_id(stream)
@@ -115,11 +124,11 @@ def _scratch(t: torch.Tensor, stream: int, call: str) -> tuple[int, int, int, in
         held = _CAPTURED.get(key)
         if held is None or held[0] != capture or capture < 0:  # below 0: a capture of unknown id
             held = _CAPTURED[key] = capture, _Scratch(device)
-        return held[1].get(call, t.shape[-1])
+        return held[1].get(call, *sizes)
     held = _SCRATCH.get(key)
     if held is None:
         held = _SCRATCH.setdefault(key, _Scratch(device))
-    return held.get(call, t.shape[-1])
+    return held.get(call, *sizes)
 
 
 def paged_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, page_table: torch.Tensor,
@@ -140,7 +149,7 @@ def paged_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch
     """
     stream = _stream(q)
     return _native.tensor_calls().paged_attention(q, key_cache, value_cache, page_table, lens, scale, window, k_scale,
-                                                  v_scale, out, *_scratch(q, stream, "paged_attention"), stream)
+                                                  v_scale, out, *_scratch(q, stream, "paged_attention", *q.shape[-1:]), stream)
 
 
 def tree_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, page_table: torch.Tensor,
@@ -161,7 +170,7 @@ def tree_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.
     stream = _stream(q)
     return _native.tensor_calls().tree_attention(q, key_cache, value_cache, page_table, past_lens, seq_lens, visible,
                                                  depths, scale, window, k_scale, v_scale, out,
-                                                 *_scratch(q, stream, "tree_attention"), stream)
+                                                 *_scratch(q, stream, "tree_attention", *q.shape[-1:]), stream)
 
 
 def keep_tokens(key_caches, value_caches, page_table: torch.Tensor, past_lens: torch.Tensor, path: torch.Tensor,

@@ -31,7 +31,7 @@ def test_cpu_tensors_are_refused():
     with pytest.raises(TypeError, match="sequence"):
         keep_tokens(3, [key], table, lens, table, lens)
     with pytest.raises(TypeError, match="must be a torch.Tensor"):
-        _native.tensor_calls().verify_tokens(*[None] * 7, 0)
+        _native.tensor_calls().verify_tokens(*[None] * 7, 0, 0, 0, 0, 0)
 
 
 def test_tree_tables_of_a_tree():
@@ -148,7 +148,7 @@ def test_tree_attention_refusals_of_the_library():
 
 # What a call gets beside its arguments proper.
 _TREE_SCRATCH = {"ws": 4096, "wsb": 1 << 30, "counters": 4096, "ints": _native.PL_ATTENTION_COUNTER_INTS, "stream": None}
-_VERIFY_SCRATCH = {"stream": None}
+_VERIFY_SCRATCH = {"ws": 4096, "wsb": 1 << 30, "counters": 4096, "ints": 1 << 20, "stream": None}
 
 
 def test_verification_refusals_of_the_library():
@@ -166,6 +166,10 @@ def test_verification_refusals_of_the_library():
     assert _refused(call, good, parents=p) == _native.PL_ERR_ARG  # probabilities of a tree
     for name in ("logits", "tokens", "uniforms", "path", "counts", "next"):
         assert _refused(call, good, **{name: None}) == _native.PL_ERR_ARG
+    assert _refused(call, good, nodes=1025) == _native.PL_ERR_LIMIT
+    assert _refused(call, good, wsb=lib.pl_verify_workspace_bytes(2, 5, 16) - 1) == _native.PL_ERR_ARG
+    assert _refused(call, good, ints=lib.pl_verify_counter_ints(2, 5) - 1) == _native.PL_ERR_ARG
+    assert _refused(call, good, counters=None) == _native.PL_ERR_ARG
     assert call(*{**good, "rows": 0}.values()) == 0
 
 
