@@ -25,6 +25,7 @@ struct tree_args {
   int32_t tok0, toks;           // the tokens of this launch
   int32_t col_tiles, slices;    // workers: col_tiles for each slice
   float per_group;              // 1 / group
+  int32_t once;                 // keys and values are read once and stay in no cache
 };
 
 namespace {
@@ -128,7 +129,7 @@ struct tree_run {
   bool whole_pairs;
 };
 template <int ATOM, int TILES>
-__device__ __forceinline__ tree_run find_run(const tree_args& a, int slice, int lane) {
+__device__ __forceinline__ tree_run find_run(const tree_args& a, int slice, int lane, bool one_of_many = false) {
   tree_run r;
   // Each wave works out the deal for itself: 64 rows to a look, no barrier.
   constexpr int kLooks = 2;  // that stay in registers
@@ -150,9 +151,10 @@ __device__ __forceinline__ tree_run find_run(const tree_args& a, int slice, int 
   }
   total = __builtin_amdgcn_readlane(scan_sum(total), 63) * a.kv_heads;
   longest = __builtin_amdgcn_readlane(scan_max(longest), 63);
-  const bool whole_pairs =
-      choose_whole<TILES>(a.slices, total, a.rows * a.kv_heads, longest);
-  const int per = (total + a.slices - 1) / a.slices;
+  // where asked for, one workgroup on a CU for many atoms (see paged_attention.hip)
+  const int slices = one_of_many && total >= 8 * kCus ? min(a.slices, kCus) : a.slices;
+  const bool whole_pairs = choose_whole<TILES>(slices, total, a.rows * a.kv_heads, longest);
+  const int per = (total + slices - 1) / slices;
   r.from = (int)min((int64_t)slice * per, (int64_t)total);
   r.to = min(total - per, r.from) + per;
   r.per = per, r.total = total, r.whole_pairs = whole_pairs;
@@ -201,6 +203,9 @@ __device__ __forceinline__ column_place place_of(const tree_args& a, int col, in
 }
 
 // The weights of a column's eight tokens of a tile as 16-bit parts, two tokens to a word.
+// No part is negative, or 0 beside the first, so that an infinite value stays one: bf16
+// takes the rest of the weight 2^-20 larger, as in all weights alike and in their sum
+// (fp16 ends too early for that).
 template <int DT>
 __device__ __forceinline__ void weight_parts(const float* p, pl_u32x4* part) {
   constexpr int kParts = kWeightParts<DT>;
@@ -210,9 +215,11 @@ __device__ __forceinline__ void weight_parts(const float* p, pl_u32x4* part) {
 #pragma unroll
     for (int k = 0; k < kParts; ++k) {
       const uint32_t z = k + 1 < kParts ? pack2_down<DT>(x, y) : pack2<DT>(x, y);
-      if (k + 1 < kParts) x -= unpack<DT>(z, 0), y -= unpack<DT>(z, 1);
-      // no part negative, or 0 beside the others: an infinite value stays one
-      part[k][j] = k ? at_least_smallest<DT>(z, part[0][j]) : z;
+      if (k + 1 < kParts) {
+        constexpr float kMore = DT == PL_BF16 ? 1.f + 0x1p-20f : 1.f;
+        x = fmaf(x, kMore, -unpack<DT>(z, 0)), y = fmaf(y, kMore, -unpack<DT>(z, 1));
+      }
+      part[k][j] = k && DT == PL_F16 ? at_least_smallest<DT>(z, part[0][j]) : z;
     }
   }
 }
@@ -332,9 +339,8 @@ __device__ __forceinline__ void add_nonfinite(const tree_args& a, const tree_spa
 // Raises the references of columns whose scores have gone far above them: the largest
 // score takes the place.  They stay while no score is more than kSlack above them, so
 // weights reach 2^kSlack, and the outputs are rescaled at a few tiles only.
-template <int TOKENS, int V, int C>
-__device__ __forceinline__ void rescale(const float (*p)[TOKENS], float scale2, float* m, float* l,
-                                        pl_f32x4 (*o)[V]) {
+template <int TOKENS, int V, int C, typename L>
+__device__ __forceinline__ void rescale(const float (*p)[TOKENS], float scale2, float* m, L* l, pl_f32x4 (*o)[V]) {
   float top[C];
   bool beyond = false;
 #pragma unroll
@@ -342,13 +348,12 @@ __device__ __forceinline__ void rescale(const float (*p)[TOKENS], float scale2, 
     top[c] = p[c][0];
 #pragma unroll
     for (int j = 1; j < TOKENS; ++j) top[c] = fmaxf(top[c], p[c][j]);
-    top[c] = column_max(top[c]) * scale2;
-    beyond = beyond || top[c] > m[c] + kSlack;
+    beyond = beyond || top[c] * scale2 > m[c] + kSlack;  // of this lane's tokens
   }
   if (!__any(beyond)) return;
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    top[c] = fmaxf(top[c], m[c]);
+    top[c] = fmaxf(column_max(top[c]) * scale2, m[c]);
     const float keep = exp2_fast(m[c] - (top[c] == -INFINITY ? 0.f : top[c]));
     l[c] *= keep;
 #pragma unroll
@@ -357,12 +362,20 @@ __device__ __forceinline__ void rescale(const float (*p)[TOKENS], float scale2, 
   }
 }
 
-// Adds up a tile's values by the columns' weights (16-bit models).
+// Adds up a tile's values by the columns' weights, and the weights themselves, as the
+// values of an element that is 1 everywhere: a product more on units that have little
+// to do beside the vector unit (16-bit models).
 template <int DT, int CT, int DP, int C>
 __device__ __forceinline__ void add_values(const uint32_t (*v)[shape<DT, CT, DP>::kVWords],
                                            const pl_u32x4 (*part)[kWeightParts<DT>],
-                                           pl_f32x4 (*o)[shape<DT, CT, DP>::V]) {
+                                           pl_f32x4 (*o)[shape<DT, CT, DP>::V], pl_f32x4* l) {
   typedef shape<DT, CT, DP> S;
+  constexpr uint32_t kOnes = DT == PL_BF16 ? 0x3f803f80u : 0x3c003c00u;
+  const pl_u32x4 ones = {kOnes, kOnes, kOnes, kOnes};
+#pragma unroll
+  for (int k = 0; k < kWeightParts<DT>; ++k)
+#pragma unroll
+    for (int c = 0; c < C; ++c) l[c] = pl_mfma_chunk<DT>(ones, part[c][k], l[c]);
 #pragma unroll
   for (int i = 0; i < S::V / 2; ++i) {
     uint32_t word[8];

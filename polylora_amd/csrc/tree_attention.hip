@@ -18,7 +18,7 @@ constexpr int waves_per_simd() {
   return DP == 256 || (DT == PL_F32 && DP == 128 && C == 2) ? 1 : 2;
 }
 
-template <int DT, int CT, int DP, int C, bool FULL>
+template <int DT, int CT, int DP, int C, bool FULL, bool STREAM>
 __global__ __launch_bounds__(kThreads, (waves_per_simd<DT, DP, C>())) void pl_tree_attention_kernel(tree_args a) {
   typedef shape<DT, CT, DP> S;
   typedef typename pl_traits<DT>::T T;
@@ -34,7 +34,8 @@ __global__ __launch_bounds__(kThreads, (waves_per_simd<DT, DP, C>())) void pl_tr
   const int li = lane & 15, lg = lane >> 4;
   const tree_worker me = worker_of(a);
   const int ct = me.ct, slice = me.slice;
-  const tree_run run = find_run<S::kAtom, S::kAtom / (kWaves * S::kTile)>(a, slice, lane);
+  const tree_run run = find_run<S::kAtom, S::kAtom / (kWaves * S::kTile)>(
+      a, slice, lane, DT != PL_F32 && DP <= 128 && C == 1 && a.dim * S::kCsize >= 128 && a.col_tiles == 1);
   const int from = run.from, to = run.to, per = run.per;
   const bool whole_pairs = run.whole_pairs;
   if (from >= run.total) return;
@@ -72,12 +73,13 @@ __global__ __launch_bounds__(kThreads, (waves_per_simd<DT, DP, C>())) void pl_tr
     pl_u32x4 q_own[kQueryLds ? 1 : C][kQueryLds ? 1 : S::kSteps];
     shared_u32x4* q_lds = reinterpret_cast<shared_u32x4*>(s_q) + lane;
     pl_f32x4 o[C][S::V];
-    float m[C], l[C];
+    float m[C];
+    typename std::conditional<DT == PL_F32, float, pl_f32x4>::type l[C];  // fp32: of this lane's tokens
     // this lane's column of each 16: its token (-1: none that counts) and the first place that it sees
     int t[C], first[C], all_from = 0;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      m[c] = -INFINITY, l[c] = 0.f;
+      m[c] = -INFINITY, l[c] = {};
 #pragma unroll
       for (int i = 0; i < S::V; ++i) o[c][i] = pl_f32x4{0.f, 0.f, 0.f, 0.f};
       const int in = c * kCols + li;
@@ -157,7 +159,7 @@ __global__ __launch_bounds__(kThreads, (waves_per_simd<DT, DP, C>())) void pl_tr
 #pragma unroll
         for (int n = 0; n < S::kKeyLoads; ++n) {
           uint32_t x[4];
-          load_words<4, false>(b, key_off[n], 0, x);
+          load_words<4, STREAM>(b, key_off[n], 0, x);
           keys[u][n] = pl_u32x4{x[0], x[1], x[2], x[3]};
         }
       }
@@ -175,7 +177,7 @@ __global__ __launch_bounds__(kThreads, (waves_per_simd<DT, DP, C>())) void pl_tr
           for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int n = 0; n < S::kPieces; ++n)
-              load_words<S::kVWords / S::kPieces, false>(b, value_off[n], j * w.value_slot,
+              load_words<S::kVWords / S::kPieces, STREAM>(b, value_off[n], j * w.value_slot,
                                                           v[4 * u + j] + n * (S::kVWords / S::kPieces));
         }
         const tile_place<S::kSubs> here = place;
@@ -220,7 +222,7 @@ __global__ __launch_bounds__(kThreads, (waves_per_simd<DT, DP, C>())) void pl_tr
 #pragma unroll
           for (int j = 0; j < S::kTokens; ++j) {
             p[c][j] = exp2_fast(fmaf(p[c][j], scale2, -ref));
-            l[c] += p[c][j];
+            if constexpr (DT == PL_F32) l[c] += p[c][j];
           }
           if constexpr (DT != PL_F32) weight_parts<DT>(p[c], part[c]);
         }
@@ -238,7 +240,7 @@ __global__ __launch_bounds__(kThreads, (waves_per_simd<DT, DP, C>())) void pl_tr
             if (i % 2) __builtin_amdgcn_sched_barrier(0);
           }
         } else {
-          add_values<DT, CT, DP, C>(v, part, o);
+          add_values<DT, CT, DP, C>(v, part, o, l);
         }
         tile = next;
       } while (tile < end);
@@ -258,8 +260,12 @@ __global__ __launch_bounds__(kThreads, (waves_per_simd<DT, DP, C>())) void pl_tr
     const pl_buffer parts = P::all(a.parts, 2u * kWorkersMax * C);
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      l[c] = column_sum(l[c]);
-      if (lg == 0) s_m[wave][c * kCols + li] = m[c], s_l[wave][c * kCols + li] = l[c];
+      float sum;
+      if constexpr (DT == PL_F32)
+        sum = column_sum(l[c]);
+      else
+        sum = l[c].x;
+      if (lg == 0) s_m[wave][c * kCols + li] = m[c], s_l[wave][c * kCols + li] = sum;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
 #pragma unroll
@@ -324,12 +330,15 @@ template <int DT, int CT, int DP, int C>
 void launch_columns(tree_args a, int64_t atoms_most, hipStream_t s) {
   const int columns = a.toks * a.group;
   a.col_tiles = (columns + C * kCols - 1) / (C * kCols);
+  a.once = a.once && a.col_tiles == 1;
   a.slices = slices_of(atoms_most, kCus * waves_per_simd<DT, DP, C>(), a.col_tiles);
   const dim3 grid((unsigned)(a.slices * a.col_tiles));
-  if (a.dim == DP)
-    pl_tree_attention_kernel<DT, CT, DP, C, true><<<grid, kThreads, 0, s>>>(a);
+  if (a.dim != DP)
+    pl_tree_attention_kernel<DT, CT, DP, C, false, false><<<grid, kThreads, 0, s>>>(a);
+  else if (a.once)
+    pl_tree_attention_kernel<DT, CT, DP, C, true, true><<<grid, kThreads, 0, s>>>(a);
   else
-    pl_tree_attention_kernel<DT, CT, DP, C, false><<<grid, kThreads, 0, s>>>(a);
+    pl_tree_attention_kernel<DT, CT, DP, C, true, false><<<grid, kThreads, 0, s>>>(a);
 }
 
 // Columns above which 16-bit models take the other kernel.
@@ -437,6 +446,8 @@ extern "C" int pl_tree_attention(int32_t dtype, int32_t cache_dtype, const void*
   a.k_scale = k_scale, a.v_scale = v_scale, a.out = out, a.scale = scale, a.rows = rows, a.row_len = row_len;
   a.heads = heads, a.kv_heads = kv_heads, a.dim = dim, a.window = window, a.group = heads / kv_heads, a.per_group = 1.f / (float)a.group;
   a.parts = static_cast<float*>(workspace), a.counters = counters;
+  // lines are marked as read once where a pool of pages is too large for the last cache
+  a.once = 2ll * num_pages * ((int64_t)kv_heads * dim * page_size) * pl_cache_elem_size(cache_dtype) > (256 << 20);
   // atoms at most: every row as long as its pages or its window allow
   int64_t longest = (int64_t)max_pages * page_size;
   if (window > 0 && longest > (int64_t)window + row_len + 31) longest = (int64_t)window + row_len + 31;

@@ -53,8 +53,96 @@ __device__ __forceinline__ void load_to_lds(uint32_t to, uintptr_t p, uint32_t b
                : "memory");
 }
 
+// Joins n parts of columns [in0, in1) (numbers of sixteens: the first part's, and from the
+// second on first + step * part) and puts out what comes of them.  A thread has kItems
+// places in hand, kBatch parts of each at a time: parts come from where every XCD
+// sees them, and what counts is how many are on their way.
+template <typename T, int DP, bool FULL>
+__device__ __forceinline__ void join_columns(const tree_args& a, pl_buffer parts, int first, int others, int step, int n,
+                                             int row, int col0, int in0, int in1, int live, int hk, float v_scale,
+                                             int threads) {
+  typedef part_layout<DP> P;
+  constexpr int kItems = 4, kBatch = 2;
+  const int items = (in1 - in0) * (DP / 4);
+  for (int i0 = (int)threadIdx.x; i0 < items; i0 += kItems * threads) {
+    float top[kItems], sum[kItems];
+    pl_f32x4 y[kItems];
+#pragma unroll
+    for (int s = 0; s < kItems; ++s) top[s] = -INFINITY, sum[s] = 0.f, y[s] = pl_f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int k0 = 0; k0 < n; k0 += kBatch) {
+      pl_f32x4 x[kItems][kBatch];
+      pl_f32x2 ml[kItems][kBatch];
+#pragma unroll
+      for (int s = 0; s < kItems; ++s)
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          const int i = min(i0 + s * threads, items - 1), in = in0 + i / (DP / 4), d = i % (DP / 4) * 4;
+          const int k = min(k0 + j, n - 1);  // the last again, with no weight
+          const uint32_t part = (uint32_t)((k ? others + step * k : first) + in / kCols) * P::kBytes;
+          x[s][j] = __builtin_bit_cast(
+              pl_f32x4, __builtin_amdgcn_raw_buffer_load_b128(parts, part + P::at(in % kCols, d), 0, kAgentScope));
+          ml[s][j] = __builtin_bit_cast(
+              pl_f32x2, __builtin_amdgcn_raw_buffer_load_b64(parts, part + P::sums(in % kCols), 0, kAgentScope));
+        }
+#pragma unroll
+      for (int s = 0; s < kItems; ++s) {
+        float high = top[s];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          ml[s][j].x = k0 + j < n ? ml[s][j].x : -INFINITY;
+          high = fmaxf(high, ml[s][j].x);
+        }
+        const float ref = high == -INFINITY ? 0.f : high, keep = exp2_fast(top[s] - ref);
+        sum[s] *= keep, y[s] *= keep, top[s] = high;
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          const float f = exp2_fast(ml[s][j].x - ref);
+          sum[s] += f * ml[s][j].y, y[s] += f * x[s][j];
+        }
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < kItems; ++s) {
+      const int i = i0 + s * threads;
+      if (i < items)
+        put_output<T, FULL>(a, row, col0, in0 + i / (DP / 4), live, hk, i % (DP / 4) * 4, y[s], sum[s], v_scale);
+    }
+  }
+}
+
+// The parts of pairs that are cut into many: a workgroup to each sixteen of columns of a
+// pair, where one that arrives last would have all of them to itself.
+constexpr int kJoinThreads = 256;
 template <int DT, int CT, int DP, bool FULL>
-__global__ __launch_bounds__(kWideThreads, 2) void pl_tree_wide_kernel(tree_args a, int across) {
+__global__ __launch_bounds__(kJoinThreads) void pl_tree_join_kernel(tree_args a) {
+  typedef wide<DT, CT, DP> S;
+  typedef typename pl_traits<DT>::T T;
+  constexpr int kSixteens = kWideWaves * S::C;
+  const int lane = (int)threadIdx.x & 63;
+  const int sixteen = (int)blockIdx.x % kSixteens, ct = (int)blockIdx.x / kSixteens % a.col_tiles;
+  const int pair = (int)blockIdx.x / kSixteens / a.col_tiles, row = pair / a.kv_heads, hk = pair % a.kv_heads;
+  const int col0 = ct * wide_columns(DP), cols = min(wide_columns(DP), a.toks * a.group - col0);
+  const int in0 = sixteen * kCols, in1 = min(in0 + kCols, cols);
+  if (in0 >= in1) return;
+  // the deal, and the atoms before this row
+  const tree_run run = find_run<S::kAtom, S::kAtom / 128>(a, 0, lane);
+  if (run.whole_pairs) return;
+  int before = 0;
+  for (int b = lane; b < row; b += 64) before += span_of<S::kAtom>(a, a.past[b], a.seq_lens ? a.seq_lens[b] : a.row_len).atoms;
+  before = __builtin_amdgcn_readlane(scan_sum(before), 63) * a.kv_heads;
+  const tree_span r = span_of<S::kAtom>(a, a.past[row], a.seq_lens ? a.seq_lens[row] : a.row_len);
+  const int pair_start = before + hk * r.atoms;
+  const int w0 = pair_start / run.per, w1 = (pair_start + r.atoms - 1) / run.per;
+  if (w0 == w1) return;  // in one piece: its worker has put it out
+  const int live = max(0, min(cols, (min(r.n, a.tok0 + a.toks) - a.tok0) * a.group - col0));
+  const int slot1 = 2 * (w0 * a.col_tiles + ct), slot0 = slot1 + (w0 * run.per == pair_start ? 0 : 1);
+  join_columns<T, DP, FULL>(a, part_layout<DP>::all(a.parts, 2u * kWorkersMax / 2 * kSixteens), slot0 * kSixteens,
+                            slot1 * kSixteens, 2 * a.col_tiles * kSixteens, w1 - w0 + 1, row, col0, in0, in1, live, hk,
+                            CT == PL_F8E4M3 ? a.v_scale[hk] : 1.f, kJoinThreads);
+}
+
+template <int DT, int CT, int DP, bool FULL>
+__global__ __launch_bounds__(kWideThreads, 2) void pl_tree_wide_kernel(tree_args a, int across, int join_later) {
   typedef wide<DT, CT, DP> S;
   typedef typename pl_traits<DT>::T T;
   constexpr int C = S::C, kParts = kWeightParts<DT>;
@@ -119,7 +207,8 @@ __global__ __launch_bounds__(kWideThreads, 2) void pl_tree_wide_kernel(tree_args
     const int live = max(0, min(cols, (min(r.n, a.tok0 + a.toks) - a.tok0) * a.group - col0));
 
     pl_f32x4 o[C][S::V];
-    float m[C], l[C];
+    float m[C];
+    pl_f32x4 l[C];
     int t[C], first[C], all_from = 0;
     pl_u32x4 q[C][S::kSteps];
     const float signed_scale = a.scale * 1.44269504088896f * (CT == PL_F8E4M3 ? as_scalar(a.k_scale)[hk] : 1.f);
@@ -127,7 +216,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void pl_tree_wide_kernel(tree_args
     const uint32_t flip = signed_scale < 0.f ? 0x80008000u : 0u;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      m[c] = -INFINITY, l[c] = 0.f;
+      m[c] = -INFINITY, l[c] = pl_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < S::V; ++i) o[c][i] = pl_f32x4{0.f, 0.f, 0.f, 0.f};
       const int in = (wc + c * across) * kCols + li;
@@ -145,7 +234,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void pl_tree_wide_kernel(tree_args
         q[c][n] ^= flip;
       }
     }
-    if (a.window > 0) all_from = __builtin_amdgcn_readlane(scan_max(all_from), 63);
+    all_from = a.window > 0 ? __builtin_amdgcn_readlane(scan_max(all_from), 63) : 0;
 
     // a line's last column sees the most; no column that counts, no token
     const int last_t = uniform(place_of(a, max(0, col0 + live - 1), hk).token);
@@ -186,6 +275,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void pl_tree_wide_kernel(tree_args
     };
 
     bool nonfinite = false;  // values of a mixed unit were infinities or NaN
+    uint32_t all_held = 0;   // which 16 tokens of the stage lie on pages that the table holds
     // A unit: 32 tokens of the stage.
     auto unit = [&](int buffer, int u, int tile) __attribute__((always_inline)) {
       const uint8_t* mem = s_mem + buffer * 2 * S::kSide + u * 32 * S::kRow;
@@ -194,25 +284,38 @@ __global__ __launch_bounds__(kWideThreads, 2) void pl_tree_wide_kernel(tree_args
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int c = 0; c < C; ++c) s[h][c] = pl_f32x4{0.f, 0.f, 0.f, 0.f};
+      // all keys of a step asked for before the first product: a wave has little else to
+      // wait behind
+      constexpr int kAhead = S::kKeyLoads < 4 ? S::kKeyLoads : 4;
 #pragma unroll
-      for (int n = 0; n < S::kKeyLoads; ++n)
+      for (int n0 = 0; n0 < S::kKeyLoads; n0 += kAhead) {
+        pl_u32x4 keys[kAhead][2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const pl_u32x4 k = *reinterpret_cast<const shared_u32x4*>(mem + h * 16 * S::kRow + key_at[n]);
-          if constexpr (CT == PL_F8E4M3) {
-            const pl_u32x4 x = {widen<DT, false>(k.x), widen<DT, true>(k.x), widen<DT, false>(k.y),
-                                widen<DT, true>(k.y)};
-            const pl_u32x4 y = {widen<DT, false>(k.z), widen<DT, true>(k.z), widen<DT, false>(k.w),
-                                widen<DT, true>(k.w)};
+        for (int n = 0; n < kAhead; ++n)
 #pragma unroll
-            for (int c = 0; c < C; ++c) s[h][c] = pl_mfma_chunk<DT>(x, q[c][2 * n], s[h][c]);
+          for (int h = 0; h < 2; ++h)
+            keys[n][h] = *reinterpret_cast<const shared_u32x4*>(mem + h * 16 * S::kRow + key_at[n0 + n]);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int c = 0; c < C; ++c) s[h][c] = pl_mfma_chunk<DT>(y, q[c][2 * n + 1], s[h][c]);
-          } else {
+        for (int n = 0; n < kAhead; ++n)
 #pragma unroll
-            for (int c = 0; c < C; ++c) s[h][c] = pl_mfma_chunk<DT>(k, q[c][n], s[h][c]);
+          for (int h = 0; h < 2; ++h) {
+            const pl_u32x4 k = keys[n][h];
+            if constexpr (CT == PL_F8E4M3) {
+              const pl_u32x4 x = {widen<DT, false>(k.x), widen<DT, true>(k.x), widen<DT, false>(k.y),
+                                  widen<DT, true>(k.y)};
+              const pl_u32x4 y = {widen<DT, false>(k.z), widen<DT, true>(k.z), widen<DT, false>(k.w),
+                                  widen<DT, true>(k.w)};
+#pragma unroll
+              for (int c = 0; c < C; ++c) s[h][c] = pl_mfma_chunk<DT>(x, q[c][2 * (n0 + n)], s[h][c]);
+#pragma unroll
+              for (int c = 0; c < C; ++c) s[h][c] = pl_mfma_chunk<DT>(y, q[c][2 * (n0 + n) + 1], s[h][c]);
+            } else {
+#pragma unroll
+              for (int c = 0; c < C; ++c) s[h][c] = pl_mfma_chunk<DT>(k, q[c][n0 + n], s[h][c]);
+            }
           }
-        }
+      }
       uint32_t v[S::kTokens][S::kVWords];
 #pragma unroll
       for (int j = 0; j < S::kTokens; ++j)
@@ -227,7 +330,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void pl_tree_wide_kernel(tree_args
       for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int j = 0; j < S::kTokens; ++j) p[c][j] = s[j / 4][c][j % 4];
-      const bool held[2] = {uniform(s_held[buffer][2 * u]) != 0, uniform(s_held[buffer][2 * u + 1]) != 0};
+      const bool held[2] = {(all_held >> 2 * u & 1) != 0, (all_held >> 2 * u & 2) != 0};
       if (__builtin_expect(!(tile >= all_from && tile + 32 <= min(r.past, r.len) && held[0] && held[1]), 0))
         nonfinite |= mask_tile<DT, CT, DP, C>(a, r, row, t, first, tile, held, lane, p, v);
       rescale<S::kTokens, S::V, C>(p, scale2, m, l, o);
@@ -237,13 +340,10 @@ __global__ __launch_bounds__(kWideThreads, 2) void pl_tree_wide_kernel(tree_args
         // nothing alive yet: any finite reference gives weights of 0
         const float ref = (m[c] == -INFINITY ? 0.f : m[c]) - kLift;
 #pragma unroll
-        for (int j = 0; j < S::kTokens; ++j) {
-          p[c][j] = exp2_fast(fmaf(p[c][j], scale2, -ref));
-          l[c] += p[c][j];
-        }
+        for (int j = 0; j < S::kTokens; ++j) p[c][j] = exp2_fast(fmaf(p[c][j], scale2, -ref));
         weight_parts<DT>(p[c], part[c]);
       }
-      add_values<DT, CT, DP, C>(v, part, o);
+      add_values<DT, CT, DP, C>(v, part, o, l);
     };
 
     constexpr int kStage = S::kUnits * 32;
@@ -254,6 +354,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void pl_tree_wide_kernel(tree_args
       __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
       __syncthreads();
       if (base + kStage < end) load_stage(buffer ^ 1, base + kStage);
+      all_held = (uint32_t)__ballot(lane < 2 * S::kUnits && s_held[buffer][min(lane, 2 * S::kUnits - 1)]);
       for (int u = wt; u < S::kUnits && base + u * 32 < end; u += behind) {
         if (wc * kCols < live) unit(buffer, u, base + u * 32);
       }
@@ -278,9 +379,8 @@ __global__ __launch_bounds__(kWideThreads, 2) void pl_tree_wide_kernel(tree_args
     constexpr int kPitch = DP + 4;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      l[c] = column_sum(l[c]);
       __syncthreads();
-      if (lg == 0) s_m[wave][li] = m[c], s_l[wave][li] = l[c];
+      if (lg == 0) s_m[wave][li] = m[c], s_l[wave][li] = l[c].x;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
 #pragma unroll
@@ -308,7 +408,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void pl_tree_wide_kernel(tree_args
           put_part<DP>(parts, slot * kSixteens, in, d, x, top, sum);
       }
     }
-    if (!complete) {
+    if (!complete && !join_later) {
       // Parts are acknowledged from where every XCD sees them before the arrival
       // is counted, and the last to arrive asks for them there after that.
       const int w0 = pair_start / per, w1 = (pair_start + r.atoms - 1) / per;
@@ -325,40 +425,8 @@ __global__ __launch_bounds__(kWideThreads, 2) void pl_tree_wide_kernel(tree_args
         // the first part is its workgroup's second when that workgroup began earlier
         const int slot1 = 2 * (w0 * a.col_tiles + ct), slot0 = slot1 + (w0 * per == pair_start ? 0 : 1);
         const int n = w1 - w0 + 1;
-        constexpr int kBatch = 4;
-        for (int i = tid; i < cols * (DP / 4); i += kWideThreads) {
-          const int in = i / (DP / 4), d = i % (DP / 4) * 4;
-          float top = -INFINITY, sum = 0.f;
-          pl_f32x4 y = {0.f, 0.f, 0.f, 0.f};
-          for (int k0 = 0; k0 < n; k0 += kBatch) {
-            pl_f32x4 x[kBatch];
-            pl_f32x2 ml[kBatch];
-#pragma unroll
-            for (int j = 0; j < kBatch; ++j) {
-              const int k = min(k0 + j, n - 1);  // the last again, with no weight
-              const uint32_t part =
-                  (uint32_t)((k ? slot1 + 2 * a.col_tiles * k : slot0) * kSixteens + in / kCols) * P::kBytes;
-              x[j] = __builtin_bit_cast(
-                  pl_f32x4, __builtin_amdgcn_raw_buffer_load_b128(parts, part + P::at(in % kCols, d), 0, kAgentScope));
-              ml[j] = __builtin_bit_cast(
-                  pl_f32x2, __builtin_amdgcn_raw_buffer_load_b64(parts, part + P::sums(in % kCols), 0, kAgentScope));
-            }
-            float high = top;
-#pragma unroll
-            for (int j = 0; j < kBatch; ++j) {
-              ml[j].x = k0 + j < n ? ml[j].x : -INFINITY;
-              high = fmaxf(high, ml[j].x);
-            }
-            const float ref = high == -INFINITY ? 0.f : high, keep = exp2_fast(top - ref);
-            sum *= keep, y *= keep, top = high;
-#pragma unroll
-            for (int j = 0; j < kBatch; ++j) {
-              const float f = exp2_fast(ml[j].x - ref);
-              sum += f * ml[j].y, y += f * x[j];
-            }
-          }
-          put_output<T, FULL>(a, row, col0, in, live, hk, d, y, sum, v_scale);
-        }
+        join_columns<T, DP, FULL>(a, parts, slot0 * kSixteens, slot1 * kSixteens, 2 * a.col_tiles * kSixteens, n, row, col0,
+                                  0, cols, live, hk, v_scale, kWideThreads);
       }
     }
     __syncthreads();  // the shared arrays are free again
@@ -372,6 +440,9 @@ __global__ __launch_bounds__(kWideThreads, 2) void pl_tree_wide_kernel(tree_args
   }
 }
 
+// Slices to a pair above which parts are joined by a launch of their own.
+constexpr int kManyParts = 3;
+
 template <int DT, int CT, int DP>
 void launch_wide(tree_args a, int64_t atoms_most, hipStream_t s) {
   const int columns = a.toks * a.group, most = wide_columns(DP);
@@ -380,10 +451,16 @@ void launch_wide(tree_args a, int64_t atoms_most, hipStream_t s) {
   int across = 1;
   while (across < kWideWaves && across * kCols * wide<DT, CT, DP>::C < columns) across *= 2;
   const dim3 grid((unsigned)(a.slices * a.col_tiles));
-  if (a.dim == DP)
-    pl_tree_wide_kernel<DT, CT, DP, true><<<grid, kWideThreads, 0, s>>>(a, across);
-  else
-    pl_tree_wide_kernel<DT, CT, DP, false><<<grid, kWideThreads, 0, s>>>(a, across);
+  const int64_t pairs = (int64_t)a.rows * a.kv_heads;
+  const int later = a.slices > kManyParts * pairs;
+  const dim3 joins((unsigned)(later ? pairs * a.col_tiles * kWideWaves * wide<DT, CT, DP>::C : 0));
+  if (a.dim == DP) {
+    pl_tree_wide_kernel<DT, CT, DP, true><<<grid, kWideThreads, 0, s>>>(a, across, later);
+    if (later) pl_tree_join_kernel<DT, CT, DP, true><<<joins, kJoinThreads, 0, s>>>(a);
+  } else {
+    pl_tree_wide_kernel<DT, CT, DP, false><<<grid, kWideThreads, 0, s>>>(a, across, later);
+    if (later) pl_tree_join_kernel<DT, CT, DP, false><<<joins, kJoinThreads, 0, s>>>(a);
+  }
 }
 
 template <int DT, int CT>
