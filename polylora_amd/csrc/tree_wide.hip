@@ -18,7 +18,8 @@
 namespace {
 
 constexpr int kWideThreads = kWideWaves * 64;
-constexpr int kStageBytes = 64 << 10;
+constexpr int kStageBytes = 32 << 10;
+constexpr int kBuffers = 4;  // one is read, three are on their way
 
 template <int DT, int CT, int DP>
 struct wide : shape<DT, CT, DP> {
@@ -27,12 +28,13 @@ struct wide : shape<DT, CT, DP> {
   static constexpr int kRow = DP * S::kCsize;   // bytes of a token in LDS
   static constexpr int kSlots = kRow / 16;      // its pieces
   static constexpr int kFit = kStageBytes / (2 * 32 * kRow);
-  static constexpr int kUnits = kFit < 8 ? kFit : 8;  // of a stage, 32 tokens each
+  static constexpr int kUnits = kFit < 4 ? kFit : 4;  // of a stage, 32 tokens each
   static constexpr int kSide = kUnits * 32 * kRow;    // bytes of a stage's keys, then as many of values
   static constexpr int kChunks = kSide / 1024;        // loads of a wave: 64 lanes, 16 bytes each
   static constexpr int kChunkRows = 1024 / kRow;
   static constexpr int kJoin = kWideWaves * kCols * (DP + 4) * 4;
-  static constexpr int kLds = 2 * 2 * kSide > kJoin ? 2 * 2 * kSide : kJoin;
+  static constexpr int kOwn = kChunks / kWideWaves;   // a wave's, of keys and again of values
+  static constexpr int kLds = kBuffers * 2 * kSide > kJoin ? kBuffers * 2 * kSide : kJoin;
   // What a row's pieces are turned by.
   static __device__ __forceinline__ int turn(int row) {
     return kSlots >= 16 ? row & 15 : kSlots == 8 ? row >> 1 & 7 : row >> 2 & 3;
@@ -149,12 +151,15 @@ __global__ __launch_bounds__(kWideThreads, 2) void pl_tree_wide_kernel(tree_args
   constexpr float kLift = DT == PL_F16 ? 15.f - kSlack : 0.f;
   __shared__ __attribute__((aligned(1024))) uint8_t s_mem[S::kLds];
   __shared__ float s_m[kWideWaves][kCols], s_l[kWideWaves][kCols];
-  __shared__ int s_held[2][2 * S::kUnits];
+  __shared__ int s_held[kBuffers][2 * S::kUnits];
   __shared__ int s_last;
   const int tid = (int)threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int li = lane & 15, lg = lane >> 4;
   const int wc = wave % across, wt = wave / across, behind = kWideWaves / across;
+  // Of a SIMD's two waves one goes first, so that they are not both at their products or
+  // both at their weights (16 x 64 drafts over 8192: 230 -> 217 us).
+  if (wave < kWideWaves / 2) __builtin_amdgcn_s_setprio(1);
   const tree_worker me = worker_of(a);
   const int ct = me.ct, slice = me.slice;
   const tree_run run = find_run<S::kAtom, S::kAtom / 128>(a, slice, lane);
@@ -254,22 +259,34 @@ __global__ __launch_bounds__(kWideThreads, 2) void pl_tree_wide_kernel(tree_args
     const uint32_t key_span = 15 * w.key_slot + (uint32_t)a.dim * S::kCsize;
     const uint32_t value_span = 15 * w.value_slot + (uint32_t)a.dim * S::kCsize;
 
-    // One stage's keys and values, a kilobyte at a time; 16 tokens share a page.
+    // One stage's keys and values, a kilobyte at a time; 16 tokens share a page.  Its
+    // pages are asked for a stage ahead.  What is not there is asked for with no bytes, so
+    // that every stage is as many loads.
+    int ids[S::kOwn];
+    auto look_up = [&](int base) __attribute__((always_inline)) {
+#pragma unroll
+      for (int k = 0; k < S::kOwn; ++k) {
+        const int token = base + ((wave + k * kWideWaves) * S::kChunkRows & ~15);
+        // no look-up past the end: the table's row may end there
+        ids[k] = token < end ? w.pages[token >> w.shift] : -1;
+      }
+    };
     auto load_stage = [&](int buffer, int base) __attribute__((always_inline)) {
       const uint32_t lds = lds_address(s_mem) + buffer * 2 * S::kSide;
-      tile_place<1> place[S::kChunks / kWideWaves];
 #pragma unroll
-      for (int k = 0; k < S::kChunks / kWideWaves; ++k)
-        place[k] = place_tile<1>(w, base + ((wave + k * kWideWaves) * S::kChunkRows & ~15));
-#pragma unroll
-      for (int k = 0; k < S::kChunks / kWideWaves; ++k) {
+      for (int k = 0; k < S::kOwn; ++k) {
         const int chunk = wave + k * kWideWaves, row0 = chunk * S::kChunkRows;
         const int in = (row0 & 15) + lane / S::kSlots;  // of the 16 tokens
         const int piece = lane % S::kSlots ^ S::turn(in);
-        if (row0 % 16 == 0 && lane == 0) s_held[buffer][row0 / 16] = place[k].held[0];
-        if (place[k].held[0] && (FULL || piece * 16 < a.dim * S::kCsize)) {
-          load_to_lds(lds + chunk * 1024, place[k].key[0], key_span, in * w.key_slot + piece * 16);
-          load_to_lds(lds + S::kSide + chunk * 1024, place[k].value[0], value_span, in * w.value_slot + piece * 16);
+        const bool held = ids[k] >= 0 && ids[k] < w.num_pages;
+        const int64_t page = held ? ids[k] : 0;
+        const uint32_t slot = (uint32_t)(base + (row0 & ~15)) & ((1u << w.shift) - 1);
+        if (row0 % 16 == 0 && lane == 0) s_held[buffer][row0 / 16] = held;
+        if (FULL || piece * 16 < a.dim * S::kCsize) {
+          load_to_lds(lds + chunk * 1024, w.key + page * w.key_page + (uint64_t)slot * w.key_slot, held ? key_span : 0,
+                      in * w.key_slot + piece * 16);
+          load_to_lds(lds + S::kSide + chunk * 1024, w.value + page * w.value_page + (uint64_t)slot * w.value_slot,
+                      held ? value_span : 0, in * w.value_slot + piece * 16);
         }
       }
     };
@@ -347,18 +364,27 @@ __global__ __launch_bounds__(kWideThreads, 2) void pl_tree_wide_kernel(tree_args
     };
 
     constexpr int kStage = S::kUnits * 32;
-    int buffer = 0;
-    if (begin < end) load_stage(0, begin);
-    for (int base = begin; base < end; base += kStage, buffer ^= 1) {
-      // this stage is there, and nobody reads the one before it any more
-      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-      __syncthreads();
-      if (base + kStage < end) load_stage(buffer ^ 1, base + kStage);
-      all_held = (uint32_t)__ballot(lane < 2 * S::kUnits && s_held[buffer][min(lane, 2 * S::kUnits - 1)]);
-      for (int u = wt; u < S::kUnits && base + u * 32 < end; u += behind) {
-        if (wc * kCols < live) unit(buffer, u, base + u * 32);
+    if (begin < end) {
+#pragma unroll
+      for (int i = 0; i < kBuffers - 1; ++i) {
+        look_up(begin + i * kStage);
+        load_stage(i, begin + i * kStage);
       }
+      look_up(begin + (kBuffers - 1) * kStage);
     }
+    int buffer = 0;
+    for (int base = begin; base < end; base += kStage, buffer = (buffer + 1) % kBuffers) {
+      // this stage is there (all but the two behind it), and nobody reads the one before it any more
+      constexpr int kBehind = (kBuffers - 2) * 2 * S::kOwn;
+      __builtin_amdgcn_s_waitcnt(0x0F70 | (kBehind & 15) | (kBehind >> 4) << 14);  // vmcnt
+      __syncthreads();
+      load_stage((buffer + kBuffers - 1) % kBuffers, base + (kBuffers - 1) * kStage);
+      look_up(base + kBuffers * kStage);
+      all_held = (uint32_t)__ballot(lane < 2 * S::kUnits && s_held[buffer][min(lane, 2 * S::kUnits - 1)]);
+      for (int u = wt; u < S::kUnits && base + u * 32 < end; u += behind)
+        if (wc * kCols < live) unit(buffer, u, base + u * 32);
+    }
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the join writes where loads are on their way
     if (__builtin_expect(nonfinite, 0))
       for (int base = begin; base < end; base += kStage)
         for (int u = wt; u < S::kUnits && base + u * 32 < end; u += behind) {
