@@ -114,16 +114,12 @@ def keep_tokens(cache, table, past, path, counts):
 
 def first_above(weights, number: float) -> int:
     """The first place whose running sum is above number times the sum; the last of any weight where none is."""
-    total = math.fsum(weights)
-    upto = 0.0
-    last = -1
-    for v, w in enumerate(weights):
-        if w > 0:
-            upto += w
-            last = v
-            if upto > number * total:
-                return v
-    return last
+    upto = weights.cumsum(0)
+    above = ((upto > number * upto[-1]) & (weights > 0)).nonzero()
+    if len(above):
+        return int(above[0])
+    some = (weights > 0).nonzero()
+    return int(some[-1]) if len(some) else -1
 
 
 def verify_tokens(logits, tokens, uniforms, parents=None, draft_probs=None, temperature=None, seq_lens=None):
@@ -140,28 +136,27 @@ def verify_tokens(logits, tokens, uniforms, parents=None, draft_probs=None, temp
         nodes, token = [0], -1
         while True:
             node = nodes[-1]
-            x = logits[b, node].double().tolist()
-            top = max((v for v in x if v == v), default=-math.inf)
-            if any(not v < math.inf for v in x) or top == -math.inf or not 0 <= heat < math.inf:
+            x = logits[b, node].double()
+            if not vocab or not bool((x < math.inf).all()) or float(x.max()) == -math.inf or not 0 <= heat < math.inf:
                 token = -1
                 break
-            best = x.index(top)
-            e = [0.0] * vocab if heat == 0 else [math.exp((v - top) / heat) for v in x]
+            best = int((x == x.max()).nonzero()[0])
+            e = torch.exp((x - x.max()) / (heat or 1.0))
             u = float(uniforms[b, node])
             if draft_probs is not None:
                 q = None
                 if node + 1 < n:
-                    q = draft_probs[b, node].double().tolist()
-                    d, z = int(tokens[b, node + 1]), math.fsum(e)
-                    if d == best if heat == 0 else 0 <= d < vocab and u * q[d] * z < e[d]:
+                    q = draft_probs[b, node].double()
+                    d, z = int(tokens[b, node + 1]), float(e.sum())
+                    if d == best if heat == 0 else 0 <= d < vocab and u * float(q[d]) * z < float(e[d]):
                         nodes.append(node + 1)
                         continue
                 if heat == 0:
                     token = best
                 else:
                     last = float(uniforms[b, n - 1])
-                    rest = [0.0] * vocab if q is None else [max(ev - qv * z, 0.0) for ev, qv in zip(e, q)]
-                    token = first_above(rest if sum(rest) > 0 else e, last)
+                    rest = torch.zeros_like(e) if q is None else (e - q * z).clamp(min=0)
+                    token = first_above(rest if float(rest.sum()) > 0 else e, last)
                 break
             token = best if heat == 0 else first_above(e, u)
             after = [c for c in range(node + 1, n)

@@ -145,7 +145,7 @@ _SIGNATURES: dict[str, tuple] = {
         c_int32, c_int32, c_int32, c_int32, c_int32, c_float, c_int32, c_void_p, c_void_p, c_void_p, c_void_p,
         c_int64, c_void_p, c_int64, c_void_p,
     ),
-    "pl_tree_attention_workspace_bytes": (c_int32,),
+    "pl_tree_attention_workspace_bytes": (c_int32, c_int32),
     "pl_keep_tokens": (
         c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_void_p, c_int64,
         c_int32, c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_int32, c_void_p,

@@ -54,7 +54,8 @@ __device__ __forceinline__ tree_span span_of(const tree_args& a, int past, int n
   const bool live = r.n > a.tok0 && past >= 0;
   r.len = live ? (int)min((int64_t)past + r.n, cap) : 0;
   const int64_t first = (int64_t)past + (a.visible ? 0 : a.tok0) - a.window + 1;
-  r.first = live && a.window > 0 ? (int)max(first, (int64_t)0) : 0;
+  // (a window that begins behind the pages' end sees nothing of them)
+  r.first = live && a.window > 0 ? (int)min(max(first, (int64_t)0), (int64_t)r.len) : 0;
   r.base = r.first & ~31;
   r.atoms = max(1, (r.len - r.base + ATOM - 1) / ATOM);  // an empty row's output is an atom too
   return r;
@@ -256,7 +257,7 @@ __device__ __forceinline__ uint32_t column_sees(const tree_args& a, const tree_s
 __device__ __forceinline__ int first_seen(const tree_args& a, const tree_span& r, int row, int t) {
   if (a.window <= 0 || t < 0) return 0;
   const int depth = a.depths ? max(a.depths[row * a.depths_row + t], 0) : t;
-  return (int)max((int64_t)r.past + depth - a.window + 1, (int64_t)0);
+  return (int)min(max((int64_t)r.past + depth - a.window + 1, (int64_t)0), (int64_t)INT32_MAX);
 }
 
 // Takes out what a mixed tile's columns do not see: their scores, the values of slots

@@ -377,10 +377,12 @@ int launch(int32_t dtype, int32_t cache_dtype, tree_args a, int64_t atoms_most, 
 
 static_assert(PL_ATTENTION_COUNTER_INTS == kWorkersMax * kCounterStride, "one counter per workgroup");
 
-extern "C" int64_t pl_tree_attention_workspace_bytes(int32_t dim) {
-  // two parts of a worker: one on each CU of 256 columns (128 of large heads) or two of 32
+extern "C" int64_t pl_tree_attention_workspace_bytes(int32_t dim, int32_t columns) {
+  if (dim < 1 || dim > kHeadDimMax || columns < 0) return 0;
+  // two parts of a worker: of up to 32 columns, two workers on a CU, or one of 256 (128 of large heads)
   const int dp = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
-  return dim < 1 || dim > kHeadDimMax ? 0 : 2ll * kCus * wide_columns(dp) / kCols * part_floats(dp) * (int64_t)sizeof(float);
+  const int64_t sixteens = columns <= narrow_columns(dp) ? 2ll * kWorkersMax * 2 : 2ll * kCus * wide_columns(dp) / kCols;
+  return sixteens * part_floats(dp) * (int64_t)sizeof(float);
 }
 
 extern "C" int pl_tree_attention(int32_t dtype, int32_t cache_dtype, const void* q, const int64_t* q_strides,
@@ -430,10 +432,12 @@ extern "C" int pl_tree_attention(int32_t dtype, int32_t cache_dtype, const void*
     pl_set_error("%s: out overlaps q", what);
     return PL_ERR_ARG;
   }
-  if (!workspace || workspace_bytes < pl_tree_attention_workspace_bytes(dim) || !counters ||
+  const int64_t all_columns = (int64_t)row_len * (heads / kv_heads);
+  const int32_t columns = (int32_t)(all_columns < kColumnsMax ? all_columns : kColumnsMax);
+  if (!workspace || workspace_bytes < pl_tree_attention_workspace_bytes(dim, columns) || !counters ||
       counter_ints < PL_ATTENTION_COUNTER_INTS) {
     pl_set_error("%s: workspace of %lld bytes and %lld counters, %lld and %d needed", what, (long long)workspace_bytes,
-                 (long long)counter_ints, (long long)pl_tree_attention_workspace_bytes(dim), PL_ATTENTION_COUNTER_INTS);
+                 (long long)counter_ints, (long long)pl_tree_attention_workspace_bytes(dim, columns), PL_ATTENTION_COUNTER_INTS);
     return PL_ERR_ARG;
   }
   tree_args a;

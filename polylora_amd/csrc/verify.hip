@@ -14,28 +14,33 @@
 // Weights and sums are 64-bit: a sum of 10^5 weights decides between tokens whose
 // borders lie 10^-6 apart and less, and a running sum in fp32 is off by as much.
 //
-// A launch looks at all tokens of all rows at once, a wave to each piece of a token's
-// logits, which it reads once into registers: the piece's largest, then the sum of
-// its weights beside that.  The wave of a token's last piece to end puts the
-// sums together and says where the row would go from there; whoever says so
-// last for a row follows its tokens.  Where a large batch does not run all at
-// once, tokens lie in the grid's order before those behind them, and a workgroup
-// leaves out a token that a row is known to have turned away from: what it would
-// have found counts for nothing.  Drawing from what is left of p beside q needs
+// A launch looks at all tokens of all rows at once, a wave to a piece of a token's
+// logits, which it reads once into registers: the largest, then the sum of weights
+// beside that.  Few tokens are spread over workgroups of four pieces, and the one
+// that ends last for a token puts the sums together and says where the row would
+// go from there; of many, each has a workgroup.  Who says so last for a row follows
+// its tokens.  Where a large batch does not run all at once, tokens lie in
+// the grid's order before those behind them, and a workgroup leaves out a token
+// that a row is known to have turned away from: what it would have found counts
+// for nothing.  Drawing from what is left of p beside q needs
 // Z first, and is a second launch, over one token of each row.
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
-constexpr int kVec = 4;          // logits of a lane's load
+constexpr int kVec = 4, kPasses = 4;  // logits of a lane's load, and its loads to a piece
+constexpr int kPiece = 64 * kVec * kPasses;
 constexpr int kNodesMax = 1024;  // tokens of a row
 constexpr int kVocabMax = 1 << 24;
-// Loads of a lane to a piece: pieces of 1024 logits for few rows, that all CUs take
-// part, of 2048 above kManyPieces of those, whose beginnings and ends cost less.
-constexpr int kFewPasses = 4, kManyPasses = 8;
-constexpr int kManyPieces = 8192;
+// Threads of a workgroup that takes a token whole, and tokens of a call from which on they
+// fill the GPU: what a workgroup costs besides its logits is then paid once a
+// token, and of the tokens behind others only a few begin before those are done.
+constexpr int kWholeThreads = 1024;
+constexpr int kWholeTokens = 256;
+constexpr int kFewPieces = 64;  // up to these a token is a workgroup of kThreads: less to wait for
+constexpr int kWholePieces = 1024;  // whose sums fit beside it
 // Workgroups above which some end before others begin, so that looking for tokens
 // that no row reaches is worth its wait.
-constexpr int kResident = 1024;
+constexpr int kResident = 1024, kWholeResident = 256;
 
 struct verify_args {
   const void* logits;
@@ -85,33 +90,40 @@ __device__ __forceinline__ unsigned long long verdict(int child, int token) {
 }
 constexpr int kDraw = -2;  // the token is to be drawn
 
-// 2^t for t <= 0, to 2e-13: the power of two of the nearest integer times the
-// exponential's series for the rest.
+// 2^t, |t| up to 1000, to 2e-14 of it: the power of two of the nearest integer, which the
+// sum with 1.5 * 2^52 holds in its lowest bits and adds to the exponent, times the
+// Chebyshev interpolation of degree 9 of 2^f for the rest, f in [-1/2, 1/2] (computed
+// from its definition in 60 digits).
 __device__ __forceinline__ double exp2_64(double t) {
-  const double n = __builtin_rint(t);
-  const double f = (t - n) * 0.69314718055994530942;
-  double p = 1.0 / 39916800.0;
-  p = fma(p, f, 1.0 / 3628800.0);
-  p = fma(p, f, 1.0 / 362880.0);
-  p = fma(p, f, 1.0 / 40320.0);
-  p = fma(p, f, 1.0 / 5040.0);
-  p = fma(p, f, 1.0 / 720.0);
-  p = fma(p, f, 1.0 / 120.0);
-  p = fma(p, f, 1.0 / 24.0);
-  p = fma(p, f, 1.0 / 6.0);
-  p = fma(p, f, 0.5);
-  p = fma(p, f, 1.0);
-  p = fma(p, f, 1.0);
-  return __builtin_ldexp(p, (int)n);
+  constexpr double kRound = 6755399441055744.0;
+  const double n = t + kRound, f = t - (n - kRound);
+  double p = 0x1.b6571de2f2351p-24;
+  p = fma(p, f, 0x1.63ef969a64d3cp-20);
+  p = fma(p, f, 0x1.ffcb76789860fp-17);
+  p = fma(p, f, 0x1.43088e257f341p-13);
+  p = fma(p, f, 0x1.5d87fe908f88ap-10);
+  p = fma(p, f, 0x1.3b2ab72b175eep-7);
+  p = fma(p, f, 0x1.c6b08d7044119p-5);
+  p = fma(p, f, 0x1.ebfbdff8149f2p-3);
+  p = fma(p, f, 0x1.62e42fefa39f7p-1);
+  p = fma(p, f, 0x1.000000000003dp+0);
+  const uint64_t bits = __builtin_bit_cast(uint64_t, p);
+  const uint32_t high = (uint32_t)(bits >> 32) + ((uint32_t)__builtin_bit_cast(uint64_t, n) << 20);
+  return __builtin_bit_cast(double, (uint64_t)high << 32 | (uint32_t)bits);
 }
 
-// The weight of a logit beside the largest, `per` = log2(e) / temperature.  -inf
-// gives 0, NaN gives NaN.
+// The weight of a logit (no NaN) beside a reference, `per` = log2(e) / temperature; never less
+// than 2^-1000, what -infinity gives.
+__device__ __forceinline__ double weight_least(float x, float top, double per) {
+  return exp2_64(fmax(((double)x - (double)top) * per, -1000.0));
+}
+// And with 0 for -infinity.
 __device__ __forceinline__ double weight(float x, float top, double per) {
-  const double t = ((double)x - (double)top) * per;
-  return t < -1000.0 ? 0.0 : t != t ? t : exp2_64(t);
+  return x == -INFINITY ? 0.0 : weight_least(x, top, per);
 }
-
+// A piece's sum of weights without what those put in that stand for 0 (the choice in each of them took a
+// tenth of a large batch's time).
+__device__ __forceinline__ double without_least(double z) { return z < 0x1p-900 ? 0.0 : z; }
 
 template <typename V>
 __device__ __forceinline__ V wave_max(V x) {
@@ -123,31 +135,52 @@ __device__ __forceinline__ V wave_min(V x) {
   for (int d = 1; d < 64; d *= 2) x = min(x, __shfl_xor(x, d));
   return x;
 }
-__device__ __forceinline__ double wave_sum(double x) {
-  for (int d = 1; d < 64; d *= 2) x += __shfl_xor(x, d);
-  return x;
+// The sum of a wave's numbers, in lane 63: shifts by 1, 2, 4 and 8 inside rows of 16, then each
+// row's last lane into the rows above.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double from_lower(double x) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, ROWS, 0xf, false);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
+__device__ __forceinline__ double wave_sum(double x) {
+  x += from_lower<0x111, 0xf>(x), x += from_lower<0x112, 0xf>(x);
+  x += from_lower<0x114, 0xf>(x), x += from_lower<0x118, 0xf>(x);
+  x += from_lower<0x142, 0xa>(x);
+  return x + from_lower<0x143, 0xc>(x);
+}
+template <int THREADS>
 struct block_store {
-  double d[kWaves];
-  int i[kWaves];
-  float f[kWaves];
+  double d[THREADS / 64];
+  int i[THREADS / 64];
+  float f[THREADS / 64];
 };
-__device__ __forceinline__ int block_min(int x, block_store& s) {
+template <int THREADS>
+__device__ __forceinline__ int block_min(int x, block_store<THREADS>& s) {
   x = wave_min(x);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) s.i[threadIdx.x >> 6] = x;
   __syncthreads();
-  return min(min(s.i[0], s.i[1]), min(s.i[2], s.i[3]));
+  x = s.i[0];
+#pragma unroll
+  for (int w = 1; w < THREADS / 64; ++w) x = min(x, s.i[w]);
+  return x;
 }
-__device__ __forceinline__ float block_max(float x, block_store& s) {
+template <int THREADS>
+__device__ __forceinline__ float block_max(float x, block_store<THREADS>& s) {
   x = wave_max(x);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) s.f[threadIdx.x >> 6] = x;
   __syncthreads();
-  return fmaxf(fmaxf(s.f[0], s.f[1]), fmaxf(s.f[2], s.f[3]));
+  x = s.f[0];
+#pragma unroll
+  for (int w = 1; w < THREADS / 64; ++w) x = fmaxf(x, s.f[w]);
+  return x;
 }
 // The sum of all threads' numbers before this thread's, and of all.
-__device__ __forceinline__ double block_before(double x, double& total, block_store& s) {
+template <int THREADS>
+__device__ __forceinline__ double block_before(double x, double& total, block_store<THREADS>& s) {
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
   double run = x;
   for (int d = 1; d < 64; d *= 2) {
@@ -159,7 +192,8 @@ __device__ __forceinline__ double block_before(double x, double& total, block_st
   __syncthreads();
   double before = run - x;  // (exact enough: see draw_place)
   total = 0.0;
-  for (int w = 0; w < kWaves; ++w) {
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) {
     before += w < wave ? s.d[w] : 0.0;
     total += s.d[w];
   }
@@ -167,12 +201,12 @@ __device__ __forceinline__ double block_before(double x, double& total, block_st
 }
 
 // The first place in [0, n) whose running sum, from `before` on, passes `target`: weights
-// by `weight_of`, 1024 places at a time.  Where rounding leaves none, the last place of
+// by `weight_of`, four places of a thread at a time.  Where rounding leaves none, the last place of
 // any weight (-1: none).
-template <typename W>
-__device__ __forceinline__ int draw_place(int n, double before, double target, block_store& s, W weight_of) {
+template <int THREADS, typename W>
+__device__ __forceinline__ int draw_place(int n, double before, double target, block_store<THREADS>& s, W weight_of) {
   int last = -1;
-  for (int v0 = 0; v0 < n; v0 += kThreads * kVec) {
+  for (int v0 = 0; v0 < n; v0 += THREADS * kVec) {
     double w[kVec], mine = 0.0, all;
 #pragma unroll
     for (int e = 0; e < kVec; ++e) {
@@ -199,10 +233,10 @@ __device__ __forceinline__ int draw_place(int n, double before, double target, b
 
 // The piece of `pieces` whose running sum passes `target`, and the sum before it; sums by
 // `sum_of`.  (The last piece of any weight where rounding leaves none, -1 where none has.)
-template <typename S>
-__device__ __forceinline__ int draw_piece(int pieces, double target, double& before, block_store& s, double* s_before,
-                                          S sum_of) {
-  const int each = (pieces + kThreads - 1) / kThreads, first = (int)threadIdx.x * each;
+template <int THREADS, typename S>
+__device__ __forceinline__ int draw_piece(int pieces, double target, double& before, block_store<THREADS>& s,
+                                          double* s_before, S sum_of) {
+  const int each = (pieces + THREADS - 1) / THREADS, first = (int)threadIdx.x * each;
   double mine = 0.0, total;
   for (int i = first; i < min(first + each, pieces); ++i) mine += sum_of(i);
   double upto = block_before(mine, total, s);
@@ -257,13 +291,13 @@ __device__ __forceinline__ unsigned long long peek(const unsigned long long* p) 
 }
 
 // Follows a row's verdicts (all there), writes what comes out and clears them.
-template <int DT>
+template <int THREADS, int DT>
 __device__ __forceinline__ void follow(const row_of<DT>& r, int drawn, unsigned long long* s_verdict, int* s_path) {
   const verify_args& a = r.a;
   const int tid = (int)threadIdx.x;
   unsigned long long* verdicts = a.verdicts + (int64_t)r.b * a.nodes;
   __shared__ int s_count, s_token;
-  for (int i = tid; i < a.nodes; i += kThreads) {
+  for (int i = tid; i < a.nodes; i += THREADS) {
     s_verdict[i] = peek(verdicts + i);
     s_path[i] = -1;
     __hip_atomic_store(verdicts + i, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -280,7 +314,7 @@ __device__ __forceinline__ void follow(const row_of<DT>& r, int drawn, unsigned 
     s_count = count, s_token = token == kDraw ? drawn : token;
   }
   __syncthreads();
-  for (int i = tid; i < a.nodes; i += kThreads) a.path[(int64_t)r.b * a.nodes + i] = s_path[i];
+  for (int i = tid; i < a.nodes; i += THREADS) a.path[(int64_t)r.b * a.nodes + i] = s_path[i];
   if (tid == 0) a.counts[r.b] = s_count, a.next[r.b] = s_token;
 }
 
@@ -296,11 +330,148 @@ __device__ __forceinline__ int arrive(int32_t* counter, int add, int* s_old) {
 
 constexpr int kOut = 1 << 20;  // of an arrival: the token was left out
 
-template <int DT, int PASSES>
-__global__ __launch_bounds__(kThreads, 4) void pl_verify_nodes_kernel(verify_args a) {
-  typedef typename pl_traits<DT>::T T;
-  constexpr int kPiece = 64 * kVec * PASSES;
-  __shared__ block_store store;
+// Whether a token is out of a row's reach: a token on the way to it is known to go elsewhere.
+template <int THREADS, int DT>
+__device__ __forceinline__ bool out_of_reach(const row_of<DT>& r, int node, const unsigned long long* verdicts,
+                                             int* s_path) {
+  for (int i = (int)threadIdx.x; i <= node; i += THREADS) {
+    const int up = i == 0 ? -1 : r.parent(i);
+    const unsigned long long v = up >= 0 && up < i ? peek(verdicts + up) : 0;
+    // the token before it, or a mark
+    s_path[i] = up < 0 || up >= i ? -1 : v && (int)(v >> 32) - 2 != i ? -2 : up;
+  }
+  __syncthreads();
+  int i = node;
+  while (i > 0) i = s_path[i];
+  __syncthreads();
+  return i == -2;
+}
+
+// A piece of a row's logits in registers; `none` past their end.
+template <typename T>
+__device__ __forceinline__ void load_piece(const T* x, int lo, int vocab, float (&y)[kPasses][kVec], float none) {
+  const int lane = (int)threadIdx.x & 63;
+  // rows have the alignment of their elements alone
+#pragma unroll
+  for (int k = 0; k < kPasses; ++k) {
+    const int v = lo + (k * 64 + lane) * kVec;
+    if (v + kVec <= vocab) {
+      T t[kVec];
+      __builtin_memcpy(t, x + v, sizeof(t));
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) y[k][e] = (float)t[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) y[k][e] = v + e < vocab ? (float)x[v + e] : none;
+    }
+  }
+}
+
+// A piece's sum (in lane 63) beside `ref`, which rises to its largest logit where that is none yet, or
+// so far above that weights would leave 64 bits (2^500).
+template <int DT>
+__device__ __forceinline__ piece_sum sum_piece(const row_of<DT>& r, const float (&y)[kPasses][kVec], int lo, float& ref) {
+  const int lane = (int)threadIdx.x & 63;
+  float top = -INFINITY;
+  bool bad = false;
+#pragma unroll
+  for (int k = 0; k < kPasses; ++k)
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) {
+      bad = bad || !(y[k][e] < INFINITY);
+      top = fmaxf(top, y[k][e]);
+    }
+  if (__any(bad)) return {NAN, top, INT32_MAX};
+  if (r.greedy()) {
+    top = wave_max(top);
+    int best = INT32_MAX;
+#pragma unroll
+    for (int k = 0; k < kPasses; ++k)
+#pragma unroll
+      for (int e = 0; e < kVec; ++e)
+        if (y[k][e] == top) best = min(best, lo + (k * 64 + lane) * kVec + e);
+    return {0.0, top, wave_min(best)};
+  }
+  if (__any(ref == -INFINITY || ((double)top - (double)ref) * r.per > 500.0)) ref = wave_max(top);
+  if (ref == -INFINITY) return {0.0, ref, INT32_MAX};
+  double z = 0.0;
+#pragma unroll
+  for (int k = 0; k < kPasses; ++k) {
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) z += weight_least(y[k][e], ref, r.per);
+    __builtin_amdgcn_sched_barrier(0);  // a few at a time: other waves fill the gaps
+  }
+  return {without_least(wave_sum(z)), ref, INT32_MAX};
+}
+
+// Where the row goes from a token, from its pieces' sums.
+template <int THREADS, int DT, typename S>
+__device__ __forceinline__ unsigned long long resolve(const row_of<DT>& r, int node, S sum_at,
+                                                      block_store<THREADS>& store, double* s_before) {
+  const verify_args& a = r.a;
+  const int tid = (int)threadIdx.x;
+  const auto* x = r.logits(node);
+  float top = -INFINITY;
+  bool bad = !r.sane();
+  for (int i = tid; i < a.pieces; i += THREADS) {
+    const piece_sum p = sum_at(i);
+    top = fmaxf(top, p.top), bad = bad || p.z != p.z;
+  }
+  top = block_max(top, store);
+  bad = block_min(bad ? 0 : 1, store) == 0 || top == -INFINITY;
+  if (bad) return verdict(-1, -1);
+  int child = -1, token = -1, best = INT32_MAX;
+  if (r.greedy()) {
+    for (int i = tid; i < a.pieces; i += THREADS) {
+      const piece_sum p = sum_at(i);
+      if (p.top == top) best = min(best, p.best);
+    }
+    best = block_min(best, store);
+  }
+  auto scaled = [&](int i) {
+    const piece_sum p = sum_at(i);
+    return p.top == -INFINITY ? 0.0 : p.z * weight(p.top, top, r.per);
+  };
+  double z = 0.0;
+  if (!r.greedy()) {
+    double mine = 0.0;
+    for (int i = tid; i < a.pieces; i += THREADS) mine += scaled(i);
+    block_before(mine, z, store);
+  }
+  if (a.draft_probs) {
+    token = r.greedy() ? best : kDraw;
+    if (node + 1 < r.n) {
+      const int64_t d = r.token(node + 1);
+      const bool known = d >= 0 && d < a.vocab;
+      const bool go = r.greedy() ? d == best
+                                 : known && (double)r.uniform_of(node) * (double)r.probs(node)[d] * z <
+                                                weight((float)x[d], top, r.per);
+      child = go ? node + 1 : -1;
+    }
+    if (tid == 0) a.totals[(int64_t)r.b * a.nodes + node] = node_sum{z, top, 0};
+  } else {
+    token = best;
+    if (!r.greedy()) {
+      const double target = (double)r.uniform_of(node) * z;
+      double before = 0.0;
+      const int piece = draw_piece(a.pieces, target, before, store, s_before, scaled), lo = piece * kPiece;
+      token = piece < 0 ? -1
+                        : lo + draw_place(min(kPiece, a.vocab - lo), before, target, store,
+                                          [&](int v) { return weight((float)x[lo + v], top, r.per); });
+    }
+    int c = INT32_MAX;
+    for (int i = node + 1 + tid; i < r.n; i += THREADS)
+      if (r.parent(i) == node && r.token(i) == token) c = min(c, i);
+    c = block_min(c, store);
+    child = c == INT32_MAX ? -1 : c;
+  }
+  return verdict(child, token);
+}
+
+// A wave to each piece of a token.
+template <int DT>
+__global__ __launch_bounds__(kThreads) void pl_verify_nodes_kernel(verify_args a) {
+  __shared__ block_store<kThreads> store;
   __shared__ double s_before;
   __shared__ unsigned long long s_verdict[kNodesMax];
   __shared__ int s_path[kNodesMax];
@@ -311,79 +482,18 @@ __global__ __launch_bounds__(kThreads, 4) void pl_verify_nodes_kernel(verify_arg
   const row_of<DT> r(a, b);
   unsigned long long* verdicts = a.verdicts + (int64_t)b * a.nodes;
   bool out = node >= r.n;
-  if (a.look && node > 0 && !out) {
-    // out of reach if a token on the way to it is known to go elsewhere
-    for (int i = tid; i <= node; i += kThreads) {
-      const int up = i == 0 ? -1 : r.parent(i);
-      const unsigned long long v = up >= 0 && up < i ? peek(verdicts + up) : 0;
-      // the token before it, or a mark
-      s_path[i] = up < 0 || up >= i ? -1 : v && (int)(v >> 32) - 2 != i ? -2 : up;
-    }
-    __syncthreads();
-    int i = node;
-    while (i > 0) i = s_path[i];
-    out = i == -2;
-    __syncthreads();
-  }
+  if (a.look && node > 0 && !out) out = out_of_reach<kThreads>(r, node, verdicts, s_path);
   piece_sum* sums = a.sums + ((int64_t)b * a.nodes + node) * a.pieces;
-  const T* x = r.logits(node);
-  if (!out) {
-    const int piece = group * kWaves + wave, lo = piece * kPiece, hi = min(lo + kPiece, a.vocab);
-    if (piece < a.pieces) {
-      float y[PASSES][kVec];
-      // rows have the alignment of their elements alone
-#pragma unroll
-      for (int k = 0; k < PASSES; ++k) {
-        const int v = lo + (k * 64 + lane) * kVec;
-        if (v + kVec <= hi) {
-          T t[kVec];
-          __builtin_memcpy(t, x + v, sizeof(t));
-#pragma unroll
-          for (int e = 0; e < kVec; ++e) y[k][e] = (float)t[e];
-        } else {
-#pragma unroll
-          for (int e = 0; e < kVec; ++e) y[k][e] = v + e < hi ? (float)x[v + e] : -INFINITY;
-        }
-      }
-      float top = -INFINITY;
-      bool bad = false;
-#pragma unroll
-      for (int k = 0; k < PASSES; ++k)
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) {
-          bad = bad || !(y[k][e] < INFINITY);
-          top = fmaxf(top, y[k][e]);
-        }
-      bad = __any(bad);
-      top = wave_max(top);
-      piece_sum sum = {0.0, top, INT32_MAX};
-      if (bad || top == -INFINITY) {
-        sum.z = bad ? NAN : 0.0;
-      } else if (r.greedy()) {
-        int best = INT32_MAX;
-#pragma unroll
-        for (int k = 0; k < PASSES; ++k)
-#pragma unroll
-          for (int e = 0; e < kVec; ++e)
-            if (y[k][e] == top) best = min(best, lo + (k * 64 + lane) * kVec + e);
-        sum.best = wave_min(best);
-      } else {
-        double z = 0.0;
-#pragma unroll
-        for (int k = 0; k < PASSES; ++k) {
-#pragma unroll
-          for (int e = 0; e < kVec; ++e) z += weight(y[k][e], top, r.per);
-          __builtin_amdgcn_sched_barrier(0);  // a few at a time: other waves fill the gaps
-        }
-        sum.z = wave_sum(z);
-      }
-      if (lane == 0) {
-        unsigned long long* to = reinterpret_cast<unsigned long long*>(sums + piece);
-        __hip_atomic_store(to, __builtin_bit_cast(unsigned long long, sum.z), __ATOMIC_RELAXED,
-                           __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_store(to + 1, (unsigned long long)(uint32_t)sum.best << 32 | __float_as_uint(sum.top),
-                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      }
+  const int piece = group * kWaves + wave;
+  if (!out && piece < a.pieces) {
+    float y[kPasses][kVec], ref = -INFINITY;
+    load_piece(r.logits(node), piece * kPiece, a.vocab, y, -INFINITY);
+    const piece_sum sum = sum_piece(r, y, piece * kPiece, ref);
+    if (lane == 63) {
+      unsigned long long* to = reinterpret_cast<unsigned long long*>(sums + piece);
+      __hip_atomic_store(to, __builtin_bit_cast(unsigned long long, sum.z), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_store(to + 1, (unsigned long long)(uint32_t)sum.best << 32 | __float_as_uint(sum.top),
+                         __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
   }
   int32_t* arrivals = a.node_arrivals + (int64_t)b * a.nodes + node;
@@ -391,164 +501,147 @@ __global__ __launch_bounds__(kThreads, 4) void pl_verify_nodes_kernel(verify_arg
   if ((before & (kOut - 1)) != a.groups - 1) return;
   out = out || before >= kOut;
   if (tid == 0) __hip_atomic_store(arrivals, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  // the last of this token: where the row goes from here
+  // the last of this token
   if (!out) {
-    auto sum_at = [&](int i) {
-      const unsigned long long* from = reinterpret_cast<const unsigned long long*>(sums + i);
-      const unsigned long long z = peek(from), rest = peek(from + 1);
-      return piece_sum{__builtin_bit_cast(double, z), __uint_as_float((uint32_t)rest), (int)(rest >> 32)};
-    };
-    float top = -INFINITY;
-    bool bad = !r.sane();
-    for (int i = tid; i < a.pieces; i += kThreads) {
-      const piece_sum p = sum_at(i);
-      top = fmaxf(top, p.top), bad = bad || p.z != p.z;
-    }
-    top = block_max(top, store);
-    bad = block_min(bad ? 0 : 1, store) == 0 || top == -INFINITY;
-    int child = -1, token = -1;
-    if (!bad) {
-      int best = INT32_MAX;
-      for (int i = tid; r.greedy() && i < a.pieces; i += kThreads) {
-        const piece_sum p = sum_at(i);
-        if (p.top == top) best = min(best, p.best);
-      }
-      if (r.greedy()) best = block_min(best, store);
-      auto scaled = [&](int i) {
-        const piece_sum p = sum_at(i);
-        return p.top == -INFINITY ? 0.0 : p.z * weight(p.top, top, r.per);
-      };
-      double z = 0.0;
-      if (!r.greedy()) {
-        double mine = 0.0;
-        for (int i = tid; i < a.pieces; i += kThreads) mine += scaled(i);
-        block_before(mine, z, store);
-      }
-      if (a.draft_probs) {
-        token = r.greedy() ? best : kDraw;
-        if (node + 1 < r.n) {
-          const int64_t d = r.token(node + 1);
-          const bool known = d >= 0 && d < a.vocab;
-          const bool go = r.greedy() ? d == best
-                                     : known && (double)r.uniform_of(node) * (double)r.probs(node)[d] * z <
-                                                    weight((float)x[d], top, r.per);
-          child = go ? node + 1 : -1;
-        }
-        if (tid == 0) a.totals[(int64_t)b * a.nodes + node] = node_sum{z, top, 0};
-      } else {
-        token = best;
-        if (!r.greedy()) {
-          const double target = (double)r.uniform_of(node) * z;
-          double sum_before = 0.0;
-          const int piece = draw_piece(a.pieces, target, sum_before, store, &s_before, scaled);
-          const int lo = piece * kPiece;
-          token = piece < 0 ? -1
-                            : lo + draw_place(min(kPiece, a.vocab - lo), sum_before, target, store,
-                                              [&](int v) { return weight((float)x[lo + v], top, r.per); });
-        }
-        int c = INT32_MAX;
-        for (int i = node + 1 + tid; i < r.n; i += kThreads)
-          if (r.parent(i) == node && r.token(i) == token) c = min(c, i);
-        c = block_min(c, store);
-        child = c == INT32_MAX ? -1 : c;
-      }
-    }
-    if (tid == 0)
-      __hip_atomic_store(verdicts + node, verdict(child, token), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const unsigned long long v = resolve(
+        r, node,
+        [&](int i) {
+          const unsigned long long* from = reinterpret_cast<const unsigned long long*>(sums + i);
+          const unsigned long long z = peek(from), rest = peek(from + 1);
+          return piece_sum{__builtin_bit_cast(double, z), __uint_as_float((uint32_t)rest), (int)(rest >> 32)};
+        },
+        store, &s_before);
+    if (tid == 0) __hip_atomic_store(verdicts + node, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   if (a.draft_probs) return;  // the second launch follows the row
   if (arrive(a.row_arrivals + b, 1, &s_old) != a.nodes - 1) return;
   if (tid == 0) __hip_atomic_store(a.row_arrivals + b, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  follow(r, -1, s_verdict, s_path);
+  follow<kThreads>(r, -1, s_verdict, s_path);
 }
 
-// A line's rows: what follows the token where each stops, drawn from max(e - q Z, 0) there.
-template <int DT, int PASSES>
-__global__ __launch_bounds__(kThreads) void pl_verify_draw_kernel(verify_args a) {
-  typedef typename pl_traits<DT>::T T;
-  constexpr int kPiece = 64 * kVec * PASSES;
-  __shared__ block_store store;
+// A workgroup to each token, its waves taking pieces in turn.
+template <int DT, int THREADS>
+__global__ __launch_bounds__(THREADS, 8) void pl_verify_whole_kernel(verify_args a) {
+  __shared__ block_store<THREADS> store;
   __shared__ double s_before;
+  __shared__ piece_sum s_sums[THREADS == kThreads ? kFewPieces : kWholePieces];
   __shared__ unsigned long long s_verdict[kNodesMax];
   __shared__ int s_path[kNodesMax];
   __shared__ int s_old;
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int group = (int)(blockIdx.x % a.groups), b = (int)(blockIdx.x / a.groups);
+  const int b = (int)(blockIdx.x % a.rows), node = (int)(blockIdx.x / a.rows);
+  const row_of<DT> r(a, b);
+  unsigned long long* verdicts = a.verdicts + (int64_t)b * a.nodes;
+  bool out = node >= r.n;
+  if (a.look && node > 0 && !out) out = out_of_reach<THREADS>(r, node, verdicts, s_path);
+  if (!out) {
+    constexpr int kStep = THREADS / 64;
+    float y[kPasses][kVec], ref = -INFINITY;
+    for (int piece = wave; piece < a.pieces; piece += kStep) {
+      load_piece(r.logits(node), piece * kPiece, a.vocab, y, -INFINITY);
+      const piece_sum sum = sum_piece(r, y, piece * kPiece, ref);
+      if (lane == 63) s_sums[piece] = sum;
+    }
+    __syncthreads();
+    const unsigned long long v = resolve(r, node, [&](int i) { return s_sums[i]; }, store, &s_before);
+    // what a draw may ask for once more
+    if (a.draft_probs)
+      for (int i = tid; i < a.pieces; i += THREADS)
+        a.sums[((int64_t)b * a.nodes + node) * a.pieces + i] = s_sums[i];
+    if (tid == 0) __hip_atomic_store(verdicts + node, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  if (a.draft_probs) return;  // the second launch follows the row
+  if (arrive(a.row_arrivals + b, 1, &s_old) != a.nodes - 1) return;
+  if (tid == 0) __hip_atomic_store(a.row_arrivals + b, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  follow<THREADS>(r, -1, s_verdict, s_path);
+}
+
+// A line's rows: what follows the token where each stops, drawn from max(e - q Z, 0) there.
+// THREADS: of a workgroup, which takes a row whole (kWholeThreads) or a few pieces.
+template <int DT, int THREADS>
+__global__ __launch_bounds__(THREADS) void pl_verify_draw_kernel(verify_args a) {
+  typedef typename pl_traits<DT>::T T;
+  constexpr bool kWhole = THREADS == kWholeThreads;
+  __shared__ block_store<THREADS> store;
+  __shared__ double s_before;
+  __shared__ double s_rests[kWhole ? kWholePieces : 1];
+  __shared__ unsigned long long s_verdict[kNodesMax];
+  __shared__ int s_path[kNodesMax];
+  __shared__ int s_old;
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int groups = kWhole ? 1 : a.groups;
+  const int group = (int)(blockIdx.x % groups), b = (int)(blockIdx.x / groups);
   const row_of<DT> r(a, b);
   const unsigned long long* verdicts = a.verdicts + (int64_t)b * a.nodes;
   // the first token that goes nowhere; those before it all go to the next
   int stop = INT32_MAX;
-  for (int i = tid; i < r.n; i += kThreads)
+  for (int i = tid; i < r.n; i += THREADS)
     if (verdicts[i] >> 32 == 1) stop = min(stop, i);
   stop = block_min(stop, store);
   const bool draws = stop < r.n && (int)(uint32_t)verdicts[min(stop, a.nodes - 1)] == kDraw;
   __syncthreads();
   int drawn = -1;
+  const node_sum total = draws ? a.totals[(int64_t)b * a.nodes + stop] : node_sum{0.0, 0.f, 0};
+  const T* x = r.logits(draws ? stop : 0);
+  const float* q = draws && stop + 1 < r.n ? r.probs(stop) : nullptr;
+  auto rest_of = [&](double e, float qv) { return fmax(e - (double)qv * total.z, 0.0); };
+  double* rests = a.rests + (int64_t)b * a.pieces;
   if (draws) {
-    const node_sum total = a.totals[(int64_t)b * a.nodes + stop];
-    const T* x = r.logits(stop);
-    const float* q = stop + 1 < r.n ? r.probs(stop) : nullptr;
-    auto rest_of = [&](float y, float qv) {
-      const double e = weight(y, total.top, r.per);
-      return fmax(e - (double)qv * total.z, 0.0);
-    };
-    double* rests = a.rests + (int64_t)b * a.pieces;
-    const int piece = group * kWaves + wave, lo = piece * kPiece, hi = min(lo + kPiece, a.vocab);
-    if (piece < a.pieces) {
+    for (int piece = group * (THREADS / 64) + wave; piece < a.pieces; piece += THREADS / 64 * groups) {
+      float y[kPasses][kVec], p[kPasses][kVec] = {};
+      load_piece(x, piece * kPiece, a.vocab, y, -INFINITY);
+      if (q) load_piece(q, piece * kPiece, a.vocab, p, 0.f);
       double z = 0.0;
-#pragma unroll 4
-      for (int k = 0; k < PASSES; ++k) {
-        const int v = lo + (k * 64 + lane) * kVec;
-        T t[kVec];
-        float p[kVec] = {0.f, 0.f, 0.f, 0.f};
-        if (v + kVec <= hi) {
-          __builtin_memcpy(t, x + v, sizeof(t));
-          if (q) __builtin_memcpy(p, q + v, sizeof(p));
 #pragma unroll
-          for (int e = 0; e < kVec; ++e) z += rest_of((float)t[e], p[e]);
-        } else {
-          for (int e = 0; v + e < hi; ++e) z += rest_of((float)x[v + e], q ? q[v + e] : 0.f);
-        }
+      for (int k = 0; k < kPasses; ++k) {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e)
+          z += rest_of(weight_least(y[k][e], total.top, r.per), p[k][e]);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      z = wave_sum(z);
-      if (lane == 0)
-        __hip_atomic_store(reinterpret_cast<unsigned long long*>(rests + piece),
-                           __builtin_bit_cast(unsigned long long, z), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      z = without_least(wave_sum(z));
+      if (lane == 63) {
+        if constexpr (kWhole)
+          s_rests[piece] = z;
+        else
+          __hip_atomic_store(reinterpret_cast<unsigned long long*>(rests + piece),
+                             __builtin_bit_cast(unsigned long long, z), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
     }
-    if (arrive(a.row_arrivals + b, 1, &s_old) != a.groups - 1) return;
+  }
+  if constexpr (kWhole) {
+    __syncthreads();
+  } else {
+    // all of a row's, whatever they found: the last one clears what they have read
+    if (arrive(a.row_arrivals + b, 1, &s_old) != groups - 1) return;
     if (tid == 0) __hip_atomic_store(a.row_arrivals + b, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  if (draws) {
     auto rest_at = [&](int i) {
-      return __builtin_bit_cast(double, peek(reinterpret_cast<const unsigned long long*>(rests + i)));
+      if constexpr (kWhole)
+        return s_rests[i];
+      else
+        return __builtin_bit_cast(double, peek(reinterpret_cast<const unsigned long long*>(rests + i)));
     };
     const float u = r.uniform_of(r.n - 1);
-    double mine = 0.0, all;
-    for (int i = tid; i < a.pieces; i += kThreads) mine += rest_at(i);
+    double mine = 0.0, all, before = 0.0;
+    for (int i = tid; i < a.pieces; i += THREADS) mine += rest_at(i);
     block_before(mine, all, store);
-    if (q && !(all > 0.0)) {
-      // p and q agree everywhere: from p itself
-      const piece_sum* sums = a.sums + ((int64_t)b * a.nodes + stop) * a.pieces;
-      auto scaled = [&](int i) {
-        return sums[i].top == -INFINITY ? 0.0 : sums[i].z * weight(sums[i].top, total.top, r.per);
-      };
-      const double target = (double)u * total.z;
-      double before = 0.0;
-      const int at = draw_piece(a.pieces, target, before, store, &s_before, scaled);
-      if (at >= 0)
-        drawn = at * kPiece + draw_place(min(kPiece, a.vocab - at * kPiece), before, target, store,
-                                         [&](int v) { return weight((float)x[at * kPiece + v], total.top, r.per); });
-    } else {
-      const double target = (double)u * all;
-      double before = 0.0;
-      const int at = draw_piece(a.pieces, target, before, store, &s_before, rest_at);
-      if (at >= 0)
-        drawn = at * kPiece + draw_place(min(kPiece, a.vocab - at * kPiece), before, target, store, [&](int v) {
-                  return rest_of((float)x[at * kPiece + v], q ? q[at * kPiece + v] : 0.f);
-                });
-    }
-  } else if (group != 0) {
-    return;
+    // where p and q agree everywhere, from p itself
+    const bool whole = q && !(all > 0.0);
+    if (whole) q = nullptr, all = total.z;
+    const double target = (double)u * all;
+    const piece_sum* sums = a.sums + ((int64_t)b * a.nodes + stop) * a.pieces;
+    const int at = draw_piece(a.pieces, target, before, store, &s_before, [&](int i) {
+      if (!whole) return rest_at(i);
+      return sums[i].top == -INFINITY ? 0.0 : sums[i].z * weight(sums[i].top, total.top, r.per);
+    });
+    if (at >= 0)
+      drawn = at * kPiece + draw_place(min(kPiece, a.vocab - at * kPiece), before, target, store, [&](int v) {
+                return rest_of(weight((float)x[at * kPiece + v], total.top, r.per), q ? q[at * kPiece + v] : 0.f);
+              });
   }
-  follow(r, drawn, s_verdict, s_path);
+  follow<THREADS>(r, drawn, s_verdict, s_path);
 }
 
 // Rows of no token.
@@ -557,33 +650,26 @@ __global__ __launch_bounds__(kThreads) void pl_verify_none_kernel(int32_t* count
   if (b < rows) counts[b] = 0, next[b] = -1;
 }
 
-// How a call is cut: pieces of a token's logits, and the workgroups that take them.
-struct verify_cut {
-  int passes, pieces, groups;
-};
-verify_cut cut_of(int64_t rows, int64_t nodes, int64_t vocab) {
-  verify_cut c;
-  const int64_t few = (vocab + 64 * kVec * kFewPasses - 1) / (64 * kVec * kFewPasses);
-  c.passes = rows * nodes * few > kManyPieces ? kManyPasses : kFewPasses;
-  const int64_t piece = 64 * kVec * c.passes;
-  c.pieces = (int)((vocab + piece - 1) / piece);
-  c.groups = (c.pieces + kWaves - 1) / kWaves;
-  if (c.groups == 0) c.groups = 1;
-  return c;
-}
+int pieces_of(int64_t vocab) { return (int)((vocab + kPiece - 1) / kPiece); }
 
-template <int DT, int PASSES>
-int launch(const verify_args& a, hipStream_t s) {
+template <int DT>
+int launch(const verify_args& a, bool whole, hipStream_t s) {
   const char* what = "pl_verify_tokens";
-  pl_verify_nodes_kernel<DT, PASSES><<<dim3((unsigned)(a.rows * a.nodes * a.groups)), kThreads, 0, s>>>(a);
+  const unsigned tokens = (unsigned)(a.rows * a.nodes);
+  if (whole && a.pieces <= kFewPieces)
+    pl_verify_whole_kernel<DT, kThreads><<<dim3(tokens), kThreads, 0, s>>>(a);
+  else if (whole)
+    pl_verify_whole_kernel<DT, kWholeThreads><<<dim3(tokens), kWholeThreads, 0, s>>>(a);
+  else
+    pl_verify_nodes_kernel<DT><<<dim3(tokens * a.groups), kThreads, 0, s>>>(a);
   const int rc = pl_launch_status(what);
   if (rc || !a.draft_probs) return rc;
-  pl_verify_draw_kernel<DT, PASSES><<<dim3((unsigned)(a.rows * a.groups)), kThreads, 0, s>>>(a);
+  // one token of each row
+  if (a.rows >= kWholeTokens && a.pieces <= kWholePieces)
+    pl_verify_draw_kernel<DT, kWholeThreads><<<dim3((unsigned)a.rows), kWholeThreads, 0, s>>>(a);
+  else
+    pl_verify_draw_kernel<DT, kThreads><<<dim3((unsigned)(a.rows * a.groups)), kThreads, 0, s>>>(a);
   return pl_launch_status(what);
-}
-template <int DT>
-int launch(const verify_args& a, int passes, hipStream_t s) {
-  return passes == kFewPasses ? launch<DT, kFewPasses>(a, s) : launch<DT, kManyPasses>(a, s);
 }
 
 int64_t whole_pieces(int64_t bytes) { return (bytes + 255) / 256 * 256; }
@@ -592,10 +678,9 @@ int64_t whole_pieces(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
 extern "C" int64_t pl_verify_workspace_bytes(int32_t rows, int32_t nodes, int32_t vocab) {
   if (rows < 0 || nodes < 0 || vocab < 0) return 0;
-  const verify_cut c = cut_of(rows, nodes, vocab);
-  const int64_t n = (int64_t)rows * nodes;
-  return whole_pieces(n * c.pieces * (int64_t)sizeof(piece_sum)) + whole_pieces(n * (int64_t)sizeof(node_sum)) +
-         whole_pieces((int64_t)rows * c.pieces * 8);
+  const int64_t n = (int64_t)rows * nodes, pieces = pieces_of(vocab);
+  return whole_pieces(n * pieces * (int64_t)sizeof(piece_sum)) + whole_pieces(n * (int64_t)sizeof(node_sum)) +
+         whole_pieces((int64_t)rows * pieces * 8);
 }
 extern "C" int64_t pl_verify_counter_ints(int32_t rows, int32_t nodes) {
   return rows < 0 || nodes < 0 ? 0 : 3ll * rows * nodes + rows;
@@ -650,20 +735,21 @@ extern "C" int pl_verify_tokens(int32_t dtype, const void* logits, int64_t ld_ro
     pl_verify_none_kernel<<<dim3((unsigned)((rows + kThreads - 1) / kThreads)), kThreads, 0, s>>>(counts, next, rows);
     return pl_launch_status(what);
   }
-  const verify_cut c = cut_of(rows, nodes, vocab);
-  a.pieces = c.pieces, a.groups = c.groups;
-  const int64_t blocks = (int64_t)rows * nodes * c.groups, n = (int64_t)rows * nodes;
-  if (!pl_grid_fits(blocks, kThreads) || blocks > INT32_MAX) {
+  const int64_t n = (int64_t)rows * nodes;
+  a.pieces = pieces_of(vocab), a.groups = a.pieces > kWaves ? (a.pieces + kWaves - 1) / kWaves : 1;
+  const bool whole = n >= kWholeTokens && a.pieces <= kWholePieces;
+  const int64_t blocks = whole ? n : n * a.groups;
+  if (!pl_grid_fits(n * a.groups, kWholeThreads)) {
     pl_set_error("%s: too many rows (%d)", what, rows);
     return PL_ERR_LIMIT;
   }
-  a.look = blocks > kResident;
+  a.look = blocks > (whole && a.pieces > kFewPieces ? kWholeResident : kResident);
   uint8_t* at = static_cast<uint8_t*>(workspace);
-  a.sums = reinterpret_cast<piece_sum*>(at), at += whole_pieces(n * c.pieces * (int64_t)sizeof(piece_sum));
+  a.sums = reinterpret_cast<piece_sum*>(at), at += whole_pieces(n * a.pieces * (int64_t)sizeof(piece_sum));
   a.totals = reinterpret_cast<node_sum*>(at), at += whole_pieces(n * (int64_t)sizeof(node_sum));
   a.rests = reinterpret_cast<double*>(at);
   a.verdicts = reinterpret_cast<unsigned long long*>(counters);
   a.node_arrivals = counters + 2 * n, a.row_arrivals = counters + 3 * n;
-  if (dtype == PL_F32) return launch<PL_F32>(a, c.passes, s);
-  return dtype == PL_BF16 ? launch<PL_BF16>(a, c.passes, s) : launch<PL_F16>(a, c.passes, s);
+  if (dtype == PL_F32) return launch<PL_F32>(a, whole, s);
+  return dtype == PL_BF16 ? launch<PL_BF16>(a, whole, s) : launch<PL_F16>(a, whole, s);
 }

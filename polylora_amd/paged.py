@@ -149,7 +149,7 @@ def paged_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch
     """
     stream = _stream(q)
     return _native.tensor_calls().paged_attention(q, key_cache, value_cache, page_table, lens, scale, window, k_scale,
-                                                  v_scale, out, *_scratch(q, stream, "paged_attention", *q.shape[-1:]), stream)
+                                                  v_scale, out, *_scratch(q, stream, "paged_attention", *(q.shape[-1:] or (0,))), stream)
 
 
 def tree_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, page_table: torch.Tensor,
@@ -168,9 +168,13 @@ def tree_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.
     the tree.  scale, scales, precision, ``out`` and rows that see nothing are ``paged_attention``'s; padding tokens get 0.
     """
     stream = _stream(q)
+    # columns of the products: the workspace goes by whether they are few
+    fits = q.dim() == 4 and key_cache.dim() == 4
+    columns = q.shape[1] * q.shape[2] // max(1, key_cache.shape[1]) if fits else 0
     return _native.tensor_calls().tree_attention(q, key_cache, value_cache, page_table, past_lens, seq_lens, visible,
                                                  depths, scale, window, k_scale, v_scale, out,
-                                                 *_scratch(q, stream, "tree_attention", *q.shape[-1:]), stream)
+                                                 *_scratch(q, stream, "tree_attention", *(q.shape[-1:] or (0,)), min(columns, 64)),
+                                                 stream)
 
 
 def keep_tokens(key_caches, value_caches, page_table: torch.Tensor, past_lens: torch.Tensor, path: torch.Tensor,

@@ -136,13 +136,14 @@ def test_tree_attention_refusals_of_the_library():
     assert _refused(call, good, out=p) == _native.PL_ERR_ARG  # over q
     assert _refused(call, good, value=p + 8) == _native.PL_ERR_ALIGN
     assert _refused(call, good, heads=3) == _native.PL_ERR_ARG
-    assert _refused(call, good, wsb=lib.pl_tree_attention_workspace_bytes(16) - 1) == _native.PL_ERR_ARG
+    assert _refused(call, good, wsb=lib.pl_tree_attention_workspace_bytes(16, 4) - 1) == _native.PL_ERR_ARG
     assert _refused(call, good, counters=None) == _native.PL_ERR_ARG
     assert _refused(call, good, ints=16) == _native.PL_ERR_ARG
-    assert _refused(call, good, heads=4098, qs=_i64(1 << 20, 1 << 17, 16)) == _native.PL_ERR_LIMIT
+    assert _refused(call, good, heads=2050, qs=_i64(1 << 20, 1 << 17, 16)) == _native.PL_ERR_LIMIT
     assert _refused(call, good, keys=_i64(64, 32, 1 << 30)) == _native.PL_ERR_LIMIT
     assert _refused(call, good, rows=1 << 20, cols=1 << 26, ld=1 << 26, out=1 << 60) == _native.PL_ERR_LIMIT
-    assert lib.pl_tree_attention_workspace_bytes(0) == lib.pl_tree_attention_workspace_bytes(257) == 0
+    need = lib.pl_tree_attention_workspace_bytes
+    assert need(0, 4) == need(257, 4) == need(64, -1) == 0 and need(64, 32) < need(64, 33)
     assert call(*{**good, "rows": 0}.values()) == 0 and call(*{**good, "m": 0}.values()) == 0
 
 

@@ -172,12 +172,12 @@ def test_append_refuses(gpu):
 
 
 def check_tree(gpu, dtype, past, seq, m, heads, kv_heads, dim, page, tree=True, fp8=False, order="head", window=None,
-               scale=None, seed=0, holes=False, shared=False, extra=0, q_gain=1.5):
+               scale=None, seed=0, holes=False, shared=False, extra=0, q_gain=1.5, columns=0):
     gen = torch.Generator().manual_seed(seed + dim + heads + m)
     rows = len(past)
     new = [min(m, n) for n in (seq or [m] * rows)]
-    key, value, table, ks, vs = pool(gen, rows, [max(0, p) + max(0, n) for p, n in zip(past, new)], kv_heads, dim, page,
-                                     dtype, fp8)
+    held = [min(max(0, p) + max(0, n), (columns or 10**9) * page) for p, n in zip(past, new)]
+    key, value, table, ks, vs = pool(gen, rows, held, kv_heads, dim, page, dtype, fp8)
     if holes:
         table[::2, 0] = -1
         table[1::2, 0] = key.shape[0]
@@ -266,6 +266,32 @@ def test_tree_attention_of_long_and_of_many_rows(gpu, dtype, rows, m, heads, kv_
     check_tree(gpu, dtype, past, None, m, heads, kv_heads, dim, 16, tree=m > 1)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,group,tree,window", [(300, 8, False, None), (300, 8, False, 40), (130, 20, True, None),
+                                                 (130, 20, True, 150), (600, 2, False, 7)])
+def test_tree_attention_of_more_columns_than_one_launch_takes(gpu, dtype, m, group, tree, window):
+    check_tree(gpu, dtype, [0, 37, 300], [m, m // 3, m - 1], m, group, 1, 32, 16, tree, window=window)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m", [5, 30])
+def test_tree_attention_where_the_table_ends_before_the_row(gpu, dtype, m):
+    """Tokens behind the table's last column are left out, of the drafts and of what lies before them."""
+    check_tree(gpu, dtype, [60, 64, 200, 0], None, m, 8, 2, 64, 16, columns=4)
+    check_tree(gpu, dtype, [60, 64, 200, 0], None, m, 8, 2, 64, 16, tree=False, columns=4, window=33)
+
+
+def test_tree_attention_of_lengths_near_32_bits(gpu):
+    q = torch.ones(2, 3, 4, 64, device=gpu, dtype=torch.bfloat16)
+    key = torch.ones(2, 2, 16, 64, device=gpu, dtype=torch.bfloat16)
+    table = torch.tensor([[0, 1]] * 2, dtype=torch.int32, device=gpu)
+    past = torch.tensor([2**31 - 1, 2**31 - 3], dtype=torch.int32, device=gpu)
+    for heads in (4, 2):
+        for window in (None, 5, 2**31 - 1):
+            got = tree_attention(q[:, :, :heads], key, key, table, past, window=window)
+            assert torch.equal(got, torch.zeros_like(got) if window == 5 else torch.ones_like(got))
+
+
 def test_one_drafted_token_is_the_single_tokens_attention(gpu):
     gen = torch.Generator().manual_seed(3)
     lens = [40, 300, 1]
@@ -289,12 +315,14 @@ def test_tree_attention_takes_empty_batches(gpu):
         assert not tree_attention(q, key, key, table, past).any()
 
 
-def test_tree_attention_reads_nothing_that_no_token_sees(gpu):
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads", [4, 40])
+def test_tree_attention_reads_nothing_that_no_token_sees(gpu, dtype, heads):
     """NaN in places beyond the row's tokens, before every window and at drafts that a token does not see."""
     gen = torch.Generator().manual_seed(6)
     page, m, past = 16, 6, 70
-    key, value, table, _, _ = pool(gen, 1, [past + m], 2, 64, page, torch.bfloat16)
-    q = torch.randn(1, m, 4, 64, generator=gen).bfloat16()
+    key, value, table, _, _ = pool(gen, 1, [past + m], 2, 64, page, dtype)
+    q = torch.randn(1, m, heads, 64, generator=gen).to(dtype)
     parents = torch.tensor([[-1, 0, 0, 1, 2, 4]], dtype=torch.int32)
     depths, visible = tree_tables(parents)
     lens = torch.tensor([past], dtype=torch.int32)
@@ -310,20 +338,22 @@ def test_tree_attention_reads_nothing_that_no_token_sees(gpu):
         assert torch.equal(got[:, t], clean[:, t]), t
 
 
-def test_tree_attention_infinities_and_nan_stay_where_they_are(gpu):
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads", [2, 24])
+def test_tree_attention_infinities_and_nan_stay_where_they_are(gpu, dtype, heads):
     gen = torch.Generator().manual_seed(7)
-    key, value, table, _, _ = pool(gen, 1, [90], 1, 64, 16, torch.bfloat16)
-    q = torch.randn(1, 5, 2, 64, generator=gen).bfloat16()
+    key, value, table, _, _ = pool(gen, 1, [90], 1, 64, 16, dtype)
+    q = torch.randn(1, 5, heads, 64, generator=gen).to(dtype)
     q[0, 2, 1, 5] = float("nan")
     at = plain.place(table, 0, 30, key.shape[0], 16)
     value[at[0], :, at[1], 7] = float("inf")
     lens = torch.tensor([85], dtype=torch.int32)
     got = tree_attention(q.to(gpu), key.to(gpu), value.to(gpu), table.to(gpu), lens.to(gpu)).cpu()
-    nan = torch.zeros(5, 2, 64, dtype=torch.bool)
+    nan = torch.zeros(5, heads, 64, dtype=torch.bool)
     nan[2, 1] = True
     assert torch.equal(got[0].isnan(), nan)
     assert bool((got[0, :, :, 7] == float("inf")).logical_or(nan[:, :, 7]).all())
-    assert int(got.isinf().sum()) == 9
+    assert int(got.isinf().sum()) == 5 * heads - 1
 
 
 def test_tree_attention_refuses(gpu):
@@ -472,6 +502,27 @@ def test_verification_of_many_rows(gpu, kind):
     gen = torch.Generator().manual_seed(2)
     logits, tokens, uniforms, more = drafted(gen, 700, 4, 331, torch.bfloat16, kind)
     check_verify(gpu, logits, tokens, uniforms, **more)
+
+
+@pytest.mark.parametrize("kind", ["line", "tree", "sure"])
+@pytest.mark.parametrize("rows,m,vocab", [(64, 4, 66000), (256, 2, 70001), (2, 2, 1100000)])
+def test_verification_of_many_large_rows(gpu, kind, rows, m, vocab):
+    gen = torch.Generator().manual_seed(8)
+    logits, tokens, uniforms, more = drafted(gen, rows, m, vocab, torch.bfloat16, kind, peak=4)
+    check_verify(gpu, logits, tokens, uniforms, **more)
+
+
+def test_verification_where_a_row_stops_without_a_distribution_before_others_would_draw(gpu):
+    """Many workgroups to a row, the first token's logits unusable, those behind it fine: again and again."""
+    gen = torch.Generator().manual_seed(9)
+    logits, tokens, uniforms, more = drafted(gen, 8, 5, 40000, torch.float32, "line")
+    more["seq_lens"], more["temperature"] = None, None
+    logits[::2, 0, 7] = float("nan")
+    want = plain.verify_tokens(logits, tokens, uniforms, **more)
+    args, more = (logits.to(gpu), tokens.to(gpu), uniforms.to(gpu)), on(gpu, **more)
+    for _ in range(50):
+        got = verify_tokens(*args, **more)
+        assert all(torch.equal(a.cpu(), b) for a, b in zip(got, want))
 
 
 @pytest.mark.parametrize("kind", ["line", "tree", "sure"])
