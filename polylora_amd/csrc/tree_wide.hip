@@ -263,7 +263,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void pl_tree_wide_kernel(tree_args
     // pages are asked for a stage ahead.  What is not there is asked for with no bytes, so
     // that every stage is as many loads.
     int ids[S::kOwn];
-    auto look_up = [&](int base) __attribute__((always_inline)) {
+    auto look_up = [&](int base, int (&ids)[S::kOwn]) __attribute__((always_inline)) {
 #pragma unroll
       for (int k = 0; k < S::kOwn; ++k) {
         const int token = base + ((wave + k * kWideWaves) * S::kChunkRows & ~15);
@@ -271,7 +271,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void pl_tree_wide_kernel(tree_args
         ids[k] = token < end ? w.pages[token >> w.shift] : -1;
       }
     };
-    auto load_stage = [&](int buffer, int base) __attribute__((always_inline)) {
+    auto load_stage = [&](int buffer, int base, const int(&ids)[S::kOwn]) __attribute__((always_inline)) {
       const uint32_t lds = lds_address(s_mem) + buffer * 2 * S::kSide;
 #pragma unroll
       for (int k = 0; k < S::kOwn; ++k) {
@@ -365,12 +365,12 @@ __global__ __launch_bounds__(kWideThreads, 2) void pl_tree_wide_kernel(tree_args
 
     constexpr int kStage = S::kUnits * 32;
     if (begin < end) {
+      int first_ids[kBuffers - 1][S::kOwn];
 #pragma unroll
-      for (int i = 0; i < kBuffers - 1; ++i) {
-        look_up(begin + i * kStage);
-        load_stage(i, begin + i * kStage);
-      }
-      look_up(begin + (kBuffers - 1) * kStage);
+      for (int i = 0; i < kBuffers - 1; ++i) look_up(begin + i * kStage, first_ids[i]);
+      look_up(begin + (kBuffers - 1) * kStage, ids);
+#pragma unroll
+      for (int i = 0; i < kBuffers - 1; ++i) load_stage(i, begin + i * kStage, first_ids[i]);
     }
     int buffer = 0;
     for (int base = begin; base < end; base += kStage, buffer = (buffer + 1) % kBuffers) {
@@ -378,8 +378,8 @@ __global__ __launch_bounds__(kWideThreads, 2) void pl_tree_wide_kernel(tree_args
       constexpr int kBehind = (kBuffers - 2) * 2 * S::kOwn;
       __builtin_amdgcn_s_waitcnt(0x0F70 | (kBehind & 15) | (kBehind >> 4) << 14);  // vmcnt
       __syncthreads();
-      load_stage((buffer + kBuffers - 1) % kBuffers, base + (kBuffers - 1) * kStage);
-      look_up(base + kBuffers * kStage);
+      load_stage((buffer + kBuffers - 1) % kBuffers, base + (kBuffers - 1) * kStage, ids);
+      look_up(base + kBuffers * kStage, ids);
       all_held = (uint32_t)__ballot(lane < 2 * S::kUnits && s_held[buffer][min(lane, 2 * S::kUnits - 1)]);
       for (int u = wt; u < S::kUnits && base + u * 32 < end; u += behind)
         if (wc * kCols < live) unit(buffer, u, base + u * 32);
