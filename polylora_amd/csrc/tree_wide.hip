@@ -56,28 +56,27 @@ __device__ __forceinline__ void load_to_lds(uint32_t to, uintptr_t p, uint32_t b
 }
 
 // Joins n parts of columns [in0, in1) (numbers of sixteens: the first part's, and from the
-// second on first + step * part) and puts out what comes of them.  A thread has kItems
-// places in hand, kBatch parts of each at a time: parts come from where every XCD
+// second on first + step * part) and puts out what comes of them.  A thread has ITEMS
+// places in hand, BATCH parts of each at a time: parts come from where every XCD
 // sees them, and what counts is how many are on their way.
-template <typename T, int DP, bool FULL>
+template <typename T, int DP, bool FULL, int ITEMS, int BATCH>
 __device__ __forceinline__ void join_columns(const tree_args& a, pl_buffer parts, int first, int others, int step, int n,
                                              int row, int col0, int in0, int in1, int live, int hk, float v_scale,
                                              int threads) {
   typedef part_layout<DP> P;
-  constexpr int kItems = 4, kBatch = 2;
   const int items = (in1 - in0) * (DP / 4);
-  for (int i0 = (int)threadIdx.x; i0 < items; i0 += kItems * threads) {
-    float top[kItems], sum[kItems];
-    pl_f32x4 y[kItems];
+  for (int i0 = (int)threadIdx.x; i0 < items; i0 += ITEMS * threads) {
+    float top[ITEMS], sum[ITEMS];
+    pl_f32x4 y[ITEMS];
 #pragma unroll
-    for (int s = 0; s < kItems; ++s) top[s] = -INFINITY, sum[s] = 0.f, y[s] = pl_f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int k0 = 0; k0 < n; k0 += kBatch) {
-      pl_f32x4 x[kItems][kBatch];
-      pl_f32x2 ml[kItems][kBatch];
+    for (int s = 0; s < ITEMS; ++s) top[s] = -INFINITY, sum[s] = 0.f, y[s] = pl_f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int k0 = 0; k0 < n; k0 += BATCH) {
+      pl_f32x4 x[ITEMS][BATCH];
+      pl_f32x2 ml[ITEMS][BATCH];
 #pragma unroll
-      for (int s = 0; s < kItems; ++s)
+      for (int s = 0; s < ITEMS; ++s)
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
+        for (int j = 0; j < BATCH; ++j) {
           const int i = min(i0 + s * threads, items - 1), in = in0 + i / (DP / 4), d = i % (DP / 4) * 4;
           const int k = min(k0 + j, n - 1);  // the last again, with no weight
           const uint32_t part = (uint32_t)((k ? others + step * k : first) + in / kCols) * P::kBytes;
@@ -87,24 +86,24 @@ __device__ __forceinline__ void join_columns(const tree_args& a, pl_buffer parts
               pl_f32x2, __builtin_amdgcn_raw_buffer_load_b64(parts, part + P::sums(in % kCols), 0, kAgentScope));
         }
 #pragma unroll
-      for (int s = 0; s < kItems; ++s) {
+      for (int s = 0; s < ITEMS; ++s) {
         float high = top[s];
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
+        for (int j = 0; j < BATCH; ++j) {
           ml[s][j].x = k0 + j < n ? ml[s][j].x : -INFINITY;
           high = fmaxf(high, ml[s][j].x);
         }
         const float ref = high == -INFINITY ? 0.f : high, keep = exp2_fast(top[s] - ref);
         sum[s] *= keep, y[s] *= keep, top[s] = high;
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
+        for (int j = 0; j < BATCH; ++j) {
           const float f = exp2_fast(ml[s][j].x - ref);
           sum[s] += f * ml[s][j].y, y[s] += f * x[s][j];
         }
       }
     }
 #pragma unroll
-    for (int s = 0; s < kItems; ++s) {
+    for (int s = 0; s < ITEMS; ++s) {
       const int i = i0 + s * threads;
       if (i < items)
         put_output<T, FULL>(a, row, col0, in0 + i / (DP / 4), live, hk, i % (DP / 4) * 4, y[s], sum[s], v_scale);
@@ -112,19 +111,20 @@ __device__ __forceinline__ void join_columns(const tree_args& a, pl_buffer parts
   }
 }
 
-// The parts of pairs that are cut into many: a workgroup to each sixteen of columns of a
-// pair, where one that arrives last would have all of them to itself.
-constexpr int kJoinThreads = 256;
+// The parts of pairs that are cut into many: a workgroup to every four columns of a pair,
+// where one that arrives last would have all of them to itself (1 x 16 drafts over
+// 131072 tokens, 32 parts to a pair: 7 us; 26 with sixteens and two parts at a time).
+constexpr int kJoinThreads = 128, kJoinColumns = 4;
 template <int DT, int CT, int DP, bool FULL>
 __global__ __launch_bounds__(kJoinThreads) void pl_tree_join_kernel(tree_args a) {
   typedef wide<DT, CT, DP> S;
   typedef typename pl_traits<DT>::T T;
-  constexpr int kSixteens = kWideWaves * S::C;
+  constexpr int kSixteens = kWideWaves * S::C, kShares = wide_columns(DP) / kJoinColumns;
   const int lane = (int)threadIdx.x & 63;
-  const int sixteen = (int)blockIdx.x % kSixteens, ct = (int)blockIdx.x / kSixteens % a.col_tiles;
-  const int pair = (int)blockIdx.x / kSixteens / a.col_tiles, row = pair / a.kv_heads, hk = pair % a.kv_heads;
+  const int share = (int)blockIdx.x % kShares, ct = (int)blockIdx.x / kShares % a.col_tiles;
+  const int pair = (int)blockIdx.x / kShares / a.col_tiles, row = pair / a.kv_heads, hk = pair % a.kv_heads;
   const int col0 = ct * wide_columns(DP), cols = min(wide_columns(DP), a.toks * a.group - col0);
-  const int in0 = sixteen * kCols, in1 = min(in0 + kCols, cols);
+  const int in0 = share * kJoinColumns, in1 = min(in0 + kJoinColumns, cols);
   if (in0 >= in1) return;
   // the deal, and the atoms before this row
   const tree_run run = find_run<S::kAtom, S::kAtom / 128>(a, 0, lane);
@@ -138,7 +138,7 @@ __global__ __launch_bounds__(kJoinThreads) void pl_tree_join_kernel(tree_args a)
   if (w0 == w1) return;  // in one piece: its worker has put it out
   const int live = max(0, min(cols, (min(r.n, a.tok0 + a.toks) - a.tok0) * a.group - col0));
   const int slot1 = 2 * (w0 * a.col_tiles + ct), slot0 = slot1 + (w0 * run.per == pair_start ? 0 : 1);
-  join_columns<T, DP, FULL>(a, part_layout<DP>::all(a.parts, 2u * kWorkersMax / 2 * kSixteens), slot0 * kSixteens,
+  join_columns<T, DP, FULL, 1, 8>(a, part_layout<DP>::all(a.parts, 2u * kWorkersMax / 2 * kSixteens), slot0 * kSixteens,
                             slot1 * kSixteens, 2 * a.col_tiles * kSixteens, w1 - w0 + 1, row, col0, in0, in1, live, hk,
                             CT == PL_F8E4M3 ? a.v_scale[hk] : 1.f, kJoinThreads);
 }
@@ -451,7 +451,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void pl_tree_wide_kernel(tree_args
         // the first part is its workgroup's second when that workgroup began earlier
         const int slot1 = 2 * (w0 * a.col_tiles + ct), slot0 = slot1 + (w0 * per == pair_start ? 0 : 1);
         const int n = w1 - w0 + 1;
-        join_columns<T, DP, FULL>(a, parts, slot0 * kSixteens, slot1 * kSixteens, 2 * a.col_tiles * kSixteens, n, row, col0,
+        join_columns<T, DP, FULL, 4, 2>(a, parts, slot0 * kSixteens, slot1 * kSixteens, 2 * a.col_tiles * kSixteens, n, row, col0,
                                   0, cols, live, hk, v_scale, kWideThreads);
       }
     }
@@ -479,7 +479,7 @@ void launch_wide(tree_args a, int64_t atoms_most, hipStream_t s) {
   const dim3 grid((unsigned)(a.slices * a.col_tiles));
   const int64_t pairs = (int64_t)a.rows * a.kv_heads;
   const int later = a.slices > kManyParts * pairs;
-  const dim3 joins((unsigned)(later ? pairs * a.col_tiles * kWideWaves * wide<DT, CT, DP>::C : 0));
+  const dim3 joins((unsigned)(later ? pairs * a.col_tiles * (wide_columns(DP) / kJoinColumns) : 0));
   if (a.dim == DP) {
     pl_tree_wide_kernel<DT, CT, DP, true><<<grid, kWideThreads, 0, s>>>(a, across, later);
     if (later) pl_tree_join_kernel<DT, CT, DP, true><<<joins, kJoinThreads, 0, s>>>(a);
