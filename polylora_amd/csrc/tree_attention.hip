@@ -341,8 +341,14 @@ void launch_columns(tree_args a, int64_t atoms_most, hipStream_t s) {
     pl_tree_attention_kernel<DT, CT, DP, C, true, false><<<grid, kThreads, 0, s>>>(a);
 }
 
-// Columns above which 16-bit models take the other kernel.
-constexpr int narrow_columns(int dp) { return dp == 256 ? kCols : 2 * kCols; }
+// Columns above which 16-bit models take the other kernel, which reads keys and values
+// once for all of them where this one reads them again for each 32 (16 of heads above
+// 128 elements), out of the XCD's cache mostly.  Measured in us, this one and the other, 64 rows
+// over 4096 tokens, 8 key heads of 128: 36 columns 189 and 205, 64 180 and 207, 96 240 and
+// 280, 128 268 and 252; one row over 700: 64 columns 15.5 and 21; one over 131072 in 8 bits: 64
+// columns 95 and 119, 96 130 and 179.  Heads of 256 elements: 32 columns 302 and 282, one row
+// 15 and 21, 8 bits 132 and 157; 64 columns 504 and 320.
+constexpr int narrow_columns(int dp) { return dp == 256 ? 2 * kCols : 6 * kCols; }
 
 template <int DT, int CT, int DP>
 int launch_dim(int32_t dtype, int32_t cache_dtype, const tree_args& a, int64_t atoms_most, hipStream_t s) {
@@ -379,7 +385,7 @@ static_assert(PL_ATTENTION_COUNTER_INTS == kWorkersMax * kCounterStride, "one co
 
 extern "C" int64_t pl_tree_attention_workspace_bytes(int32_t dim, int32_t columns) {
   if (dim < 1 || dim > kHeadDimMax || columns < 0) return 0;
-  // two parts of a worker: of up to 32 columns, two workers on a CU, or one of 256 (128 of large heads)
+  // two parts of a worker: of up to 32 columns each, two workers on a CU, or one of 256 (128 of large heads)
   const int dp = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
   const int64_t sixteens = columns <= narrow_columns(dp) ? 2ll * kWorkersMax * 2 : 2ll * kCus * wide_columns(dp) / kCols;
   return sixteens * part_floats(dp) * (int64_t)sizeof(float);

@@ -173,7 +173,7 @@ def tree_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.
     columns = q.shape[1] * q.shape[2] // max(1, key_cache.shape[1]) if fits else 0
     return _native.tensor_calls().tree_attention(q, key_cache, value_cache, page_table, past_lens, seq_lens, visible,
                                                  depths, scale, window, k_scale, v_scale, out,
-                                                 *_scratch(q, stream, "tree_attention", *(q.shape[-1:] or (0,)), min(columns, 64)),
+                                                 *_scratch(q, stream, "tree_attention", *(q.shape[-1:] or (0,)), min(columns, 128)),
                                                  stream)
 
 

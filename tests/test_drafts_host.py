@@ -143,7 +143,7 @@ def test_tree_attention_refusals_of_the_library():
     assert _refused(call, good, keys=_i64(64, 32, 1 << 30)) == _native.PL_ERR_LIMIT
     assert _refused(call, good, rows=1 << 20, cols=1 << 26, ld=1 << 26, out=1 << 60) == _native.PL_ERR_LIMIT
     need = lib.pl_tree_attention_workspace_bytes
-    assert need(0, 4) == need(257, 4) == need(64, -1) == 0 and need(64, 32) < need(64, 33)
+    assert need(0, 4) == need(257, 4) == need(64, -1) == 0 and need(64, 96) < need(64, 97)
     assert call(*{**good, "rows": 0}.values()) == 0 and call(*{**good, "m": 0}.values()) == 0
 
 

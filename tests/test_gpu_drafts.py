@@ -273,6 +273,28 @@ def test_tree_attention_of_more_columns_than_one_launch_takes(gpu, dtype, m, gro
     check_tree(gpu, dtype, [0, 37, 300], [m, m // 3, m - 1], m, group, 1, 32, 16, tree, window=window)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [48, 64, 80, 128, 144, 256])
+@pytest.mark.parametrize("m,group", [(16, 6), (33, 1), (8, 4), (97, 1), (16, 8), (15, 9), (52, 5)])
+def test_tree_attention_where_many_columns_begin(gpu, dtype, dim, m, group):
+    check_tree(gpu, dtype, [0, 1, 77, 400], [m, 0, m // 2, m], m, 2 * group, 2, dim, 16)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("window", [12, 33, 100, 1000])
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("heads", [12, 40])
+def test_tree_attention_of_a_window_and_many_columns(gpu, dtype, window, tree, heads):
+    check_tree(gpu, dtype, [0, 5, 64, 300, 411], [12, 12, 1, 12, 6], 12, heads, 2, 64, 16, tree, window=window)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads", [12, 40])
+def test_tree_attention_of_many_columns_where_the_table_ends_before_the_row(gpu, dtype, heads):
+    check_tree(gpu, dtype, [60, 64, 200, 0], None, 12, heads, 2, 64, 16, columns=4)
+    check_tree(gpu, dtype, [0, 0, 40], [12, 0, 12], 12, heads, 2, 128, 16, extra=2)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("m", [5, 30])
 def test_tree_attention_where_the_table_ends_before_the_row(gpu, dtype, m):
@@ -509,6 +531,15 @@ def test_verification_of_many_rows(gpu, kind):
 def test_verification_of_many_large_rows(gpu, kind, rows, m, vocab):
     gen = torch.Generator().manual_seed(8)
     logits, tokens, uniforms, more = drafted(gen, rows, m, vocab, torch.bfloat16, kind, peak=4)
+    check_verify(gpu, logits, tokens, uniforms, **more)
+
+
+@pytest.mark.parametrize("kind", ["line", "tree", "sure"])
+@pytest.mark.parametrize("rows,m,vocab,dtype", [(1500, 3, 300, torch.float32), (130, 33, 515, torch.float16),
+                                                (684, 3, 65600, torch.bfloat16)])
+def test_verification_of_thousands_of_tokens(gpu, kind, rows, m, vocab, dtype):
+    gen = torch.Generator().manual_seed(10)
+    logits, tokens, uniforms, more = drafted(gen, rows, m, vocab, dtype, kind, peak=4)
     check_verify(gpu, logits, tokens, uniforms, **more)
 
 
