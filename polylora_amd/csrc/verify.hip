@@ -31,11 +31,18 @@ constexpr int kVec = 4, kPasses = 4;  // logits of a lane's load, and its loads 
 constexpr int kPiece = 64 * kVec * kPasses;
 constexpr int kNodesMax = 1024;  // tokens of a row
 constexpr int kVocabMax = 1 << 24;
-// Threads of a workgroup that takes a token whole, and tokens of a call from which on they
-// fill the GPU: what a workgroup costs besides its logits is then paid once a
-// token, and of the tokens behind others only a few begin before those are done.
+// Threads of a workgroup that takes a token whole, and tokens of a call above which there
+// are such.  Pieces in workgroups of four spread a call over the GPU at once; where that
+// has many to follow one another, a token's workgroup pays what one costs besides
+// its logits once, and of the tokens behind others only a few begin before those are
+// done.  Measured in us, whole and spread, 32 tokens a row of 32003 bf16: 4096 tokens 90
+// and 71, 8192 111 and 126; 6 a row of 128256 in fp32: 1536 tokens 210 and 198, 2304 289 and
+// 306, 6144 639 and 741.
 constexpr int kWholeThreads = 1024;
-constexpr int kWholeTokens = 256;
+constexpr int kWholeTokens = 2048, kWholeFewTokens = 4096;
+// Rows from which on the draw beside drafts' probabilities takes one whole: 256 rows of
+// 128256 198 us for the call, 216 of pieces.
+constexpr int kWholeRows = 256;
 constexpr int kFewPieces = 64;  // up to these a token is a workgroup of kThreads: less to wait for
 constexpr int kWholePieces = 1024;  // whose sums fit beside it
 // Workgroups above which some end before others begin, so that looking for tokens
@@ -665,7 +672,7 @@ int launch(const verify_args& a, bool whole, hipStream_t s) {
   const int rc = pl_launch_status(what);
   if (rc || !a.draft_probs) return rc;
   // one token of each row
-  if (a.rows >= kWholeTokens && a.pieces <= kWholePieces)
+  if (a.rows >= kWholeRows && a.pieces <= kWholePieces)
     pl_verify_draw_kernel<DT, kWholeThreads><<<dim3((unsigned)a.rows), kWholeThreads, 0, s>>>(a);
   else
     pl_verify_draw_kernel<DT, kThreads><<<dim3((unsigned)(a.rows * a.groups)), kThreads, 0, s>>>(a);
@@ -737,7 +744,7 @@ extern "C" int pl_verify_tokens(int32_t dtype, const void* logits, int64_t ld_ro
   }
   const int64_t n = (int64_t)rows * nodes;
   a.pieces = pieces_of(vocab), a.groups = a.pieces > kWaves ? (a.pieces + kWaves - 1) / kWaves : 1;
-  const bool whole = n >= kWholeTokens && a.pieces <= kWholePieces;
+  const bool whole = n > (a.pieces > kFewPieces ? kWholeTokens : kWholeFewTokens) && a.pieces <= kWholePieces;
   const int64_t blocks = whole ? n : n * a.groups;
   if (!pl_grid_fits(n * a.groups, kWholeThreads)) {
     pl_set_error("%s: too many rows (%d)", what, rows);
