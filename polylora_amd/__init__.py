@@ -2,7 +2,8 @@
 
 Same public names as the reference package ``polylora`` (src/polylora/__init__.py:1-18).
 What a decode step does beside the Linears is in ``polylora_amd.paged`` (append
-to a paged key-value cache, attention of one new token over it) and
+to a paged key-value cache, attention of one new token or of several drafted
+ones over it), ``polylora_amd.drafts`` (which drafts stay) and
 ``polylora_amd.logits`` (penalties, biases and grammar masks), which the
 reference leaves to the wrapped model and its caller.
 """

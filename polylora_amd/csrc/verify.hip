@@ -24,6 +24,10 @@
 // that a row is known to have turned away from: what it would have found counts
 // for nothing.  Drawing from what is left of p beside q needs
 // Z first, and is a second launch, over one token of each row.
+//
+// 64-bit exponentials bound a batch: 256 rows of 6 tokens over 128256 fp32 logits take 164 us, 89
+// of them their bytes at a copy's rate; without the exponentials the time was nearly halved.
+// One row takes 18 us, two launches of look-ups and waits for the last workgroup.
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
@@ -43,7 +47,7 @@ constexpr int kWholeTokens = 2048, kWholeFewTokens = 4096;
 // Rows from which on the draw beside drafts' probabilities takes one whole: 256 rows of
 // 128256 198 us for the call, 216 of pieces.
 constexpr int kWholeRows = 256;
-constexpr int kFewPieces = 64;  // up to these a token is a workgroup of kThreads: less to wait for
+constexpr int kFewPieces = 64;  // up to these such a workgroup has kThreads: less to wait for
 constexpr int kWholePieces = 1024;  // whose sums fit beside it
 // Workgroups above which some end before others begin, so that looking for tokens
 // that no row reaches is worth its wait.
