@@ -16,18 +16,27 @@
 //
 // A launch looks at all tokens of all rows at once, a wave to a piece of a token's
 // logits, which it reads once into registers: the largest, then the sum of weights
-// beside that.  Few tokens are spread over workgroups of four pieces, and the one
-// that ends last for a token puts the sums together and says where the row would
-// go from there; of many, each has a workgroup.  Who says so last for a row follows
-// its tokens.  Where a large batch does not run all at once, tokens lie in
+// beside that.  Few tokens are spread over workgroups of four pieces, and a second
+// launch, a workgroup to a token, puts their sums together and says where the row would
+// go from there; of many, each has a workgroup that does both.  A last launch follows
+// each row.  Where a large batch does not run all at once, tokens lie in
 // the grid's order before those behind them, and a workgroup leaves out a token
 // that a row is known to have turned away from: what it would have found counts
-// for nothing.  Drawing from what is left of p beside q needs
-// Z first, and is a second launch, over one token of each row.
+// for nothing.  Drawing from what is left of p beside q needs Z first: its pieces are a
+// launch of their own, before the last.
 //
-// 64-bit exponentials bound a batch: 256 rows of 6 tokens over 128256 fp32 logits take 164 us, 89
+// What a workgroup finds goes to others from launch to launch only.  Handing it on inside of
+// one takes a release and an acquire at agent scope, 22 to 33 ns of the whole GPU's time for every
+// workgroup that has something (256 rows: 1786 us), and without them nothing promises
+// that who arrives last at a counter sees what the others have stored: neighbouring tokens' sums
+// share lines, which an XCD that has read one token's may still hold when it reads the next one's.
+//
+// 64-bit exponentials bound a batch: 256 rows of 6 tokens over 128256 fp32 logits take 180 us, 89
 // of them their bytes at a copy's rate; without the exponentials the time was nearly halved.
-// One row takes 18 us, two launches of look-ups and waits for the last workgroup.
+// One row takes 19 us, four launches that each wait for a few reads one after the other.
+// A workgroup that draws a row whole, without a launch for its pieces, was slower at any
+// number of rows (256 rows of 2 tokens over 128256 fp32 logits 93.2 and 93.2 us, 64 rows 57 and 36, 1024 rows
+// over 32003 118 and 99).
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
@@ -39,18 +48,15 @@ constexpr int kVocabMax = 1 << 24;
 // are such.  Pieces in workgroups of four spread a call over the GPU at once; where that
 // has many to follow one another, a token's workgroup pays what one costs besides
 // its logits once, and of the tokens behind others only a few begin before those are
-// done.  Measured in us, whole and spread, 32 tokens a row of 32003 bf16: 4096 tokens 90
-// and 71, 8192 111 and 126; 6 a row of 128256 in fp32: 1536 tokens 210 and 198, 2304 289 and
-// 306, 6144 639 and 741.
+// done.  Measured in us, whole and spread: 32 tokens a row of 32003 bf16, 512 tokens 33 and 29, 2048
+// 77 and 68, 4096 103 and 124; 6 a row of 128256 in fp32, 384 tokens 79 and 60, 768 123 and 107, 1536 194
+// and 197.
 constexpr int kWholeThreads = 1024;
-constexpr int kWholeTokens = 2048, kWholeFewTokens = 4096;
-// Rows from which on the draw beside drafts' probabilities takes one whole: 256 rows of
-// 128256 198 us for the call, 216 of pieces.
-constexpr int kWholeRows = 256;
+constexpr int kWholeTokens = 1024, kWholeFewTokens = 2048;
 constexpr int kFewPieces = 64;  // up to these such a workgroup has kThreads: less to wait for
 constexpr int kWholePieces = 1024;  // whose sums fit beside it
-// Workgroups above which some end before others begin, so that looking for tokens
-// that no row reaches is worth its wait.
+// Workgroups of whole tokens above which some end before others begin, so that looking for tokens
+// that no row reaches is worth its wait: of kThreads, and of kWholeThreads.
 constexpr int kResident = 1024, kWholeResident = 256;
 
 struct verify_args {
@@ -72,9 +78,7 @@ struct verify_args {
   int32_t rows, nodes, vocab, wide_tokens;
   int32_t pieces, groups;  // of a token's logits; workgroups that take them
   int32_t look;            // whether to look for tokens out of reach
-  // between launches 0: what became of each token (see verdict), and who has arrived
-  unsigned long long* verdicts;  // [rows][nodes]
-  int32_t *node_arrivals, *row_arrivals;
+  unsigned long long* verdicts;  // [rows][nodes]: what became of each token (see verdict); between calls 0
   // not cleared
   struct piece_sum* sums;   // [rows][nodes][pieces]
   struct node_sum* totals;  // [rows][nodes]
@@ -301,46 +305,6 @@ __device__ __forceinline__ unsigned long long peek(const unsigned long long* p) 
   return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// Follows a row's verdicts (all there), writes what comes out and clears them.
-template <int THREADS, int DT>
-__device__ __forceinline__ void follow(const row_of<DT>& r, int drawn, unsigned long long* s_verdict, int* s_path) {
-  const verify_args& a = r.a;
-  const int tid = (int)threadIdx.x;
-  unsigned long long* verdicts = a.verdicts + (int64_t)r.b * a.nodes;
-  __shared__ int s_count, s_token;
-  for (int i = tid; i < a.nodes; i += THREADS) {
-    s_verdict[i] = peek(verdicts + i);
-    s_path[i] = -1;
-    __hip_atomic_store(verdicts + i, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  }
-  __syncthreads();
-  if (tid == 0) {
-    int count = 0, token = -1;
-    for (int node = 0; node >= 0 && node < r.n && count < r.n;) {
-      s_path[count++] = node;
-      const unsigned long long v = s_verdict[node];
-      token = (int)(uint32_t)v;
-      node = (int)(v >> 32) - 2;
-    }
-    s_count = count, s_token = token == kDraw ? drawn : token;
-  }
-  __syncthreads();
-  for (int i = tid; i < a.nodes; i += THREADS) a.path[(int64_t)r.b * a.nodes + i] = s_path[i];
-  if (tid == 0) a.counts[r.b] = s_count, a.next[r.b] = s_token;
-}
-
-// One arrival of a workgroup, behind what it has stored (at agent scope); the count before it.
-__device__ __forceinline__ int arrive(int32_t* counter, int add, int* s_old) {
-  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-  __syncthreads();
-  if (threadIdx.x == 0)
-    *s_old = __hip_atomic_fetch_add(counter, add, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  __syncthreads();
-  return *s_old;
-}
-
-constexpr int kOut = 1 << 20;  // of an arrival: the token was left out
-
 // Whether a token is out of a row's reach: a token on the way to it is known to go elsewhere.
 template <int THREADS, int DT>
 __device__ __forceinline__ bool out_of_reach(const row_of<DT>& r, int node, const unsigned long long* verdicts,
@@ -481,53 +445,31 @@ __device__ __forceinline__ unsigned long long resolve(const row_of<DT>& r, int n
 
 // A wave to each piece of a token.
 template <int DT>
-__global__ __launch_bounds__(kThreads) void pl_verify_nodes_kernel(verify_args a) {
-  __shared__ block_store<kThreads> store;
-  __shared__ double s_before;
-  __shared__ unsigned long long s_verdict[kNodesMax];
-  __shared__ int s_path[kNodesMax];
-  __shared__ int s_old;
-  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
+__global__ __launch_bounds__(kThreads) void pl_verify_pieces_kernel(verify_args a) {
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
   const int group = (int)(blockIdx.x % a.groups);
   const int b = (int)(blockIdx.x / a.groups % a.rows), node = (int)(blockIdx.x / a.groups / a.rows);
   const row_of<DT> r(a, b);
-  unsigned long long* verdicts = a.verdicts + (int64_t)b * a.nodes;
-  bool out = node >= r.n;
-  if (a.look && node > 0 && !out) out = out_of_reach<kThreads>(r, node, verdicts, s_path);
-  piece_sum* sums = a.sums + ((int64_t)b * a.nodes + node) * a.pieces;
   const int piece = group * kWaves + wave;
-  if (!out && piece < a.pieces) {
-    float y[kPasses][kVec], ref = -INFINITY;
-    load_piece(r.logits(node), piece * kPiece, a.vocab, y, -INFINITY);
-    const piece_sum sum = sum_piece(r, y, piece * kPiece, ref);
-    if (lane == 63) {
-      unsigned long long* to = reinterpret_cast<unsigned long long*>(sums + piece);
-      __hip_atomic_store(to, __builtin_bit_cast(unsigned long long, sum.z), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      __hip_atomic_store(to + 1, (unsigned long long)(uint32_t)sum.best << 32 | __float_as_uint(sum.top),
-                         __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-  }
-  int32_t* arrivals = a.node_arrivals + (int64_t)b * a.nodes + node;
-  const int before = arrive(arrivals, out ? kOut + 1 : 1, &s_old);
-  if ((before & (kOut - 1)) != a.groups - 1) return;
-  out = out || before >= kOut;
-  if (tid == 0) __hip_atomic_store(arrivals, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  // the last of this token
-  if (!out) {
-    const unsigned long long v = resolve(
-        r, node,
-        [&](int i) {
-          const unsigned long long* from = reinterpret_cast<const unsigned long long*>(sums + i);
-          const unsigned long long z = peek(from), rest = peek(from + 1);
-          return piece_sum{__builtin_bit_cast(double, z), __uint_as_float((uint32_t)rest), (int)(rest >> 32)};
-        },
-        store, &s_before);
-    if (tid == 0) __hip_atomic_store(verdicts + node, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  }
-  if (a.draft_probs) return;  // the second launch follows the row
-  if (arrive(a.row_arrivals + b, 1, &s_old) != a.nodes - 1) return;
-  if (tid == 0) __hip_atomic_store(a.row_arrivals + b, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  follow<kThreads>(r, -1, s_verdict, s_path);
+  if (node >= r.n || piece >= a.pieces) return;
+  float y[kPasses][kVec], ref = -INFINITY;
+  load_piece(r.logits(node), piece * kPiece, a.vocab, y, -INFINITY);
+  const piece_sum sum = sum_piece(r, y, piece * kPiece, ref);
+  if (lane == 63) a.sums[((int64_t)b * a.nodes + node) * a.pieces + piece] = sum;
+}
+
+// And a workgroup to each token, for what its pieces say.
+template <int DT>
+__global__ __launch_bounds__(kThreads) void pl_verify_resolve_kernel(verify_args a) {
+  __shared__ block_store<kThreads> store;
+  __shared__ double s_before;
+  const int b = (int)(blockIdx.x % a.rows), node = (int)(blockIdx.x / a.rows);
+  const row_of<DT> r(a, b);
+  if (node >= r.n) return;
+  const int64_t at = (int64_t)b * a.nodes + node;
+  const piece_sum* sums = a.sums + at * a.pieces;
+  const unsigned long long v = resolve(r, node, [&](int i) { return sums[i]; }, store, &s_before);
+  if (threadIdx.x == 0) a.verdicts[at] = v;
 }
 
 // A workgroup to each token, its waves taking pieces in turn.
@@ -536,123 +478,140 @@ __global__ __launch_bounds__(THREADS, 8) void pl_verify_whole_kernel(verify_args
   __shared__ block_store<THREADS> store;
   __shared__ double s_before;
   __shared__ piece_sum s_sums[THREADS == kThreads ? kFewPieces : kWholePieces];
-  __shared__ unsigned long long s_verdict[kNodesMax];
   __shared__ int s_path[kNodesMax];
-  __shared__ int s_old;
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int b = (int)(blockIdx.x % a.rows), node = (int)(blockIdx.x / a.rows);
   const row_of<DT> r(a, b);
   unsigned long long* verdicts = a.verdicts + (int64_t)b * a.nodes;
-  bool out = node >= r.n;
-  if (a.look && node > 0 && !out) out = out_of_reach<THREADS>(r, node, verdicts, s_path);
-  if (!out) {
-    constexpr int kStep = THREADS / 64;
-    float y[kPasses][kVec], ref = -INFINITY;
-    for (int piece = wave; piece < a.pieces; piece += kStep) {
-      load_piece(r.logits(node), piece * kPiece, a.vocab, y, -INFINITY);
-      const piece_sum sum = sum_piece(r, y, piece * kPiece, ref);
-      if (lane == 63) s_sums[piece] = sum;
-    }
-    __syncthreads();
-    const unsigned long long v = resolve(r, node, [&](int i) { return s_sums[i]; }, store, &s_before);
-    // what a draw may ask for once more
-    if (a.draft_probs)
-      for (int i = tid; i < a.pieces; i += THREADS)
-        a.sums[((int64_t)b * a.nodes + node) * a.pieces + i] = s_sums[i];
-    if (tid == 0) __hip_atomic_store(verdicts + node, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (node >= r.n) return;
+  if (a.look && node > 0 && out_of_reach<THREADS>(r, node, verdicts, s_path)) return;
+  constexpr int kStep = THREADS / 64;
+  float y[kPasses][kVec], ref = -INFINITY;
+  for (int piece = wave; piece < a.pieces; piece += kStep) {
+    load_piece(r.logits(node), piece * kPiece, a.vocab, y, -INFINITY);
+    const piece_sum sum = sum_piece(r, y, piece * kPiece, ref);
+    if (lane == 63) s_sums[piece] = sum;
   }
-  if (a.draft_probs) return;  // the second launch follows the row
-  if (arrive(a.row_arrivals + b, 1, &s_old) != a.nodes - 1) return;
-  if (tid == 0) __hip_atomic_store(a.row_arrivals + b, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  follow<THREADS>(r, -1, s_verdict, s_path);
+  __syncthreads();
+  const unsigned long long v = resolve(r, node, [&](int i) { return s_sums[i]; }, store, &s_before);
+  // what a draw may ask for once more
+  if (a.draft_probs)
+    for (int i = tid; i < a.pieces; i += THREADS)
+      a.sums[((int64_t)b * a.nodes + node) * a.pieces + i] = s_sums[i];
+  if (tid == 0) __hip_atomic_store(verdicts + node, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// A line's rows: what follows the token where each stops, drawn from max(e - q Z, 0) there.
-// THREADS: of a workgroup, which takes a row whole (kWholeThreads) or a few pieces.
-template <int DT, int THREADS>
-__global__ __launch_bounds__(THREADS) void pl_verify_draw_kernel(verify_args a) {
+// What a row of a line draws from, max(e - q Z, 0) at the token where it stops (verdicts all there).
+template <int DT>
+struct rest_of {
   typedef typename pl_traits<DT>::T T;
-  constexpr bool kWhole = THREADS == kWholeThreads;
-  __shared__ block_store<THREADS> store;
+  const row_of<DT>& r;
+  int stop;
+  bool draws;  // the row stops, and at usable logits
+  node_sum total;
+  const T* x;
+  const float* q;  // null behind the last draft
+  __device__ __forceinline__ rest_of(const row_of<DT>& row, block_store<kThreads>& store) : r(row) {
+    const verify_args& a = r.a;
+    const unsigned long long* verdicts = a.verdicts + (int64_t)r.b * a.nodes;
+    // the first token that goes nowhere; those before it all go to the next
+    stop = INT32_MAX;
+    for (int i = (int)threadIdx.x; i < r.n; i += kThreads)
+      if (verdicts[i] >> 32 == 1) stop = min(stop, i);
+    stop = block_min(stop, store);
+    draws = stop < r.n && (int)(uint32_t)verdicts[min(stop, a.nodes - 1)] == kDraw;
+    __syncthreads();
+    total = draws ? a.totals[(int64_t)r.b * a.nodes + stop] : node_sum{0.0, 0.f, 0};
+    x = r.logits(draws ? stop : 0);
+    q = draws && stop + 1 < r.n ? r.probs(stop) : nullptr;
+  }
+  __device__ __forceinline__ double of(double e, float qv) const { return fmax(e - (double)qv * total.z, 0.0); }
+  // A piece's sum of them, in lane 63.
+  __device__ __forceinline__ double piece(int i) const {
+    float y[kPasses][kVec], p[kPasses][kVec] = {};
+    load_piece(x, i * kPiece, r.a.vocab, y, -INFINITY);
+    if (q) load_piece(q, i * kPiece, r.a.vocab, p, 0.f);
+    double z = 0.0;
+#pragma unroll
+    for (int k = 0; k < kPasses; ++k) {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) z += of(weight_least(y[k][e], total.top, r.per), p[k][e]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    return without_least(wave_sum(z));
+  }
+};
+
+// The pieces' sums of that, a wave to each.
+template <int DT>
+__global__ __launch_bounds__(kThreads) void pl_verify_rests_kernel(verify_args a) {
+  __shared__ block_store<kThreads> store;
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+  const int group = (int)(blockIdx.x % a.groups), b = (int)(blockIdx.x / a.groups);
+  const row_of<DT> r(a, b);
+  const rest_of<DT> rest(r, store);
+  const int i = group * kWaves + wave;
+  if (!rest.draws || i >= a.pieces) return;
+  const double z = rest.piece(i);
+  if (lane == 63) a.rests[(int64_t)b * a.pieces + i] = z;
+}
+
+// Follows each row.  Of lines it draws what follows the token where each stops, from the pieces' sums.
+template <int DT>
+__global__ __launch_bounds__(kThreads) void pl_verify_follow_kernel(verify_args a) {
+  __shared__ block_store<kThreads> store;
   __shared__ double s_before;
-  __shared__ double s_rests[kWhole ? kWholePieces : 1];
   __shared__ unsigned long long s_verdict[kNodesMax];
   __shared__ int s_path[kNodesMax];
-  __shared__ int s_old;
-  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int groups = kWhole ? 1 : a.groups;
-  const int group = (int)(blockIdx.x % groups), b = (int)(blockIdx.x / groups);
+  __shared__ int s_count, s_token;
+  const int tid = (int)threadIdx.x, b = (int)blockIdx.x;
   const row_of<DT> r(a, b);
-  const unsigned long long* verdicts = a.verdicts + (int64_t)b * a.nodes;
-  // the first token that goes nowhere; those before it all go to the next
-  int stop = INT32_MAX;
-  for (int i = tid; i < r.n; i += THREADS)
-    if (verdicts[i] >> 32 == 1) stop = min(stop, i);
-  stop = block_min(stop, store);
-  const bool draws = stop < r.n && (int)(uint32_t)verdicts[min(stop, a.nodes - 1)] == kDraw;
-  __syncthreads();
+  unsigned long long* verdicts = a.verdicts + (int64_t)b * a.nodes;
   int drawn = -1;
-  const node_sum total = draws ? a.totals[(int64_t)b * a.nodes + stop] : node_sum{0.0, 0.f, 0};
-  const T* x = r.logits(draws ? stop : 0);
-  const float* q = draws && stop + 1 < r.n ? r.probs(stop) : nullptr;
-  auto rest_of = [&](double e, float qv) { return fmax(e - (double)qv * total.z, 0.0); };
-  double* rests = a.rests + (int64_t)b * a.pieces;
-  if (draws) {
-    for (int piece = group * (THREADS / 64) + wave; piece < a.pieces; piece += THREADS / 64 * groups) {
-      float y[kPasses][kVec], p[kPasses][kVec] = {};
-      load_piece(x, piece * kPiece, a.vocab, y, -INFINITY);
-      if (q) load_piece(q, piece * kPiece, a.vocab, p, 0.f);
-      double z = 0.0;
-#pragma unroll
-      for (int k = 0; k < kPasses; ++k) {
-#pragma unroll
-        for (int e = 0; e < kVec; ++e)
-          z += rest_of(weight_least(y[k][e], total.top, r.per), p[k][e]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      z = without_least(wave_sum(z));
-      if (lane == 63) {
-        if constexpr (kWhole)
-          s_rests[piece] = z;
-        else
-          __hip_atomic_store(reinterpret_cast<unsigned long long*>(rests + piece),
-                             __builtin_bit_cast(unsigned long long, z), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (a.draft_probs) {
+    rest_of<DT> rest(r, store);
+    if (rest.draws) {
+      const double* rests = a.rests + (int64_t)b * a.pieces;
+      const float u = r.uniform_of(r.n - 1);
+      double mine = 0.0, all, before = 0.0;
+      for (int i = tid; i < a.pieces; i += kThreads) mine += rests[i];
+      block_before(mine, all, store);
+      // where p and q agree everywhere, from p itself
+      const bool whole = rest.q && !(all > 0.0);
+      if (whole) rest.q = nullptr, all = rest.total.z;
+      const double target = (double)u * all;
+      const piece_sum* sums = a.sums + ((int64_t)b * a.nodes + rest.stop) * a.pieces;
+      const int at = draw_piece(a.pieces, target, before, store, &s_before, [&](int i) {
+        if (!whole) return rests[i];
+        return sums[i].top == -INFINITY ? 0.0 : sums[i].z * weight(sums[i].top, rest.total.top, r.per);
+      });
+      if (at >= 0) {
+        const int lo = at * kPiece;
+        drawn = lo + draw_place(min(kPiece, a.vocab - lo), before, target, store, [&](int v) {
+                  return rest.of(weight((float)rest.x[lo + v], rest.total.top, r.per), rest.q ? rest.q[lo + v] : 0.f);
+                });
       }
     }
   }
-  if constexpr (kWhole) {
-    __syncthreads();
-  } else {
-    // all of a row's, whatever they found: the last one clears what they have read
-    if (arrive(a.row_arrivals + b, 1, &s_old) != groups - 1) return;
-    if (tid == 0) __hip_atomic_store(a.row_arrivals + b, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  for (int i = tid; i < a.nodes; i += kThreads) {
+    s_verdict[i] = verdicts[i];
+    s_path[i] = -1;
+    verdicts[i] = 0;  // as the next call expects them
   }
-  if (draws) {
-    auto rest_at = [&](int i) {
-      if constexpr (kWhole)
-        return s_rests[i];
-      else
-        return __builtin_bit_cast(double, peek(reinterpret_cast<const unsigned long long*>(rests + i)));
-    };
-    const float u = r.uniform_of(r.n - 1);
-    double mine = 0.0, all, before = 0.0;
-    for (int i = tid; i < a.pieces; i += THREADS) mine += rest_at(i);
-    block_before(mine, all, store);
-    // where p and q agree everywhere, from p itself
-    const bool whole = q && !(all > 0.0);
-    if (whole) q = nullptr, all = total.z;
-    const double target = (double)u * all;
-    const piece_sum* sums = a.sums + ((int64_t)b * a.nodes + stop) * a.pieces;
-    const int at = draw_piece(a.pieces, target, before, store, &s_before, [&](int i) {
-      if (!whole) return rest_at(i);
-      return sums[i].top == -INFINITY ? 0.0 : sums[i].z * weight(sums[i].top, total.top, r.per);
-    });
-    if (at >= 0)
-      drawn = at * kPiece + draw_place(min(kPiece, a.vocab - at * kPiece), before, target, store, [&](int v) {
-                return rest_of(weight((float)x[at * kPiece + v], total.top, r.per), q ? q[at * kPiece + v] : 0.f);
-              });
+  __syncthreads();
+  if (tid == 0) {
+    int count = 0, token = -1;
+    for (int node = 0; node >= 0 && node < r.n && count < r.n;) {
+      s_path[count++] = node;
+      const unsigned long long v = s_verdict[node];
+      token = (int)(uint32_t)v;
+      node = (int)(v >> 32) - 2;
+    }
+    s_count = count, s_token = token == kDraw ? drawn : token;
   }
-  follow<THREADS>(r, drawn, s_verdict, s_path);
+  __syncthreads();
+  for (int i = tid; i < a.nodes; i += kThreads) a.path[(int64_t)b * a.nodes + i] = s_path[i];
+  if (tid == 0) a.counts[b] = s_count, a.next[b] = s_token;
 }
 
 // Rows of no token.
@@ -666,20 +625,23 @@ int pieces_of(int64_t vocab) { return (int)((vocab + kPiece - 1) / kPiece); }
 template <int DT>
 int launch(const verify_args& a, bool whole, hipStream_t s) {
   const char* what = "pl_verify_tokens";
-  const unsigned tokens = (unsigned)(a.rows * a.nodes);
-  if (whole && a.pieces <= kFewPieces)
-    pl_verify_whole_kernel<DT, kThreads><<<dim3(tokens), kThreads, 0, s>>>(a);
-  else if (whole)
-    pl_verify_whole_kernel<DT, kWholeThreads><<<dim3(tokens), kWholeThreads, 0, s>>>(a);
-  else
-    pl_verify_nodes_kernel<DT><<<dim3(tokens * a.groups), kThreads, 0, s>>>(a);
-  const int rc = pl_launch_status(what);
-  if (rc || !a.draft_probs) return rc;
-  // one token of each row
-  if (a.rows >= kWholeRows && a.pieces <= kWholePieces)
-    pl_verify_draw_kernel<DT, kWholeThreads><<<dim3((unsigned)a.rows), kWholeThreads, 0, s>>>(a);
-  else
-    pl_verify_draw_kernel<DT, kThreads><<<dim3((unsigned)(a.rows * a.groups)), kThreads, 0, s>>>(a);
+  const dim3 tokens((unsigned)a.rows * (unsigned)a.nodes), rows((unsigned)a.rows);
+  int rc;
+  if (whole && a.pieces <= kFewPieces) {
+    pl_verify_whole_kernel<DT, kThreads><<<tokens, kThreads, 0, s>>>(a);
+  } else if (whole) {
+    pl_verify_whole_kernel<DT, kWholeThreads><<<tokens, kWholeThreads, 0, s>>>(a);
+  } else {
+    pl_verify_pieces_kernel<DT><<<dim3(tokens.x * (unsigned)a.groups), kThreads, 0, s>>>(a);
+    if ((rc = pl_launch_status(what))) return rc;
+    pl_verify_resolve_kernel<DT><<<tokens, kThreads, 0, s>>>(a);
+  }
+  if ((rc = pl_launch_status(what))) return rc;
+  if (a.draft_probs) {
+    pl_verify_rests_kernel<DT><<<dim3(rows.x * (unsigned)a.groups), kThreads, 0, s>>>(a);
+    if ((rc = pl_launch_status(what))) return rc;
+  }
+  pl_verify_follow_kernel<DT><<<rows, kThreads, 0, s>>>(a);
   return pl_launch_status(what);
 }
 
@@ -694,7 +656,7 @@ extern "C" int64_t pl_verify_workspace_bytes(int32_t rows, int32_t nodes, int32_
          whole_pieces((int64_t)rows * pieces * 8);
 }
 extern "C" int64_t pl_verify_counter_ints(int32_t rows, int32_t nodes) {
-  return rows < 0 || nodes < 0 ? 0 : 3ll * rows * nodes + rows;
+  return rows < 0 || nodes < 0 ? 0 : 2ll * rows * nodes;
 }
 
 extern "C" int pl_verify_tokens(int32_t dtype, const void* logits, int64_t ld_row, int64_t ld_node,
@@ -748,19 +710,18 @@ extern "C" int pl_verify_tokens(int32_t dtype, const void* logits, int64_t ld_ro
   }
   const int64_t n = (int64_t)rows * nodes;
   a.pieces = pieces_of(vocab), a.groups = a.pieces > kWaves ? (a.pieces + kWaves - 1) / kWaves : 1;
-  const bool whole = n > (a.pieces > kFewPieces ? kWholeTokens : kWholeFewTokens) && a.pieces <= kWholePieces;
-  const int64_t blocks = whole ? n : n * a.groups;
+  const bool few = a.pieces <= kFewPieces;
+  const bool whole = n > (few ? kWholeFewTokens : kWholeTokens) && a.pieces <= kWholePieces;
   if (!pl_grid_fits(n * a.groups, kWholeThreads)) {
     pl_set_error("%s: too many rows (%d)", what, rows);
     return PL_ERR_LIMIT;
   }
-  a.look = blocks > (whole && a.pieces > kFewPieces ? kWholeResident : kResident);
+  a.look = whole && n > (few ? kResident : kWholeResident);
   uint8_t* at = static_cast<uint8_t*>(workspace);
   a.sums = reinterpret_cast<piece_sum*>(at), at += whole_pieces(n * a.pieces * (int64_t)sizeof(piece_sum));
   a.totals = reinterpret_cast<node_sum*>(at), at += whole_pieces(n * (int64_t)sizeof(node_sum));
   a.rests = reinterpret_cast<double*>(at);
   a.verdicts = reinterpret_cast<unsigned long long*>(counters);
-  a.node_arrivals = counters + 2 * n, a.row_arrivals = counters + 3 * n;
   if (dtype == PL_F32) return launch<PL_F32>(a, whole, s);
   return dtype == PL_BF16 ? launch<PL_BF16>(a, whole, s) : launch<PL_F16>(a, whole, s);
 }
