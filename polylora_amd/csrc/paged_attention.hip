@@ -521,19 +521,8 @@ __global__ __launch_bounds__(kThreads, (shape<DT, CT, DP>::kWavesPerSimd)) void 
       }
     }
     if (!complete) {
-      // Parts are acknowledged from where every XCD sees them before the arrival
-      // is counted, and the last to arrive asks for them there after that.
       const int w0 = pair_start / per, w1 = (pair_start + r.atoms - 1) / per;
-      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-      __syncthreads();
-      if (tid == 0) {
-        int32_t* counter = a.counters + w0 * kCounterStride;
-        const int old = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        s_last = old == w1 - w0;
-        if (s_last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      }
-      __syncthreads();
-      if (s_last) {
+      if (arrive_last(a.counters + w0 * kCounterStride, w1 - w0, &s_last)) {
         // the first part is its workgroup's second when that workgroup began earlier
         const int slot0 = 2 * w0 + (w0 * per == pair_start ? 0 : 1);
         join_parts<DP>(parts, slot0, 2 * w0, 2, w1 - w0 + 1, cols, &s_o[0][0][0],
@@ -633,6 +622,10 @@ extern "C" int pl_paged_attention(int32_t dtype, int32_t cache_dtype, const void
                  (long long)workspace_bytes, (long long)counter_ints,
                  (long long)pl_paged_attention_workspace_bytes(dim), PL_ATTENTION_COUNTER_INTS);
     return PL_ERR_ARG;
+  }
+  if (!on_a_line(workspace)) {
+    pl_set_error("pl_paged_attention: the workspace must begin at whole %d bytes", kLine);
+    return PL_ERR_ALIGN;
   }
   attend_args a;
   a.q = q, a.q_row = q_strides[0], a.q_head = q_strides[1];

@@ -202,11 +202,14 @@ __device__ __forceinline__ void store4(T* p, pl_f32x4 x) {
   const T y[4] = {(T)x.x, (T)x.y, (T)x.z, (T)x.w};
   __builtin_memcpy(p, y, sizeof(y));
 }
+constexpr int kLine = 128;  // bytes of an L2's line, which a workspace begins with
+inline bool on_a_line(const void* p) { return reinterpret_cast<uintptr_t>(p) % kLine == 0; }
 // Floats of one part: o [kCols][DP], then m and l of each column.
 constexpr int part_floats(int dp) { return kCols * dp + 2 * kCols; }
 template <int DP>
 struct part_layout {
   static constexpr uint32_t kBytes = 4u * part_floats(DP);
+  static_assert(kBytes % kLine == 0, "no line holds two workgroups' parts (arrive_last)");
   static __device__ __forceinline__ pl_buffer all(const float* parts, uint32_t n) {
     return make_buffer(reinterpret_cast<uintptr_t>(parts), n * kBytes);
   }
@@ -218,6 +221,30 @@ struct part_layout {
 // them and from there, 16 bytes at a time.  No cache has to be invalidated for
 // that (16 rows of up to 3229 tokens 18.9 -> 17.0 us, with stores of 8 bytes 17.3).
 constexpr int kAgentScope = 16;
+
+// Arrival of a workgroup whose parts of a pair are stored: whether it is the last of `others` + 1,
+// which then may read what the others have stored.  Every thread calls it; the counter is 0 again
+// behind the last.
+//
+// The order is the hardware's: a wave's stores at agent scope go through its XCD's L2 to memory, and
+// vmcnt counts them until they are there; every wave has waited for its own, and the barrier
+// for the others', before the arrival is counted, and the last one asks for the parts after its
+// own count has come back.  No L2 answers it from an older copy: a part is whole 128-byte lines of one workgroup, nobody asks
+// for them before all have arrived, and a launch begins with the L2s invalidated.  (Records that share lines
+// between workgroups have no such promise.)  A release and an acquire at the counter instead write
+// back and invalidate a whole L2 at every arrival: 64 rows of 8 drafts over 4096 tokens 156 -> 178 us, 64
+// rows over 8192 tokens in 8 bits 108 -> 131.
+__device__ __forceinline__ bool arrive_last(int32_t* counter, int others, int* s_last) {
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const int old = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    *s_last = old == others;
+    if (old == others) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  return *s_last != 0;
+}
 
 // Joins n parts (the first in slot `slot0`, part w in slot `slot` + `step` w) and
 // hands each 4 finished elements of a column to `store`.  A thread takes 4

@@ -302,19 +302,8 @@ __global__ __launch_bounds__(kThreads, (waves_per_simd<DT, DP, C>())) void pl_tr
         put_part<DP>(parts, slot * C, in, d, x, top, sum);
     }
     if (!complete) {
-      // Parts are acknowledged from where every XCD sees them before the arrival
-      // is counted, and the last to arrive asks for them there after that.
       const int w0 = pair_start / per, w1 = (pair_start + r.atoms - 1) / per;
-      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-      __syncthreads();
-      if (tid == 0) {
-        int32_t* counter = a.counters + (w0 * a.col_tiles + ct) * kCounterStride;
-        const int old = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        s_last = old == w1 - w0;
-        if (s_last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      }
-      __syncthreads();
-      if (s_last) {
+      if (arrive_last(a.counters + (w0 * a.col_tiles + ct) * kCounterStride, w1 - w0, &s_last)) {
         // the first part is its workgroup's second when that workgroup began earlier
         const int slot1 = 2 * (w0 * a.col_tiles + ct), slot0 = slot1 + (w0 * per == pair_start ? 0 : 1);
         for (int c = 0; c < C; ++c)
@@ -452,6 +441,10 @@ extern "C" int pl_tree_attention(int32_t dtype, int32_t cache_dtype, const void*
     pl_set_error("%s: workspace of %lld bytes and %lld counters, %lld and %d needed", what, (long long)workspace_bytes,
                  (long long)counter_ints, (long long)pl_tree_attention_workspace_bytes(dim, columns), PL_ATTENTION_COUNTER_INTS);
     return PL_ERR_ARG;
+  }
+  if (!on_a_line(workspace)) {
+    pl_set_error("%s: the workspace must begin at whole %d bytes", what, kLine);
+    return PL_ERR_ALIGN;
   }
   tree_args a;
   a.q = q, a.q_row = q_strides[0], a.q_token = q_strides[1], a.q_head = q_strides[2];

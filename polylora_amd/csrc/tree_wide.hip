@@ -444,19 +444,8 @@ __global__ __launch_bounds__(kWideThreads, 2) void pl_tree_wide_kernel(tree_args
       }
     }
     if (!complete && !join_later) {
-      // Parts are acknowledged from where every XCD sees them before the arrival
-      // is counted, and the last to arrive asks for them there after that.
       const int w0 = pair_start / per, w1 = (pair_start + r.atoms - 1) / per;
-      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-      __syncthreads();
-      if (tid == 0) {
-        int32_t* counter = a.counters + (w0 * a.col_tiles + ct) * kCounterStride;
-        const int old = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        s_last = old == w1 - w0;
-        if (s_last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      }
-      __syncthreads();
-      if (s_last) {
+      if (arrive_last(a.counters + (w0 * a.col_tiles + ct) * kCounterStride, w1 - w0, &s_last)) {
         // the first part is its workgroup's second when that workgroup began earlier
         const int slot1 = 2 * (w0 * a.col_tiles + ct), slot0 = slot1 + (w0 * per == pair_start ? 0 : 1);
         const int n = w1 - w0 + 1;
