@@ -18,7 +18,9 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstdint>
 #include <exception>
+#include <mutex>
 #include <optional>
 #include <string>
 #include <vector>
@@ -125,6 +127,15 @@ class OnDevice {
  private:
   std::optional<c10::DeviceGuard> guard_;
 };
+
+// Calls on one stream share a workspace and counters, and some are several launches, between
+// which those hold the call's own: another thread's call on the stream waits for
+// the last of them.  (Taken without the GIL.  Streams that share one of these locks wait for each other's
+// launches alone.)
+std::mutex& launches_on(int device, void* stream) {
+  static std::mutex locks[64];
+  return locks[(reinterpret_cast<uintptr_t>(stream) / 64 + (uintptr_t)device) % 64];
+}
 
 void check_type(const at::Tensor& t, const char* name, at::ScalarType type, int device) {
   if (t.scalar_type() != type)
@@ -359,6 +370,7 @@ PyObject* paged_attention(PyObject* const* a) {
   at::Tensor out = given ? *given : at::empty(q.sizes(), q.options());
   int rc;
   Py_BEGIN_ALLOW_THREADS;
+  const std::lock_guard<std::mutex> together(launches_on(device, stream));
   rc = pl_paged_attention(code, c.code, q.const_data_ptr(), q.strides().data(), c.key, c.key_strides, c.value,
                           c.value_strides, c.num_pages, c.page_size, c.table, c.table_ld, c.max_pages, lens, r32, h32,
                           c.kv_heads, d32, (float)scale, (int32_t)window, c.k_scale, c.v_scale, out.data_ptr(),
@@ -518,6 +530,7 @@ PyObject* tree_attention(PyObject* const* a) {
   at::Tensor out = given ? *given : at::empty(q.sizes(), q.options());
   int rc;
   Py_BEGIN_ALLOW_THREADS;
+  const std::lock_guard<std::mutex> together(launches_on(device, stream));
   rc = pl_tree_attention(code, c.code, q.const_data_ptr(), q.strides().data(), c.key, c.key_strides, c.value,
                          c.value_strides, c.num_pages, c.page_size, c.table, c.table_ld, c.max_pages, past, seq, masks,
                          mask_row, mask_token, w32, depth.p, depth.ld, r32, m32, h32, c.kv_heads, d32, (float)scale,
@@ -628,6 +641,7 @@ PyObject* verify_tokens(PyObject* const* a) {
   at::Tensor next = at::empty({rows}, ints.dtype(at::kLong));
   int rc;
   Py_BEGIN_ALLOW_THREADS;
+  const std::lock_guard<std::mutex> together(launches_on(device, stream));
   rc = pl_verify_tokens(code, logits.const_data_ptr(), logits.stride(0), logits.stride(1), tokens.const_data_ptr(),
                         (int32_t)tokens.element_size(), tokens.stride(0),
                         static_cast<const float*>(uniforms.const_data_ptr()), uniforms.stride(0), tree.p, tree.ld,

@@ -2,13 +2,17 @@
 
 from __future__ import annotations
 
+from concurrent.futures import ThreadPoolExecutor
+
 import pytest
 import torch
 
 from oracle import drafts as plain
 from polylora_amd.drafts import verify_tokens
+from polylora_amd.paged import paged_attention, tree_attention
 
 from .test_gpu_drafts import random_parents
+from .test_gpu_paged import pool
 
 pytestmark = pytest.mark.gpu
 
@@ -51,3 +55,50 @@ def test_verification_of_other_inputs_in_each_call(gpu, rows, m, vocab, dtype, t
         want = plain.verify_tokens(*args, **more)
         for name, a, b in zip(("path", "counts", "next"), got, want):
             assert torch.equal(a.cpu(), b), (seed, name, (a.cpu() != b).nonzero().tolist())
+
+
+# ----------------------------------------------------------------------------- threads
+
+
+def on_one_stream(calls, repeats=30):
+    """What each call gives where each is a thread's and all threads launch on one stream, which has no scratch yet."""
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+
+    def work(call):
+        with torch.cuda.stream(stream):
+            return [call() for _ in range(repeats)]
+
+    with ThreadPoolExecutor(len(calls)) as threads:
+        got = list(threads.map(work, calls))
+    torch.cuda.synchronize()
+    return got
+
+
+def test_verification_from_threads_that_share_a_stream(gpu):
+    """A call is several launches: those of another on the stream do not come between them."""
+    calls, want = [], []
+    for seed, (rows, m, vocab, tree) in enumerate([(3, 6, 40000, False), (7, 4, 9001, False), (5, 6, 20000, True)]):
+        *args, more = drafted_on(gpu, seed, rows, m, vocab, torch.float32, tree)
+        calls.append(lambda args=args, more=more: verify_tokens(*args, **more))
+        want.append(plain.verify_tokens(*args, **more))
+    for kept, w in zip(on_one_stream(calls), want):
+        for got in kept:
+            assert all(torch.equal(a.cpu(), b) for a, b in zip(got, w))
+
+
+def test_attention_from_threads_that_share_a_stream(gpu):
+    """Many columns and few rows are two launches; one thread has single tokens over the same pages."""
+    gen = torch.Generator().manual_seed(1)
+    key, value, table, _, _ = pool(gen, 2, [3000, 2500], 2, 64, 16, torch.bfloat16)
+    key, value, table = key.nan_to_num(0.0).to(gpu), value.nan_to_num(0.0).to(gpu), table.to(gpu)
+    past = torch.tensor([2900, 2400], dtype=torch.int32, device=gpu)
+    calls = []
+    for m in (40, 64, 9):  # 160 and 256 columns, and 36
+        q = torch.randn(2, m, 8, 64, generator=gen).bfloat16().to(gpu)
+        calls.append(lambda q=q: tree_attention(q, key, value, table, past))
+    one = torch.randn(2, 8, 64, generator=gen).bfloat16().to(gpu)
+    calls.append(lambda: paged_attention(one, key, value, table, past))
+    want = [call() for call in calls]
+    for kept, w in zip(on_one_stream(calls), want):
+        assert all(torch.equal(got, w) for got in kept)
