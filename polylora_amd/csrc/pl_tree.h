@@ -33,11 +33,12 @@ namespace {
 constexpr int kCus = 256;
 constexpr int kWorkersMax = 2 * kCus;
 
-// Parts of 16 bits that a weight enters its product as.  One would add its rounding (2^-8 in
-// bf16) to every weight; two leave the output its own rounding alone (1.7e-3 in bf16 against 64
-// bits, as in fp32 rounded once) for a fifth more time where products bound it.
+// Parts of 16 bits that a weight enters its product as: three bf16 hold it whole, two fp16 keep
+// 2^-21 of it, as in paged_attention.hip.  Two bf16 keep 17 of its 24 bits, and small differences
+// of values come out wrong by percents; the third takes (bf16, 32 query heads over 8 of 128) 64 x 8 drafts over 4096
+// tokens 153 -> 155 us, 64 x 16 183 -> 187, 64 x 32 240 -> 267, 16 over 131072 in 8 bits 91 -> 103.
 template <int DT>
-constexpr int kWeightParts = 2;
+constexpr int kWeightParts = DT == PL_BF16 ? 3 : 2;
 // log2 of how far scores may pass the maximum that weights are taken against, and of
 // what fp16 weights are multiplied by, that their parts keep small ones: to 2^15.
 constexpr float kSlack = 8.f;
@@ -204,9 +205,7 @@ __device__ __forceinline__ column_place place_of(const tree_args& a, int col, in
 }
 
 // The weights of a column's eight tokens of a tile as 16-bit parts, two tokens to a word.
-// No part is negative, or 0 beside the first, so that an infinite value stays one: bf16
-// takes the rest of the weight 2^-20 larger, as in all weights alike and in their sum
-// (fp16 ends too early for that).
+// No part is negative, or 0 beside the first, so that an infinite value stays one.
 template <int DT>
 __device__ __forceinline__ void weight_parts(const float* p, pl_u32x4* part) {
   constexpr int kParts = kWeightParts<DT>;
@@ -215,12 +214,10 @@ __device__ __forceinline__ void weight_parts(const float* p, pl_u32x4* part) {
     float x = p[2 * j], y = p[2 * j + 1];
 #pragma unroll
     for (int k = 0; k < kParts; ++k) {
-      const uint32_t z = k + 1 < kParts ? pack2_down<DT>(x, y) : pack2<DT>(x, y);
-      if (k + 1 < kParts) {
-        constexpr float kMore = DT == PL_BF16 ? 1.f + 0x1p-20f : 1.f;
-        x = fmaf(x, kMore, -unpack<DT>(z, 0)), y = fmaf(y, kMore, -unpack<DT>(z, 1));
-      }
-      part[k][j] = k && DT == PL_F16 ? at_least_smallest<DT>(z, part[0][j]) : z;
+      // bf16's last part is exact either way
+      const uint32_t z = k + 1 < kParts || DT == PL_BF16 ? pack2_down<DT>(x, y) : pack2<DT>(x, y);
+      x -= unpack<DT>(z, 0), y -= unpack<DT>(z, 1);
+      part[k][j] = k ? at_least_smallest<DT>(z, part[0][j]) : z;
     }
   }
 }

@@ -102,3 +102,38 @@ def test_attention_from_threads_that_share_a_stream(gpu):
     want = [call() for call in calls]
     for kept, w in zip(on_one_stream(calls), want):
         assert all(torch.equal(got, w) for got in kept)
+
+
+# ----------------------------------------------------------------------------- weights of a drafted token's attention
+
+
+@pytest.mark.parametrize("dtype,fp8", [(torch.float32, False), (torch.bfloat16, False), (torch.float16, False),
+                                       (torch.bfloat16, True), (torch.float16, True)])
+@pytest.mark.parametrize("heads", [4, 40])  # 20 and 200 columns: both kernels
+@pytest.mark.parametrize("dim", [64, 144])
+def test_weights_are_held_in_32_bits(gpu, dtype, fp8, heads, dim):
+    """Two values, 1 and -1, with weights 1 and exp(-d), d down to 2^-13: out is tanh(d / 2), a small difference.
+
+    Weights are off by 2^-22 at most (of exp2's argument and result a unit each of fp32, half of one in their sum); two
+    fp16 parts keep 2^-21 of one.  Half of that, over the sum of weights, which is nearly 2, and the output's own rounding."""
+    d = torch.tensor([2.0**-e * f for e in (7, 9, 11, 12, 13) for f in (1.0, 1.25, 1.75)], dtype=torch.float64)
+    rows, m = len(d), 5
+    key = torch.zeros(rows, 1, 16, dim, dtype=dtype)
+    value = torch.zeros(rows, 1, 16, dim, dtype=dtype)
+    value[:, :, 0], value[:, :, 1] = 1.0, -1.0
+    key[:, 0, 1, 3] = -1.0 if fp8 else -d.to(dtype)
+    more = {}
+    if fp8:
+        key, value = (x.to(torch.float8_e4m3fn) for x in (key, value))
+        more = {"k_scale": torch.ones(1, device=gpu), "v_scale": torch.ones(1, device=gpu)}
+    q = torch.zeros(rows, m, heads, dim, dtype=dtype)
+    q[..., 3] = d.to(dtype)[:, None, None] if fp8 else 1.0
+    table = torch.arange(rows, dtype=torch.int32)[:, None]
+    got = tree_attention(q.to(gpu), key.to(gpu), value.to(gpu), table.to(gpu),
+                         torch.full((rows,), 2, dtype=torch.int32, device=gpu),
+                         visible=torch.zeros(m, 1, dtype=torch.int32, device=gpu), scale=1.0, **more)
+    want = torch.tanh(d / 2)[:, None, None, None].expand(got.shape)
+    weight = 2.0**-22 + (2.0**-21 if dtype == torch.float16 else 0.0)
+    tol = torch.finfo(dtype).eps / 2 * want + weight / 2
+    err = (got.cpu().double() - want).abs()
+    assert bool((err <= tol).all()), float((err / tol).max())
