@@ -60,7 +60,7 @@ __device__ __forceinline__ void load_to_lds(uint32_t to, uintptr_t p, uint32_t b
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                :
                : "s"(uniform((int)to)), "v"(lane_off), "s"(r)
-               : "memory");
+               : "memory", "m0");
 }
 
 // Joins n parts of columns [in0, in1) (numbers of sixteens: the first part's, and from the
