@@ -8,10 +8,10 @@ import pytest
 import torch
 
 from oracle import drafts as plain
-from polylora_amd.drafts import verify_tokens
+from polylora_amd.drafts import tree_tables, verify_tokens
 from polylora_amd.paged import paged_attention, tree_attention
 
-from .test_gpu_drafts import random_parents
+from .test_gpu_drafts import random_parents, seen_of
 from .test_gpu_paged import pool
 
 pytestmark = pytest.mark.gpu
@@ -137,3 +137,61 @@ def test_weights_are_held_in_32_bits(gpu, dtype, fp8, heads, dim):
     tol = torch.finfo(dtype).eps / 2 * want + weight / 2
     err = (got.cpu().double() - want).abs()
     assert bool((err <= tol).all()), float((err / tol).max())
+
+
+# ----------------------------------------------------------------------------- infinities and NaN that some tokens see
+
+
+@pytest.mark.parametrize("dtype,fp8", [(torch.float32, False), (torch.bfloat16, False), (torch.float16, False),
+                                       (torch.bfloat16, True), (torch.float16, True)])
+@pytest.mark.parametrize("dim", [64, 80, 256])
+@pytest.mark.parametrize("heads", [2, 40])  # 16 and 320 columns
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("window", [None, 40])
+def test_infinities_and_nan_reach_the_tokens_that_see_them_and_no_others(gpu, dtype, fp8, dim, heads, tree, window):
+    """Among the drafts, in the tile where they begin and where windows begin: each comes out, whatever its weight, at its
+    element of the tokens that see its place; all else is what finite values in its place give, bit for bit."""
+    gen = torch.Generator().manual_seed(dim + heads)
+    rows, m, page = 2, 8, 16
+    past = [133, 77]
+    key, value, table, ks, vs = pool(gen, rows, [p + m for p in past], 1, dim, page, dtype, fp8)
+    q = (torch.randn(rows, m, heads, dim, generator=gen) * (0.2 if fp8 else 1.0)).to(dtype)
+    depths = seen = None
+    more = {"k_scale": ks, "v_scale": vs, "visible": None, "depths": None}
+    if tree:
+        parents = random_parents(gen, rows, m)
+        depths, visible = tree_tables(parents)
+        seen = seen_of(visible, m)
+        more.update(visible=visible, depths=depths)
+    bits = value.view(torch.uint8) if fp8 else value
+    inf = float("inf")
+    kinds = [0x7F, 0xFF] if fp8 else [inf, -inf, float("nan")]
+    hit = torch.zeros(rows, m, dim, 3, dtype=torch.bool)  # +inf, -inf and NaN that a token sees at an element
+    clean = bits.clone()
+    for b in range(rows):
+        places = [past[b] + j for j in range(m)] + [past[b] - 1, past[b] - 6]
+        if window:  # places where some windows begin and others do not reach
+            places += [past[b] - window + j for j in range(m + 1)]
+        for i, p in enumerate(places):
+            at = plain.place(table, b, p, key.shape[0], page)
+            # elements at both ends and in the middle, the same one for several places
+            for d in (i % 3, dim // 2 + i, dim - 1 - i % 2):
+                kind = (i + d) % len(kinds)
+                bits[at[0], 0, at[1], d] = kinds[kind]
+                clean[at[0], 0, at[1], d] = 0
+                for t in range(m):
+                    if p in plain.seen_places(past[b], m, t, m, None if seen is None else seen[b, t].tolist(),
+                                              None if depths is None else int(depths[b, t]), window):
+                        hit[b, t, d, 2 if fp8 else kind] = True
+    some = hit.any(-1).sum(1)
+    assert bool((some == m).any()) and bool(((some > 0) & (some < m)).any())  # seen by all, and by a part of the tokens
+    args = (table.to(gpu), torch.tensor(past, dtype=torch.int32, device=gpu))
+    more = {name: None if t is None else t.to(gpu) for name, t in more.items()}
+    got = tree_attention(q.to(gpu), key.to(gpu), value.to(gpu), *args, window=window, **more).cpu()
+    want = tree_attention(q.to(gpu), key.to(gpu), clean.view(value.dtype).to(gpu), *args, window=window, **more).cpu()
+    assert not want.isnan().any() and not want.isinf().any()
+    nan = hit[..., 2] | (hit[..., 0] & hit[..., 1])
+    for name, where, x in (("nan", nan, float("nan")), ("+inf", hit[..., 0] & ~nan, inf), ("-inf", hit[..., 1] & ~nan, -inf)):
+        want = torch.where(where[:, :, None], x, want)
+    same = (got == want) | (got.isnan() & want.isnan())
+    assert bool(same.all()), [(i, float(got[tuple(i)]), float(want[tuple(i)])) for i in (~same).nonzero().tolist()[:5]]
