@@ -53,7 +53,11 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
 }
 // 16 bytes to a lane, from p + lane_off to LDS at `to` + 16 * lane.  The wait for it is the
-// caller's, before the barrier behind which the stage is read.
+// caller's, before the barrier behind which the stage is read.  (The compiler sets m0 where it wants it
+// and keeps nothing else there, but may take it to be still what it set: so it is named, and the
+// warning about reserved registers is off.)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void load_to_lds(uint32_t to, uintptr_t p, uint32_t bytes, uint32_t lane_off) {
   const pl_u32x4 r = {(uint32_t)uniform((int)(uint32_t)p), (uint32_t)uniform((int)(p >> 32)), (uint32_t)uniform((int)bytes),
                       0x00027000u};
@@ -62,6 +66,7 @@ __device__ __forceinline__ void load_to_lds(uint32_t to, uintptr_t p, uint32_t b
                : "s"(uniform((int)to)), "v"(lane_off), "s"(r)
                : "memory", "m0");
 }
+#pragma clang diagnostic pop
 
 // Joins n parts of columns [in0, in1) (numbers of sixteens: the first part's, and from the
 // second on first + step * part) and puts out what comes of them.  A thread has ITEMS
