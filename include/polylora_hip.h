@@ -655,7 +655,8 @@ int pl_paged_attention(int32_t dtype, int32_t cache_dtype, const void* q,
  * does one that sees nothing; nothing is read at a place that no live token of the
  * row sees.  Depths below 0 count as 0.  q [rows][row_len][heads][dim] with strides of
  * row, token and head, out contiguous and apart from q.  Workspace
- * (pl_tree_attention_workspace_bytes(dim, row_len * heads / kv_heads) bytes) and
+ * (pl_tree_attention_workspace_bytes(dim, columns) bytes, columns row_len * heads /
+ * kv_heads, or 1 in fp32) and
  * counters as above; the two may share them where they follow one another.  At most
  * 1024 query heads to a key head. */
 int64_t pl_tree_attention_workspace_bytes(int32_t dim, int32_t columns);

@@ -381,9 +381,10 @@ static_assert(PL_ATTENTION_COUNTER_INTS == kWorkersMax * kCounterStride, "one co
 
 extern "C" int64_t pl_tree_attention_workspace_bytes(int32_t dim, int32_t columns) {
   if (dim < 1 || dim > kHeadDimMax || columns < 0) return 0;
-  // two parts of a worker: of up to 32 columns each, two workers on a CU, or one of 256 (128 of large heads)
+  // two parts of a worker: of up to kWorkersMax workers of 32 columns each (16 of large heads), or, of
+  // 16-bit models, of one on a CU of 256 (128)
   const int dp = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
-  const int64_t sixteens = columns <= narrow_columns(dp) ? 2ll * kWorkersMax * 2 : 2ll * kCus * wide_columns(dp) / kCols;
+  const int64_t sixteens = columns <= narrow_columns(dp) ? 2ll * kWorkersMax * (dp == 256 ? 1 : 2) : 2ll * kCus * wide_columns(dp) / kCols;
   return sixteens * part_floats(dp) * (int64_t)sizeof(float);
 }
 
@@ -435,11 +436,12 @@ extern "C" int pl_tree_attention(int32_t dtype, int32_t cache_dtype, const void*
     return PL_ERR_ARG;
   }
   const int64_t all_columns = (int64_t)row_len * (heads / kv_heads);
-  const int32_t columns = (int32_t)(all_columns < kColumnsMax ? all_columns : kColumnsMax);
-  if (!workspace || workspace_bytes < pl_tree_attention_workspace_bytes(dim, columns) || !counters ||
-      counter_ints < PL_ATTENTION_COUNTER_INTS) {
+  // (fp32 has the kernel for few columns alone)
+  const int32_t columns = dtype == PL_F32 ? 1 : (int32_t)(all_columns < kColumnsMax ? all_columns : kColumnsMax);
+  const int64_t need = pl_tree_attention_workspace_bytes(dim, columns);
+  if (!workspace || workspace_bytes < need || !counters || counter_ints < PL_ATTENTION_COUNTER_INTS) {
     pl_set_error("%s: workspace of %lld bytes and %lld counters, %lld and %d needed", what, (long long)workspace_bytes,
-                 (long long)counter_ints, (long long)pl_tree_attention_workspace_bytes(dim, columns), PL_ATTENTION_COUNTER_INTS);
+                 (long long)counter_ints, (long long)need, PL_ATTENTION_COUNTER_INTS);
     return PL_ERR_ARG;
   }
   if (!on_a_line(workspace)) {

@@ -168,8 +168,8 @@ def tree_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.
     the tree.  scale, scales, precision, ``out`` and rows that see nothing are ``paged_attention``'s; padding tokens get 0.
     """
     stream = _stream(q)
-    # columns of the products: the workspace goes by whether they are few
-    fits = q.dim() == 4 and key_cache.dim() == 4
+    # columns of the products: the workspace goes by whether they are few, which those of fp32 count as
+    fits = q.dim() == 4 and key_cache.dim() == 4 and q.dtype != torch.float32
     columns = q.shape[1] * q.shape[2] // max(1, key_cache.shape[1]) if fits else 0
     return _native.tensor_calls().tree_attention(q, key_cache, value_cache, page_table, past_lens, seq_lens, visible,
                                                  depths, scale, window, k_scale, v_scale, out,

@@ -23,3 +23,22 @@ def test_attention_workspaces_begin_with_a_line(shift):
                 lens=p, rows=2, heads=2, kv=2, dim=16, scale=1.0, window=0, ksc=None, vsc=None, out=1 << 20)
     good.update(_TREE_SCRATCH)
     assert _refused(lib.pl_paged_attention, good, ws=4096 + shift) == _native.PL_ERR_ALIGN
+
+
+def test_attention_workspaces_are_no_larger_than_what_is_launched_takes():
+    """Two parts of 512 workers of 16 columns of heads above 128 elements, of 32 below; fp32 has no kernel for more columns."""
+    lib = _native.load()
+    need = lib.pl_tree_attention_workspace_bytes
+    part = {64: 16 * (64 + 2) * 4, 128: 16 * (128 + 2) * 4, 256: 16 * (256 + 2) * 4}  # 16 columns, and two sums to each
+    for dim, dp, sixteens in ((16, 64, 2), (64, 64, 2), (80, 128, 2), (128, 128, 2), (144, 256, 1), (256, 256, 1)):
+        assert need(dim, 1) == need(dim, 32) == 2 * 512 * sixteens * part[dp]
+        assert need(dim, 1) <= 17 << 20
+    s, p = _i64(1 << 20, 64 * 40, 64), 4096
+    good = dict(dtype=0, cache=0, q=p, qs=s, key=p, keys=_i64(2048, 1024, 64), value=p, values=_i64(2048, 1024, 64), pages=4,
+                page=16, table=p, ld=2, cols=2, past=p, seq=None, visible=None, vrow=0, vtoken=0, words=0, depths=None,
+                drow=0, rows=2, m=9, heads=40, kv=1, dim=64, scale=1.0, window=0, ksc=None, vsc=None, out=1 << 40)
+    good.update(_TREE_SCRATCH)
+    # fp32 of 360 columns takes what one column does: no later check finds fault but the workspace's place
+    assert _refused(lib.pl_tree_attention, good, ws=4096 + 64, wsb=need(64, 1)) == _native.PL_ERR_ALIGN
+    assert _refused(lib.pl_tree_attention, good, ws=4096 + 64, wsb=need(64, 1) - 1) == _native.PL_ERR_ARG
+    assert _refused(lib.pl_tree_attention, good, ws=4096 + 64, wsb=need(64, 1), dtype=1, cache=1) == _native.PL_ERR_ARG
