@@ -712,7 +712,9 @@ extern "C" int pl_verify_tokens(int32_t dtype, const void* logits, int64_t ld_ro
   a.pieces = pieces_of(vocab), a.groups = a.pieces > kWaves ? (a.pieces + kWaves - 1) / kWaves : 1;
   const bool few = a.pieces <= kFewPieces;
   const bool whole = n > (few ? kWholeFewTokens : kWholeTokens) && a.pieces <= kWholePieces;
-  if (!pl_grid_fits(n * a.groups, kWholeThreads)) {
+  // the first launch's workgroups, and the pieces' of a draw
+  if (!(whole ? pl_grid_fits(n, few ? kThreads : kWholeThreads) : pl_grid_fits(n * a.groups, kThreads)) ||
+      !pl_grid_fits(draft_probs ? (int64_t)rows * a.groups : rows, kThreads)) {
     pl_set_error("%s: too many rows (%d)", what, rows);
     return PL_ERR_LIMIT;
   }

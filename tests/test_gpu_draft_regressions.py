@@ -195,3 +195,21 @@ def test_infinities_and_nan_reach_the_tokens_that_see_them_and_no_others(gpu, dt
         want = torch.where(where[:, :, None], x, want)
     same = (got == want) | (got.isnan() & want.isnan())
     assert bool(same.all()), [(i, float(got[tuple(i)]), float(want[tuple(i)])) for i in (~same).nonzero().tolist()[:5]]
+
+
+# ----------------------------------------------------------------------------- sizes
+
+
+def test_verification_of_more_rows_than_their_pieces_would_fit_a_grid(gpu):
+    """Tokens that are taken whole are as many workgroups, not as many as they have pieces."""
+    gen = torch.Generator().manual_seed(2)
+    rows, m, vocab = 4096, 33, 128256
+    logits = (torch.randn(1, m, vocab, generator=gen) * 4.5).to(gpu).expand(rows, m, vocab)
+    uniforms = torch.rand(rows, m, generator=gen)
+    tokens = logits[0].argmax(-1).cpu().roll(1).expand(rows, m).clone()
+    got = verify_tokens(logits, tokens.to(gpu), uniforms.to(gpu))
+    some = torch.randperm(rows, generator=gen)[:24]
+    want = plain.verify_tokens(logits[:24], tokens[some], uniforms[some])
+    assert int(want[1].max()) > 1
+    for a, b in zip(got, want):
+        assert torch.equal(a.cpu()[some], b)
