@@ -469,7 +469,7 @@ void launch_vec(const append_args& a, const norm_args* n, int vec, dim3 grid, hi
 }
 
 template <int DT, int CT>
-int launch(append_args a, norm_args* n, int vec, hipStream_t s) {
+int launch(const char* what, append_args a, norm_args* n, int vec, hipStream_t s) {
   // places of a head that a thread may keep
   a.turns = (a.interleaved && vec > 1 ? 2 * a.half : a.half) / vec;
   a.units = a.turns + (a.dim - 2 * a.half) / vec;
@@ -495,11 +495,11 @@ int launch(append_args a, norm_args* n, int vec, hipStream_t s) {
     launch_vec<DT, CT, true>(a, n, vec, grid, s);
   else
     launch_vec<DT, CT, false>(a, n, vec, grid, s);
-  return pl_launch_status("pl_rope_append");
+  return pl_launch_status(what);
 }
 
 // Both entry points; `n` null for the one without norms and depths.
-int append(int32_t dtype, int32_t cache_dtype, const void* q,
+int append(const char* what, int32_t dtype, int32_t cache_dtype, const void* q,
            const int64_t* q_strides, const void* k, const int64_t* k_strides,
            const void* v, const int64_t* v_strides, void* q_out, void* k_out,
            void* key_cache, const int64_t* key_strides, void* value_cache,
@@ -510,20 +510,20 @@ int append(int32_t dtype, int32_t cache_dtype, const void* q,
            const float* cos, const float* sin, int32_t positions, int32_t rot,
            int32_t interleaved, const float* k_scale, const float* v_scale,
            norm_args* n, void* stream) {
-  const int rc = pl_check_paged("pl_rope_append", dtype, cache_dtype, key_cache, key_strides,
+  const int rc = pl_check_paged(what, dtype, cache_dtype, key_cache, key_strides,
                                 value_cache, value_strides, num_pages, page_size, page_table,
                                 table_ld, max_pages, rows, heads, kv_heads, dim, k_scale, v_scale);
   if (rc) return rc;
   if (row_len < 0 || rot < 0 || rot > dim || rot % 2 != 0 || positions < 0) {
-    pl_set_error("pl_rope_append: bad sizes (row_len %d, rot %d of %d, positions %d)", row_len, rot,
-                 dim, positions);
+    pl_set_error("%s: bad sizes (row_len %d, rot %d of %d, positions %d)", what, row_len, rot, dim,
+                 positions);
     return PL_ERR_ARG;
   }
   const int64_t tokens = (int64_t)rows * row_len;
   if (tokens == 0) return PL_OK;
   if (!q || !k || !v || !q_out || !q_strides || !k_strides || !v_strides || !past_lens ||
       (rot > 0 && positions > 0 && (!cos || !sin))) {
-    pl_set_error("pl_rope_append: null pointer");
+    pl_set_error("%s: null pointer", what);
     return PL_ERR_ARG;
   }
   const int64_t es = pl_elem_size(dtype), q_bytes = tokens * heads * dim * es;
@@ -537,17 +537,17 @@ int append(int32_t dtype, int32_t cache_dtype, const void* q,
   for (int i = 0; i < 3; ++i)
     if (pl_ranges_meet(q_out, q_bytes, inputs[i], reaches[i]) ||
         pl_ranges_meet(k_out, k_out ? k_bytes : 0, inputs[i], reaches[i])) {
-      pl_set_error("pl_rope_append: an output overlaps an input");
+      pl_set_error("%s: an output overlaps an input", what);
       return PL_ERR_ARG;
     }
   if (!pl_grid_fits(tokens, kThreads)) {
-    pl_set_error("pl_rope_append: too many tokens (%lld)", (long long)tokens);
+    pl_set_error("%s: too many tokens (%lld)", what, (long long)tokens);
     return PL_ERR_LIMIT;
   }
   if (num_pages > 0 && (key_cache == value_cache ||
                         !pl_elements_apart(key_strides, num_pages, kv_heads, page_size, dim) ||
                         !pl_elements_apart(value_strides, num_pages, kv_heads, page_size, dim))) {
-    pl_set_error("pl_rope_append: elements of the caches share their places");
+    pl_set_error("%s: elements of the caches share their places", what);
     return PL_ERR_ARG;
   }
   append_args a;
@@ -579,10 +579,11 @@ int append(int32_t dtype, int32_t cache_dtype, const void* q,
   while (vec > 1 && !whole(vec)) vec /= 2;
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (cache_dtype == PL_F8E4M3)
-    return dtype == PL_BF16 ? launch<PL_BF16, PL_F8E4M3>(a, n, vec, s)
-                            : launch<PL_F16, PL_F8E4M3>(a, n, vec, s);
-  if (dtype == PL_F32) return launch<PL_F32, PL_F32>(a, n, vec, s);
-  return dtype == PL_BF16 ? launch<PL_BF16, PL_BF16>(a, n, vec, s) : launch<PL_F16, PL_F16>(a, n, vec, s);
+    return dtype == PL_BF16 ? launch<PL_BF16, PL_F8E4M3>(what, a, n, vec, s)
+                            : launch<PL_F16, PL_F8E4M3>(what, a, n, vec, s);
+  if (dtype == PL_F32) return launch<PL_F32, PL_F32>(what, a, n, vec, s);
+  return dtype == PL_BF16 ? launch<PL_BF16, PL_BF16>(what, a, n, vec, s)
+                          : launch<PL_F16, PL_F16>(what, a, n, vec, s);
 }
 
 }  // namespace
@@ -595,7 +596,7 @@ extern "C" int pl_rope_append(int32_t dtype, int32_t cache_dtype, const void* q,
     int32_t row_len, int32_t heads, int32_t kv_heads, int32_t dim, const float* cos, const float* sin,
     int32_t positions, int32_t rot, int32_t interleaved, const float* k_scale, const float* v_scale,
     void* stream) {
-  return append(dtype, cache_dtype, q, q_strides, k, k_strides, v, v_strides, q_out, k_out, key_cache, key_strides,
+  return append("pl_rope_append", dtype, cache_dtype, q, q_strides, k, k_strides, v, v_strides, q_out, k_out, key_cache, key_strides,
                 value_cache, value_strides, num_pages, page_size, page_table, table_ld, max_pages, past_lens, seq_lens,
                 rows, row_len, heads, kv_heads, dim, cos, sin, positions, rot, interleaved, k_scale, v_scale, nullptr, stream);
 }
@@ -609,16 +610,17 @@ extern "C" int pl_norm_rope_append(int32_t dtype, int32_t cache_dtype, const voi
     int32_t positions, int32_t rot, int32_t interleaved, const float* k_scale, const float* v_scale,
     const void* q_norm, const void* k_norm, int32_t norm_dtype,
     float eps, const int32_t* depths, int64_t depths_ld, void* stream) {
+  const char* what = "pl_norm_rope_append";
   if ((q_norm || k_norm) && norm_dtype != PL_F32 && norm_dtype != dtype) {
-    pl_set_error("pl_norm_rope_append: the norms' weights are fp32 or of the model's type (got %d)", norm_dtype);
+    pl_set_error("%s: the norms' weights are fp32 or of the model's type (got %d)", what, norm_dtype);
     return PL_ERR_ARG;
   }
   if (!(eps > 0.f && eps < INFINITY)) {
-    pl_set_error("pl_norm_rope_append: eps must be positive and finite (got %g)", (double)eps);
+    pl_set_error("%s: eps must be positive and finite (got %g)", what, (double)eps);
     return PL_ERR_ARG;
   }
   norm_args n = {q_norm, k_norm, norm_dtype == PL_F32, eps, depths, depths_ld, 1};
-  return append(dtype, cache_dtype, q, q_strides, k, k_strides, v, v_strides, q_out, k_out, key_cache, key_strides,
+  return append(what, dtype, cache_dtype, q, q_strides, k, k_strides, v, v_strides, q_out, k_out, key_cache, key_strides,
                 value_cache, value_strides, num_pages, page_size, page_table, table_ld, max_pages, past_lens, seq_lens,
                 rows, row_len, heads, kv_heads, dim, cos, sin, positions, rot, interleaved, k_scale, v_scale, &n, stream);
 }

@@ -42,3 +42,18 @@ def test_attention_workspaces_are_no_larger_than_what_is_launched_takes():
     assert _refused(lib.pl_tree_attention, good, ws=4096 + 64, wsb=need(64, 1)) == _native.PL_ERR_ALIGN
     assert _refused(lib.pl_tree_attention, good, ws=4096 + 64, wsb=need(64, 1) - 1) == _native.PL_ERR_ARG
     assert _refused(lib.pl_tree_attention, good, ws=4096 + 64, wsb=need(64, 1), dtype=1, cache=1) == _native.PL_ERR_ARG
+
+
+@pytest.mark.parametrize("name", ["pl_rope_append", "pl_norm_rope_append"])
+def test_append_refusals_name_the_function_that_was_called(name):
+    lib = _native.load()
+    s, p = _i64(64, 32, 16), 4096
+    good = dict(dtype=1, cache=1, q=p, qs=s, k=2 * p, ks=s, v=3 * p, vs=s, out=1 << 20, k_out=None, key=p, keys=s, value=2 * p,
+                values=s, pages=4, page=16, table=p, ld=2, cols=2, past=p, seq=None, rows=1, m=2, heads=2, kv=2, dim=16,
+                cos=p, sin=p, positions=8, rot=16, inter=0, ksc=None, vsc=None)
+    if name == "pl_norm_rope_append":
+        good.update(qn=p, kn=p, norm=1, eps=1e-6, depths=None, depths_ld=0)
+    good["stream"] = None
+    for bad in (dict(dim=24), dict(rot=3), dict(past=None), dict(out=p), dict(value=p), dict(rows=1 << 30)):
+        _refused(getattr(lib, name), good, **bad)
+        assert lib.pl_last_error().decode().startswith(name + ": "), (bad, lib.pl_last_error())
