@@ -600,7 +600,8 @@ int pl_rope_append(int32_t dtype, int32_t cache_dtype, const void* q, const int6
 /* The same with the norms of queries and keys of each head before the rotation,
  *   x / sqrt(mean(x^2) + eps) * w,
  * in fp32 like the rest, w the head's dim weights of q_norm or k_norm (the model's
- * type or PL_F32, norm_dtype for both; NULL for no norm of these), eps positive;
+ * type or PL_F32, norm_dtype for both; NULL for no norm of these), eps positive
+ * (without norms anything);
  * and, unless depths is NULL, with position past_lens[b] + depths[b * depths_ld + t]
  * in the angles (depths_ld 0: one list that all rows share).  The token's place
  * in the pages stays past_lens[b] + t. */

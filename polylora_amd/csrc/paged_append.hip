@@ -615,7 +615,7 @@ extern "C" int pl_norm_rope_append(int32_t dtype, int32_t cache_dtype, const voi
     pl_set_error("%s: the norms' weights are fp32 or of the model's type (got %d)", what, norm_dtype);
     return PL_ERR_ARG;
   }
-  if (!(eps > 0.f && eps < INFINITY)) {
+  if ((q_norm || k_norm) && !(eps > 0.f && eps < INFINITY)) {
     pl_set_error("%s: eps must be positive and finite (got %g)", what, (double)eps);
     return PL_ERR_ARG;
   }

@@ -57,3 +57,16 @@ def test_append_refusals_name_the_function_that_was_called(name):
     for bad in (dict(dim=24), dict(rot=3), dict(past=None), dict(out=p), dict(value=p), dict(rows=1 << 30)):
         _refused(getattr(lib, name), good, **bad)
         assert lib.pl_last_error().decode().startswith(name + ": "), (bad, lib.pl_last_error())
+
+
+def test_append_without_norms_does_not_look_at_eps():
+    """Refused for what comes after eps, not for it."""
+    lib = _native.load()
+    s, p = _i64(64, 32, 16), 4096
+    good = dict(dtype=1, cache=1, q=p, qs=s, k=2 * p, ks=s, v=3 * p, vs=s, out=1 << 20, k_out=None, key=p, keys=s, value=2 * p,
+                values=s, pages=4, page=16, table=p, ld=2, cols=2, past=p, seq=None, rows=1, m=2, heads=2, kv=2, dim=24,
+                cos=p, sin=p, positions=8, rot=16, inter=0, ksc=None, vsc=None, qn=None, kn=None, norm=1, eps=0.0, depths=p,
+                depths_ld=2, stream=None)
+    for eps in (0.0, -1.0, float("nan")):
+        assert _refused(lib.pl_norm_rope_append, good, eps=eps) == _native.PL_ERR_LIMIT  # the head size
+        assert _refused(lib.pl_norm_rope_append, good, eps=eps, kn=p) == _native.PL_ERR_ARG

@@ -9,7 +9,7 @@ import torch
 
 from oracle import drafts as plain
 from polylora_amd.drafts import tree_tables, verify_tokens
-from polylora_amd.paged import paged_attention, tree_attention
+from polylora_amd.paged import paged_attention, rope_append, rope_table, tree_attention
 
 from .test_gpu_drafts import random_parents, seen_of
 from .test_gpu_paged import pool
@@ -213,3 +213,19 @@ def test_verification_of_more_rows_than_their_pieces_would_fit_a_grid(gpu):
     assert int(want[1].max()) > 1
     for a, b in zip(got, want):
         assert torch.equal(a.cpu()[some], b)
+
+
+# ----------------------------------------------------------------------------- append
+
+
+def test_append_by_depths_without_norms_takes_any_eps(gpu):
+    gen = torch.Generator().manual_seed(3)
+    key, value, table, _, _ = pool(gen, 2, [9, 20], 1, 32, 16, torch.float32)
+    x = torch.randn(2, 4, 1, 32, generator=gen).to(gpu)
+    past = torch.tensor([3, 14], dtype=torch.int32, device=gpu)
+    depths = torch.tensor([0, 1, 1, 2], dtype=torch.int32, device=gpu)
+    args = (x, x, x, key.to(gpu), value.to(gpu), table.to(gpu), past, *rope_table(32, 32, device=gpu))
+    want = rope_append(*args, depths=depths)
+    assert torch.equal(rope_append(*args, depths=depths, eps=0.0), want)
+    with pytest.raises(RuntimeError, match="eps"):
+        rope_append(*args, depths=depths, eps=0.0, k_norm=torch.ones(32, device=gpu))
