@@ -20,8 +20,9 @@ __all__ = ["tree_tables", "verify_tokens"]
 def tree_tables(parents: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """(depths, visible) of trees of tokens: int32 ``[..., M]`` and ``[..., M, ceil(M / 32)]``.
 
-    ``parents[..., t]`` is the token before token t, less than t; a token whose parent is negative is a root.  visible has
-    the bits of each token and its ancestors, as ``paged.tree_attention`` takes them.
+    ``parents[..., t]`` is the token before token t, less than t; a token whose parent is negative is a root, as is one
+    whose parent is not before it.  visible has the bits of each token and its ancestors, as ``paged.tree_attention``
+    takes them.
     """
     if parents.dtype not in (torch.int32, torch.int64) or parents.dim() == 0:
         raise TypeError("tree_tables takes int32 or int64 parents [..., M]")
@@ -31,7 +32,7 @@ def tree_tables(parents: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     bits = torch.zeros(*parents.shape, 32 * words, dtype=torch.bool, device=parents.device)
     for t in range(m):
         parent = parents[..., t : t + 1].long()
-        has = parent >= 0
+        has = (parent >= 0) & (parent < t)
         parent = parent.clamp(0, max(0, t - 1))
         depths[..., t : t + 1] = torch.where(has, depths.gather(-1, parent) + 1, 0)
         before = bits.gather(-2, parent[..., None].expand(*parent.shape, 32 * words))[..., 0, :]

@@ -3,8 +3,10 @@
 from __future__ import annotations
 
 import pytest
+import torch
 
 from polylora_amd import _native
+from polylora_amd.drafts import tree_tables
 
 from .test_drafts_host import _TREE_SCRATCH, _i64, _refused
 
@@ -70,3 +72,14 @@ def test_append_without_norms_does_not_look_at_eps():
     for eps in (0.0, -1.0, float("nan")):
         assert _refused(lib.pl_norm_rope_append, good, eps=eps) == _native.PL_ERR_LIMIT  # the head size
         assert _refused(lib.pl_norm_rope_append, good, eps=eps, kn=p) == _native.PL_ERR_ARG
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_a_token_whose_parent_is_not_before_it_is_a_root(dtype):
+    """Token 0 as its own parent too: it was one deeper than a root, and all tokens behind it."""
+    parents = torch.tensor([[0, 0, 1, 1, 9], [-1, 1, 0, 4, 2], [-7, 2**30, 1, 0, 4]], dtype=dtype)
+    depths, visible = tree_tables(parents)
+    assert depths.tolist() == [[0, 1, 2, 2, 0], [0, 0, 1, 0, 2], [0, 0, 1, 1, 0]]
+    assert visible[..., 0].tolist() == [[1, 3, 7, 11, 16], [1, 2, 5, 8, 21], [1, 2, 6, 9, 16]]
+    depths, visible = tree_tables(parents[:, :0])
+    assert depths.shape == (3, 0) and visible.shape == (3, 0, 0)
