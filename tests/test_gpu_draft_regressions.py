@@ -9,9 +9,10 @@ import torch
 
 from oracle import drafts as plain
 from polylora_amd.drafts import tree_tables, verify_tokens
-from polylora_amd.paged import paged_attention, rope_append, rope_table, tree_attention
+from polylora_amd.paged import keep_tokens, paged_attention, rope_append, rope_table, tree_attention
 
 from .test_gpu_drafts import random_parents, seen_of
+from .test_gpu_draft_steps import VOCAB, Server, Weights, plain_logits
 from .test_gpu_paged import pool
 
 pytestmark = pytest.mark.gpu
@@ -229,3 +230,47 @@ def test_append_by_depths_without_norms_takes_any_eps(gpu):
     assert torch.equal(rope_append(*args, depths=depths, eps=0.0), want)
     with pytest.raises(RuntimeError, match="eps"):
         rope_append(*args, depths=depths, eps=0.0, k_norm=torch.ones(32, device=gpu))
+
+
+# ----------------------------------------------------------------------------- whole steps of lines with probabilities
+
+
+def test_steps_over_lines_with_probabilities(gpu):
+    """Each pass's logits are those of the row's tokens alone, and what stays and follows is what the definition has."""
+    gen = torch.Generator().manual_seed(4)
+    w = Weights(gpu, torch.float32)
+    rows = [torch.randint(0, VOCAB, (n,), generator=gen).tolist() for n in (3, 20, 35)]
+    server = Server(gpu, w, rows, 128)
+    heat = torch.tensor([0.0, 0.8, 1.1])
+    kept = refused = 0
+    for _ in range(10):
+        m = int(torch.randint(2, 7, (), generator=gen))
+        n = torch.randint(1, m + 1, (len(rows),), generator=gen).int()
+        drafts, q = torch.zeros(len(rows), m - 1, dtype=torch.int64), torch.zeros(len(rows), m - 1, VOCAB)
+        want = [[] for _ in rows]
+        for b, tokens in enumerate(rows):
+            for t in range(m):
+                behind = plain_logits(w, tokens + drafts[b, :t].tolist()).cpu()
+                want[b].append(behind)
+                if t < m - 1:
+                    near = behind.float() + 1.5 * torch.randn(VOCAB, generator=gen)
+                    q[b, t] = torch.softmax(near / float(heat[b] or 1), -1)
+                    drafts[b, t] = int(torch.multinomial(q[b, t], 1, generator=gen)) if heat[b] else int(near.argmax())
+        ids = torch.cat((torch.tensor([r[-1:] for r in rows]), drafts), 1)
+        uniforms = torch.rand(len(rows), m, generator=gen)
+        logits = server.forward(ids.to(gpu), n.to(gpu))
+        for b in range(len(rows)):
+            for t in range(int(n[b])):
+                # fp32 sums of other orders, over logits of size 10 (the greedy steps' bound)
+                assert float((logits[b, t].cpu().double() - want[b][t]).abs().max()) < 1e-4
+        more = dict(draft_probs=q, temperature=heat, seq_lens=n)
+        path, counts, following = verify_tokens(logits, ids.to(gpu), uniforms.to(gpu),
+                                                **{k: v.to(gpu) for k, v in more.items()})
+        for a, b in zip((path, counts, following), plain.verify_tokens(logits.cpu(), ids, uniforms, **more)):
+            assert torch.equal(a.cpu(), b)
+        keep_tokens(server.keys, server.values, server.table, server.lens, path, counts)
+        server.lens += counts
+        for b, c in enumerate(counts.tolist()):
+            rows[b] += ids[b, 1:c].tolist() + [int(following[b])]
+            kept, refused = kept + c - 1, refused + int(n[b]) - c
+    assert kept > 5 and refused > 5
