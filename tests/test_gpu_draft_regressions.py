@@ -274,3 +274,51 @@ def test_steps_over_lines_with_probabilities(gpu):
             rows[b] += ids[b, 1:c].tolist() + [int(following[b])]
             kept, refused = kept + c - 1, refused + int(n[b]) - c
     assert kept > 5 and refused > 5
+
+
+# ----------------------------------------------------------------------------- shared scratch
+
+
+SHAPES = [(700, 4, 331, torch.bfloat16, True), (3, 5, 9001, torch.float32, False), (1100, 2, 66000, torch.bfloat16, False),
+          (1, 1024, 50, torch.float32, True), (600, 4, 1500, torch.float16, False), (1, 1024, 50, torch.float32, False),
+          (40, 30, 66000, torch.bfloat16, True), (5, 1, 4097, torch.float32, False)]
+
+
+def test_verification_of_one_shape_after_another(gpu):
+    """A stream's counters are as the next call wants them, whatever its sizes and the kernels that they choose, and an
+    attention's in between."""
+    key = torch.randn(40, 1, 16, 64, generator=torch.Generator().manual_seed(1)).to(gpu)
+    table = torch.arange(40, dtype=torch.int32, device=gpu)[None]
+    past = torch.tensor([600], dtype=torch.int32, device=gpu)
+    q = torch.randn(1, 5, 8, 64, generator=torch.Generator().manual_seed(2)).to(gpu)
+    with torch.cuda.stream(torch.cuda.Stream()):
+        attended = tree_attention(q, key, key, table, past)
+        for turn in range(2):
+            for i, shape in enumerate(SHAPES[::-1] if turn else SHAPES):
+                *args, more = drafted_on(gpu, 10 * turn + i, *shape)
+                got = verify_tokens(*args, **more)
+                want = plain.verify_tokens(*args, **more)
+                for a, b in zip(got, want):
+                    assert torch.equal(a.cpu(), b), (turn, shape)
+                assert torch.equal(tree_attention(q, key, key, table, past), attended)
+
+
+def test_verification_of_many_tokens_in_a_graph(gpu):
+    """Replays with other inputs, eager calls of other sizes between them."""
+    for shape in (SHAPES[0], SHAPES[2], SHAPES[4], SHAPES[6]):
+        *args, more = drafted_on(gpu, 0, *shape)
+        verify_tokens(*args, **more)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = verify_tokens(*args, **more)
+        for seed in (1, 2, 3):
+            *others, also = drafted_on(gpu, seed, *shape)
+            for a, b in zip([*args, *more.values()], [*others, *also.values()]):
+                a.copy_(b)
+            graph.replay()
+            *small, rest = drafted_on(gpu, seed, 3, 5, 9001, torch.float32, False)
+            for got, want in ((out, plain.verify_tokens(*others, **also)),
+                              (verify_tokens(*small, **rest), plain.verify_tokens(*small, **rest))):
+                for a, b in zip(got, want):
+                    assert torch.equal(a.cpu(), b), (seed, shape)
