@@ -658,7 +658,8 @@ int pl_paged_attention(int32_t dtype, int32_t cache_dtype, const void* q,
  * row, token and head, out contiguous and apart from q.  Workspace
  * (pl_tree_attention_workspace_bytes(dim, columns) bytes, columns row_len * heads /
  * kv_heads, or 1 in fp32) and
- * counters as above; the two may share them where they follow one another.  At most
+ * counters as above; the two may share them where they follow one another (a call may be
+ * several launches: other threads' calls wait for the last).  At most
  * 1024 query heads to a key head. */
 int64_t pl_tree_attention_workspace_bytes(int32_t dim, int32_t columns);
 
@@ -709,7 +710,8 @@ int pl_keep_tokens(int32_t dtype, int32_t layers, void* const* key_caches,
  * and 2^24 logits to a token.  Workspace (pl_verify_workspace_bytes, 128-byte aligned,
  * not cleared) and counters (pl_verify_counter_ints int32s, 8-byte aligned, zero before
  * the first launch and zero again after each call) are not shared by calls that
- * overlap. */
+ * overlap, those of other threads on the stream among them: a call is up to four
+ * launches. */
 int64_t pl_verify_workspace_bytes(int32_t rows, int32_t nodes, int32_t vocab);
 int64_t pl_verify_counter_ints(int32_t rows, int32_t nodes);
 

@@ -40,7 +40,8 @@ constexpr int kWorkersMax = 2 * kCus;
 template <int DT>
 constexpr int kWeightParts = DT == PL_BF16 ? 3 : 2;
 // log2 of how far scores may pass the maximum that weights are taken against, and of
-// what fp16 weights are multiplied by, that their parts keep small ones: to 2^15.
+// what fp16 weights are multiplied by, that their parts keep small ones: to 2^15.  (They end
+// at 2^-31 of the largest, 2^-39 where the maximum lags by all of it, in their sum as in the output.)
 constexpr float kSlack = 8.f;
 
 // A row's tokens that count, for the tokens of this launch.

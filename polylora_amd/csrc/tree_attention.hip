@@ -11,8 +11,8 @@
 //
 // Few columns are bound by memory, more by the chain from a tile's scores to its weights to
 // its products.  Measured, bf16, 32 query heads over 8 of 128: 8 tokens of 64 rows over up
-// to 4096 (C = 2) 151 us, 3.7 TB/s; 4 tokens (C = 1) 115 us, 4.9 TB/s; 6 tokens of one row over
-// 700 14.3 us, a chain of reads and the waves' join; 16 tokens over 131072 in 8 bits 95 us.
+// to 4096 (C = 2) 155 us, 3.6 TB/s; 4 tokens (C = 1) 113 us, 4.9 TB/s; 6 tokens of one row over
+// 700 14.2 us, a chain of reads and the waves' join; 16 tokens over 131072 in 8 bits 103 us.
 #include "pl_tree.h"
 
 namespace {
@@ -340,10 +340,10 @@ void launch_columns(tree_args a, int64_t atoms_most, hipStream_t s) {
 // Columns above which 16-bit models take the other kernel, which reads keys and values
 // once for all of them where this one reads them again for each 32 (16 of heads above
 // 128 elements), out of the XCD's cache mostly.  Measured in us, this one and the other, 64 rows
-// over 4096 tokens, 8 key heads of 128: 36 columns 189 and 205, 64 180 and 207, 96 240 and
-// 280, 128 268 and 252; one row over 700: 64 columns 15.5 and 21; one over 131072 in 8 bits: 64
-// columns 95 and 119, 96 130 and 179.  Heads of 256 elements: 32 columns 302 and 282, one row
-// 15 and 21, 8 bits 132 and 157; 64 columns 504 and 320.
+// over 4096 tokens, 8 key heads of 128: 36 columns 183 and 209, 64 185 and 215, 96 223 and
+// 263, 128 262 and 273 (252 with weights in two parts); one row over 700: 64 columns 15.9 and 22, 128 16.4
+// and 24; one over 131072 in 8 bits: 64 columns 110 and 129, 96 143 and 182, 128 175 and 184.  Heads of 256
+// elements: 32 columns 299 and 292, one row 15.5 and 23, 8 bits 131 and 163; 64 columns 494 and 320.
 constexpr int narrow_columns(int dp) { return dp == 256 ? 2 * kCols : 6 * kCols; }
 
 template <int DT, int CT, int DP>

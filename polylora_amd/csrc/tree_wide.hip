@@ -15,12 +15,12 @@
 // that 16 rows' pieces of one place, which the keys' product asks for, lie in 16
 // different quarters of the banks.
 //
-// Measured, bf16, 32 query heads over 8 of 128: 64 drafts of 16 rows over 8192 tokens 190 to
-// 220 us by the rows' lengths (49 us of products at the rate of a large one, 65 of bytes);
-// of one row 54.  A unit of 32 tokens by 32 columns takes a wave about 2100 cycles, nearly the
-// sum of its 832 of products and 950 of weights: the two waves of a SIMD overlap little.  A
-// weight in one part of 16 bits would take a fifth of the time (230 -> 184 us) and
-// lose the output's precision (kWeightParts).
+// Measured, bf16, 32 query heads over 8 of 128: 64 drafts of 16 rows over 8192 tokens 195 to 250 us
+// by the rows' lengths (49 us of products at the rate of a large one, 65 of bytes);
+// of one row 57.  With weights in two parts of 16 bits a unit of 32 tokens by 32 columns took a wave about
+// 2100 cycles, nearly the sum of its 832 of products and 950 of weights: the two waves of a SIMD
+// overlap little.  The third part, which holds the rest of the weight (kWeightParts), adds 288 of products
+// and took 64 rows of 32 drafts over 4096 tokens from 240 to 267 us; one part alone took a fifth less than two.
 #include "pl_tree.h"
 
 namespace {
@@ -471,7 +471,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void pl_tree_wide_kernel(tree_args
 
 // Slices to a pair above which parts are joined by a launch of their own, in many workgroups;
 // up to it the last workgroup of a pair joins them, and saves the launch.  In us, always apart
-// / from 2 / from 4 on: 64 drafts of 16 rows over 8192 232 / 246 / 234, over 1024 69 / 69 / 65.5,
+// / from 2 / from 4 on (weights in two parts): 64 drafts of 16 rows over 8192 232 / 246 / 234, over 1024 69 / 69 / 65.5,
 // 32 rows of 16 over 2000 89 / 78 / 78.
 constexpr int kManyParts = 3;
 

@@ -31,11 +31,11 @@
 // that who arrives last at a counter sees what the others have stored: neighbouring tokens' sums
 // share lines, which an XCD that has read one token's may still hold when it reads the next one's.
 //
-// 64-bit exponentials bound a batch: 256 rows of 6 tokens over 128256 fp32 logits take 180 us, 89
+// 64-bit exponentials bound a batch: 256 rows of 6 tokens over 128256 fp32 logits take 170 to 190 us, 89
 // of them their bytes at a copy's rate; without the exponentials the time was nearly halved.
 // One row takes 19 us, four launches that each wait for a few reads one after the other.
-// A workgroup that draws a row whole, without a launch for its pieces, was slower at any
-// number of rows (256 rows of 2 tokens over 128256 fp32 logits 93.2 and 93.2 us, 64 rows 57 and 36, 1024 rows
+// A workgroup that draws a row whole, without a launch for its pieces, was faster at no
+// number of rows (256 rows of 2 tokens over 128256 fp32 logits 93 and 93 us, 64 rows 57 and 36, 1024 rows
 // over 32003 118 and 99).
 namespace {
 
