@@ -19,8 +19,8 @@
 // beside that.  Few tokens are spread over workgroups of four pieces, and a second
 // launch, a workgroup to a token, puts their sums together and says where the row would
 // go from there; of many, each has a workgroup that does both.  A last launch follows
-// each row.  Where a large batch does not run all at once, tokens lie in
-// the grid's order before those behind them, and a workgroup leaves out a token
+// each row.  Many tokens' workgroups do not run all at once: tokens lie in the grid's
+// order before those behind them, and a workgroup leaves out a token
 // that a row is known to have turned away from: what it would have found counts
 // for nothing.  Drawing from what is left of p beside q needs Z first: its pieces are a
 // launch of their own, before the last.
@@ -55,9 +55,6 @@ constexpr int kWholeThreads = 1024;
 constexpr int kWholeTokens = 1024, kWholeFewTokens = 2048;
 constexpr int kFewPieces = 64;  // up to these such a workgroup has kThreads: less to wait for
 constexpr int kWholePieces = 1024;  // whose sums fit beside it
-// Workgroups of whole tokens above which some end before others begin, so that looking for tokens
-// that no row reaches is worth its wait: of kThreads, and of kWholeThreads.
-constexpr int kResident = 1024, kWholeResident = 256;
 
 struct verify_args {
   const void* logits;
@@ -77,7 +74,6 @@ struct verify_args {
   int64_t* next;     // [rows]
   int32_t rows, nodes, vocab, wide_tokens;
   int32_t pieces, groups;  // of a token's logits; workgroups that take them
-  int32_t look;            // whether to look for tokens out of reach
   unsigned long long* verdicts;  // [rows][nodes]: what became of each token (see verdict); between calls 0
   // not cleared
   struct piece_sum* sums;   // [rows][nodes][pieces]
@@ -484,7 +480,7 @@ __global__ __launch_bounds__(THREADS, 8) void pl_verify_whole_kernel(verify_args
   const row_of<DT> r(a, b);
   unsigned long long* verdicts = a.verdicts + (int64_t)b * a.nodes;
   if (node >= r.n) return;
-  if (a.look && node > 0 && out_of_reach<THREADS>(r, node, verdicts, s_path)) return;
+  if (node > 0 && out_of_reach<THREADS>(r, node, verdicts, s_path)) return;
   constexpr int kStep = THREADS / 64;
   float y[kPasses][kVec], ref = -INFINITY;
   for (int piece = wave; piece < a.pieces; piece += kStep) {
@@ -718,7 +714,6 @@ extern "C" int pl_verify_tokens(int32_t dtype, const void* logits, int64_t ld_ro
     pl_set_error("%s: too many rows (%d)", what, rows);
     return PL_ERR_LIMIT;
   }
-  a.look = whole && n > (few ? kResident : kWholeResident);
   uint8_t* at = static_cast<uint8_t*>(workspace);
   a.sums = reinterpret_cast<piece_sum*>(at), at += whole_pieces(n * a.pieces * (int64_t)sizeof(piece_sum));
   a.totals = reinterpret_cast<node_sum*>(at), at += whole_pieces(n * (int64_t)sizeof(node_sum));
