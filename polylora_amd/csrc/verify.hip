@@ -693,6 +693,10 @@ extern "C" int pl_verify_tokens(int32_t dtype, const void* logits, int64_t ld_ro
                  (long long)workspace_bytes, (long long)counter_ints, (long long)need, (long long)ints);
     return PL_ERR_ARG;
   }
+  if (reinterpret_cast<uintptr_t>(workspace) % 128 != 0 || reinterpret_cast<uintptr_t>(counters) % 8 != 0) {
+    pl_set_error("%s: the workspace must begin at whole 128 bytes, the counters at whole 8", what);
+    return PL_ERR_ALIGN;
+  }
   verify_args a;
   a.logits = logits, a.ld_row = ld_row, a.ld_node = ld_node, a.tokens = tokens, a.ld_tokens = ld_tokens;
   a.uniforms = uniforms, a.ld_uniforms = ld_uniforms, a.parents = parents, a.ld_parents = ld_parents;

@@ -8,7 +8,7 @@ import torch
 from polylora_amd import _native
 from polylora_amd.drafts import tree_tables
 
-from .test_drafts_host import _TREE_SCRATCH, _i64, _refused
+from .test_drafts_host import _TREE_SCRATCH, _VERIFY_SCRATCH, _i64, _refused
 
 
 @pytest.mark.parametrize("shift", [16, 64])
@@ -83,3 +83,14 @@ def test_a_token_whose_parent_is_not_before_it_is_a_root(dtype):
     assert visible[..., 0].tolist() == [[1, 3, 7, 11, 16], [1, 2, 5, 8, 21], [1, 2, 6, 9, 16]]
     depths, visible = tree_tables(parents[:, :0])
     assert depths.shape == (3, 0) and visible.shape == (3, 0, 0)
+
+
+def test_verification_scratch_is_aligned_as_the_header_says():
+    lib = _native.load()
+    p = 4096
+    good = dict(dtype=0, logits=p, row=80, node=16, tokens=p, token_bytes=8, ld_tokens=5, uniforms=p, ld_uniforms=5,
+                parents=None, ld_parents=0, probs=p, probs_row=64, probs_node=16, heat=p, seq=None, rows=2, nodes=5,
+                vocab=16, path=p, counts=p, next=p)
+    good.update(_VERIFY_SCRATCH)
+    for bad in (dict(ws=p + 8), dict(ws=p + 64), dict(counters=p + 4)):
+        assert _refused(lib.pl_verify_tokens, good, **bad) == _native.PL_ERR_ALIGN
